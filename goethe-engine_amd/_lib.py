@@ -1,5 +1,5 @@
-"""ctypes binding of libgse.so (include/gse.h), in the style of goethe_engine/gc_c.py:58-77 (bind with an ABI check,
-size-first structs) and gc_c.py:222-227 (a negative return code becomes RuntimeError with the library's last error).
+"""ctypes binding of libgse.so (include/gse.h, include/gsp.h), in the style of goethe_engine/gc_c.py:58-77 (bind with an ABI
+check, size-first structs) and gc_c.py:222-227 (a negative return code becomes RuntimeError with the library's last error).
 
 torch is imported before the library is loaded so that libgse.so binds to the HIP runtime torch already mapped (both
 carry the soname libamdhip64.so.7): one runtime, so torch's streams and device pointers are valid in libgse calls.
@@ -12,7 +12,7 @@ from collections import OrderedDict
 import numpy as np
 import torch
 
-ABI_MAJOR, ABI_MINOR = 1, 4
+ABI_MAJOR, ABI_MINOR = 1, 5
 PATH_MAIN, PATH_DEEP, PATH_EXACT = 0, 1, 2  # gse_row_paths codes
 OK, E_ARG, E_DEVICE, E_UNSUPPORTED, E_CAPACITY = 0, -1, -4, -5, -7
 F32, BF16 = 0, 1
@@ -28,6 +28,8 @@ BATCH_NO_PLAN_WAIT = 4
 BATCH_NO_SPLIT = 8  # (ABI 1.3)
 BATCH_SUBBIN_FINISH = 16  # (ABI 1.4, testing)
 MAX_LOGPROBS = 64
+P_F64, P_F32, P_BF16, P_F16 = 0, 1, 2, 3  # types of probability rows (gsp.h)
+STEP_OK, STEP_FULL, STEP_BAD = 0, 1, 2
 P_ = C.POINTER
 
 PATH = os.environ.get("GSE_LIB", os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgse.so"))
@@ -90,6 +92,36 @@ class PickBatch(C.Structure):
                 ("out_ld", C.c_int64), ("stream", C.c_void_p)]
 
 
+class Chains(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("requests", C.c_uint32), ("vocab", C.c_uint32), ("max_drafts", C.c_uint32),
+                ("drafts", C.c_uint32), ("target_type", C.c_uint32), ("draft_type", C.c_uint32),
+                ("reserved", C.c_uint32), ("target", C.c_void_p), ("target_ld", C.c_int64), ("draft", C.c_void_p),
+                ("draft_ld", C.c_int64), ("begin", C.c_void_p), ("token", C.c_void_p), ("coin", C.c_void_p),
+                ("u", C.c_void_p), ("emit_len", C.c_void_p), ("emit_tokens", C.c_void_p), ("emit_probs", C.c_void_p),
+                ("emit_ld", C.c_int64), ("status", C.c_void_p), ("stream", C.c_void_p)]
+
+
+class Pages(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("requests", C.c_uint32), ("page", C.c_uint32), ("pool", C.c_uint32),
+                ("max_pages", C.c_uint32), ("reserved", C.c_uint32), ("table", C.c_void_p), ("table_ld", C.c_int64), ("ring", C.c_void_p), ("counters", C.c_void_p),
+                ("counters_out", C.c_void_p)]
+
+
+class Step(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("max_tokens", C.c_uint32), ("keep", C.c_void_p), ("add", C.c_void_p),
+                ("depth", C.c_void_p), ("begin", C.c_void_p), ("slot", C.c_void_p), ("pos", C.c_void_p),
+                ("req", C.c_void_p), ("seq_len", C.c_void_p), ("status", C.c_void_p), ("stream", C.c_void_p)]
+
+
+class Path(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("requests", C.c_uint32), ("tokens", C.c_uint32), ("caches", C.c_uint32),
+                ("slot", C.c_void_p), ("anchor", C.c_void_p), ("emit_len", C.c_void_p), ("emit_nodes", C.c_void_p),
+                ("emit_ld", C.c_int64), ("cache", C.c_void_p), ("cache_stride", C.c_int64), ("cache_ptrs", C.c_void_p),
+                ("align", C.c_uint32), ("page", C.c_uint32), ("pages", C.c_uint32), ("chunks", C.c_uint32),
+                ("chunk_bytes", C.c_uint32), ("reserved", C.c_uint32), ("page_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("chunk_stride", C.c_int64), ("stream", C.c_void_p)]
+
+
 SIGNATURES = dict(
     gse_abi_version=(C.c_uint32, []),
     gse_open=(C.c_int, [P_(OpenParams), P_(C.c_void_p)]),
@@ -109,10 +141,15 @@ SIGNATURES = dict(
     gse_last_error=(C.c_char_p, [C.c_void_p]),
     gse_close=(None, [C.c_void_p]),
 )
+ROUND_SIGNATURES = dict(  # include/gsp.h
+    gsp_verify_chains=(C.c_int, [C.c_void_p, P_(Chains)]),
+    gsp_pages_step=(C.c_int, [C.c_void_p, P_(Pages), P_(Step)]),
+    gsp_keep_path=(C.c_int, [C.c_void_p, P_(Path)]),
+)
 
 
 def bind(path=PATH):
-    """The library at path with its gse.h signatures; refuses a different ABI major or an older minor."""
+    """The library at path with its gse.h and gsp.h signatures; refuses a different ABI major or an older minor."""
     if not os.path.exists(path):
         raise RuntimeError(f"{path} is not built: run __graft_entry__.build() (hipcc --offload-arch=gfx950)")
     L = C.CDLL(path)
@@ -122,6 +159,9 @@ def bind(path=PATH):
     v = L.gse_abi_version()
     if v >> 16 != ABI_MAJOR or (v & 0xFFFF) < ABI_MINOR:
         raise RuntimeError(f"{path}: C ABI {v >> 16}.{v & 0xFFFF}, this module needs {ABI_MAJOR}.{ABI_MINOR}+")
+    for n, (res, args) in ROUND_SIGNATURES.items():
+        f = getattr(L, n)
+        f.restype, f.argtypes = res, args
     return L
 
 

@@ -1,4 +1,4 @@
-// Host side of the C ABI in include/gse.h: handle, device workspace, argument checks, launches.
+// Host side of the C ABI in include/gse.h and include/gsp.h: handle, device workspace, argument checks, launches.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -11,6 +11,7 @@
 
 #include "gse_dev.h"
 #include "gse_int.h"
+#include "gsp_int.h"
 
 struct gse_handle {
   int device = 0;
@@ -593,6 +594,71 @@ GSE_API int gse_pack_mask(gse_handle *h, const uint8_t *bools, int64_t bool_ld, 
   DeviceGuard g(h->device);
   hipError_t e = gse::launch_pack(bools, bool_ld, (int)rows, (int)vocab, words, words_ld, (hipStream_t)stream);
   return e == hipSuccess ? GSE_OK : hip_fail(h, e, "pack launch");
+}
+
+GSE_API int gsp_verify_chains(gse_handle *h, const gsp_chains *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsp_chains c;
+  if (!take(in, c)) return fail(h, GSE_E_ARG, "null or short gsp_chains");
+  if (c.requests == 0) return GSE_OK;
+  if (!c.target || !c.begin || !c.u || !c.emit_len || !c.emit_tokens || !c.status)
+    return fail(h, GSE_E_ARG, "target, begin, u, emit_len, emit_tokens and status are required");
+  if (c.drafts > 0 && (!c.token || !c.coin)) return fail(h, GSE_E_ARG, "drafts need token and coin");
+  if (c.target_type > GSP_F16 || (c.draft && c.draft_type > GSP_F16))
+    return fail(h, GSE_E_ARG, "target type %u, draft type %u", c.target_type, c.draft_type);
+  if (c.vocab == 0 || c.target_ld < (int64_t)c.vocab || (c.draft && c.draft_ld < (int64_t)c.vocab))
+    return fail(h, GSE_E_ARG, "vocab 0, target_ld < vocab or draft_ld < vocab");
+  // (token, draft and request numbers are ints in the kernels, one past a row's last token too)
+  if (c.vocab > (1u << 30) || c.max_drafts > (1u << 30) || (uint64_t)c.drafts + c.requests > (1u << 30))
+    return fail(h, GSE_E_UNSUPPORTED, "vocab %u, max_drafts %u, %u drafts of %u requests: at most 2^30", c.vocab, c.max_drafts,
+                c.drafts, c.requests);
+  if (c.emit_ld <= (int64_t)c.max_drafts) return fail(h, GSE_E_ARG, "emit_ld must be > max_drafts");
+  DeviceGuard g(h->device);
+  hipError_t e = gse::launch_chains(rows_ws(h), c, (hipStream_t)c.stream);
+  return e == hipSuccess ? GSE_OK : hip_fail(h, e, "chain launch");
+}
+
+GSE_API int gsp_pages_step(gse_handle *h, const gsp_pages *pages, const gsp_step *step) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsp_pages p;
+  gsp_step t;
+  if (!take(pages, p) || !take(step, t)) return fail(h, GSE_E_ARG, "null or short gsp_pages / gsp_step");
+  if (p.requests == 0) return GSE_OK;
+  if (!p.table || !p.ring || !p.counters || !p.counters_out)
+    return fail(h, GSE_E_ARG, "table, ring, counters and counters_out are required");
+  if (!t.add || !t.begin || !t.seq_len || !t.status || (t.max_tokens > 0 && !t.slot))
+    return fail(h, GSE_E_ARG, "add, begin, slot, seq_len and status are required");
+  if (p.page == 0 || p.pool == 0 || p.max_pages == 0) return fail(h, GSE_E_ARG, "page, pool and max_pages must be > 0");
+  if (p.table_ld < (int64_t)p.max_pages) return fail(h, GSE_E_ARG, "table_ld < max_pages");
+  if (p.pool > (uint32_t)INT32_MAX || (uint64_t)p.max_pages * p.page > (uint64_t)INT32_MAX)
+    return fail(h, GSE_E_UNSUPPORTED, "%u pages, %u pages of %u tokens a request: at most 2^31 - 1 pages, and as many tokens",
+                p.pool, p.max_pages, p.page);
+  if (p.requests > (1u << 30) || t.max_tokens > (1u << 30))
+    return fail(h, GSE_E_UNSUPPORTED, "%u requests, %u tokens: at most 2^30", p.requests, t.max_tokens);
+  DeviceGuard g(h->device);
+  hipError_t e = gse::launch_pages(p, t, (hipStream_t)t.stream);
+  return e == hipSuccess ? GSE_OK : hip_fail(h, e, "page step launch");
+}
+
+GSE_API int gsp_keep_path(gse_handle *h, const gsp_path *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsp_path p;
+  if (!take(in, p)) return fail(h, GSE_E_ARG, "null or short gsp_path");
+  if (p.requests == 0 || p.caches == 0 || p.tokens == 0) return GSE_OK;
+  if (!p.slot || !p.anchor || !p.emit_len || !p.emit_nodes || (!p.cache && !p.cache_ptrs))
+    return fail(h, GSE_E_ARG, "slot, anchor, emit_len, emit_nodes and cache or cache_ptrs are required");
+  if (p.page == 0 || p.pages == 0 || p.chunks == 0 || p.chunk_bytes == 0 || p.emit_ld <= 0)
+    return fail(h, GSE_E_ARG, "page, pages, chunks, chunk_bytes and emit_ld must be > 0");
+  if (p.page_stride < 0 || p.token_stride < 0 || p.chunk_stride < 0)
+    return fail(h, GSE_E_ARG, "page_stride, token_stride and chunk_stride must be >= 0");
+  if (p.cache_ptrs && (p.align == 0 || (p.align & (p.align - 1))))
+    return fail(h, GSE_E_ARG, "align %u is no power of two", p.align);
+  if ((uint64_t)p.chunks * p.chunk_bytes > (1u << 30) || (uint64_t)p.chunks * p.chunk_bytes * p.caches > (1u << 30))
+    return fail(h, GSE_E_UNSUPPORTED, "%u caches of %llu bytes a token: at most 2^30 bytes in all", p.caches,
+                (unsigned long long)p.chunks * p.chunk_bytes);
+  DeviceGuard g(h->device);
+  hipError_t e = gse::launch_path(p, (hipStream_t)p.stream);
+  return e == hipSuccess ? GSE_OK : hip_fail(h, e, "path launch");
 }
 
 GSE_API int gse_profile(gse_handle *h, float *ms, uint32_t n, uint32_t *calls) {

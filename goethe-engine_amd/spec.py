@@ -7,6 +7,8 @@
   mss_batch(p, kids, seeds, idxs)  many independent nodes in one launch
   verify_tree(reqs, ...)           one verify round of many requests' draft trees in one call (gse_verify_tree): every
                                    node decided on the device, the walk done there, one copy of the results back
+  verify_chains(target, ...)       many requests' drafted chains against rows of target probabilities, with the random
+                                   numbers given, in one call (gsp_verify_chains); nothing leaves the device
   pick_batch(x, n, t, seeds, ats)  the drafter's children of many nodes in one call (gse_draft_pick)
   qprob(x, t)                      q = softmax(float64(x) / t) of drafter rows on the device (gse_qprob)
   Tree / as_tree                   spec.py:22-67: the proposal tree the scheduler fits and the engine walks
@@ -289,6 +291,14 @@ class VerifyCall:
             res.append((tk, nd, why))
         return res
 
+    def keep_path(self, step, caches, heads_first=False):
+        """engine.py:299-305's commit on the device, on the current stream after launch(): moves every request's accepted
+        path in the paged caches (paged.keep_path) from the slots that the round's nodes were written to (step: the
+        paged.StepMap of this round, its requests this call's, add = each one's nodes) to the slots after its anchor. The
+        paged.PageTable's next step keeps emit_len tokens of each request (call.e_len)."""
+        from . import paged
+        paged.keep_path(caches, step.slot, self.keep[0], self.e_len, self.e_node, heads_first=heads_first)
+
     def _build(self, reqs, nout0, emit_ld):
         dev = _device()
         sizes = [len(r["tokens"]) + 1 for r in reqs]
@@ -432,6 +442,105 @@ def _stack_targets(ts, sizes, dev):
                 return torch.as_strided(base, (int(sum(sizes)), base.shape[1]), base.stride())
         return torch.cat([t.to(dev) for t in ts])
     return torch.cat([(t if isinstance(t, torch.Tensor) else torch.from_numpy(np.asarray(t))).to(dev) for t in ts])
+
+
+# ---- drafted chains against rows of probabilities ------------------------------------------------------------------
+
+_PROB = {torch.float64: _lib.P_F64, torch.float32: _lib.P_F32, torch.bfloat16: _lib.P_BF16, torch.float16: _lib.P_F16}
+
+
+class Chains:
+    """verify_chains' device results: emit_len int32 [R], tokens int32 [R, max_drafts + 1] (-1 past emit_len), probs fp32 of
+    the same shape (the target's weight of each emitted token, 0 past them), status int32 [R] (_lib.WALK_OK, or WALK_ERROR:
+    the row to draw from held no valid token; emit_len then counts the accepted drafts alone)."""
+
+    def __init__(self, emit_len, tokens, probs, status):
+        self.emit_len, self.tokens, self.probs, self.status = emit_len, tokens, probs, status
+
+    def tolist(self):
+        """Per request (emitted tokens, "error" or None), as verify_tree reports them."""
+        n, t, st = self.emit_len.cpu().tolist(), self.tokens.cpu().tolist(), self.status.cpu().tolist()
+        return [(t[a][:n[a]], "error" if st[a] != _lib.WALK_OK else None) for a in range(len(n))]
+
+
+def _prob_rows(x, what, rows, v=None):
+    """[>= rows, V] probability rows with unit column stride."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _PROB:
+        raise ValueError(f"{what} must be a [rows, V] tensor of float64, float32, bfloat16 or float16")
+    if x.shape[0] < rows or (v is not None and x.shape[1] != v):
+        raise ValueError(f"{what} of {tuple(x.shape)}, need {rows} rows" + (f" of {v}" if v is not None else ""))
+    if x.shape[1] and (x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
+        x = x.contiguous()
+    return x
+
+
+def _i32(x, dev):
+    """Integers as a contiguous int32 device tensor; values outside int32 keep their sign (at its ends)."""
+    t = x if isinstance(x, torch.Tensor) else torch.tensor(np.asarray(x, dtype=np.int64))
+    if t.is_floating_point() or t.dtype == torch.bool:
+        raise ValueError(f"expected integers, got {t.dtype}")
+    if t.dtype != torch.int32:
+        t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+    return t.to(dev).contiguous()
+
+
+def _f64(x, dev):
+    t = x if isinstance(x, torch.Tensor) else torch.from_numpy(np.asarray(x, np.float64))
+    return t.to(dev, torch.float64).contiguous()
+
+
+def verify_chains(target, tokens, begin, coins, u, draft=None, max_drafts=None):
+    """Drafted chains (one draft per position) of R requests against the target's probabilities, in one
+    gsp_verify_chains call on the current stream, asynchronously: a Chains of device tensors.
+
+    tokens [D]: request r's drafts are tokens[begin[r]:begin[r + 1]] (begin [R + 1]; a token outside the vocabulary ends its
+    chain, so padded batches pad with -1); target [D + R, V]: row begin[r] + r + i the target's distribution after r's first
+    i drafts (fp64, fp32, bf16 or fp16, any row stride, used in place: softmax rows, dist_batch's); draft [D, V]: the
+    distribution each draft was drawn from (any of these types, qprob's), None for a deterministic drafter; coins [D] and
+    u [R]: numbers in [0, 1) (fp64). Draft x is accepted while coin * q(x) < p(x); at the first that is not, the token is
+    drawn with u from max(p - q, 0), after the last one from the row that follows. A chain of one draft is mss with one kid.
+    max_drafts: the longest chain a request may have (default: from begin, which then has to be on the host)."""
+    if max_drafts is None:
+        if isinstance(begin, torch.Tensor) and begin.device.type != "cpu":
+            raise ValueError("begin is on the device: max_drafts is required")
+        ends = [int(k) for k in begin]
+        max_drafts = max([b - a for a, b in zip(ends, ends[1:])] + [0])
+    for x in (tokens, begin, coins, u):
+        if isinstance(x, torch.Tensor) and x.dim() != 1:
+            raise ValueError("tokens, begin, coins and u must have one dimension")
+    k, d = int(max_drafts), len(tokens)
+    n = len(begin) - 1
+    if n < 0 or k < 0:
+        raise ValueError("begin must have one entry more than there are requests, max_drafts be >= 0")
+    target = _prob_rows(target, "target", d + n)
+    v = target.shape[1]
+    if draft is not None:
+        draft = _prob_rows(draft, "draft", d, v)
+    if len(coins) != d or len(u) != n or v == 0:
+        raise ValueError(f"{d} tokens and {n} requests need as many coins and draws, got {len(coins)} and {len(u)} (V = {v})")
+    dev = target.device if target.device.type == "cuda" else _device()
+    for x in (draft, tokens, begin, coins, u):
+        if isinstance(x, torch.Tensor) and x.device.type == "cuda" and x.device != dev:
+            raise ValueError(f"tensors on {x.device} and {dev}")
+    target = target.to(dev)
+    tokens, begin, coins, u = _i32(tokens, dev), _i32(begin, dev), _f64(coins, dev), _f64(u, dev)
+    out = Chains(torch.empty(n, dtype=torch.int32, device=dev), torch.empty((n, k + 1), dtype=torch.int32, device=dev),
+                 torch.empty((n, k + 1), dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.int32, device=dev))
+    if n == 0:
+        return out
+    c = _lib.Chains()
+    c.size = C.sizeof(_lib.Chains)
+    c.requests, c.vocab, c.max_drafts, c.drafts = n, v, k, d
+    c.target_type, c.target, c.target_ld = _PROB[target.dtype], target.data_ptr(), max(target.stride(0), v)
+    if draft is not None and d:
+        draft = draft.to(dev)
+        c.draft_type, c.draft, c.draft_ld = _PROB[draft.dtype], draft.data_ptr(), max(draft.stride(0), v)
+    c.begin, c.token, c.coin, c.u = begin.data_ptr(), tokens.data_ptr(), coins.data_ptr(), u.data_ptr()
+    c.emit_len, c.emit_tokens, c.emit_probs = out.emit_len.data_ptr(), out.tokens.data_ptr(), out.probs.data_ptr()
+    c.emit_ld, c.status = k + 1, out.status.data_ptr()
+    c.stream = torch.cuda.current_stream(dev).cuda_stream
+    _lib.handle(dev.index, 1, v).call("gsp_verify_chains", C.byref(c))
+    return out
 
 
 # ---- the drafter's selection (spec.py:151-159) ---------------------------------------------------------------------

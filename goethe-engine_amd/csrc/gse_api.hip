@@ -279,6 +279,7 @@ gse::RowsWs rows_ws(const gse_handle *h) {
   w.seg = (double *)h->tseg;
   w.last = h->plast;
   w.tick = h->ptick;
+  w.ticks = (int)std::max(h->max_rows, gse::TICKS);
   w.mass = h->ppart;
   w.top = h->ptop;
   w.st = h->tstate;
@@ -613,6 +614,8 @@ GSE_API int gsp_verify_chains(gse_handle *h, const gsp_chains *in) {
     return fail(h, GSE_E_UNSUPPORTED, "vocab %u, max_drafts %u, %u drafts of %u requests: at most 2^30", c.vocab, c.max_drafts,
                 c.drafts, c.requests);
   if (c.emit_ld <= (int64_t)c.max_drafts) return fail(h, GSE_E_ARG, "emit_ld must be > max_drafts");
+  if (!gse::chains_fit(rows_ws(h), c))
+    return fail(h, GSE_E_CAPACITY, "vocab %u, the handle was opened for %u", c.vocab, h->max_vocab);
   DeviceGuard g(h->device);
   hipError_t e = gse::launch_chains(rows_ws(h), c, (hipStream_t)c.stream);
   return e == hipSuccess ? GSE_OK : hip_fail(h, e, "chain launch");

@@ -225,13 +225,18 @@ struct TreeLaunch {
 
 // The workspace of the row passes (gse_rows.hip): per row, `slices` slices of RS tokens.
 constexpr int RS = 4096;
+// Slice tickets of a handle, at least: a call whose rows need no other room per row (a chain's slice sums are few) takes
+// this many of them in one launch, whatever the handle was opened for (512 chains over 262144 bf16 tokens through a handle
+// of 64 rows, one workgroup a slice: eight launches 260 us, one 173).
+constexpr uint32_t TICKS = 4096;
 struct RowsWs {
   int rows, slices;
   int round;        // workgroups of one resident round (four per CU)
   double *sum;      // [rows][slices] slice sums
   double *seg;      // [rows][slices][64] segment sums
   int32_t *last;    // [rows][slices] last token with a positive weight
-  uint32_t *tick;   // [rows] slice tickets, zero between calls
+  int ticks;        // max(rows, TICKS)
+  uint32_t *tick;   // [ticks] slice tickets, zero between calls
   Fx *mass;         // [rows][slices] slice masses
   uint64_t *top;    // [rows][slices][GSE_MAX_KIDS] the slices' best entries
   TreeNode *st;     // [rows] state of a node between launches (its ticket zero between calls)
@@ -283,7 +288,7 @@ constexpr Layout plan_layout(uint32_t R, uint32_t V, uint32_t target, bool tree)
     L.ppart = put((size_t)R * S * (CH / RS) * sizeof(Fx));
     L.plast = put((size_t)R * S * (CH / RS) * sizeof(int32_t));
     L.ptop = put((size_t)R * S * (CH / RS) * GSE_MAX_KIDS * sizeof(uint64_t));
-    L.ptick = put((size_t)R * sizeof(uint32_t));
+    L.ptick = put((size_t)(R > TICKS ? R : TICKS) * sizeof(uint32_t));
     L.plist = put((size_t)(GSE_MAX_KIDS + 1) * R * sizeof(uint32_t));  // the nodes of each residual pass
     L.pcnt = put((GSE_MAX_KIDS + 1) * sizeof(uint32_t));
   }

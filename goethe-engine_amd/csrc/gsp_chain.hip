@@ -12,9 +12,9 @@ namespace gse {
 
 namespace {
 
-constexpr int CT = 256;          // threads of a slice's workgroup
+constexpr int CT = 256;          // threads of a workgroup
 constexpr int CW = CT / WAVE;
-constexpr int CS = 8;            // steps that the last slice's search takes at once (CT partial sums each, in LDS)
+constexpr int WGS_MAX = 48;      // workgroups of a request, at most
 
 template <int T>
 constexpr int SIZE = T == GSP_F64 ? 8 : T == GSP_F32 ? 4 : 2;
@@ -98,295 +98,260 @@ __device__ __forceinline__ ChainEnd chain_end(const gsp_chains &c, int r, bool e
   return e;
 }
 
-// The distribution that a request's token is drawn from: weight(t) = max(p(t) - q(t), 0) (Q: q given; X: the draft x's own
-// weight dropped, else).
+// The distribution that a request's token is drawn from: weight(t) = max(p(t) - q(t), 0), q null: max(p(t), 0), and x's
+// weight 0. The kernel sums v + |v| = 2 max(v, 0), v = p - q, which is exact, one add, and unlike a maximum keeps what is not
+// finite: a NaN or an infinity anywhere in the rows makes the sum NaN or infinite. Every sum and threshold is so doubled.
 struct ChainRow {
   const char *p, *q;
   int x;
 };
 
-// A vector's weights. bad becomes NaN when a weight is not finite (NaN or infinite p or q).
-template <int PT, int QT, int VEC>
+template <int PT, int QT, int VEC, bool HQ>
 struct Weights {
+  static constexpr int Q = HQ ? QT : GSP_BF16;
   Raw<PT, VEC> p;
-  Raw<QT < 0 ? GSP_BF16 : QT, QT < 0 ? 2 : VEC> q;
+  Raw<Q, HQ ? VEC : 2> q;
   __device__ __forceinline__ void load(const ChainRow &w, int64_t t) {
     p.load(w.p, t);
-    if constexpr (QT >= 0)
-      if (w.q) q.load(w.q, t);
+    if constexpr (HQ) q.load(w.q, t);
   }
-  __device__ __forceinline__ double get(const ChainRow &w, int64_t t, int i, double &bad) const {
+  __device__ __forceinline__ double get(int i) const {
     double v = p.get(i);
-    if constexpr (QT >= 0) {
-      if (w.q) v -= q.get(i);
-    } else {
-      if (t + i == w.x) v = 0.0;
-    }
-    bad = fma(v, 0.0, bad);
-    return fmax(v, 0.0);
+    if constexpr (HQ) v -= q.get(i);
+    return v + fabs(v);
   }
 };
 
-// The same for one token.
-template <int PT, int QT>
-__device__ __forceinline__ double weight(const ChainRow &w, int64_t t, double &bad) {
+template <int PT, int QT, bool HQ>
+__device__ __forceinline__ double weight(const ChainRow &w, int t) {
   double v = value<PT>(w.p, t);
-  if constexpr (QT >= 0) {
-    if (w.q) v -= value<QT>(w.q, t);
-  } else {
-    if (t == w.x) v = 0.0;
-  }
-  bad = fma(v, 0.0, bad);
-  return fmax(v, 0.0);
+  if constexpr (HQ) v -= value<QT>(w.q, t);
+  return t == w.x ? 0.0 : v + fabs(v);
 }
 
+// A row's vectors of VEC tokens go to segments of S * 64: vector k * 64 + lane of a segment is a lane's k-th. The tokens past
+// the row's last whole vector (fewer than VEC) go with the last segment, one a lane.
 struct ChainArgs {
   gsp_chains c;
   int r0;          // first request of the launch
-  int ns, steps;   // slices of a row, steps of a slice; a step is one vector a thread
-  double *sum;     // [requests of the launch][ns]
-  uint32_t *tick;  // [requests of the launch], zero between calls
+  int nseg;        // segments of a row
+  double *sum;     // [requests of the launch][nseg]
+  uint32_t *tick;  // ticket of request k of the launch at k * tstride, zero between calls
+  int tstride;
 };
 
-struct ChainShared {
-  double part[CS * CT];
-  double wave[CW];
-  int hit[CW];
-  uint32_t ticket;
-};
-
-// Sum over the workgroup in a fixed order (every thread gets it).
-__device__ __forceinline__ double block_sum(double v, ChainShared &sh) {
-  v = wave_sum_f64(v);
-  __syncthreads();
-  if (lane_id() == 0) sh.wave[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double t = sh.wave[0];
-  for (int k = 1; k < CW; ++k) t += sh.wave[k];
-  return t;
-}
-
-// This thread's part of the weights of steps [s0, s1) of a row: whole vectors, S at a time, and after the row's last whole
-// vector the tokens that are left, one a thread.
-// (s1 - s0 is a multiple of S)
-template <int PT, int QT, int VEC, int S>
-__device__ __forceinline__ double steps_sum(const ChainRow &w, int64_t s0, int64_t s1, int V) {
-  const int nv = V / VEC, tid = threadIdx.x;
-  double acc = 0.0, bad = 0.0;
-  for (int64_t s = s0; s < s1; s += S) {
-    Weights<PT, QT, VEC> x[S];
-#pragma unroll
-    for (int k = 0; k < S; ++k) {
-      const int64_t i = (s + k) * CT + tid;  // (past the end: the last vector again, its weights dropped)
-      x[k].load(w, min(i, (int64_t)nv - 1) * VEC);
-    }
-#pragma unroll
-    for (int k = 0; k < S; ++k) {
-      const int64_t i = (s + k) * CT + tid;
-      double a = 0.0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) a += x[k].get(w, min(i, (int64_t)nv - 1) * VEC, e, bad);
-      acc += i < nv ? a : 0.0;
-    }
-  }
-  return acc + bad;
-}
-
-// The tokens after a row's last whole vector belong to the step after it, as this thread's single token.
-template <int PT, int QT, int VEC>
+template <int PT, int QT, int VEC, bool HQ>
 __device__ __forceinline__ double tail_weight(const ChainRow &w, int V) {
-  const int t = V / VEC * VEC + (int)threadIdx.x;
-  double bad = 0.0;
-  const double v = t < V ? weight<PT, QT>(w, t, bad) : 0.0;
-  return v + bad;
+  const int t = V / VEC * VEC + lane_id();
+  return t < V ? weight<PT, QT, HQ>(w, t) : 0.0;
 }
 
-// The first token of steps [s0, s1) (tail: and of the row's tail) with a positive weight whose prefix, from `before` on, reaches
-// thr; the last one with a positive weight when rounding leaves none, -1 when there is none at all. By the workgroup.
-template <int PT, int QT, int VEC>
-__device__ __noinline__ int search(const ChainRow &w, int64_t s0, int64_t s1, bool tail, int V, double before, double thr,
-                                   ChainShared &sh) {
-  const int nv = V / VEC, tid = threadIdx.x, lane = lane_id(), wv = tid >> 6;
-  int last = -1;
-  double bad = 0.0;
-  for (int64_t s = s0; s < s1; s += CS) {
-    // the vectors' sums, then every thread a run of CS of them in vocabulary order
-    __syncthreads();
-    for (int k = 0; k < CS; ++k) {
-      const int64_t i = (s + k) * CT + tid;
-      double a = 0.0;
-      if (i < nv && s + k < s1) {
-        Weights<PT, QT, VEC> x;
-        x.load(w, i * VEC);
+// The sum of a segment (last: with the row's tail), by one wave; every lane gets it.
+template <int PT, int QT, int VEC, int S, bool HQ>
+__device__ __forceinline__ double segment_sum(const ChainRow &w, int seg, bool last, int V) {
+  const int nv = V / VEC, i0 = seg * (S * WAVE), lane = lane_id();
+  double a = 0.0;
+  if (i0 + S * WAVE <= nv && (w.x < i0 * VEC || w.x >= (i0 + S * WAVE) * VEC)) {  // whole, and w.x not in it
+    Weights<PT, QT, VEC, HQ> x[S];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) a += x.get(w, i * VEC, e, bad);
-      }
-      sh.part[k * CT + tid] = a;
-    }
-    __syncthreads();
-    double run[CS], tot = 0.0;
-    for (int k = 0; k < CS; ++k) tot += run[k] = sh.part[tid * CS + k];
-    const double inc = wave_incl_scan_f64(tot);
-    if (lane == WAVE - 1) sh.wave[wv] = inc;
-    __syncthreads();
-    double base = before;
-    for (int k = 0; k < wv; ++k) base += sh.wave[k];
-    const double up = shfl_up_f64(inc, 1);  // (by every lane: a lane that does not take part gives nothing)
-    double at = lane > 0 ? base + up : base;
-    int hit = -1, pos = -1;  // this thread's first vector that reaches thr, its last with a weight
-    double hat = 0.0;
-    for (int k = 0; k < CS; ++k) {
-      const double nx = at + run[k];
-      if (run[k] > 0.0) {
-        pos = tid * CS + k;
-        if (hit < 0 && !(nx < thr)) {
-          hit = pos;
-          hat = at;
-        }
-      }
-      at = nx;
-    }
-    const uint64_t hm = ballot64(hit >= 0), pm = ballot64(pos >= 0);
-    // (a thread's run may pass thr where the wave's scan, in another order, had not: the first thread counts)
-    const int src = hm ? (int)__builtin_ctzll(hm) : pm ? 63 - (int)__builtin_clzll(pm) : 0;
-    const int vec = __shfl(hm ? hit : pos, src, WAVE);
-    const double vat = shfl_f64(hat, src);
-    for (int k = 0; k < CW; ++k) before += sh.wave[k];
-    __syncthreads();
-    if (lane == 0) {
-      sh.hit[wv] = hm ? vec : pm ? -2 - vec : -1;
-      sh.wave[wv] = vat;
-    }
-    __syncthreads();
-    int at_vec = -1;
-    double from = 0.0;
-    for (int k = CW - 1; k >= 0; --k) {
-      if (sh.hit[k] >= 0) {
-        at_vec = sh.hit[k];
-        from = sh.wave[k];
-      }
-    }
-    int lv = -1;
-    for (int k = 0; k < CW; ++k)
-      if (sh.hit[k] < -1) lv = -2 - sh.hit[k];
-    const int v = at_vec >= 0 ? at_vec : lv;
-    if (v >= 0) {  // the vector's tokens, the same in every thread
-      const int64_t t0 = (s * CT + v) * VEC;
-      Weights<PT, QT, VEC> x;
-      x.load(w, t0);
-      int found = -1;
+    for (int k = 0; k < S; ++k) x[k].load(w, (int64_t)(i0 + k * WAVE + lane) * VEC);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const double a = x.get(w, t0, e, bad);
-        from += a;
-        if (a > 0.0) {
-          last = (int)t0 + e;
-          if (at_vec >= 0 && found < 0 && !(from < thr)) found = last;
-        }
-      }
-      if (at_vec >= 0) return found >= 0 ? found : last;
+    for (int k = 0; k < S; ++k) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) a += x[k].get(e);
+    }
+  } else {
+    for (int i = i0 + lane; i < min(i0 + S * WAVE, nv); i += WAVE) {
+      Weights<PT, QT, VEC, HQ> x;
+      x.load(w, (int64_t)i * VEC);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) a += i * VEC + e == w.x ? 0.0 : x.get(e);
     }
   }
-  if (tail) {
-    for (int t = nv * VEC; t < V; ++t) {
-      const double a = weight<PT, QT>(w, t, bad);
-      before += a;
-      if (a > 0.0) {
-        last = t;
-        if (!(before < thr)) return t;
-      }
-    }
-  }
-  return last;
+  if (last) a += tail_weight<PT, QT, VEC, HQ>(w, V);
+  return wave_sum_f64(a);
 }
 
-// One workgroup a slice of a request's row: the chain's end (every workgroup finds it: its drafts' values are cached after
-// the first), the slice's sum, and the ticket whose last holder searches the row.
+// The first token of a segment (last: and of the row's tail) with a positive weight whose prefix, from `before` on, reaches
+// thr (found); the last token with a positive weight when none does, -1 when there is none. before becomes the prefix after
+// the segment where none does. By one wave; every lane gets it.
+template <int PT, int QT, int VEC, int S, bool HQ>
+__device__ __forceinline__ int segment_search(const ChainRow &w, int seg, bool last, int V, double &before, double thr,
+                                              bool &found) {
+  const int nv = V / VEC, i0 = seg * (S * WAVE), lane = lane_id();
+  int lst = -1;
+  constexpr int H = S < 4 ? S : 4;  // vectors a lane loads at once
+  Weights<PT, QT, VEC, HQ> x[H];
+#pragma unroll
+  for (int k = 0; k < S; ++k) {
+    if (k % H == 0 && nv > 0) {  // (past the last vector: that one again, not counted)
+#pragma unroll
+      for (int j = 0; j < H; ++j) x[j].load(w, (int64_t)min(i0 + (k + j) * WAVE + lane, nv - 1) * VEC);
+    }
+    const int i = i0 + k * WAVE + lane;
+    double b[VEC], a = 0.0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a += b[e] = i < nv && i * VEC + e != w.x ? x[k % H].get(e) : 0.0;
+    const double inc = before + wave_incl_scan_f64(a), up = shfl_up_f64(inc, 1);
+    // this lane's tokens: the first that reaches thr, the last with a weight
+    double at = lane > 0 ? up : before;
+    int hit = -1, pos = -1;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      at += b[e];
+      if (b[e] > 0.0) {
+        pos = i * VEC + e;
+        if (hit < 0 && !(at < thr)) hit = pos;
+      }
+    }
+    const uint64_t pm = ballot64(pos >= 0);
+    // the first lane whose vector reaches thr by the scan: its own sum, in another order, may stay below
+    const uint64_t hm = ballot64(pos >= 0 && !(inc < thr));
+    found = hm != 0;
+    if (found) return __builtin_amdgcn_readlane(hit >= 0 ? hit : pos, (int)__builtin_ctzll(hm));
+    if (pm) lst = __builtin_amdgcn_readlane(pos, 63 - (int)__builtin_clzll(pm));
+    before = shfl_f64(inc, WAVE - 1);
+  }
+  if (last) {
+    const int t = V / VEC * VEC + lane;
+    const double b = tail_weight<PT, QT, VEC, HQ>(w, V);
+    const double inc = before + wave_incl_scan_f64(b);
+    const uint64_t pm = ballot64(b > 0.0), hm = ballot64(b > 0.0 && !(inc < thr));
+    found = hm != 0;
+    if (found) return __builtin_amdgcn_readlane(t, (int)__builtin_ctzll(hm));
+    if (pm) lst = __builtin_amdgcn_readlane(t, 63 - (int)__builtin_clzll(pm));
+    before = shfl_f64(inc, WAVE - 1);
+  }
+  return lst;
+}
+
+// The token drawn from a row whose segments are summed, by one wave; -1: an error.
+template <int PT, int QT, int VEC, int S, bool HQ>
+__device__ __forceinline__ int chain_draw(const ChainRow &w, const double *sum, int nseg, int V, double u, double &total) {
+  constexpr int NB = 8;  // 64 sums each, loaded at once: a row of up to 512 segments waits for one round of loads
+  const int lane = lane_id();
+  double x[NB];
+  auto block = [&](int b0) {
+#pragma unroll
+    for (int k = 0; k < NB; ++k) x[k] = b0 + k * WAVE + lane < nseg ? ld_ag(&sum[b0 + k * WAVE + lane]) : 0.0;
+  };
+  total = 0.0;
+  for (int b0 = 0; b0 < nseg; b0 += NB * WAVE) {
+    block(b0);
+    double t = 0.0;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) t += x[k];
+    total += wave_sum_f64(t);
+  }
+  if (!(total > 0.0 && total < INFINITY)) return -1;
+  const double thr = u * total;
+  double before = 0.0, lb = 0.0;
+  int lst = -1;  // the segment that the draw falls into: the first that reaches thr, else the last with a weight
+  bool hit = false;
+  for (int b0 = 0; b0 < nseg && !hit; b0 += NB * WAVE) {
+    if (nseg > NB * WAVE) block(b0);
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      if (hit || b0 + k * WAVE >= nseg) continue;
+      const double inc = before + wave_incl_scan_f64(x[k]);
+      const uint64_t pos = ballot64(x[k] > 0.0), hm = ballot64(x[k] > 0.0 && !(inc < thr));
+      hit = hm != 0;
+      if (pos) {
+        const int l = hit ? (int)__builtin_ctzll(hm) : 63 - (int)__builtin_clzll(pos);
+        lst = b0 + k * WAVE + l;
+        lb = l > 0 ? shfl_f64(inc, l - 1) : before;
+      }
+      before = shfl_f64(inc, WAVE - 1);
+    }
+  }
+  bool found = false;
+  return segment_search<PT, QT, VEC, S, HQ>(w, lst, lst == nseg - 1, V, lb, thr, found);
+}
+
+// The same from p alone, nothing summed yet: where p is nowhere above q. One wave over the row twice; only rounding (of p and
+// q to their types, of the product with the coin) leads here.
+template <int PT, int QT, int VEC, int S>
+__device__ __noinline__ int chain_draw_again(const char *p, int nseg, int V, double u) {
+  const ChainRow w{p, nullptr, -1};
+  double total = 0.0, before = 0.0;
+#pragma unroll 1
+  for (int i = 0; i < nseg; ++i) total += segment_sum<PT, QT, VEC, S, false>(w, i, i == nseg - 1, V);
+  if (!(total > 0.0 && total < INFINITY)) return -1;
+  int lst = -1;
+  bool found = false;
+#pragma unroll 1
+  for (int i = 0; i < nseg && !found; ++i) {
+    const int j = segment_search<PT, QT, VEC, S, false>(w, i, i == nseg - 1, V, before, u * total, found);
+    if (j >= 0) lst = j;
+  }
+  return lst;
+}
+
+// gridDim.x workgroups a request. Every wave finds the chain's end by itself (its drafts' values are cached after the first),
+// then sums its share of the row's segments; the last workgroup's first wave (by a ticket) draws the token. No barrier but
+// the ticket's, nothing in LDS but its answer.
 template <int PT, int QT, int S>
-__global__ __launch_bounds__(CT) void chain_kernel(ChainArgs a) {
-  constexpr int VEC = 16 / (QT >= 0 && SIZE<QT < 0 ? 0 : QT> > SIZE<PT> ? SIZE<QT < 0 ? 0 : QT> : SIZE<PT>);
-  __shared__ ChainShared sh;
+__global__ __launch_bounds__(CT) __attribute__((amdgpu_waves_per_eu(4, 8))) void chain_kernel(ChainArgs a) {
+  constexpr int QS = QT < 0 ? 0 : SIZE<QT < 0 ? 0 : QT>;
+  constexpr int VEC = 16 / (QS > SIZE<PT> ? QS : SIZE<PT>);
+  __shared__ uint32_t ticket;
   const gsp_chains &c = a.c;
-  const int s = blockIdx.x, k = blockIdx.y, r = a.r0 + k, tid = threadIdx.x, lane = lane_id(), V = (int)c.vocab;
-  const ChainEnd e = chain_end<PT, QT>(c, r, s == 0 && tid < WAVE);
-  ChainRow w;
-  w.p = row_of<PT>(c.target, c.target_ld, e.row);
-  w.q = nullptr;
-  w.x = -1;
+  const int k = blockIdx.y, r = a.r0 + k, tid = threadIdx.x, lane = lane_id(), V = (int)c.vocab;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * CW + (tid >> 6)));  // the wave among the request's
+  const int waves = (int)gridDim.x * CW;
+  const ChainEnd e = chain_end<PT, QT>(c, r, wv == 0);
+  ChainRow w{row_of<PT>(c.target, c.target_ld, e.row), nullptr, -1};
   if (e.x >= 0) {
     if constexpr (QT >= 0) w.q = row_of<QT>(c.draft, c.draft_ld, e.row - r);
     else w.x = e.x;
   }
-  const int nv = V / VEC;
-  double total = 0.0;
+  double *sum = a.sum + (int64_t)k * a.nseg;
+  auto sums = [&](auto hq) {
+    for (int i = wv; i < a.nseg; i += waves) {
+      const double t = segment_sum<PT, QT, VEC, S, decltype(hq)::value>(w, i, i == a.nseg - 1, V);
+      if (lane == 0) st_ag(&sum[i], t);
+    }
+  };
   if (e.a >= 0) {
-    const int64_t s0 = (int64_t)s * a.steps;
-    double part = nv > 0 ? steps_sum<PT, QT, VEC, S>(w, s0, s0 + a.steps, V) : 0.0;
-    if (s == a.ns - 1) part += tail_weight<PT, QT, VEC>(w, V);
-    total = block_sum(part, sh);
+    if constexpr (QT >= 0) {
+      if (w.q) sums(std::true_type{});
+      else sums(std::false_type{});
+    } else {
+      sums(std::false_type{});
+    }
   }
-  double *sum = a.sum + (int64_t)k * a.ns;
-  if (tid == 0) {
-    st_ag(&sum[s], total);
-    store_wait();
-    sh.ticket = ticket_add(&a.tick[k]);
-  }
+  store_wait();
   __syncthreads();
-  if (sh.ticket != (uint32_t)(a.ns - 1)) return;
+  if (tid == 0) ticket = ticket_add(&a.tick[k * a.tstride]);
+  __syncthreads();
+  if (ticket != gridDim.x - 1 || tid >= WAVE) return;
   int j = -1;
   if (e.a >= 0) {
-    total = 0.0;
-    for (int i0 = 0; i0 < a.ns; i0 += WAVE) total += wave_sum_f64(i0 + lane < a.ns ? ld_ag(&sum[i0 + lane]) : 0.0);
-    int64_t s0 = 0, s1 = (int64_t)a.ns * a.steps;
-    bool tail = true;
-    double before = 0.0, thr = 0.0;
-    if (total == 0.0 && e.x >= 0) {  // p is nowhere above q: drawn from p itself, by this workgroup alone
-      w.q = nullptr;
-      w.x = -1;
-      total = block_sum((nv > 0 ? steps_sum<PT, QT, VEC, S>(w, s0, s1, V) : 0.0) + tail_weight<PT, QT, VEC>(w, V), sh);
-      thr = c.u[r] * total;
-    } else if (total > 0.0) {
-      thr = c.u[r] * total;
-      int at = -1, lst = -1;  // the slice that the draw falls into
-      double lb = 0.0;
-      for (int i0 = 0; i0 < a.ns && at < 0; i0 += WAVE) {
-        const double x = i0 + lane < a.ns ? ld_ag(&sum[i0 + lane]) : 0.0;
-        const double inc = before + wave_incl_scan_f64(x);
-        const uint64_t hit = ballot64(x > 0.0 && !(inc < thr)), pos = ballot64(x > 0.0);
-        if (hit) {
-          const int l = (int)__builtin_ctzll(hit);
-          at = i0 + l;
-          if (l > 0) before = shfl_f64(inc, l - 1);
-        } else {
-          if (pos) {
-            const int l = 63 - (int)__builtin_clzll(pos);
-            lst = i0 + l;
-            lb = l > 0 ? shfl_f64(inc, l - 1) : before;
-          }
-          before = shfl_f64(inc, WAVE - 1);
-        }
-      }
-      if (at < 0) {
-        at = lst;
-        before = lb;
-      }
-      s0 = (int64_t)at * a.steps;
-      s1 = s0 + a.steps;
-      tail = at == a.ns - 1;
+    const double u = c.u[r];
+    double total = 0.0;
+    if constexpr (QT >= 0) {
+      if (w.q) j = chain_draw<PT, QT, VEC, S, true>(w, sum, a.nseg, V, u, total);
+      else j = chain_draw<PT, QT, VEC, S, false>(w, sum, a.nseg, V, u, total);
+    } else {
+      j = chain_draw<PT, QT, VEC, S, false>(w, sum, a.nseg, V, u, total);
     }
-    if (total > 0.0 && total < INFINITY) j = search<PT, QT, VEC>(w, s0, s1, tail, V, before, thr, sh);
+    if (total == 0.0 && e.x >= 0) j = chain_draw_again<PT, QT, VEC, S>(w.p, a.nseg, V, u);
   }
-  if (tid == 0) {
+  if (lane == 0) {
     const int n = max(e.a, 0);
     c.emit_len[r] = n + (j >= 0 ? 1 : 0);
     c.status[r] = j >= 0 ? GSE_WALK_OK : GSE_WALK_ERROR;
     c.emit_tokens[r * c.emit_ld + n] = j;
     if (c.emit_probs) c.emit_probs[r * c.emit_ld + n] = j >= 0 ? (float)value<PT>(w.p, j) : 0.0f;
-    a.tick[k] = 0;
+    a.tick[k * a.tstride] = 0;
   }
 }
 
 }  // namespace
+
+bool chains_fit(const RowsWs &w, const gsp_chains &c) {  // (the longest segments over the narrowest vectors)
+  return (int64_t)c.vocab / (2 * 8 * WAVE) + 1 <= (int64_t)w.rows * w.slices * 64;
+}
 
 hipError_t launch_chains(const RowsWs &w, const gsp_chains &c, hipStream_t s) {
   auto go = [&](auto pt, auto qt) {
@@ -397,23 +362,27 @@ hipError_t launch_chains(const RowsWs &w, const gsp_chains &c, hipStream_t s) {
     a.c = c;
     a.sum = w.seg;
     a.tick = w.tick;
-    const int64_t all = ((int64_t)c.vocab / VEC + CT - 1) / CT;  // steps of a row (0: the tail alone)
-    const int64_t cap = (int64_t)w.rows * w.slices * 64;         // slice sums that the workspace holds
-    const int64_t most = min((int64_t)w.rows, (int64_t)65535);   // requests of a launch
-    const int64_t rows = min((int64_t)c.requests, most);
-    // The steps of a slice: as few as keep the launch at two resident rounds of workgroups.
-    int64_t steps = 1;
-    while (steps < 8 && rows * ((all + steps - 1) / steps) > 2 * (int64_t)w.round) steps *= 2;
-    while ((all + steps - 1) / steps > cap) steps *= 2;
-    a.steps = (int)steps;
-    a.ns = (int)max((int64_t)1, (all + steps - 1) / steps);
-    const int64_t per = min(rows, cap / a.ns);
+    const int64_t nv = (int64_t)c.vocab / VEC;
+    const int64_t cap = (int64_t)w.rows * w.slices * 64;         // segment sums that the workspace holds
+    const int64_t rows = min((int64_t)c.requests, min((int64_t)w.ticks, (int64_t)65535));  // requests of a launch, at most
+    // One resident round of workgroups over the launch, as long as a wave has a segment; the longest segments that leave
+    // every wave one.
+    auto segs = [&](int64_t S) { return max((int64_t)1, (nv + S * WAVE - 1) / (S * WAVE)); };
+    int64_t most = max((int64_t)1, min((int64_t)(w.round) / rows, (int64_t)WGS_MAX));
+    if (segs(8) >= 8 * CW * most) most *= 4;
+    int S = 8;
+    while (S > 1 && segs(S) < most * CW) S /= 2;
+    while (S < 8 && segs(S) > cap) S *= 2;
+    a.nseg = (int)segs(S);
+    const int64_t wgs = min(most, (a.nseg + CW - 1) / (int64_t)CW);
+    const int64_t per = min(rows, cap / a.nseg);
+    a.tstride = (int)min((int64_t)w.ticks / per, (int64_t)64);
     for (int64_t r0 = 0; r0 < (int64_t)c.requests; r0 += per) {
       a.r0 = (int)r0;
-      const dim3 grid((uint32_t)a.ns, (uint32_t)min(per, (int64_t)c.requests - r0));
-      if (steps == 1) hipLaunchKernelGGL((chain_kernel<P, Q, 1>), grid, dim3(CT), 0, s, a);
-      else if (steps == 2) hipLaunchKernelGGL((chain_kernel<P, Q, 2>), grid, dim3(CT), 0, s, a);
-      else if (steps == 4) hipLaunchKernelGGL((chain_kernel<P, Q, 4>), grid, dim3(CT), 0, s, a);
+      const dim3 grid((uint32_t)wgs, (uint32_t)min(per, (int64_t)c.requests - r0));
+      if (S == 1) hipLaunchKernelGGL((chain_kernel<P, Q, 1>), grid, dim3(CT), 0, s, a);
+      else if (S == 2) hipLaunchKernelGGL((chain_kernel<P, Q, 2>), grid, dim3(CT), 0, s, a);
+      else if (S == 4) hipLaunchKernelGGL((chain_kernel<P, Q, 4>), grid, dim3(CT), 0, s, a);
       else hipLaunchKernelGGL((chain_kernel<P, Q, 8>), grid, dim3(CT), 0, s, a);
     }
   };

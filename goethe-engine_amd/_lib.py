@@ -241,12 +241,19 @@ class Handle:
             pass
 
 
+def raw_stream(device):
+    """The hipStream_t of the current stream of a device (0.1 us; torch.cuda.current_stream's object takes 2)."""
+    if not torch.cuda.is_initialized():
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def handle(device, rows, vocab):
     """The handle of (device, current stream) that fits rows x vocab, reopened larger on demand. Calls on two streams
     may overlap on the device, so each stream gets its own workspace; at most MAX_HANDLES stay cached."""
-    if not torch.cuda.is_available():
+    if not _handles and not torch.cuda.is_available():
         raise RuntimeError("goethe-engine_amd needs a HIP device (torch.cuda.is_available() is False)")
-    key = (device, torch.cuda.current_stream(device).cuda_stream)
+    key = (device, raw_stream(device))
     with _lock:
         h = _handles.get(key)
         if h is None or h.rows < rows or h.vocab < vocab:

@@ -659,6 +659,8 @@ GSE_API int gsp_keep_path(gse_handle *h, const gsp_path *in) {
   if ((uint64_t)p.chunks * p.chunk_bytes > (1u << 30) || (uint64_t)p.chunks * p.chunk_bytes * p.caches > (1u << 30))
     return fail(h, GSE_E_UNSUPPORTED, "%u caches of %llu bytes a token: at most 2^30 bytes in all", p.caches,
                 (unsigned long long)p.chunks * p.chunk_bytes);
+  if ((uint64_t)p.pages * p.page > UINT32_MAX)
+    return fail(h, GSE_E_UNSUPPORTED, "%u pages of %u tokens: at most 2^32 - 1 slots", p.pages, p.page);
   DeviceGuard g(h->device);
   hipError_t e = gse::launch_path(p, (hipStream_t)p.stream);
   return e == hipSuccess ? GSE_OK : hip_fail(h, e, "path launch");

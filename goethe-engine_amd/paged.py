@@ -19,13 +19,14 @@ A round of chains needs no move: its accepted drafts are already consecutive (sp
 step's keep).
 """
 import ctypes as C
+import math
 
 import numpy as np
 import torch
 
 from . import _lib
 from .sampling import _device
-from .spec import _i32
+from .spec import _count, _vec
 
 
 class StepMap:
@@ -41,9 +42,9 @@ class StepMap:
 
 
 def _state(t, what, dev, dims):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims or t.device != dev:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != dims or t.device != dev:
         raise ValueError(f"{what} must be an int32 tensor of {dims} dimension(s) on {dev}")
-    if t.shape[-1] and t.stride(-1) != 1:
+    if not t.is_contiguous() and t.stride(-1) != 1:
         raise ValueError(f"{what} must have unit stride")
     return t
 
@@ -78,6 +79,7 @@ class PageTable:
             raise ValueError("requests, pool, page and max_pages must be > 0")
         if self.requests > 1 and table.stride(0) < self.max_pages:
             raise ValueError("table rows overlap")
+        self.table_ld = table.stride(0) if self.requests > 1 else self.max_pages
         self.counters, self.page, self.device = self._counters(counters), page, dev
 
     def _counters(self, t):
@@ -108,56 +110,55 @@ class PageTable:
         the map (default: the sum of add, which then has to be on the host). into: counters of the same size that receive
         the new state; this table's own then stay as they were (pages taken are the same if the step is made again).
         Returns a StepMap."""
-        if len(add) != self.requests or (keep is not None and len(keep) != self.requests):
-            raise ValueError(f"add and keep must have {self.requests} entries")
+        r, dev = self.requests, self.device
+        if _count(add) != r or (keep is not None and _count(keep) != r):
+            raise ValueError(f"add and keep must have {r} entries")
         if max_tokens is None:
             if isinstance(add, torch.Tensor) and add.device.type != "cpu":
                 raise ValueError("add is on the device: max_tokens is required")
             max_tokens = sum(max(int(k), 0) for k in add)
-        n, r, dev = int(max_tokens), self.requests, self.device
+        n = int(max_tokens)
         if not 0 <= n <= 1 << 30:
             raise ValueError(f"max_tokens {n} is not in [0, 2^30]")
-        if depth is not None and len(depth) < n:
+        if depth is not None and _count(depth) < n:
             raise ValueError(f"depth must have {n} entries")
-        if into is not None:
+        if into is None:
+            into = self.counters
+        elif into is not self.counters:
             self._counters(into)
             if 0 < abs(into.data_ptr() - self.counters.data_ptr()) < 4 * into.numel():
                 raise ValueError("into overlaps the table's counters")
         if dev.type != "cuda":
             raise RuntimeError("goethe-engine_amd needs a HIP device (the table's state is on the host)")
-        for x in (add, keep, depth):
-            if isinstance(x, torch.Tensor) and x.device.type == "cuda" and x.device != dev:
-                raise ValueError(f"tensors on {x.device} and {dev}")
-        add = _i32(add, dev)
-        keep = _i32(keep, dev) if keep is not None else None
-        depth = _i32(depth, dev) if depth is not None else None
-        i32 = dict(dtype=torch.int32, device=dev)
-        m = StepMap(torch.empty(r + 1, **i32), torch.empty(n, dtype=torch.int64, device=dev), torch.empty(n, **i32),
-                    torch.empty(n, **i32), torch.empty(r, **i32), torch.empty(r, **i32),
-                    into if into is not None else self.counters)
-        p = _lib.Pages()
-        p.size = C.sizeof(_lib.Pages)
-        p.requests, p.page, p.pool, p.max_pages = r, self.page, self.ring.numel(), self.max_pages
-        p.table, p.table_ld, p.ring = self.table.data_ptr(), self.table.stride(0) if r > 1 else self.max_pages, self.ring.data_ptr()
-        p.counters, p.counters_out = self.counters.data_ptr(), m.counters.data_ptr()
-        t = _lib.Step()
-        t.size, t.max_tokens = C.sizeof(_lib.Step), n
-        t.keep = keep.data_ptr() if keep is not None else None
-        t.add = add.data_ptr()
-        t.depth = depth.data_ptr() if depth is not None else None
-        t.begin, t.slot, t.pos, t.req = m.begin.data_ptr(), m.slot.data_ptr(), m.pos.data_ptr(), m.req.data_ptr()
-        t.seq_len, t.status = m.seq_len.data_ptr(), m.status.data_ptr()
-        t.stream = torch.cuda.current_stream(dev).cuda_stream
+        i32 = torch.int32
+        add = _vec(add, i32, dev)
+        keep = _vec(keep, i32, dev) if keep is not None else None
+        depth = _vec(depth, i32, dev) if depth is not None else None
+        slot = torch.empty(n, dtype=torch.int64, device=dev)
+        pos, req, begin, seq, status = torch.empty(2 * n + 3 * r + 1, dtype=i32, device=dev).split_with_sizes((n, n, r + 1, r, r))
+        p = _lib.Pages(_PAGES, r, self.page, self.ring.shape[0], self.max_pages, 0, self.table.data_ptr(), self.table_ld,
+                       self.ring.data_ptr(), self.counters.data_ptr(), into.data_ptr())
+        t = _lib.Step(_STEP, n, keep.data_ptr() if keep is not None else None, add.data_ptr(),
+                      depth.data_ptr() if depth is not None else None, begin.data_ptr(), slot.data_ptr(), pos.data_ptr(),
+                      req.data_ptr(), seq.data_ptr(), status.data_ptr(), _lib.raw_stream(dev.index))
         _lib.handle(dev.index, 1, 1).call("gsp_pages_step", C.byref(p), C.byref(t))
-        return m
+        return StepMap(begin, slot, pos, req, seq, status, into)
 
 
-def _layout(shape, stride, size, heads_first):
+_PAGES, _STEP, _PATH = C.sizeof(_lib.Pages), C.sizeof(_lib.Step), C.sizeof(_lib.Path)
+
+
+def _layout(shape, stride, size, heads_first, dense=False):
     """(pages, page, chunks, chunk bytes, page / token / chunk strides in bytes) of one cache's [pages, page, ...] or, heads
-    first, [pages, heads, page, ...]: a token's data as equal contiguous chunks."""
+    first, [pages, heads, page, ...]: a token's data as equal contiguous chunks. dense: the tensor has no gaps."""
     need = 4 if heads_first else 3
-    if len(shape) < need or any(k < 1 for k in shape):
+    if len(shape) < need or 0 in shape:
         raise ValueError(f"a cache of shape {tuple(shape)}: [pages, {'heads, page' if heads_first else 'page, ...'}] is wanted")
+    if dense:  # (sizes from the shape: a dimension of one may have any stride)
+        token = math.prod(shape[need - 1:]) * size
+        if heads_first:
+            return shape[0], shape[2], shape[1], token, shape[1] * shape[2] * token, token, shape[2] * token
+        return shape[0], shape[1], 1, token, shape[1] * token, token, 0
     if any(s == 0 and k > 1 for k, s in zip(shape, stride)):
         raise ValueError("a cache must not be an expanded tensor")
 
@@ -195,7 +196,7 @@ class Caches:
         for t in self.tensors:
             if t.shape != t0.shape or t.stride() != t0.stride() or t.dtype != t0.dtype or t.device != t0.device:
                 raise ValueError("caches must have one shape, layout, type and device")
-        self.layout = _layout(t0.shape, t0.stride(), t0.element_size(), self.heads_first)
+        self.layout = _layout(t0.shape, t0.stride(), t0.element_size(), self.heads_first, t0.is_contiguous())
         ptrs = [t.data_ptr() for t in self.tensors]
         if len(set(ptrs)) < len(ptrs):
             raise ValueError("the same cache twice")
@@ -210,7 +211,8 @@ def keep_path(caches, slot, anchor, emit_len, emit_nodes, heads_first=False):
     caches: a Caches, or one stacked tensor [n, pages, page, ...] (heads_first: [n, pages, heads, page, ...]); slot: StepMap.slot
     of the round; anchor, emit_len int32 [R], emit_nodes int32 [R, ld]: gse_verify_tree's (VerifyCall.keep_path passes
     them). Nodes ascend along a path and requests share no slots; entries out of range and negative slots are skipped."""
-    if isinstance(caches, Caches):
+    stacked = not isinstance(caches, Caches)
+    if not stacked:
         n, layout, dev = len(caches.tensors), caches.layout, caches.device
     else:
         if not isinstance(caches, torch.Tensor) or caches.dim() < 4:
@@ -218,30 +220,28 @@ def keep_path(caches, slot, anchor, emit_len, emit_nodes, heads_first=False):
         if caches.shape[0] > 1 and caches.stride(0) == 0:
             raise ValueError("a cache must not be an expanded tensor")
         n, dev = caches.shape[0], caches.device
-        layout = _layout(caches.shape[1:], caches.stride()[1:], caches.element_size(), heads_first)
-    r = len(anchor)
-    if len(emit_len) != r or emit_nodes.dim() != 2 or emit_nodes.shape[0] != r:
+        layout = _layout(caches.shape[1:], caches.stride()[1:], caches.element_size(), heads_first, caches.is_contiguous())
+    r = _count(anchor)
+    if _count(emit_len) != r or emit_nodes.dim() != 2 or emit_nodes.shape[0] != r:
         raise ValueError(f"anchor, emit_len and emit_nodes must have one entry per request ({r})")
     if not isinstance(slot, torch.Tensor) or slot.dtype != torch.int64 or slot.dim() != 1:
         raise ValueError("slot must be an int64 tensor of one dimension")
     if dev.type != "cuda":
         raise RuntimeError("goethe-engine_amd needs a HIP device (the caches are on the host)")
-    for x in (slot, anchor, emit_len, emit_nodes):
-        if isinstance(x, torch.Tensor) and x.device.type == "cuda" and x.device != dev:
-            raise ValueError(f"tensors on {x.device} and {dev}")
-    if r == 0 or n == 0 or emit_nodes.shape[1] == 0:
+    if slot.device != dev:
+        raise ValueError(f"slot on {slot.device}, the caches on {dev}")
+    ld = emit_nodes.shape[1]
+    if r == 0 or n == 0 or ld == 0:
         return
-    slot = slot.to(dev).contiguous()
-    anchor, emit_len, emit_nodes = _i32(anchor, dev), _i32(emit_len, dev), _i32(emit_nodes, dev)
-    p = _lib.Path()
-    p.size = C.sizeof(_lib.Path)
-    p.requests, p.tokens, p.caches = r, slot.numel(), n
-    p.slot, p.anchor, p.emit_len = slot.data_ptr(), anchor.data_ptr(), emit_len.data_ptr()
-    p.emit_nodes, p.emit_ld = emit_nodes.data_ptr(), emit_nodes.shape[1]
-    if isinstance(caches, Caches):
-        p.cache_ptrs, p.align = caches.ptrs.data_ptr(), caches.align
+    slot = slot.contiguous()
+    i32 = torch.int32
+    anchor, emit_len, emit_nodes = _vec(anchor, i32, dev), _vec(emit_len, i32, dev), _vec(emit_nodes, i32, dev)
+    pages, page, chunks, size, page_stride, token_stride, chunk_stride = layout
+    if stacked:
+        base, stride, ptrs, align = caches.data_ptr(), caches.stride(0) * caches.element_size(), None, 0
     else:
-        p.cache, p.cache_stride = caches.data_ptr(), caches.stride(0) * caches.element_size()
-    p.pages, p.page, p.chunks, p.chunk_bytes, p.page_stride, p.token_stride, p.chunk_stride = layout
-    p.stream = torch.cuda.current_stream(dev).cuda_stream
+        base, stride, ptrs, align = None, 0, caches.ptrs.data_ptr(), caches.align
+    p = _lib.Path(_PATH, r, slot.shape[0], n, slot.data_ptr(), anchor.data_ptr(), emit_len.data_ptr(), emit_nodes.data_ptr(), ld,
+                  base, stride, ptrs, align, page, pages, chunks, size, 0, page_stride, token_stride, chunk_stride,
+                  _lib.raw_stream(dev.index))
     _lib.handle(dev.index, 1, 1).call("gsp_keep_path", C.byref(p))

@@ -467,26 +467,31 @@ def _prob_rows(x, what, rows, v=None):
     """[>= rows, V] probability rows with unit column stride."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _PROB:
         raise ValueError(f"{what} must be a [rows, V] tensor of float64, float32, bfloat16 or float16")
-    if x.shape[0] < rows or (v is not None and x.shape[1] != v):
+    n, cols = x.shape
+    if n < rows or (v is not None and cols != v):
         raise ValueError(f"{what} of {tuple(x.shape)}, need {rows} rows" + (f" of {v}" if v is not None else ""))
-    if x.shape[1] and (x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
+    ld, step = x.stride()
+    if cols and (step != 1 or (n > 1 and ld < cols)):
         x = x.contiguous()
     return x
 
 
-def _i32(x, dev):
-    """Integers as a contiguous int32 device tensor; values outside int32 keep their sign (at its ends)."""
-    t = x if isinstance(x, torch.Tensor) else torch.tensor(np.asarray(x, dtype=np.int64))
-    if t.is_floating_point() or t.dtype == torch.bool:
-        raise ValueError(f"expected integers, got {t.dtype}")
-    if t.dtype != torch.int32:
-        t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
-    return t.to(dev).contiguous()
-
-
-def _f64(x, dev):
-    t = x if isinstance(x, torch.Tensor) else torch.from_numpy(np.asarray(x, np.float64))
-    return t.to(dev, torch.float64).contiguous()
+def _vec(x, dtype, dev):
+    """Numbers as a contiguous device tensor of dtype (int32: values outside it keep their sign, at its ends)."""
+    if isinstance(x, torch.Tensor):
+        if x.dtype is dtype and x.device == dev and x.is_contiguous():
+            return x
+        if x.device != dev and x.device.type == "cuda":
+            raise ValueError(f"tensors on {x.device} and {dev}")
+    elif dtype is torch.int32:
+        x = torch.from_numpy(np.asarray(x, np.int64))
+    else:
+        x = torch.from_numpy(np.asarray(x, np.float64))
+    if dtype is torch.int32 and x.dtype is not torch.int32:
+        if x.is_floating_point() or x.dtype is torch.bool:
+            raise ValueError(f"expected integers, got {x.dtype}")
+        x = x.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
+    return x.to(dev, dtype).contiguous()
 
 
 def verify_chains(target, tokens, begin, coins, u, draft=None, max_drafts=None):
@@ -505,42 +510,50 @@ def verify_chains(target, tokens, begin, coins, u, draft=None, max_drafts=None):
             raise ValueError("begin is on the device: max_drafts is required")
         ends = [int(k) for k in begin]
         max_drafts = max([b - a for a, b in zip(ends, ends[1:])] + [0])
-    for x in (tokens, begin, coins, u):
-        if isinstance(x, torch.Tensor) and x.dim() != 1:
-            raise ValueError("tokens, begin, coins and u must have one dimension")
-    k, d = int(max_drafts), len(tokens)
-    n = len(begin) - 1
+    k = int(max_drafts)
+    d, n, nc, nu = _count(tokens), _count(begin) - 1, _count(coins), _count(u)
     if n < 0 or k < 0:
         raise ValueError("begin must have one entry more than there are requests, max_drafts be >= 0")
     target = _prob_rows(target, "target", d + n)
     v = target.shape[1]
     if draft is not None:
         draft = _prob_rows(draft, "draft", d, v)
-    if len(coins) != d or len(u) != n or v == 0:
-        raise ValueError(f"{d} tokens and {n} requests need as many coins and draws, got {len(coins)} and {len(u)} (V = {v})")
-    dev = target.device if target.device.type == "cuda" else _device()
-    for x in (draft, tokens, begin, coins, u):
-        if isinstance(x, torch.Tensor) and x.device.type == "cuda" and x.device != dev:
-            raise ValueError(f"tensors on {x.device} and {dev}")
-    target = target.to(dev)
-    tokens, begin, coins, u = _i32(tokens, dev), _i32(begin, dev), _f64(coins, dev), _f64(u, dev)
-    out = Chains(torch.empty(n, dtype=torch.int32, device=dev), torch.empty((n, k + 1), dtype=torch.int32, device=dev),
-                 torch.empty((n, k + 1), dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.int32, device=dev))
+    if nc != d or nu != n or v == 0:
+        raise ValueError(f"{d} tokens and {n} requests need as many coins and draws, got {nc} and {nu} (V = {v})")
+    dev = target.device
+    if dev.type != "cuda":
+        dev = _device()
+        target = target.to(dev)
+    tokens, begin = _vec(tokens, torch.int32, dev), _vec(begin, torch.int32, dev)
+    coins, u = _vec(coins, torch.float64, dev), _vec(u, torch.float64, dev)
+    i32 = torch.int32
+    out = Chains(torch.empty(n, dtype=i32, device=dev), torch.empty((n, k + 1), dtype=i32, device=dev),
+                 torch.empty((n, k + 1), dtype=torch.float32, device=dev), torch.empty(n, dtype=i32, device=dev))
     if n == 0:
         return out
-    c = _lib.Chains()
-    c.size = C.sizeof(_lib.Chains)
-    c.requests, c.vocab, c.max_drafts, c.drafts = n, v, k, d
-    c.target_type, c.target, c.target_ld = _PROB[target.dtype], target.data_ptr(), max(target.stride(0), v)
+    q, q_type, q_ld = None, 0, 0
     if draft is not None and d:
-        draft = draft.to(dev)
-        c.draft_type, c.draft, c.draft_ld = _PROB[draft.dtype], draft.data_ptr(), max(draft.stride(0), v)
-    c.begin, c.token, c.coin, c.u = begin.data_ptr(), tokens.data_ptr(), coins.data_ptr(), u.data_ptr()
-    c.emit_len, c.emit_tokens, c.emit_probs = out.emit_len.data_ptr(), out.tokens.data_ptr(), out.probs.data_ptr()
-    c.emit_ld, c.status = k + 1, out.status.data_ptr()
-    c.stream = torch.cuda.current_stream(dev).cuda_stream
+        if draft.device != dev:
+            draft = _vec(draft, draft.dtype, dev)
+        q, q_type, q_ld = draft.data_ptr(), _PROB[draft.dtype], max(draft.stride(0), v)
+    stream = _lib.raw_stream(dev.index)
+    c = _lib.Chains(_CHAINS, n, v, k, d, _PROB[target.dtype], q_type, 0, target.data_ptr(), max(target.stride(0), v), q, q_ld,
+                    begin.data_ptr(), tokens.data_ptr(), coins.data_ptr(), u.data_ptr(), out.emit_len.data_ptr(),
+                    out.tokens.data_ptr(), out.probs.data_ptr(), k + 1, out.status.data_ptr(), stream)
     _lib.handle(dev.index, 1, v).call("gsp_verify_chains", C.byref(c))
     return out
+
+
+_CHAINS = C.sizeof(_lib.Chains)
+
+
+def _count(x):
+    """Entries of a one-dimensional tensor, array or list."""
+    if isinstance(x, torch.Tensor):
+        if x.dim() != 1:
+            raise ValueError("tokens, begin, coins and u must have one dimension")
+        return x.shape[0]
+    return len(x)
 
 
 # ---- the drafter's selection (spec.py:151-159) ---------------------------------------------------------------------

@@ -178,3 +178,10 @@ def test_cache_layouts(ge):
     assert lay(t, True) == (6, 3, 4, 16, 192, 16, 48)            # [pages, 4 heads, 3 tokens, 8]
     assert lay(t.transpose(1, 2)) == (6, 3, 4, 16, 192, 16, 48)
     assert lay(torch.zeros(5, 4, 7, dtype=torch.uint8)) == (5, 4, 1, 7, 28, 7, 0)
+    # without gaps: the same, also where a dimension of one has a stride of its own
+    dense = lambda t, hf=False: ge.paged._layout(t.shape, t.stride(), t.element_size(), hf, t.is_contiguous())  # noqa: E731
+    assert dense(t) == lay(t) and dense(t, True) == lay(t, True)
+    one = torch.zeros(400, dtype=torch.uint8).as_strided((5, 1, 2, 6), (12, 77, 6, 1))
+    assert one.is_contiguous() and dense(one) == (5, 1, 1, 12, 12, 12, 0)
+    one = torch.zeros(400, dtype=torch.uint8).as_strided((5, 2, 1, 6), (12, 6, 77, 1))
+    assert one.is_contiguous() and dense(one, True) == (5, 1, 2, 6, 12, 6, 6)

@@ -16,8 +16,8 @@ namespace {
 // Every workgroup (of ST threads) forms the sums itself (16 bytes a request, from cache), ST requests at a time, one a thread,
 // so no workgroup waits for another; then it takes its tiles of ST of the chunk's tokens and its share of the pages given
 // back. The state is read from counters and written to counters_out by one workgroup: when they are the same array, by a
-// second launch. Bound by the chain of state, scan, search and page reads, 4 us for a request, 6 for 512; 2^20 tokens write
-// 17 MB in 13 us.
+// second launch. Bound by the chain of state, scan, search and page reads: 3.9 us for a request, 6.1 for 512; 1024 requests with
+// a map of 2^20 entries (17 MB written) 10.9 us.
 
 struct Req {       // a request's part of the step
   int64_t kept, add;
@@ -74,15 +74,15 @@ __device__ __forceinline__ int find(const uint32_t *first, int n, uint32_t x) {
   return lo;
 }
 
-// The exclusive prefix of the thread's s over the workgroup, on top of carry, which becomes the sum after it.
+// The exclusive prefix of the thread's s over the workgroup, on top of carry, which becomes the sum after it; inc: the
+// inclusive prefix in the wave, wave: the waves' sums (scanned by every wave; added up one after the other, the step of 1024
+// requests took 13.2 us).
 template <int N>
 __device__ __forceinline__ int64_t block_prefix(int64_t s, int64_t inc, int64_t &carry, const int64_t (&wave)[N]) {
-  int64_t base = carry + inc - s;
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    if (k < (int)(threadIdx.x >> 6)) base += wave[k];
-    carry += wave[k];
-  }
+  const int lane = lane_id(), wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint64_t to = wave_incl_scan_u64(lane < N ? (uint64_t)wave[lane] : 0ull);
+  const int64_t base = carry + inc - s + (wv > 0 ? (int64_t)shfl_u64(to, wv - 1) : 0);
+  carry += (int64_t)lane63(to);
   return base;
 }
 
@@ -288,8 +288,8 @@ __global__ __launch_bounds__(PT) void path_kernel(gsp_path a, uint32_t vecs) {
 
 hipError_t launch_pages(const gsp_pages &p, const gsp_step &t, hipStream_t s) {
   // A thread a request, up to 1024 (96 requests: workgroups of 256 with a request a thread 4.5 us, with four 5.8; 512: 6.2 with
-  // 512 threads, 6.8 with 256 of two); 2^18 threads over the tokens: every workgroup forms the sums anew (1024 requests,
-  // 2^20 tokens: 2^17, 2^18, 2^19 threads 14.6, 13.1, 17.9 us).
+  // 512 threads, 6.8 with 256 of four); 2^18 threads over the tokens: every workgroup forms the sums anew (1024 requests,
+  // 2^20 tokens: 2^17, 2^18, 2^19 threads 12.2, 10.9, 13.1 us).
   constexpr int64_t threads = 1 << 18;
   auto go = [&](auto st) {
     constexpr int ST = decltype(st)::value;

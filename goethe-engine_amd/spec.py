@@ -297,6 +297,9 @@ class VerifyCall:
         paged.StepMap of this round, its requests this call's, add = each one's nodes) to the slots after its anchor. The
         paged.PageTable's next step keeps emit_len tokens of each request (call.e_len)."""
         from . import paged
+        if step.begin.shape[0] != self.n_req + 1 or step.slot.shape[0] < self.nodes:
+            raise ValueError(f"a step of {step.begin.shape[0] - 1} requests and {step.slot.shape[0]} slots for a round of "
+                             f"{self.n_req} and {self.nodes} nodes")
         paged.keep_path(caches, step.slot, self.keep[0], self.e_len, self.e_node, heads_first=heads_first)
 
     def _build(self, reqs, nout0, emit_ld):

@@ -222,6 +222,23 @@ def test_special_values(ge, gpu):
         assert want[8][0] == [300] and want[10][0] == [13, 699] and len(want[9][0]) == 1
 
 
+@pytest.mark.parametrize("target", list(TYPES))
+def test_smallest_weights_count(ge, gpu, target):
+    """Rows whose weights are the type's smallest (fp64: small ones): they are summed and drawn from like any other,
+    subnormal or not."""
+    tiny = {"f64": 2.0 ** -1000, "f32": 2.0 ** -149, "bf16": 2.0 ** -133, "f16": 2.0 ** -24}[target]
+    v, rng = 3001, np.random.default_rng(18)
+    t = torch.zeros((8, v), dtype=TYPES[target], device=gpu)
+    at = rng.choice(v, 5, replace=False)
+    for k, x in enumerate(at):
+        t[:, int(x)] = tiny * (k + 1)
+    p = t.double().cpu().numpy()
+    assert (p[0] > 0).sum() == 5
+    b = dict(target=t, tokens=np.zeros(0, np.int32), begin=[0] * 9, coins=np.zeros(0), u=np.linspace(0.01, 0.99, 8), draft=None)
+    want = _check(ge, b, p, None)
+    assert len({w[0][0] for w in want}) > 2
+
+
 def test_nothing_left_with_a_one_hot_draft(ge, gpu):
     """A deterministic draft that holds all of its row's mass and is rejected all the same (0.9 < coin) is drawn again; and
     a NaN at the draft's own token does not count among the rest."""

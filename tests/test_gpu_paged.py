@@ -368,6 +368,8 @@ def test_rounds_of_trees(ge, gpu):
         call = ge.spec.VerifyCall(reqs)
         call.launch()
         call.keep_path(m, caches)
+        with pytest.raises(ValueError):
+            call.keep_path(t.step([1] * r, keep=call.e_len, into=torch.zeros_like(t.counters)), caches)  # another round's
         keep = call.e_len
         for k, (new, path, why) in enumerate(call.result()):
             assert why is None and len(new) == len(path)

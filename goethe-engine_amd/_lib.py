@@ -95,7 +95,7 @@ class PickBatch(C.Structure):
 class Chains(C.Structure):
     _fields_ = [("size", C.c_uint32), ("requests", C.c_uint32), ("vocab", C.c_uint32), ("max_drafts", C.c_uint32),
                 ("drafts", C.c_uint32), ("target_type", C.c_uint32), ("draft_type", C.c_uint32),
-                ("reserved", C.c_uint32), ("target", C.c_void_p), ("target_ld", C.c_int64), ("draft", C.c_void_p),
+                ("u_rows", C.c_uint32), ("target", C.c_void_p), ("target_ld", C.c_int64), ("draft", C.c_void_p),
                 ("draft_ld", C.c_int64), ("begin", C.c_void_p), ("token", C.c_void_p), ("coin", C.c_void_p),
                 ("u", C.c_void_p), ("emit_len", C.c_void_p), ("emit_tokens", C.c_void_p), ("emit_probs", C.c_void_p),
                 ("emit_ld", C.c_int64), ("status", C.c_void_p), ("stream", C.c_void_p)]
@@ -103,8 +103,8 @@ class Chains(C.Structure):
 
 class Pages(C.Structure):
     _fields_ = [("size", C.c_uint32), ("requests", C.c_uint32), ("page", C.c_uint32), ("pool", C.c_uint32),
-                ("max_pages", C.c_uint32), ("reserved", C.c_uint32), ("table", C.c_void_p), ("table_ld", C.c_int64), ("ring", C.c_void_p), ("counters", C.c_void_p),
-                ("counters_out", C.c_void_p)]
+                ("max_pages", C.c_uint32), ("reserved", C.c_uint32), ("table", C.c_void_p), ("table_ld", C.c_int64),
+                ("ring", C.c_void_p), ("counters", C.c_void_p), ("counters_out", C.c_void_p)]
 
 
 class Step(C.Structure):

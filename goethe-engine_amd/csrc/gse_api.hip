@@ -604,6 +604,7 @@ GSE_API int gsp_verify_chains(gse_handle *h, const gsp_chains *in) {
   if (c.requests == 0) return GSE_OK;
   if (!c.target || !c.begin || !c.u || !c.emit_len || !c.emit_tokens || !c.status)
     return fail(h, GSE_E_ARG, "target, begin, u, emit_len, emit_tokens and status are required");
+  if (c.u_rows > 1) return fail(h, GSE_E_ARG, "u_rows %u", c.u_rows);
   if (c.drafts > 0 && (!c.token || !c.coin)) return fail(h, GSE_E_ARG, "drafts need token and coin");
   if (c.target_type > GSP_F16 || (c.draft && c.draft_type > GSP_F16))
     return fail(h, GSE_E_ARG, "target type %u, draft type %u", c.target_type, c.draft_type);

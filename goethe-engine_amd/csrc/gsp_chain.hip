@@ -5,6 +5,14 @@
 // q_i(x_i) > 0 and coin_i q_i(x_i) < p_i(x_i): with probability min(1, p / q). At the first draft a that is not, the token
 // comes from max(p_a - q_a, 0), which makes its law p_a again; after the last one from p_n. The tests read two values per
 // draft, so what has to be read is one row of p per request, and one of q where a draft was rejected.
+//
+// A request's row is cut into segments that a wave sums alone, 16 bytes a lane and load, in fp64 (a token is an index: sums in
+// fp32 would move it); the last workgroup in, by a ticket, finds the segment, then the token that u times the sum falls
+// into. One launch, whatever the chains' lengths. Bound by memory in large calls: 512 chains over 262144 bf16 tokens read
+// 390 MB in 76 us, 5.1 TB/s (a large copy: 5.1), 6.9 VALU instructions a token; a call of few rows is the chain of
+// dependent reads offsets, drafts, their weights, the row, the sums, the token's segment: 6.1 us for one chain over 128256
+// fp32 tokens. One workgroup a request and two passes took 2260 and 275 us; a workgroup a slice of 32 KB (8192 of them, each
+// through the first three reads and a ticket) 173 us.
 #include "gse_dev.h"
 #include "gsp_int.h"
 
@@ -14,7 +22,9 @@ namespace {
 
 constexpr int CT = 256;          // threads of a workgroup
 constexpr int CW = CT / WAVE;
-constexpr int WGS_MAX = 48;      // workgroups of a request, at most
+// Workgroups of a request, at most: each ends with an atomic on the request's ticket. One chain over 128256 fp32 tokens with 8,
+// 16, 32, 48, 64, 128: 7.3, 6.1, 6.2, 6.1, 6.6, 6.7 us; 16 chains over 151936 fp64 tokens 19.4, 14.9, 13.2, 10.2, 11.1, 11.1.
+constexpr int WGS_MAX = 48;
 
 template <int T>
 constexpr int SIZE = T == GSP_F64 ? 8 : T == GSP_F32 ? 4 : 2;
@@ -136,7 +146,9 @@ struct ChainArgs {
   int r0;          // first request of the launch
   int nseg;        // segments of a row
   double *sum;     // [requests of the launch][nseg]
-  uint32_t *tick;  // ticket of request k of the launch at k * tstride, zero between calls
+  // The ticket of request k of the launch at k * tstride, zero between calls. A cache line apart where there is room: side by
+  // side, the atomics of all requests queue for one line (16 chains of 64 workgroups 20.6 us, apart 12.5).
+  uint32_t *tick;
   int tstride;
 };
 
@@ -327,7 +339,7 @@ __global__ __launch_bounds__(CT) __attribute__((amdgpu_waves_per_eu(4, 8))) void
   if (ticket != gridDim.x - 1 || tid >= WAVE) return;
   int j = -1;
   if (e.a >= 0) {
-    const double u = c.u[r];
+    const double u = c.u[c.u_rows ? e.row : (int64_t)r];
     double total = 0.0;
     if constexpr (QT >= 0) {
       if (w.q) j = chain_draw<PT, QT, VEC, S, true>(w, sum, a.nseg, V, u, total);
@@ -365,8 +377,10 @@ hipError_t launch_chains(const RowsWs &w, const gsp_chains &c, hipStream_t s) {
     const int64_t nv = (int64_t)c.vocab / VEC;
     const int64_t cap = (int64_t)w.rows * w.slices * 64;         // segment sums that the workspace holds
     const int64_t rows = min((int64_t)c.requests, min((int64_t)w.ticks, (int64_t)65535));  // requests of a launch, at most
-    // One resident round of workgroups over the launch, as long as a wave has a segment; the longest segments that leave
-    // every wave one.
+    // One resident round of workgroups over the launch, as long as a wave has a segment; the longest segments that leave every
+    // wave one (the last workgroup reads their sums). Where a wave would have eight of the longest or more, four times as
+    // many workgroups: rows with and without q even out (512 chains over 262144 bf16 tokens 84 -> 78 us; 64 over 128256 fp32
+    // tokens, a segment or two a wave, are slower so: 15.3 -> 21).
     auto segs = [&](int64_t S) { return max((int64_t)1, (nv + S * WAVE - 1) / (S * WAVE)); };
     int64_t most = max((int64_t)1, min((int64_t)(w.round) / rows, (int64_t)WGS_MAX));
     if (segs(8) >= 8 * CW * most) most *= 4;

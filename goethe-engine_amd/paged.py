@@ -135,7 +135,8 @@ class PageTable:
         keep = _vec(keep, i32, dev) if keep is not None else None
         depth = _vec(depth, i32, dev) if depth is not None else None
         slot = torch.empty(n, dtype=torch.int64, device=dev)
-        pos, req, begin, seq, status = torch.empty(2 * n + 3 * r + 1, dtype=i32, device=dev).split_with_sizes((n, n, r + 1, r, r))
+        ints = torch.empty(2 * n + 3 * r + 1, dtype=i32, device=dev)
+        pos, req, begin, seq, status = ints.split_with_sizes((n, n, r + 1, r, r))
         p = _lib.Pages(_PAGES, r, self.page, self.ring.shape[0], self.max_pages, 0, self.table.data_ptr(), self.table_ld,
                        self.ring.data_ptr(), self.counters.data_ptr(), into.data_ptr())
         t = _lib.Step(_STEP, n, keep.data_ptr() if keep is not None else None, add.data_ptr(),

@@ -505,8 +505,10 @@ def verify_chains(target, tokens, begin, coins, u, draft=None, max_drafts=None):
     chain, so padded batches pad with -1); target [D + R, V]: row begin[r] + r + i the target's distribution after r's first
     i drafts (fp64, fp32, bf16 or fp16, any row stride, used in place: softmax rows, dist_batch's); draft [D, V]: the
     distribution each draft was drawn from (any of these types, qprob's), None for a deterministic drafter; coins [D] and
-    u [R]: numbers in [0, 1) (fp64). Draft x is accepted while coin * q(x) < p(x); at the first that is not, the token is
-    drawn with u from max(p - q, 0), after the last one from the row that follows. A chain of one draft is mss with one kid.
+    u [R], or [D + R] (one per target row: the row drawn from says which): numbers in [0, 1) (fp64). Draft x is accepted
+    while coin * q(x) < p(x); at the first that is not, the token is drawn with u from max(p - q, 0), after the last one
+    from the row that follows. Coin i = uniform(mix(seed, SALT_ACC), nout + i) and u of row i = uniform(mix(seed, SALT_RES),
+    nout + i) make a strict request's decisions (engine.py:278-283).
     max_drafts: the longest chain a request may have (default: from begin, which then has to be on the host)."""
     if max_drafts is None:
         if isinstance(begin, torch.Tensor) and begin.device.type != "cpu":
@@ -521,8 +523,8 @@ def verify_chains(target, tokens, begin, coins, u, draft=None, max_drafts=None):
     v = target.shape[1]
     if draft is not None:
         draft = _prob_rows(draft, "draft", d, v)
-    if nc != d or nu != n or v == 0:
-        raise ValueError(f"{d} tokens and {n} requests need as many coins and draws, got {nc} and {nu} (V = {v})")
+    if nc != d or nu not in (n, d + n) or v == 0:
+        raise ValueError(f"{d} tokens and {n} requests need {d} coins and {n} or {d + n} draws, got {nc} and {nu} (V = {v})")
     dev = target.device
     if dev.type != "cuda":
         dev = _device()
@@ -539,10 +541,10 @@ def verify_chains(target, tokens, begin, coins, u, draft=None, max_drafts=None):
         if draft.device != dev:
             draft = _vec(draft, draft.dtype, dev)
         q, q_type, q_ld = draft.data_ptr(), _PROB[draft.dtype], max(draft.stride(0), v)
-    stream = _lib.raw_stream(dev.index)
-    c = _lib.Chains(_CHAINS, n, v, k, d, _PROB[target.dtype], q_type, 0, target.data_ptr(), max(target.stride(0), v), q, q_ld,
-                    begin.data_ptr(), tokens.data_ptr(), coins.data_ptr(), u.data_ptr(), out.emit_len.data_ptr(),
-                    out.tokens.data_ptr(), out.probs.data_ptr(), k + 1, out.status.data_ptr(), stream)
+    c = _lib.Chains(_CHAINS, n, v, k, d, _PROB[target.dtype], q_type, int(nu > n), target.data_ptr(),
+                    max(target.stride(0), v), q, q_ld, begin.data_ptr(), tokens.data_ptr(), coins.data_ptr(), u.data_ptr(),
+                    out.emit_len.data_ptr(), out.tokens.data_ptr(), out.probs.data_ptr(), k + 1, out.status.data_ptr(),
+                    _lib.raw_stream(dev.index))
     _lib.handle(dev.index, 1, v).call("gsp_verify_chains", C.byref(c))
     return out
 

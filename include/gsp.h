@@ -32,7 +32,7 @@ typedef struct gsp_chains {
   uint32_t drafts;          /* entries of token and coin, rows of draft; target has drafts + requests rows */
   uint32_t target_type;     /* GSP_* */
   uint32_t draft_type;
-  uint32_t reserved;
+  uint32_t u_rows;          /* 0: u has one draw per request; 1: one per target row, and the row drawn from says which */
   const void *target;       /* [drafts + requests][target_ld]: weights, each row of any positive sum */
   int64_t target_ld;
   const void *draft;        /* [drafts][draft_ld], or NULL: every draft one-hot (a deterministic drafter) */
@@ -40,13 +40,13 @@ typedef struct gsp_chains {
   const int32_t *begin;     /* [requests + 1] */
   const int32_t *token;     /* [drafts] */
   const double *coin;       /* [drafts] in [0, 1): draft i is accepted iff q_i(x_i) > 0 and coin q_i(x_i) < p_i(x_i) */
-  const double *u;          /* [requests] in [0, 1): the draw of the token after the accepted drafts */
+  const double *u;          /* [requests], or [drafts + requests], in [0, 1): the draw of the token after the accepted drafts */
   int32_t *emit_len;        /* [requests] accepted drafts + 1 (GSE_WALK_ERROR: without the token that could not be drawn) */
   int32_t *emit_tokens;     /* [requests][emit_ld]: columns [0, max_drafts] written, -1 past the emitted tokens */
   float *emit_probs;        /* [requests][emit_ld] the target's weight of each emitted token; 0 past them; or NULL */
   int64_t emit_ld;          /* >= max_drafts + 1 */
   uint32_t *status;         /* [requests] GSE_WALK_OK, or GSE_WALK_ERROR: the row to draw from holds a NaN or an infinity
-                             * or no positive weight, or begin is not in order (nothing emitted) */
+                             * or no positive weight (or sums to an infinity), or begin is not in order (nothing emitted) */
   void *stream;
 } gsp_chains;
 

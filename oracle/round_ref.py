@@ -31,7 +31,8 @@ def draw(w, u):
 
 
 def chain(p, q, tokens, coins, u):
-    """p [n + 1, V], q [n, V] or None, of one request: (emitted tokens, target weights of them, error)."""
+    """p [n + 1, V], q [n, V] or None, of one request (u: one draw, or one per row): (emitted tokens, target weights of them,
+    error)."""
     p = np.asarray(p, np.float64)
     v = p.shape[1]
     out, i, w = [], 0, None
@@ -48,7 +49,7 @@ def chain(p, q, tokens, coins, u):
             break
         out.append(x)
         i += 1
-    t = draw(p[i] if w is None else w, u)
+    t = draw(p[i] if w is None else w, u[i] if np.ndim(u) else u)
     probs = [float(p[k][x]) for k, x in enumerate(out)]
     if t >= 0:
         out.append(t)
@@ -57,12 +58,15 @@ def chain(p, q, tokens, coins, u):
 
 
 def chains(target, draft, tokens, begin, coins, u):
-    """Per request chain()'s answer; begin as verify_chains takes it."""
+    """Per request chain()'s answer; begin as verify_chains takes it, u per request or per target row."""
     res = []
+    per_row = len(u) > len(begin) - 1
     for r in range(len(begin) - 1):
         b, e = int(begin[r]), int(begin[r + 1])
+        if per_row:
+            u_r = np.asarray(u, np.float64)[b + r:e + r + 1]
         res.append(chain(target[b + r:e + r + 1], draft[b:e] if draft is not None else None, [int(x) for x in tokens[b:e]],
-                         coins[b:e], u[r]))
+                         coins[b:e], u_r if per_row else u[r]))
     return res
 
 

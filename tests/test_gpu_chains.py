@@ -95,6 +95,19 @@ def test_one_hot_drafts_accepted(ge, gpu, target):
     assert {len(w[0]) for w in want} >= {1, 2, 3}
 
 
+@pytest.mark.parametrize("kind", ["f32-bf16", "bf16-none"])
+def test_a_draw_per_target_row(ge, gpu, kind):
+    """u with an entry per target row: the one of the row drawn from is read."""
+    target, draft = (None if k == "none" else k for k in kind.split("-"))
+    rng = np.random.default_rng(19)
+    lens = [3, 0, 1, 5, 2, 4, 4, 4]
+    b, p, q = _batch(rng, lens, 4001, target, draft, gpu)
+    b["u"] = rng.random(len(b["tokens"]) + len(lens))
+    for coins in (b["coins"], b["coins"] * 0, b["coins"] * 0 + 0.999):
+        b["coins"] = coins
+        _check(ge, b, p, q)
+
+
 def test_row_starts_at_every_alignment(ge, gpu):
     """Rows that start at any element of a 16-byte vector, target and draft apart."""
     rng = np.random.default_rng(2)
@@ -163,7 +176,7 @@ def test_c_refusals(ge, gpu):
                          (dict(coin=None), lib.E_ARG, "token and coin"), (dict(target_type=4), lib.E_ARG, "type"),
                          (dict(draft_type=9), lib.E_ARG, "type"), (dict(target_ld=499), lib.E_ARG, "target_ld"),
                          (dict(draft_ld=1), lib.E_ARG, "draft_ld"), (dict(vocab=0), lib.E_ARG, "vocab"),
-                         (dict(emit_ld=2), lib.E_ARG, "emit_ld"), (dict(size=4), lib.E_ARG, "short"),
+                         (dict(emit_ld=2), lib.E_ARG, "emit_ld"), (dict(u_rows=2), lib.E_ARG, "u_rows"), (dict(size=4), lib.E_ARG, "short"),
                          (dict(max_drafts=(1 << 30) + 1, emit_ld=1 << 40), lib.E_UNSUPPORTED, "2^30"),
                          (dict(drafts=1 << 30), lib.E_UNSUPPORTED, "2^30")):
         got, n, t, st = _raw(ge, h, b, 2, gpu, **kw)
@@ -405,11 +418,7 @@ def test_draws_follow_the_residual(ge, gpu):
             for k in range(r)]
     tree = ge.spec.verify_tree(reqs)
     coins = [ora.uniform(ora.mix(seeds[k], spo.SALT_ACC), nout + i) for k in range(r) for i in range(lens[k])]
-    # the walk's last token: SALT_RES at a strict node with kids, the plain draw at a leaf
-    u = []
-    for k in range(r):
-        a = len(tree[k][0]) - 1
-        u.append(ora.uniform(ora.mix(seeds[k], spo.SALT_RES), nout + a) if a < lens[k] else ora.uniform(seeds[k], nout + a))
+    u = [ora.uniform(ora.mix(seeds[k], spo.SALT_RES), nout + i) for k in range(r) for i in range(lens[k] + 1)]  # per row
     got = ge.spec.verify_chains(p, tok, begin, coins, u, draft=q)
     for k in range(r):
         toks, path, _ = tree[k]

@@ -50,8 +50,9 @@ typedef struct gsp_chains {
   void *stream;
 } gsp_chains;
 
-/* A paged cache's bookkeeping, in the caller's device arrays: which pages each request holds, and the free pages as a
- * ring (a queue: steps take from its head and give back at its tail, so that neither writes what the other reads). */
+/* A paged cache's bookkeeping, in the caller's device arrays: which pages each request holds (a page belongs to one), and the
+ * free pages as a ring (a queue: steps take from its head and give back at its tail, so that neither writes what the other
+ * reads). Steps over the same arrays must follow one another on the device. */
 typedef struct gsp_pages {
   uint32_t size;
   uint32_t requests;

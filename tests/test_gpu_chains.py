@@ -2,6 +2,7 @@
 (a draw within rounding of a prefix border has a probability of about 1e-13), the target's weights as their fp32
 roundings, exactly."""
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -183,6 +184,9 @@ def test_c_refusals(ge, gpu):
         assert got == rc and text in h.L.gse_last_error(h.h).decode(), (kw, got, h.L.gse_last_error(h.h))
         assert (n == -7).all() and (t == -7).all() and (st == -7).all()
     assert _raw(ge, h, b, 2, gpu, requests=0)[0] == 0
+    small = lib.Handle(gpu.index, 1, 64)  # (room for a row of 2 * 64 segments)
+    got, n, t, st = _raw(ge, small, b, 2, gpu, vocab=200000, target_ld=200000, draft_ld=200000)
+    assert got == lib.E_CAPACITY and "200000" in small.L.gse_last_error(small.h).decode() and (n == -7).all()
     with pytest.raises(ValueError):
         ge.spec.verify_chains(**{**b, "begin": torch.tensor(b["begin"], device=gpu)})  # its longest chain is not known
 
@@ -376,6 +380,53 @@ def test_in_a_graph(ge, gpu):
             assert o.tolist() == [(w[0], None) for w in want]
             eager = ge.spec.verify_chains(**dev, max_drafts=5)
             assert eager.tolist() == o.tolist()
+
+
+def test_two_graphs_of_one_handle(ge, gpu):
+    """Two captured calls that share a stream's workspace, replayed in turn on it."""
+    rng = np.random.default_rng(20)
+    sets = [_batch(rng, lens, v, "bf16", "f32", gpu) for lens, v in (([2, 4, 0], 30011), ([1] * 40, 7001))]
+    want = [[(w[0], None) for w in rr.chains(p, q, *(b[n] for n in ("tokens", "begin", "coins", "u")))] for b, p, q in sets]
+    devs = []
+    for b, _, _ in sets:
+        d = {k: torch.from_numpy(np.asarray(x)).to(gpu) if not isinstance(x, torch.Tensor) else x for k, x in b.items()}
+        devs.append(dict(d, begin=d["begin"].int()))
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        graphs, outs = [], []
+        for d in devs:
+            ge.spec.verify_chains(**d, max_drafts=4)  # (opens the stream's handle, at this vocabulary)
+        s.synchronize()
+        for d in devs:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=s):
+                outs.append(ge.spec.verify_chains(**d, max_drafts=4))
+        for k in (0, 1, 1, 0, 0, 1):
+            outs[k].tokens.fill_(-9)
+            graphs[k].replay()
+            assert outs[k].tolist() == want[k]
+            assert ge.spec.verify_chains(**devs[1 - k], max_drafts=4).tolist() == want[1 - k]
+
+
+def test_two_threads_on_one_stream(ge, gpu):
+    """Calls of two threads on the same stream share its handle: one after the other on the device."""
+    rng = np.random.default_rng(21)
+    sets = [_batch(rng, [3, 1, 0, 5], 20001, "f32", "f32", gpu) for _ in range(2)]
+    want = [[(w[0], None) for w in rr.chains(p, q, *(b[n] for n in ("tokens", "begin", "coins", "u")))] for b, p, q in sets]
+    bad = []
+
+    def work(k):
+        for _ in range(30):
+            if ge.spec.verify_chains(**sets[k][0]).tolist() != want[k]:
+                bad.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_two_streams(ge, gpu):

@@ -9,14 +9,13 @@ engine.py:299-305 commit on the host from lengths copied back.
 
 A round of tree verification, nothing of which waits for the host:
 
-    step = pages.step(add=nodes, keep=emit_len, depth=depth, max_tokens=n)   # emit_len: of the round before
+    step = pages.step(add=prompts)                       # the first tokens; then, round by round:
     ...                                                  # the model writes its keys and values to step.slot
     call.launch()                                        # spec.VerifyCall over the target's logits
-    call.keep_path(step, caches)                         # the accepted path moves behind its anchor
-    emit_len = call.e_len
+    step = call.commit(step, pages, caches, add=nodes, depth=depth, max_tokens=n)
 
-A round of chains needs no move: its accepted drafts are already consecutive (spec.verify_chains' emit_len goes to the next
-step's keep).
+commit is keep_path, the accepted path moved behind its anchor, and the step that keeps it and adds the next round's nodes. A
+round of chains needs no move: its accepted drafts are already consecutive (spec.verify_chains(...).commit).
 """
 import ctypes as C
 import math

@@ -302,6 +302,14 @@ class VerifyCall:
                              f"{self.n_req} and {self.nodes} nodes")
         paged.keep_path(caches, step.slot, self.keep[0], self.e_len, self.e_node, heads_first=heads_first)
 
+    def commit(self, step, pages, caches, add, depth=None, max_tokens=None, ends=None, heads_first=False):
+        """engine.py:299-305's commit and the next round's layout, on the device: keep_path(step, caches), then the
+        paged.PageTable's step that keeps each request's accepted tokens (none where ends[r]: it gives its pages back) and
+        adds the next round's (paged.PageTable.step's add, depth, max_tokens). Returns the next round's paged.StepMap."""
+        self.keep_path(step, caches, heads_first)
+        kept = self.e_len if self.ld >= self.longest else self.e_len.clamp(max=self.ld)  # (the tokens that result() gives)
+        return pages.step(add, keep=_kept(kept, ends), depth=depth, max_tokens=max_tokens)
+
     def _build(self, reqs, nout0, emit_ld):
         dev = _device()
         sizes = [len(r["tokens"]) + 1 for r in reqs]
@@ -426,6 +434,7 @@ class VerifyCall:
         self.dev, self.b, self.t, self.o, self.keep = dev, b, t, o, keep
         self.e_len, self.e_tok, self.e_node, self.e_st = e_len, e_tok, e_node, e_st
         self.ld, self.anchors, self.n_req, self.nodes, self.vocab = ld, anchors, len(reqs), nodes, v
+        self.longest = max(sizes)
 
 
 def _as_row(x, u, dev):
@@ -460,10 +469,26 @@ class Chains:
     def __init__(self, emit_len, tokens, probs, status):
         self.emit_len, self.tokens, self.probs, self.status = emit_len, tokens, probs, status
 
+    def commit(self, pages, add, max_tokens=None, ends=None):
+        """The round's commit and the next one's layout, on the device: the paged.PageTable's step that keeps each request's
+        anchor and accepted drafts (already consecutive; none where ends[r]) and adds the next round's tokens. Returns the
+        next round's paged.StepMap."""
+        return pages.step(add, keep=_kept(self.emit_len, ends), max_tokens=max_tokens)
+
     def tolist(self):
         """Per request (emitted tokens, "error" or None), as verify_tree reports them."""
         n, t, st = self.emit_len.cpu().tolist(), self.tokens.cpu().tolist(), self.status.cpu().tolist()
         return [(t[a][:n[a]], "error" if st[a] != _lib.WALK_OK else None) for a in range(len(n))]
+
+
+def _kept(emit_len, ends):
+    """paged.PageTable.step's keep after a round: emit_len, -1 where a request ends."""
+    if ends is None:
+        return emit_len
+    ends = torch.as_tensor(ends, dtype=torch.bool).to(emit_len.device)
+    if ends.shape != emit_len.shape:
+        raise ValueError(f"ends must have {emit_len.shape[0]} entries")
+    return emit_len.masked_fill(ends, -1)
 
 
 def _prob_rows(x, what, rows, v=None):

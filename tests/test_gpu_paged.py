@@ -437,3 +437,49 @@ def test_rounds_of_chains(ge, gpu):
             assert o.tolist() == [(c[0], None) for c in chains]
             lens = np.array([len(c[0]) for c in chains])
     assert keep.cpu().tolist() == lens.tolist() and len(set(lens.tolist())) > 1
+
+
+def test_commits(ge, gpu):
+    """VerifyCall.commit and Chains.commit: the same as the calls they stand for, requests that end among them."""
+    S = ge.sampling.SamplingParams
+    trees = [[0, 1, 0, 3], [0, 0, 2], [0]]
+    sizes, v = [5, 4, 2], 500
+    g = torch.Generator(device=gpu).manual_seed(1)
+    x = torch.randn((11, v), generator=g, device=gpu) * 3
+    best = x.argmax(1).cpu().tolist()
+    at = [0, 5, 9]
+    reqs = [dict(target=x[at[k]:at[k] + sizes[k]], parents=p, params=S(), seed=1,
+                 tokens=[(best[at[k] + par] + (k == 0 and j == 0)) % v for j, par in enumerate(p)])
+            for k, p in enumerate(trees)]
+    out = []
+    for ends in (None, [False, True, False], torch.tensor([True, False, True], device=gpu)):
+        both = []
+        for whole in (True, False):
+            t = ge.paged.PageTable(3, 40, 4, 6, device=gpu)
+            m = t.step(sizes)
+            c = torch.arange(2 * 40 * 4 * 8, device=gpu).reshape(2, 40, 4, 8).float()
+            call = ge.spec.VerifyCall(reqs)
+            call.launch()
+            if whole:
+                nxt = call.commit(m, t, c, [2, 2, 2], ends=ends)
+            else:
+                call.keep_path(m, c)
+                keep = call.e_len.tolist() if ends is None else [-1 if e else n for n, e in zip(call.e_len.tolist(), list(ends))]
+                nxt = t.step([2, 2, 2], keep=keep)
+            both.append((c, nxt.slot, nxt.pos, nxt.seq_len, t.counters, t.table, t.ring))
+        assert all(torch.equal(a, b) for a, b in zip(*both))
+        out.append(both[0])
+    assert not torch.equal(out[0][4], out[1][4]) and call.e_len.tolist()[0] > 1
+    short = ge.spec.VerifyCall(reqs, emit_ld=1)  # a walk cut at one token keeps one
+    t = ge.paged.PageTable(3, 40, 4, 6, device=gpu)
+    m = t.step(sizes)
+    short.launch()
+    assert short.commit(m, t, c, [0, 0, 0]).seq_len.tolist() == [len(r[0]) for r in short.result()] == [1, 1, 1]
+    o = ge.spec.verify_chains(torch.softmax(x[:6], 1), best[:3], [0, 3, 3, 3], [0.0] * 3, [0.5] * 3)
+    t, u = (ge.paged.PageTable(3, 40, 4, 6, device=gpu) for _ in range(2))
+    t.step([4, 1, 1]), u.step([4, 1, 1])
+    a = o.commit(t, [1, 1, 1], ends=[False, False, True])
+    b = u.step([1, 1, 1], keep=[o.emit_len.tolist()[0], 1, -1])
+    assert torch.equal(a.slot, b.slot) and torch.equal(t.counters, u.counters) and (t.length.tolist()[1:] == [1, 0])
+    with pytest.raises(ValueError):
+        o.commit(t, [1, 1, 1], ends=[True])

@@ -50,8 +50,9 @@ def _state(t, what, dev, dims):
 
 class PageTable:
     """The pages of `requests` requests over a cache of `pool` pages of `page` tokens, at most max_pages each; a page belongs to
-    one request (pages of a shared prefix are kept outside). Steps of one table follow one another on the device. State there: table int32 [requests, max_pages] (a request's pages in order), ring int32 [pool] (the free pages, a queue),
-    counters int32 [2 + 2 requests]: the queue's head and length, then length and held (pages) of each request."""
+    one request (pages of a shared prefix are kept outside). Steps of one table follow one another on the device. State there:
+    table int32 [requests, max_pages] (a request's pages in order), ring int32 [pool] (the free pages, a queue), counters int32
+    [2 + 2 requests]: the queue's head and length, then length and held (pages) of each request."""
 
     def __init__(self, requests, pool, page, max_pages, device=None):
         requests, pool, page, max_pages = int(requests), int(pool), int(page), int(max_pages)

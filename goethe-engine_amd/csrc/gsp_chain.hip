@@ -9,7 +9,7 @@
 // A request's row is cut into segments that a wave sums alone, 16 bytes a lane and load, in fp64 (a token is an index: sums in
 // fp32 would move it); the last workgroup in, by a ticket, finds the segment, then the token that u times the sum falls
 // into. One launch, whatever the chains' lengths. Bound by memory in large calls: 512 chains over 262144 bf16 tokens read
-// 390 MB in 76 us, 5.1 TB/s (a large copy: 5.1), 6.9 VALU instructions a token; a call of few rows is the chain of
+// 390 MB in 71 us, 5.5 TB/s (a large copy: 5.1), 6.9 VALU instructions a token; a call of few rows is the chain of
 // dependent reads offsets, drafts, their weights, the row, the sums, the token's segment: 6.1 us for one chain over 128256
 // fp32 tokens. One workgroup a request and two passes took 2260 and 275 us; a workgroup a slice of 32 KB (8192 of them, each
 // through the first three reads and a ticket) 173 us.
@@ -42,12 +42,20 @@ __device__ __forceinline__ double value(const char *row, int64_t t) {
 }
 
 // N consecutive values of a row of type T, as loaded (rows start at any element: the loads need no more alignment than one).
+// NT: read past the caches' keeping.
 template <int T, int N>
 struct Raw {
   static constexpr int W = SIZE<T> * N / 4;
+  typedef uint32_t Q __attribute__((ext_vector_type(W), aligned(2)));
   uint32_t w[W];
+  template <bool NT>
   __device__ __forceinline__ void load(const char *row, int64_t t) {
-    __builtin_memcpy(w, row + t * SIZE<T>, sizeof w);
+    const Q *at = (const Q *)(row + t * SIZE<T>);
+    Q q;
+    if constexpr (NT) q = __builtin_nontemporal_load(at);
+    else q = *at;
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = q[i];
   }
   __device__ __forceinline__ double get(int i) const {
     if constexpr (T == GSP_F64) return __hiloint2double((int)w[2 * i + 1], (int)w[2 * i]);
@@ -121,9 +129,10 @@ struct Weights {
   static constexpr int Q = HQ ? QT : GSP_BF16;
   Raw<PT, VEC> p;
   Raw<Q, HQ ? VEC : 2> q;
+  template <bool NT>
   __device__ __forceinline__ void load(const ChainRow &w, int64_t t) {
-    p.load(w.p, t);
-    if constexpr (HQ) q.load(w.q, t);
+    p.template load<NT>(w.p, t);
+    if constexpr (HQ) q.template load<NT>(w.q, t);
   }
   __device__ __forceinline__ double get(int i) const {
     double v = p.get(i);
@@ -159,14 +168,14 @@ __device__ __forceinline__ double tail_weight(const ChainRow &w, int V) {
 }
 
 // The sum of a segment (last: with the row's tail), by one wave; every lane gets it.
-template <int PT, int QT, int VEC, int S, bool HQ>
+template <int PT, int QT, int VEC, int S, bool HQ, bool NT>
 __device__ __forceinline__ double segment_sum(const ChainRow &w, int seg, bool last, int V) {
   const int nv = V / VEC, i0 = seg * (S * WAVE), lane = lane_id();
   double a = 0.0;
   if (i0 + S * WAVE <= nv && (w.x < i0 * VEC || w.x >= (i0 + S * WAVE) * VEC)) {  // whole, and w.x not in it
     Weights<PT, QT, VEC, HQ> x[S];
 #pragma unroll
-    for (int k = 0; k < S; ++k) x[k].load(w, (int64_t)(i0 + k * WAVE + lane) * VEC);
+    for (int k = 0; k < S; ++k) x[k].template load<NT>(w, (int64_t)(i0 + k * WAVE + lane) * VEC);
 #pragma unroll
     for (int k = 0; k < S; ++k) {
 #pragma unroll
@@ -175,7 +184,7 @@ __device__ __forceinline__ double segment_sum(const ChainRow &w, int seg, bool l
   } else {
     for (int i = i0 + lane; i < min(i0 + S * WAVE, nv); i += WAVE) {
       Weights<PT, QT, VEC, HQ> x;
-      x.load(w, (int64_t)i * VEC);
+      x.template load<NT>(w, (int64_t)i * VEC);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) a += i * VEC + e == w.x ? 0.0 : x.get(e);
     }
@@ -198,7 +207,7 @@ __device__ __forceinline__ int segment_search(const ChainRow &w, int seg, bool l
   for (int k = 0; k < S; ++k) {
     if (k % H == 0 && nv > 0) {  // (past the last vector: that one again, not counted)
 #pragma unroll
-      for (int j = 0; j < H; ++j) x[j].load(w, (int64_t)min(i0 + (k + j) * WAVE + lane, nv - 1) * VEC);
+      for (int j = 0; j < H; ++j) x[j].template load<false>(w, (int64_t)min(i0 + (k + j) * WAVE + lane, nv - 1) * VEC);
     }
     const int i = i0 + k * WAVE + lane;
     double b[VEC], a = 0.0;
@@ -287,7 +296,7 @@ __device__ __noinline__ int chain_draw_again(const char *p, int nseg, int V, dou
   const ChainRow w{p, nullptr, -1};
   double total = 0.0, before = 0.0;
 #pragma unroll 1
-  for (int i = 0; i < nseg; ++i) total += segment_sum<PT, QT, VEC, S, false>(w, i, i == nseg - 1, V);
+  for (int i = 0; i < nseg; ++i) total += segment_sum<PT, QT, VEC, S, false, false>(w, i, i == nseg - 1, V);
   if (!(total > 0.0 && total < INFINITY)) return -1;
   int lst = -1;
   bool found = false;
@@ -302,7 +311,7 @@ __device__ __noinline__ int chain_draw_again(const char *p, int nseg, int V, dou
 // gridDim.x workgroups a request. Every wave finds the chain's end by itself (its drafts' values are cached after the first),
 // then sums its share of the row's segments; the last workgroup's first wave (by a ticket) draws the token. No barrier but
 // the ticket's, nothing in LDS but its answer.
-template <int PT, int QT, int S>
+template <int PT, int QT, int S, bool NT>
 __global__ __launch_bounds__(CT) __attribute__((amdgpu_waves_per_eu(4, 8))) void chain_kernel(ChainArgs a) {
   constexpr int QS = QT < 0 ? 0 : SIZE<QT < 0 ? 0 : QT>;
   constexpr int VEC = 16 / (QS > SIZE<PT> ? QS : SIZE<PT>);
@@ -320,7 +329,7 @@ __global__ __launch_bounds__(CT) __attribute__((amdgpu_waves_per_eu(4, 8))) void
   double *sum = a.sum + (int64_t)k * a.nseg;
   auto sums = [&](auto hq) {
     for (int i = wv; i < a.nseg; i += waves) {
-      const double t = segment_sum<PT, QT, VEC, S, decltype(hq)::value>(w, i, i == a.nseg - 1, V);
+      const double t = segment_sum<PT, QT, VEC, S, decltype(hq)::value, NT>(w, i, i == a.nseg - 1, V);
       if (lane == 0) st_ag(&sum[i], t);
     }
   };
@@ -390,14 +399,20 @@ hipError_t launch_chains(const RowsWs &w, const gsp_chains &c, hipStream_t s) {
     a.nseg = (int)segs(S);
     const int64_t wgs = min(most, (a.nseg + CW - 1) / (int64_t)CW);
     const int64_t per = min(rows, cap / a.nseg);
+    // Rows that together pass the last-level cache are read around it. Bytes of one row of p and q a request, us a call over
+    // inputs in turn / the same input, cached and around: 134 MB (bf16 128 x 262144) 24.4 / 24.2 and 24.4 / 23.6; 233 MB (fp32
+    // 192 x 151936) 41.2 / 31.1 and 37.7 / 35.3; 268 MB (bf16 256 x 262144) 44.7 / 37.0 and 40.5 / 37.5; 311 MB (fp32 256) 53.4 /
+    // 44.3 and 48.6 / 46.6; 537 MB (bf16 512) 78.3 / 68.7 and 71.4 / 68.4. Smaller calls lose: 64 fp32 rows 15.0 -> 15.5.
+    const bool past = (int64_t)c.requests * c.vocab * (PS + QS) >= (int64_t)256 << 20;
     a.tstride = (int)min((int64_t)w.ticks / per, (int64_t)64);
     for (int64_t r0 = 0; r0 < (int64_t)c.requests; r0 += per) {
       a.r0 = (int)r0;
       const dim3 grid((uint32_t)wgs, (uint32_t)min(per, (int64_t)c.requests - r0));
-      if (S == 1) hipLaunchKernelGGL((chain_kernel<P, Q, 1>), grid, dim3(CT), 0, s, a);
-      else if (S == 2) hipLaunchKernelGGL((chain_kernel<P, Q, 2>), grid, dim3(CT), 0, s, a);
-      else if (S == 4) hipLaunchKernelGGL((chain_kernel<P, Q, 4>), grid, dim3(CT), 0, s, a);
-      else hipLaunchKernelGGL((chain_kernel<P, Q, 8>), grid, dim3(CT), 0, s, a);
+      if (S == 1) hipLaunchKernelGGL((chain_kernel<P, Q, 1, false>), grid, dim3(CT), 0, s, a);
+      else if (S == 2) hipLaunchKernelGGL((chain_kernel<P, Q, 2, false>), grid, dim3(CT), 0, s, a);
+      else if (S == 4) hipLaunchKernelGGL((chain_kernel<P, Q, 4, false>), grid, dim3(CT), 0, s, a);
+      else if (!past) hipLaunchKernelGGL((chain_kernel<P, Q, 8, false>), grid, dim3(CT), 0, s, a);
+      else hipLaunchKernelGGL((chain_kernel<P, Q, 8, true>), grid, dim3(CT), 0, s, a);
     }
   };
   auto by_q = [&](auto pt) {

@@ -321,6 +321,37 @@ def test_offsets_out_of_order(ge, gpu):
     assert o.tolist()[0][0] == rr.chain(p[:3], q[:2], b["tokens"][:2], b["coins"][:2], b["u"][0])[0]
 
 
+@pytest.mark.parametrize("r,drafts,dtype", [(1040, 0, "bf16"), (600, 1, "bf16"), (260, 1, "f32"), (140, 1, "f64")])
+def test_calls_past_the_last_level_cache(ge, gpu, r, drafts, dtype):
+    """Calls of more than 256 MB of rows: the same answers, over an odd vocabulary, against fp64 sums row by row."""
+    v = 130001
+    g = torch.Generator(device=gpu).manual_seed(r)
+    n = r * (drafts + 1)
+    p = torch.rand((n, v), generator=g, device=gpu).pow_(8).to(TYPES[dtype])
+    q = torch.rand((r, v), generator=g, device=gpu).pow_(8).to(TYPES[dtype]) if drafts else None
+    assert r * v * p.element_size() * (2 if drafts else 1) >= 256 << 20
+    tok = torch.randint(0, v, (r * drafts,), generator=g, device=gpu, dtype=torch.int32)
+    coin, u = (torch.rand(k, generator=g, device=gpu, dtype=torch.float64) for k in (r * drafts, r))
+    o = ge.spec.verify_chains(p, tok, torch.arange(0, r * drafts + 1, max(drafts, 1), dtype=torch.int32, device=gpu)
+                              if drafts else torch.zeros(r + 1, dtype=torch.int32, device=gpu), coin, u, draft=q, max_drafts=drafts)
+    want = []
+    for k in range(r):
+        row = p[k * (drafts + 1)].double()
+        if drafts:
+            x = int(tok[k])
+            if bool(q[k, x] > 0) and bool(coin[k] * q[k, x].double() < row[x]):
+                row, first = p[2 * k + 1].double(), [x]
+            else:
+                row, first = (row - q[k].double()).clamp(min=0), []
+        else:
+            first = []
+        c = row.cumsum(0)
+        want.append((first + [int(torch.searchsorted(c, u[k] * c[-1]))], None))
+    assert o.tolist() == want
+    if drafts:
+        assert 0 < sum(len(w[0]) for w in want) - r < r
+
+
 def test_rows_past_32_bits(ge, gpu):
     """Rows more than 2^31 elements (and 2^32 bytes) into the tensors."""
     v, d = 262144, 8198

@@ -15,7 +15,8 @@ A round of tree verification, nothing of which waits for the host:
     step = call.commit(step, pages, caches, add=nodes, depth=depth, max_tokens=n)
 
 commit is keep_path, the accepted path moved behind its anchor, and the step that keeps it and adds the next round's nodes. A
-round of chains needs no move: its accepted drafts are already consecutive (spec.verify_chains(...).commit).
+round of chains needs no move: its accepted drafts are already consecutive (spec.verify_chains(...).commit). Both commits
+keep nothing of a request that the round's step did not serve.
 """
 import ctypes as C
 import math

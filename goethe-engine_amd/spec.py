@@ -305,10 +305,12 @@ class VerifyCall:
     def commit(self, step, pages, caches, add, depth=None, max_tokens=None, ends=None, heads_first=False):
         """engine.py:299-305's commit and the next round's layout, on the device: keep_path(step, caches), then the
         paged.PageTable's step that keeps each request's accepted tokens (none where ends[r]: it gives its pages back) and
-        adds the next round's (paged.PageTable.step's add, depth, max_tokens). Returns the next round's paged.StepMap."""
+        adds the next round's (paged.PageTable.step's add, depth, max_tokens). A request that step did not serve
+        (step.status not _lib.STEP_OK) had no slots: it keeps nothing, and the tokens this round emitted for it are void.
+        Returns the next round's paged.StepMap."""
         self.keep_path(step, caches, heads_first)
         kept = self.e_len if self.ld >= self.longest else self.e_len.clamp(max=self.ld)  # (the tokens that result() gives)
-        return pages.step(add, keep=_kept(kept, ends), depth=depth, max_tokens=max_tokens)
+        return pages.step(add, keep=_kept(kept, step, ends), depth=depth, max_tokens=max_tokens)
 
     def _build(self, reqs, nout0, emit_ld):
         dev = _device()
@@ -469,11 +471,13 @@ class Chains:
     def __init__(self, emit_len, tokens, probs, status):
         self.emit_len, self.tokens, self.probs, self.status = emit_len, tokens, probs, status
 
-    def commit(self, pages, add, max_tokens=None, ends=None):
+    def commit(self, pages, add, max_tokens=None, ends=None, step=None):
         """The round's commit and the next one's layout, on the device: the paged.PageTable's step that keeps each request's
-        anchor and accepted drafts (already consecutive; none where ends[r]) and adds the next round's tokens. Returns the
-        next round's paged.StepMap."""
-        return pages.step(add, keep=_kept(self.emit_len, ends), max_tokens=max_tokens)
+        anchor and accepted drafts (already consecutive; none where ends[r]) and adds the next round's tokens. step: the
+        paged.StepMap of this round; a request that it did not serve (status not _lib.STEP_OK) had no slots, so it keeps
+        nothing, and the tokens this round emitted for it are void. Without step the caller vouches that every request
+        was served. Returns the next round's paged.StepMap."""
+        return pages.step(add, keep=_kept(self.emit_len, step, ends), max_tokens=max_tokens)
 
     def tolist(self):
         """Per request (emitted tokens, "error" or None), as verify_tree reports them."""
@@ -481,8 +485,13 @@ class Chains:
         return [(t[a][:n[a]], "error" if st[a] != _lib.WALK_OK else None) for a in range(len(n))]
 
 
-def _kept(emit_len, ends):
-    """paged.PageTable.step's keep after a round: emit_len, -1 where a request ends."""
+def _kept(emit_len, step, ends):
+    """paged.PageTable.step's keep after a round: emit_len; 0 where the round's step (None: it served every request) did not
+    serve the request, whose keys and values were then written nowhere; -1 where a request ends."""
+    if step is not None:
+        if step.status.shape != emit_len.shape:
+            raise ValueError(f"a step of {step.status.shape[0]} requests for a round of {emit_len.shape[0]}")
+        emit_len = emit_len.masked_fill(step.status != _lib.STEP_OK, 0)
     if ends is None:
         return emit_len
     ends = torch.as_tensor(ends, dtype=torch.bool).to(emit_len.device)

@@ -1,0 +1,91 @@
+"""Commits of verify rounds on the GPU (spec.VerifyCall.commit, spec.Chains.commit) where a step could not serve every request:
+lengths, tables and queues against the oracle's bookkeeping, whole numbers compared exactly."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import round_ref as rr
+
+pytestmark = pytest.mark.gpu
+
+
+def _same(t, ref, m, want):
+    for name, x in (("begin", m.begin), ("slot", m.slot), ("pos", m.pos), ("req", m.req), ("seq", m.seq_len), ("status", m.status)):
+        assert x.cpu().tolist() == [int(k) for k in want[name]], name
+    c, r = t.counters.cpu().tolist(), t.requests
+    assert c[2:2 + r] == ref.length and c[2 + r:] == [len(p) for p in ref.pages]
+    ring, table = t.ring.cpu().tolist(), t.table.cpu().tolist()
+    assert c[1] == len(ref.free) and [ring[(c[0] + i) % len(ring)] for i in range(c[1])] == list(ref.free)
+    assert [table[k][:len(p)] for k, p in enumerate(ref.pages)] == ref.pages
+    ref.check()
+
+
+# (three requests of one page each out of four; then request 1's tokens do not fit, or request 1's numbers are out of range)
+CASES = [("full", [3, 14, 4], 1), ("bad", [3, 3, 4], 2)]
+
+
+def _tables(ge, gpu, add, bad):
+    t, ref = ge.paged.PageTable(3, 4, 8, 3, device=gpu), rr.Pages(3, 4, 8, 3)
+    _same(t, ref, t.step([4, 5, 6]), ref.step([4, 5, 6]))
+    keep = [2, 40 if bad else 5, 1]
+    m, want = t.step(add, keep=keep), ref.step(add, keep)
+    _same(t, ref, m, want)
+    return t, ref, m, want
+
+
+@pytest.mark.parametrize("ends", [None, [False, True, True]])
+@pytest.mark.parametrize("name,add,status", CASES)
+def test_trees_after_a_step_that_served_not_every_request(ge, gpu, name, add, status, ends):
+    t, ref, m, want = _tables(ge, gpu, add, name == "bad")
+    assert want["status"] == [0, status, 0]
+    g = torch.Generator(device=gpu).manual_seed(2)
+    x = torch.randn((sum(add), 300), generator=g, device=gpu)
+    best = x.argmax(1).cpu().tolist()
+    at = np.concatenate([[0], np.cumsum(add)])
+    reqs = [dict(target=x[at[k]:at[k + 1]], parents=list(range(add[k] - 1)), params=ge.sampling.SamplingParams(), seed=1,
+                 tokens=best[at[k]:at[k + 1] - 1]) for k in range(3)]  # (every draft accepted)
+    call = ge.spec.VerifyCall(reqs)
+    call.launch()
+    assert call.e_len.cpu().tolist() == add
+    c = torch.arange(2 * 4 * 8 * 16, device=gpu).reshape(2, 4, 8, 16).float()
+    was = c.clone()
+    nxt = call.commit(m, t, c, [1, 1, 1], ends=ends)
+    keep = [add[0], 0, add[2]] if ends is None else [add[0], -1, -1]
+    _same(t, ref, nxt, ref.step([1, 1, 1], keep))
+    assert torch.equal(c, was)  # (chains: nothing moves)
+
+
+@pytest.mark.parametrize("ends", [None, [False, True, True]])
+@pytest.mark.parametrize("name,add,status", CASES)
+def test_chains_after_a_step_that_served_not_every_request(ge, gpu, name, add, status, ends):
+    t, ref, m, want = _tables(ge, gpu, add, name == "bad")
+    assert want["status"] == [0, status, 0]
+    drafts = [k - 1 for k in add]
+    p = torch.softmax(torch.randn((sum(add), 300), device=gpu, generator=torch.Generator(device=gpu).manual_seed(3)), 1)
+    o = ge.spec.verify_chains(p, [7] * sum(drafts), np.concatenate([[0], np.cumsum(drafts)]), [0.0] * sum(drafts), [0.5] * 3)
+    assert o.emit_len.cpu().tolist() == add  # (a coin of zero takes every draft)
+    nxt = o.commit(t, [1, 1, 1], ends=ends, step=m)
+    keep = [add[0], 0, add[2]] if ends is None else [add[0], -1, -1]
+    _same(t, ref, nxt, ref.step([1, 1, 1], keep))
+
+
+def test_a_dry_pool_commits_nothing_round_after_round(ge, gpu):
+    """A request that no page is left for keeps its length over rounds until another ends, as the loop runs: one step from the
+    next, nothing read back."""
+    t, ref = ge.paged.PageTable(2, 4, 4, 4, device=gpu), rr.Pages(2, 4, 4, 4)
+    m, want = t.step([4, 8]), ref.step([4, 8])
+    lens = [4, 8]
+    p = torch.softmax(torch.randn((8, 99), device=gpu, generator=torch.Generator(device=gpu).manual_seed(4)), 1)
+    o = None
+    for rnd in range(6):
+        ends, add = [rnd >= 3, False], [4 if rnd < 3 else 0, 4]
+        if o is None:
+            m, want = t.step(add, keep=lens), ref.step(add, lens)
+        else:
+            m = o.commit(t, add, ends=ends, step=m)
+            keep = [-1 if e else n if s == 0 else 0 for e, n, s in zip(ends, lens, want["status"])]
+            want = ref.step(add, keep)
+        _same(t, ref, m, want)
+        o = ge.spec.verify_chains(p, [1] * 6, [0, 3, 6], [0.0] * 6, [0.5] * 2)
+        lens = o.emit_len.cpu().tolist()
+    assert ref.length == [0, 12]

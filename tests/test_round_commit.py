@@ -1,0 +1,66 @@
+"""The commits of a verify round (spec.VerifyCall.commit, spec.Chains.commit) without a GPU: what they ask of the page table."""
+from types import SimpleNamespace as NS
+
+import pytest
+import torch
+
+from oracle import round_ref as rr
+
+
+class _Pages:
+    """Takes a step's arguments in the place of a paged.PageTable."""
+
+    def __init__(self):
+        self.calls = []
+
+    def step(self, add, keep=None, depth=None, max_tokens=None):
+        self.calls.append(keep.tolist())
+        return "next"
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _tree_call(ge, lens, ld=9):
+    call = ge.spec.VerifyCall.__new__(ge.spec.VerifyCall)
+    call.e_len, call.ld, call.longest = _i32(*lens), ld, 9
+    call.keep_path = lambda *a: None
+    return call
+
+
+def _chains(ge, lens):
+    return ge.spec.Chains(_i32(*lens), None, None, None)
+
+
+ENDS = [(None, [5, 0, 0, 1]), ([True, False, True, False], [-1, 0, -1, 1])]
+
+
+@pytest.mark.parametrize("ends,want", ENDS)
+def test_a_commit_keeps_nothing_of_a_request_that_was_not_served(ge, ends, want):
+    lib = ge._lib
+    step = NS(status=_i32(lib.STEP_OK, lib.STEP_FULL, lib.STEP_BAD, lib.STEP_OK))
+    lens, pages = (5, 4, 3, 1), _Pages()
+    assert _tree_call(ge, lens).commit(step, pages, None, [1] * 4, ends=ends) == "next"
+    assert _chains(ge, lens).commit(pages, [1] * 4, ends=ends, step=step) == "next"
+    assert pages.calls == [want, want]
+    cut = _Pages()  # (a walk cut at two tokens)
+    _tree_call(ge, lens, ld=2).commit(step, cut, None, [1] * 4, ends=ends)
+    assert cut.calls == [[min(k, 2) for k in want]]
+
+
+def test_a_commit_with_a_step_of_other_requests_is_refused(ge):
+    pages = _Pages()
+    with pytest.raises(ValueError, match="3 requests"):
+        _chains(ge, (1, 2)).commit(pages, [1, 1], step=NS(status=_i32(0, 0, 0)))
+    assert not pages.calls
+
+
+def test_why_a_request_that_was_not_served_keeps_nothing():
+    """The books alone cannot tell: tokens that a full step added nothing for fit the last page, and count as kept."""
+    g = rr.Pages(2, 4, 16, 4)
+    g.step([20, 32])
+    g.step([0, 0], [20, 32])
+    assert g.step([16, 0])["status"] == [1, 0]
+    m = g.step([1, 0], [5, 0])
+    assert m["status"] == [0, 0] and m["pos"] == [25]  # (20 to 24 were never written)

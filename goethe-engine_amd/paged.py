@@ -111,6 +111,10 @@ class PageTable:
         the map (default: the sum of add, which then has to be on the host). into: counters of the same size that receive
         the new state; this table's own then stay as they were (pages taken are the same if the step is made again).
         Returns a StepMap."""
+        return self._step(*self._ready(add, keep, depth, max_tokens, into))
+
+    def _ready(self, add, keep, depth, max_tokens, into=None):
+        """step's arguments as _step takes them, on the device; what is not in order is refused here."""
         r, dev = self.requests, self.device
         if _count(add) != r or (keep is not None and _count(keep) != r):
             raise ValueError(f"add and keep must have {r} entries")
@@ -135,6 +139,10 @@ class PageTable:
         add = _vec(add, i32, dev)
         keep = _vec(keep, i32, dev) if keep is not None else None
         depth = _vec(depth, i32, dev) if depth is not None else None
+        return add, keep, depth, n, into
+
+    def _step(self, add, keep, depth, n, into):
+        r, dev, i32 = self.requests, self.device, torch.int32
         slot = torch.empty(n, dtype=torch.int64, device=dev)
         ints = torch.empty(2 * n + 3 * r + 1, dtype=i32, device=dev)
         pos, req, begin, seq, status = ints.split_with_sizes((n, n, r + 1, r, r))

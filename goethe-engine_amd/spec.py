@@ -307,10 +307,12 @@ class VerifyCall:
         paged.PageTable's step that keeps each request's accepted tokens (none where ends[r]: it gives its pages back) and
         adds the next round's (paged.PageTable.step's add, depth, max_tokens). A request that step did not serve
         (step.status not _lib.STEP_OK) had no slots: it keeps nothing, and the tokens this round emitted for it are void.
-        Returns the next round's paged.StepMap."""
-        self.keep_path(step, caches, heads_first)
+        A refused call has moved nothing. Returns the next round's paged.StepMap."""
         kept = self.e_len if self.ld >= self.longest else self.e_len.clamp(max=self.ld)  # (the tokens that result() gives)
-        return pages.step(add, keep=_kept(kept, step, ends), depth=depth, max_tokens=max_tokens)
+        # (the step's arguments first: a path whose commit is then refused, and made again, would move twice)
+        ready = pages._ready(add, _kept(kept, step, ends), depth, max_tokens)
+        self.keep_path(step, caches, heads_first)
+        return pages._step(*ready)
 
     def _build(self, reqs, nout0, emit_ld):
         dev = _device()

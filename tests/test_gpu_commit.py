@@ -89,3 +89,33 @@ def test_a_dry_pool_commits_nothing_round_after_round(ge, gpu):
         o = ge.spec.verify_chains(p, [1] * 6, [0, 3, 6], [0.0] * 6, [0.5] * 2)
         lens = o.emit_len.cpu().tolist()
     assert ref.length == [0, 12]
+
+
+def test_a_refused_commit_leaves_caches_and_books(ge, gpu):
+    """Whatever a commit refuses, the one made after it moves each path once."""
+    t = ge.paged.PageTable(2, 12, 4, 4, device=gpu)
+    u = ge.paged.PageTable(2, 12, 4, 4, device=gpu)
+    parents = [[0, 0, 2, 3], [0]]
+    sizes = [5, 2]
+    x = torch.randn((7, 200), device=gpu, generator=torch.Generator(device=gpu).manual_seed(6))
+    best = x.argmax(1).cpu().tolist()
+    toks = [[(best[0] + 1) % 200, best[0], best[2], best[3]], [(best[5] + 1) % 200]]  # (the path 0, 2, 3, 4; and 0 alone)
+    at = [0, 5]
+    call = ge.spec.VerifyCall([dict(target=x[at[k]:at[k] + sizes[k]], parents=parents[k], tokens=toks[k], seed=1,
+                                    params=ge.sampling.SamplingParams()) for k in range(2)])
+    call.launch()
+    assert call.e_len.cpu().tolist() == [4, 1]
+    c = torch.arange(2 * 12 * 4 * 8, device=gpu).reshape(2, 12, 4, 8).float()
+    d = c.clone()
+    m, n = t.step(sizes), u.step(sizes)
+    was, books = c.clone(), t.counters.clone()
+    for kw in (dict(add=torch.ones(2, dtype=torch.int32, device=gpu)), dict(add=torch.ones(2), max_tokens=2), dict(add=[1]),
+               dict(add=[1, 1], depth=torch.zeros(2)), dict(add=[1, 1], ends=[True]), dict(add=[1, 1], caches=c.cpu()),
+               dict(add=[1, 1], caches=c[0, 0])):
+        with pytest.raises((ValueError, RuntimeError)):
+            call.commit(m, t, **{"caches": c, **kw})
+        assert torch.equal(c, was) and torch.equal(t.counters, books)
+    call.commit(m, t, c, [1, 1])
+    call.keep_path(n, d)
+    u.step([1, 1], keep=call.e_len)
+    assert not torch.equal(c, was) and torch.equal(c, d) and torch.equal(t.counters, u.counters)

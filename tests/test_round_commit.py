@@ -14,6 +14,12 @@ class _Pages:
         self.calls = []
 
     def step(self, add, keep=None, depth=None, max_tokens=None):
+        return self._step(*self._ready(add, keep, depth, max_tokens))
+
+    def _ready(self, add, keep, depth, max_tokens):
+        return add, keep
+
+    def _step(self, add, keep):
         self.calls.append(keep.tolist())
         return "next"
 
@@ -64,3 +70,18 @@ def test_why_a_request_that_was_not_served_keeps_nothing():
     assert g.step([16, 0])["status"] == [1, 0]
     m = g.step([1, 0], [5, 0])
     assert m["status"] == [0, 0] and m["pos"] == [25]  # (20 to 24 were never written)
+
+
+def test_a_refused_commit_moves_nothing(ge):
+    """A path that moved before its commit was refused would move again in the commit made after."""
+    call, moved = _tree_call(ge, (2, 1)), []
+    call.keep_path = lambda *a: moved.append(a)
+    step, pages = NS(status=_i32(0, 0)), ge.paged.PageTable(2, 8, 4, 4, device="cpu")
+    for kw in (dict(add=[1]), dict(add=[1, 1], ends=[True]), dict(add=[1, 1], depth=[0]), dict(add=[1, 1], max_tokens=-1)):
+        with pytest.raises(ValueError):
+            call.commit(step, pages, None, **kw)
+    with pytest.raises(RuntimeError):  # state on the host
+        call.commit(step, pages, None, [1, 1])
+    with pytest.raises(ValueError):
+        call.commit(NS(status=_i32(0, 0, 0)), pages, None, [1, 1])
+    assert not moved

@@ -99,8 +99,12 @@ __global__ __launch_bounds__(ST) void step_kernel(gsp_pages p, gsp_step t) {
     if (r0) __syncthreads();
     const int n = min(ST, R - r0), r = r0 + tid;
     Req q = {};
-    if (tid < n)
-      q = request(p, ring_ok, p.counters[2 + r], p.counters[2 + (int64_t)R + r], t.keep ? t.keep[r] : 0, t.add[r]);
+    bool ends = false;
+    if (tid < n) {
+      const int32_t keep = t.keep ? t.keep[r] : 0;
+      ends = keep < 0;
+      q = request(p, ring_ok, p.counters[2 + r], p.counters[2 + (int64_t)R + r], keep, t.add[r]);
+    }
     const int64_t it = (int64_t)wave_incl_scan_u64((uint64_t)q.add), il = (int64_t)wave_incl_scan_u64((uint64_t)q.lack);
     if (lane == WAVE - 1) {
       sh.wave[0][wv] = it;
@@ -112,9 +116,10 @@ __global__ __launch_bounds__(ST) void step_kernel(gsp_pages p, gsp_step t) {
     if (q.status == GSP_STEP_OK &&
         ((q.lack > 0 && take + q.lack > free) || (q.add > 0 && tok + q.add > (int64_t)t.max_tokens)))
       q.status = GSP_STEP_FULL;
-    if (q.status != GSP_STEP_OK) {
-      q.need = q.held;
-      q.lack = q.over = 0;
+    if (q.status != GSP_STEP_OK) {  // (a request that ends gives its pages back though what starts in its place does not fit)
+      q.need = q.status == GSP_STEP_FULL && ends ? 0 : q.held;
+      q.lack = 0;
+      q.over = q.held - q.need;
     }
     if (q.lack > 0) taken = take + q.lack;
     const int64_t ig = (int64_t)wave_incl_scan_u64((uint64_t)q.over);

@@ -70,7 +70,8 @@ typedef struct gsp_pages {
 enum {
   GSP_STEP_OK = 0,
   GSP_STEP_FULL = 1, /* not enough free pages for this request (in request order), more than max_pages, or more
-                      * tokens than max_tokens: its kept tokens count, nothing is added, its slots are -1 */
+                      * tokens than max_tokens: its kept tokens count, nothing is added, its slots are -1; it gives no
+                      * page back unless it ends (keep < 0), and then every one */
   GSP_STEP_BAD = 2   /* keep, add, length or held (for every request: head or free) out of range: the request is left as it
                       * was, its slots are -1 */
 };
@@ -79,7 +80,8 @@ typedef struct gsp_step {
   uint32_t size;
   uint32_t max_tokens;      /* entries of slot, pos, req */
   const int32_t *keep;      /* [requests] tokens of the pages held that the step before filled and that stay (an accepted
-                             * path), < 0: the request ends and gives back every page; NULL: none */
+                             * path), < 0: the request ends and gives back every page, whether or not add fits (not when
+                             * it is GSP_STEP_BAD); NULL: none */
   const int32_t *add;       /* [requests] new tokens >= 0 */
   const int32_t *depth;     /* [max_tokens] a new token's distance from its request's first (a tree node's depth), or
                              * NULL: its index among the request's new tokens */

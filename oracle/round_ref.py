@@ -110,6 +110,9 @@ class Pages:
                     self.pages[r].append(self.free.popleft())
                 back += self.pages[r][need:]
                 del self.pages[r][need:]
+            elif st == 1 and k < 0:  # (it ended: its pages are free, though what was to start in its place did not fit)
+                back += self.pages[r]
+                self.pages[r] = []
             for i in range(max(a, 0)):
                 if at + i >= max_tokens:
                     break

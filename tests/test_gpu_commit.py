@@ -119,3 +119,37 @@ def test_a_refused_commit_leaves_caches_and_books(ge, gpu):
     call.keep_path(n, d)
     u.step([1, 1], keep=call.e_len)
     assert not torch.equal(c, was) and torch.equal(c, d) and torch.equal(t.counters, u.counters)
+
+
+@pytest.mark.parametrize("room", [None, 3])
+def test_an_end_whose_successor_does_not_fit_gives_its_pages_back(ge, gpu, room):
+    """No pages left for it, a full table row, or (room) past the map's end: the ended request holds nothing after the step, in
+    place and into other counters, and the next step has its pages."""
+    for most, add in ((11, [44, 4]), (10, [41, 0])):
+        t, ref = ge.paged.PageTable(2, 10, 4, most, device=gpu), rr.Pages(2, 10, 4, most)
+        _same(t, ref, t.step([24, 16]), ref.step([24, 16]))
+        keep, into = [-1, 16], torch.zeros_like(t.counters)
+        n = sum(add) if room is None else room
+        tried = t.step(add, keep=keep, max_tokens=n, into=into)
+        m, want = t.step(add, keep=keep, max_tokens=n), ref.step(add, keep, None, n)
+        _same(t, ref, m, want)
+        assert want["status"][0] == 1 and torch.equal(into, t.counters) and torch.equal(tried.slot, m.slot)
+        assert t.held.tolist()[0] == 0 and t.free.item() == 6
+        _same(t, ref, t.step([20, 4]), ref.step([20, 4]))
+
+
+@pytest.mark.parametrize("r", [3, 300, 1500])
+def test_ends_in_a_dry_pool(ge, gpu, r):
+    """Many steps over a pool that stays dry, half the requests ending in each, their successors of any length."""
+    t, ref = ge.paged.PageTable(r, 3 * r, 4, 9, device=gpu), rr.Pages(r, 3 * r, 4, 9)
+    rng = np.random.default_rng(r)
+    kept_to, freed = np.zeros(r, np.int64), 0
+    for k in range(10):
+        keep = np.where(rng.random(r) < 0.5, -1, np.minimum(rng.integers(0, 5, r), kept_to))
+        add = rng.integers(0, 42, r)
+        held = [len(p) for p in ref.pages]
+        m, want = t.step(add, keep=keep), ref.step(add, keep)
+        _same(t, ref, m, want)
+        kept_to = np.where(np.array(want["status"]) == 0, add, 0)
+        freed += sum(held[i] for i in range(r) if keep[i] < 0 and want["status"][i] == 1)
+    assert freed > 0

@@ -85,3 +85,16 @@ def test_a_refused_commit_moves_nothing(ge):
     with pytest.raises(ValueError):
         call.commit(NS(status=_i32(0, 0, 0)), pages, None, [1, 1])
     assert not moved
+
+
+def test_an_end_gives_its_pages_back_though_what_follows_does_not_fit():
+    """Ten pages of four, six and four of them held: request 0 ends and 44 tokens in its place need eleven."""
+    g = rr.Pages(2, 10, 4, 11)
+    assert g.step([24, 16])["status"] == [0, 0]
+    m = g.step([44, 4], [-1, 16])
+    assert m["status"] == [1, 1] and m["seq"] == [0, 16] and list(g.free) == [0, 1, 2, 3, 4, 5] and not g.pages[0]
+    g.check()
+    m = g.step([20, 4], [0, 0])  # (the next step has them)
+    assert m["status"] == [0, 0] and m["seq"] == [20, 20]
+    m = g.step([2, 2], [-1, 9])  # past the pages held: left as it was
+    assert m["status"] == [0, 2]

@@ -172,6 +172,9 @@ _L = None
 # MAX_HANDLES the least recently used one leaves it and is closed once nothing references it any more.
 MAX_HANDLES = 8
 _handles = OrderedDict()
+# Handles of calls that were captured: a graph holds their workspaces' addresses, so they stay open past replacement and the
+# cache's end, until release_captured().
+_captured = set()
 
 
 def lib():
@@ -248,22 +251,46 @@ def raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+def _capturing(device):
+    """Whether a device's current stream is being captured into a graph."""
+    if device == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def handle(device, rows, vocab):
     """The handle of (device, current stream) that fits rows x vocab, reopened larger on demand. Calls on two streams
-    may overlap on the device, so each stream gets its own workspace; at most MAX_HANDLES stay cached."""
+    may overlap on the device, so each stream gets its own workspace; at most MAX_HANDLES stay cached. While the stream is
+    captured the handle has to fit already (opening one allocates and waits for the device), and it then stays open for
+    the graph's replays: until release_captured()."""
     if not _handles and not torch.cuda.is_available():
         raise RuntimeError("goethe-engine_amd needs a HIP device (torch.cuda.is_available() is False)")
     key = (device, raw_stream(device))
+    capturing = _capturing(device)
     with _lock:
         h = _handles.get(key)
         if h is None or h.rows < rows or h.vocab < vocab:
+            if capturing:
+                raise RuntimeError(f"a captured call of {rows} rows of {vocab} tokens on a stream whose handle "
+                                   + (f"holds {h.rows} of {h.vocab}" if h else "is not open")
+                                   + ": make a call of this size on the stream before the capture")
             # (a handle that is replaced or evicted is closed when its last user lets it go)
             h = Handle(device, max(rows, h.rows if h else 0, 64), max(vocab, h.vocab if h else 0))
             _handles[key] = h
             while len(_handles) > MAX_HANDLES:
                 _handles.popitem(last=False)
+        if capturing:
+            _captured.add(h)
         _handles.move_to_end(key)
         return h
+
+
+def release_captured():
+    """Lets go of the handles that captured calls use. For programs that capture anew at other sizes: call it when the graphs
+    captured so far are gone (a replay over a closed handle would write to freed memory)."""
+    with _lock:
+        _captured.clear()
 
 
 def ptr(t):

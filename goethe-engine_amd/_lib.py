@@ -175,6 +175,7 @@ _handles = OrderedDict()
 # Handles of calls that were captured: a graph holds their workspaces' addresses, so they stay open past replacement and the
 # cache's end, until release_captured().
 _captured = set()
+_device_handles = {}  # of the calls that use no workspace, by device
 
 
 def lib():
@@ -283,6 +284,27 @@ def handle(device, rows, vocab):
         if capturing:
             _captured.add(h)
         _handles.move_to_end(key)
+        return h
+
+
+def device_handle(device):
+    """A handle of the device for the calls that use no workspace: one for all streams, outside their cache, so that such
+    calls neither push out a stream's handle nor open one that its other calls then open anew. A captured call that comes
+    before any other takes a stream's (it needs the device and the error text alone)."""
+    h = _device_handles.get(device)
+    if h is not None:
+        return h
+    if not torch.cuda.is_available():
+        raise RuntimeError("goethe-engine_amd needs a HIP device (torch.cuda.is_available() is False)")
+    capturing = _capturing(device)
+    with _lock:
+        h = _device_handles.get(device)
+        if h is None and capturing:
+            h = next((k for (d, _), k in _handles.items() if d == device), None)
+            if h is None:
+                raise RuntimeError("a captured call on a device without a handle: make one call on it before the capture")
+        elif h is None:
+            h = _device_handles[device] = Handle(device, 1, 1)
         return h
 
 

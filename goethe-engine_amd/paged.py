@@ -151,7 +151,7 @@ class PageTable:
         t = _lib.Step(_STEP, n, keep.data_ptr() if keep is not None else None, add.data_ptr(),
                       depth.data_ptr() if depth is not None else None, begin.data_ptr(), slot.data_ptr(), pos.data_ptr(),
                       req.data_ptr(), seq.data_ptr(), status.data_ptr(), _lib.raw_stream(dev.index))
-        _lib.handle(dev.index, 1, 1).call("gsp_pages_step", C.byref(p), C.byref(t))
+        _lib.device_handle(dev.index).call("gsp_pages_step", C.byref(p), C.byref(t))
         return StepMap(begin, slot, pos, req, seq, status, into)
 
 
@@ -254,4 +254,4 @@ def keep_path(caches, slot, anchor, emit_len, emit_nodes, heads_first=False):
     p = _lib.Path(_PATH, r, slot.shape[0], n, slot.data_ptr(), anchor.data_ptr(), emit_len.data_ptr(), emit_nodes.data_ptr(), ld,
                   base, stride, ptrs, align, page, pages, chunks, size, 0, page_stride, token_stride, chunk_stride,
                   _lib.raw_stream(dev.index))
-    _lib.handle(dev.index, 1, 1).call("gsp_keep_path", C.byref(p))
+    _lib.device_handle(dev.index).call("gsp_keep_path", C.byref(p))

@@ -87,3 +87,25 @@ def test_a_capture_that_needs_a_handle_is_refused(ge, gpu):
         s.synchronize()
         assert x.tolist() == [1.0] * 4
         assert chains(**more).tolist() == want_m
+
+
+def test_page_calls_on_many_streams_leave_the_cache(ge, gpu):
+    """Page steps and path moves on more streams than the cache holds: every handle in it stays, and their answers agree."""
+    lib = ge._lib
+    args, want = _chains(gpu, 2003, 5)
+    assert ge.spec.verify_chains(**args).tolist() == want
+    was = list(lib._handles.items())
+    add, ref = [5, 0, 9], rr.Pages(3, 12, 4, 4)
+    slot, status = (ref.step(add)[k] for k in ("slot", "status"))
+    one = torch.zeros(1, dtype=torch.int32, device=gpu)
+    nodes = torch.tensor([[0, 3]], dtype=torch.int32, device=gpu)
+    torch.cuda.synchronize()
+    for _ in range(lib.MAX_HANDLES + 2):
+        with torch.cuda.stream(torch.cuda.Stream(gpu)):
+            t = ge.paged.PageTable(3, 12, 4, 4, device=gpu)
+            m = t.step(add)
+            c = torch.arange(12 * 4 * 8, device=gpu).reshape(1, 12, 4, 8).float()
+            ge.paged.keep_path(c, m.slot, one, one + 2, nodes)
+            assert m.slot.tolist() == slot and m.status.tolist() == status
+            assert c[0, 0, 1].tolist() == list(range(24, 32))  # (node 3's row, in the place after the anchor)
+    assert list(lib._handles.items()) == was

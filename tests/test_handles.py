@@ -19,6 +19,7 @@ def lib(ge, monkeypatch):
     monkeypatch.setattr(m, "Handle", Handle)
     monkeypatch.setattr(m, "_handles", OrderedDict())
     monkeypatch.setattr(m, "_captured", set(), raising=False)
+    monkeypatch.setattr(m, "_device_handles", {}, raising=False)
     monkeypatch.setattr(m, "stream", 0, raising=False)
     monkeypatch.setattr(m, "capturing", False, raising=False)
     monkeypatch.setattr(m, "raw_stream", lambda device: m.stream)
@@ -69,3 +70,27 @@ def test_a_capture_opens_no_handle(lib):
         with pytest.raises(RuntimeError, match="holds 64 of 100"):
             lib.handle(0, rows, vocab)
     assert lib.handle(0, 64, 100) is h and list(lib._handles.values()) == [h]
+
+
+def test_calls_without_a_workspace_leave_the_streams_handles(lib):
+    """Page steps and path moves on any number of streams push no handle out and open none in the streams' cache."""
+    a = lib.handle(0, 1, 100)
+    d = lib.device_handle(0)
+    for lib.stream in range(1, 3 * lib.MAX_HANDLES):
+        assert lib.device_handle(0) is d
+    assert list(lib._handles.values()) == [a] and d is not a and (d.rows, d.vocab) == (1, 1)
+    assert lib.device_handle(1) is not d
+
+
+def test_a_capture_opens_no_device_handle(lib):
+    lib.capturing = True
+    with pytest.raises(RuntimeError, match="before the capture"):
+        lib.device_handle(0)
+    lib.capturing = False
+    a = lib.handle(0, 1, 100)
+    lib.capturing = True
+    assert lib.device_handle(0) is a and not lib._device_handles  # (the stream's, for its error text alone)
+    with pytest.raises(RuntimeError):
+        lib.device_handle(1)
+    lib.capturing = False
+    assert lib.device_handle(0) is not a

@@ -241,7 +241,7 @@ __global__ __launch_bounds__(PT) void path_kernel(gsp_path a, uint32_t vecs) {
     if (tid < WAVE) {
       const int64_t i = i0 + lane, to = anchor + i;
       const int64_t node = i < a.emit_ld ? a.emit_nodes[r * a.emit_ld + i] : -1;  // (read ahead of the length)
-      bool moves = i < len && node >= 0 && node < a.tokens && to >= 0 && to < a.tokens && node != to;
+      bool moves = i < len && node >= 0 && node < a.tokens && anchor >= 0 && to < a.tokens && node != to;
       uint64_t s = 0, d = 0;
       if (moves) {
         s = (uint64_t)a.slot[node];

@@ -220,7 +220,8 @@ def keep_path(caches, slot, anchor, emit_len, emit_nodes, heads_first=False):
     stream: entry i = 1 .. emit_len[r] - 1 of request r's path goes from slot[emit_nodes[r, i]] to slot[anchor[r] + i].
     caches: a Caches, or one stacked tensor [n, pages, page, ...] (heads_first: [n, pages, heads, page, ...]); slot: StepMap.slot
     of the round; anchor, emit_len int32 [R], emit_nodes int32 [R, ld]: gse_verify_tree's (VerifyCall.keep_path passes
-    them). Nodes ascend along a path and requests share no slots; entries out of range and negative slots are skipped."""
+    them). Nodes ascend along a path and requests share no slots; entries out of range, negative slots and requests
+    with a negative anchor (padded ones) are skipped."""
     stacked = not isinstance(caches, Caches)
     if not stacked:
         n, layout, dev = len(caches.tensors), caches.layout, caches.device

@@ -96,7 +96,8 @@ typedef struct gsp_step {
 
 /* The accepted paths of draft trees whose nodes were written to the cache in node order: entry i of request r's path,
  * i = 1 .. emit_len[r] - 1, moves from slot[emit_nodes[r][i]] to slot[anchor[r] + i], in every cache. Nodes ascend along a
- * path (a parent comes before its children), and requests share no slots. */
+ * path (a parent comes before its children), and requests share no slots. Entries whose node, place or slot is out of range
+ * are not moved, nor is any entry of a request whose anchor is negative (a padded one). */
 typedef struct gsp_path {
   uint32_t size;
   uint32_t requests;

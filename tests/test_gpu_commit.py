@@ -153,3 +153,20 @@ def test_ends_in_a_dry_pool(ge, gpu, r):
         kept_to = np.where(np.array(want["status"]) == 0, add, 0)
         freed += sum(held[i] for i in range(r) if keep[i] < 0 and want["status"][i] == 1)
     assert freed > 0
+
+
+@pytest.mark.parametrize("anchor", [-1, -2, -(2 ** 31)])
+@pytest.mark.parametrize("depth", [4, 70])
+def test_a_request_without_an_anchor_moves_nothing(ge, gpu, anchor, depth):
+    """A padded request's anchor is negative: the places after it are other requests' (entry -anchor's is place 0)."""
+    c = torch.arange(2 * 40 * 4 * 8, device=gpu).reshape(2, 40, 4, 8).float()
+    slot = torch.arange(160, device=gpu)
+    nodes = torch.arange(80, 80 + 2 * depth, device=gpu).reshape(2, depth).int() % 160
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=gpu)  # noqa: E731
+    want = c.clone()
+    ge.paged.keep_path(c, slot, i32(anchor, anchor), i32(depth, 3), nodes)
+    assert torch.equal(c, want)
+    ge.paged.keep_path(c, slot, i32(anchor, 3), i32(depth, 3), nodes)  # (a request beside it still moves)
+    rows = want.view(2, 160, 8)
+    rows[:, 4:6] = rows[:, nodes[1, 1:3].long()].clone()
+    assert torch.equal(c, want)

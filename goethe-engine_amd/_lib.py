@@ -253,11 +253,11 @@ def raw_stream(device):
 
 
 def _capturing(device):
-    """Whether a device's current stream is being captured into a graph."""
-    if device == torch.cuda.current_device():
-        return torch.cuda.is_current_stream_capturing()
+    """Whether a device's current stream is being captured into a graph (0.5 us; torch.cuda's functions take 0.67)."""
+    if device == torch._C._cuda_getDevice():
+        return torch._C._cuda_isCurrentStreamCapturing()
     with torch.cuda.device(device):
-        return torch.cuda.is_current_stream_capturing()
+        return torch._C._cuda_isCurrentStreamCapturing()
 
 
 def handle(device, rows, vocab):

@@ -523,7 +523,13 @@ def _vec(x, dtype, dev):
         if x.device != dev and x.device.type == "cuda":
             raise ValueError(f"tensors on {x.device} and {dev}")
     elif dtype is torch.int32:
-        x = torch.from_numpy(np.asarray(x, np.int64))
+        x = np.asarray(x)
+        if x.dtype.kind not in "iub":  # (a cast would cut fractions off)
+            if x.dtype.kind != "f" or not (np.abs(x) < 2.0 ** 63).all() or (x != np.trunc(x)).any():
+                raise ValueError(f"expected integers, got {x.dtype}")
+        if x.dtype == np.uint64:
+            x = np.minimum(x, np.uint64(2 ** 63 - 1))
+        x = torch.from_numpy(x.astype(np.int64))
     else:
         x = torch.from_numpy(np.asarray(x, np.float64))
     if dtype is torch.int32 and x.dtype is not torch.int32:

@@ -1,6 +1,7 @@
 """The commits of a verify round (spec.VerifyCall.commit, spec.Chains.commit) without a GPU: what they ask of the page table."""
 from types import SimpleNamespace as NS
 
+import numpy as np
 import pytest
 import torch
 
@@ -98,3 +99,16 @@ def test_an_end_gives_its_pages_back_though_what_follows_does_not_fit():
     assert m["status"] == [0, 0] and m["seq"] == [20, 20]
     m = g.step([2, 2], [-1, 9])  # past the pages held: left as it was
     assert m["status"] == [0, 2]
+
+
+def test_numbers_that_are_no_integers_are_refused(ge):
+    """Lists and arrays as tensors: a fraction is not cut off."""
+    vec, cpu = ge.spec._vec, torch.device("cpu")
+    for bad in ([1.5, 2.0], np.array([float("nan")]), np.array([float("inf")]), [1e30], torch.ones(2), ["1"]):
+        with pytest.raises(ValueError, match="expected integers"):
+            vec(bad, torch.int32, cpu)
+    for good, want in (([], []), (np.concatenate([[0], np.cumsum([])]), [0]), ((1, -2), [1, -2]), (np.array([3, 2 ** 40]), [3, 2 ** 31 - 1]), ([-2 ** 40], [-2 ** 31]),
+                       (np.array([2 ** 64 - 1], np.uint64), [2 ** 31 - 1]), (np.array([7], np.uint8), [7]),
+                       (torch.tensor([5, -2 ** 40]), [5, -2 ** 31]), (range(3), [0, 1, 2])):
+        got = vec(good, torch.int32, cpu)
+        assert got.dtype is torch.int32 and got.tolist() == want

@@ -12,7 +12,7 @@ from collections import OrderedDict
 import numpy as np
 import torch
 
-ABI_MAJOR, ABI_MINOR = 1, 5
+ABI_MAJOR, ABI_MINOR = 1, 6
 PATH_MAIN, PATH_DEEP, PATH_EXACT = 0, 1, 2  # gse_row_paths codes
 OK, E_ARG, E_DEVICE, E_UNSUPPORTED, E_CAPACITY = 0, -1, -4, -5, -7
 F32, BF16 = 0, 1
@@ -110,7 +110,8 @@ class Pages(C.Structure):
 class Step(C.Structure):
     _fields_ = [("size", C.c_uint32), ("max_tokens", C.c_uint32), ("keep", C.c_void_p), ("add", C.c_void_p),
                 ("depth", C.c_void_p), ("begin", C.c_void_p), ("slot", C.c_void_p), ("pos", C.c_void_p),
-                ("req", C.c_void_p), ("seq_len", C.c_void_p), ("status", C.c_void_p), ("stream", C.c_void_p)]
+                ("req", C.c_void_p), ("seq_len", C.c_void_p), ("status", C.c_void_p), ("stream", C.c_void_p),
+                ("laid", C.c_void_p)]
 
 
 class Path(C.Structure):

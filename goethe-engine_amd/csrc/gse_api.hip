@@ -632,6 +632,7 @@ GSE_API int gsp_pages_step(gse_handle *h, const gsp_pages *pages, const gsp_step
     return fail(h, GSE_E_ARG, "table, ring, counters and counters_out are required");
   if (!t.add || !t.begin || !t.seq_len || !t.status || (t.max_tokens > 0 && !t.slot))
     return fail(h, GSE_E_ARG, "add, begin, slot, seq_len and status are required");
+  if (t.laid == t.status) return fail(h, GSE_E_ARG, "laid must be another step's status");
   if (p.page == 0 || p.pool == 0 || p.max_pages == 0) return fail(h, GSE_E_ARG, "page, pool and max_pages must be > 0");
   if (p.table_ld < (int64_t)p.max_pages) return fail(h, GSE_E_ARG, "table_ld < max_pages");
   if (p.pool > (uint32_t)INT32_MAX || (uint64_t)p.max_pages * p.page > (uint64_t)INT32_MAX)

@@ -101,7 +101,8 @@ __global__ __launch_bounds__(ST) void step_kernel(gsp_pages p, gsp_step t) {
     Req q = {};
     bool ends = false;
     if (tid < n) {
-      const int32_t keep = t.keep ? t.keep[r] : 0;
+      int32_t keep = t.keep ? t.keep[r] : 0;
+      if (keep > 0 && t.laid && t.laid[r] != GSP_STEP_OK) keep = 0;  // (they were written nowhere)
       ends = keep < 0;
       q = request(p, ring_ok, p.counters[2 + r], p.counters[2 + (int64_t)R + r], keep, t.add[r]);
     }

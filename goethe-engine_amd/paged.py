@@ -103,17 +103,18 @@ class PageTable:
         """int32 [1]: the number of free pages."""
         return self.counters[1:2]
 
-    def step(self, add, keep=None, depth=None, max_tokens=None, into=None):
+    def step(self, add, keep=None, depth=None, max_tokens=None, into=None, of=None):
         """One step on the current stream, asynchronously (a graph can capture it): request r's length grows by keep[r]
         tokens that an earlier step added (keep[r] < 0: it ends and gives back its pages, also where its new tokens then
         do not fit), then add[r] new tokens get pages and slots. Pages are taken in request order; those given back are free from the next step on. depth [max_tokens]:
         each new token's distance from its request's first (a tree node's depth; default: its index). max_tokens: entries of
         the map (default: the sum of add, which then has to be on the host). into: counters of the same size that receive
         the new state; this table's own then stay as they were (pages taken are the same if the step is made again).
-        Returns a StepMap."""
-        return self._step(*self._ready(add, keep, depth, max_tokens, into))
+        of: the StepMap that added the tokens which keep counts; nothing was written for a request that it did not serve, so
+        that one's keep > 0 counts as 0 (without it, the caller sees to that). Returns a StepMap."""
+        return self._step(*self._ready(add, keep, depth, max_tokens, into, of))
 
-    def _ready(self, add, keep, depth, max_tokens, into=None):
+    def _ready(self, add, keep, depth, max_tokens, into=None, of=None):
         """step's arguments as _step takes them, on the device; what is not in order is refused here."""
         r, dev = self.requests, self.device
         if _count(add) != r or (keep is not None and _count(keep) != r):
@@ -133,15 +134,19 @@ class PageTable:
             self._counters(into)
             if 0 < abs(into.data_ptr() - self.counters.data_ptr()) < 4 * into.numel():
                 raise ValueError("into overlaps the table's counters")
+        if of is not None and of.status.shape[0] != r:
+            raise ValueError(f"a step of {of.status.shape[0]} requests for a table of {r}")
         if dev.type != "cuda":
             raise RuntimeError("goethe-engine_amd needs a HIP device (the table's state is on the host)")
+        if of is not None and of.status.device != dev:
+            raise ValueError(f"a step on {of.status.device}, the table on {dev}")
         i32 = torch.int32
         add = _vec(add, i32, dev)
         keep = _vec(keep, i32, dev) if keep is not None else None
         depth = _vec(depth, i32, dev) if depth is not None else None
-        return add, keep, depth, n, into
+        return add, keep, depth, n, into, of
 
-    def _step(self, add, keep, depth, n, into):
+    def _step(self, add, keep, depth, n, into, of):
         r, dev, i32 = self.requests, self.device, torch.int32
         slot = torch.empty(n, dtype=torch.int64, device=dev)
         ints = torch.empty(2 * n + 3 * r + 1, dtype=i32, device=dev)
@@ -150,7 +155,8 @@ class PageTable:
                        self.ring.data_ptr(), self.counters.data_ptr(), into.data_ptr())
         t = _lib.Step(_STEP, n, keep.data_ptr() if keep is not None else None, add.data_ptr(),
                       depth.data_ptr() if depth is not None else None, begin.data_ptr(), slot.data_ptr(), pos.data_ptr(),
-                      req.data_ptr(), seq.data_ptr(), status.data_ptr(), _lib.raw_stream(dev.index))
+                      req.data_ptr(), seq.data_ptr(), status.data_ptr(), _lib.raw_stream(dev.index),
+                      of.status.data_ptr() if of is not None else None)
         _lib.device_handle(dev.index).call("gsp_pages_step", C.byref(p), C.byref(t))
         return StepMap(begin, slot, pos, req, seq, status, into)
 

@@ -310,7 +310,7 @@ class VerifyCall:
         A refused call has moved nothing. Returns the next round's paged.StepMap."""
         kept = self.e_len if self.ld >= self.longest else self.e_len.clamp(max=self.ld)  # (the tokens that result() gives)
         # (the step's arguments first: a path whose commit is then refused, and made again, would move twice)
-        ready = pages._ready(add, _kept(kept, step, ends), depth, max_tokens)
+        ready = pages._ready(add, _kept(kept, ends), depth, max_tokens, of=step)
         self.keep_path(step, caches, heads_first)
         return pages._step(*ready)
 
@@ -479,7 +479,7 @@ class Chains:
         paged.StepMap of this round; a request that it did not serve (status not _lib.STEP_OK) had no slots, so it keeps
         nothing, and the tokens this round emitted for it are void. Without step the caller vouches that every request
         was served. Returns the next round's paged.StepMap."""
-        return pages.step(add, keep=_kept(self.emit_len, step, ends), max_tokens=max_tokens)
+        return pages.step(add, keep=_kept(self.emit_len, ends), max_tokens=max_tokens, of=step)
 
     def tolist(self):
         """Per request (emitted tokens, "error" or None), as verify_tree reports them."""
@@ -487,13 +487,8 @@ class Chains:
         return [(t[a][:n[a]], "error" if st[a] != _lib.WALK_OK else None) for a in range(len(n))]
 
 
-def _kept(emit_len, step, ends):
-    """paged.PageTable.step's keep after a round: emit_len; 0 where the round's step (None: it served every request) did not
-    serve the request, whose keys and values were then written nowhere; -1 where a request ends."""
-    if step is not None:
-        if step.status.shape != emit_len.shape:
-            raise ValueError(f"a step of {step.status.shape[0]} requests for a round of {emit_len.shape[0]}")
-        emit_len = emit_len.masked_fill(step.status != _lib.STEP_OK, 0)
+def _kept(emit_len, ends):
+    """paged.PageTable.step's keep after a round: emit_len, -1 where a request ends."""
     if ends is None:
         return emit_len
     ends = torch.as_tensor(ends, dtype=torch.bool).to(emit_len.device)

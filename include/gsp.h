@@ -92,6 +92,9 @@ typedef struct gsp_step {
   int32_t *seq_len;         /* [requests] tokens of the request with the new ones */
   uint32_t *status;         /* [requests] GSP_STEP_* */
   void *stream;
+  const uint32_t *laid;     /* [requests] the status of the step that added the tokens which keep counts (not this step's status
+                             * array): a request that it did not serve had no slots, so a keep > 0 counts as 0 there; or
+                             * NULL: it served every request. Since ABI 1.6 */
 } gsp_step;
 
 /* The accepted paths of draft trees whose nodes were written to the cache in node order: entry i of request r's path,

@@ -77,11 +77,13 @@ class Pages:
         self.length = [0] * requests
         self.pages = [[] for _ in range(requests)]
 
-    def step(self, add, keep=None, depth=None, max_tokens=None):
-        """dict(begin, slot, pos, req, seq, status) after one step."""
+    def step(self, add, keep=None, depth=None, max_tokens=None, laid=None):
+        """dict(begin, slot, pos, req, seq, status) after one step; laid: the status of the step that added what keep counts."""
         n = len(self.length)
         max_tokens = sum(max(int(a), 0) for a in add) if max_tokens is None else max_tokens
         keep = [0] * n if keep is None else keep
+        if laid is not None:
+            keep = [min(int(k), 0) if s != 0 else k for k, s in zip(keep, laid)]
         begin, seq, status = [0], [], []
         slot, pos, req = [-1] * max_tokens, [0] * max_tokens, [-1] * max_tokens
         short, back = False, []

@@ -1,5 +1,7 @@
 """Commits of verify rounds on the GPU (spec.VerifyCall.commit, spec.Chains.commit) where a step could not serve every request:
 lengths, tables and queues against the oracle's bookkeeping, whole numbers compared exactly."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -170,3 +172,40 @@ def test_a_request_without_an_anchor_moves_nothing(ge, gpu, anchor, depth):
     rows = want.view(2, 160, 8)
     rows[:, 4:6] = rows[:, nodes[1, 1:3].long()].clone()
     assert torch.equal(c, want)
+
+
+@pytest.mark.parametrize("r", [5, 700, 1300])
+def test_keep_of_a_step_that_served_not_every_request(ge, gpu, r):
+    """PageTable.step(of=): what counts as kept is masked by that step's status, in place and into other counters."""
+    t, ref = ge.paged.PageTable(r, 2 * r, 4, 4, device=gpu), rr.Pages(r, 2 * r, 4, 4)
+    rng = np.random.default_rng(r)
+    add = rng.integers(0, 18, r)
+    m, want = t.step(add), ref.step(add)
+    _same(t, ref, m, want)
+    seen = set()
+    for k in range(8):
+        keep = np.where(rng.random(r) < 0.3, -1, rng.integers(0, 5, r))
+        nxt, laid = rng.integers(0, 9, r), want["status"]
+        into = torch.zeros_like(t.counters)
+        tried = t.step(nxt, keep=keep, into=into, of=m)
+        m = t.step(nxt, keep=keep, of=m)
+        want = ref.step(nxt, keep, laid=laid)
+        _same(t, ref, m, want)
+        assert torch.equal(into, t.counters) and torch.equal(tried.slot, m.slot)
+        seen |= set(laid)
+    assert seen == {0, 1, 2} or r == 5
+
+
+def test_the_steps_own_status_is_not_the_one_before(ge, gpu):
+    lib = ge._lib
+    t = ge.paged.PageTable(2, 8, 4, 4, device=gpu)
+    add = torch.zeros(2, dtype=torch.int32, device=gpu)
+    out = torch.full((16,), -7, dtype=torch.int64, device=gpu)
+    p = lib.Pages(C.sizeof(lib.Pages), 2, 4, 8, 4, 0, t.table.data_ptr(), 4, t.ring.data_ptr(), t.counters.data_ptr(),
+                  t.counters.data_ptr())
+    s = lib.Step(C.sizeof(lib.Step), 0, None, add.data_ptr(), None, out.data_ptr(), None, None, None, out.data_ptr(),
+                 out.data_ptr(), torch.cuda.current_stream().cuda_stream, out.data_ptr())
+    with pytest.raises(RuntimeError, match="another step"):
+        lib.device_handle(gpu.index).call("gsp_pages_step", C.byref(p), C.byref(s))
+    torch.cuda.synchronize()
+    assert (out == -7).all()

@@ -1,4 +1,5 @@
 """The commits of a verify round (spec.VerifyCall.commit, spec.Chains.commit) without a GPU: what they ask of the page table."""
+import copy
 from types import SimpleNamespace as NS
 
 import numpy as np
@@ -9,19 +10,19 @@ from oracle import round_ref as rr
 
 
 class _Pages:
-    """Takes a step's arguments in the place of a paged.PageTable."""
+    """Takes a step's arguments in the place of a paged.PageTable, and says what then counts as kept."""
 
     def __init__(self):
         self.calls = []
 
-    def step(self, add, keep=None, depth=None, max_tokens=None):
-        return self._step(*self._ready(add, keep, depth, max_tokens))
+    def step(self, add, keep=None, depth=None, max_tokens=None, of=None):
+        return self._step(*self._ready(add, keep, depth, max_tokens, of=of))
 
-    def _ready(self, add, keep, depth, max_tokens):
-        return add, keep
+    def _ready(self, add, keep, depth, max_tokens, into=None, of=None):
+        return keep, of
 
-    def _step(self, add, keep):
-        self.calls.append(keep.tolist())
+    def _step(self, keep, of):
+        self.calls.append([k if s == 0 or k < 0 else 0 for k, s in zip(keep.tolist(), of.status.tolist())])
         return "next"
 
 
@@ -57,10 +58,9 @@ def test_a_commit_keeps_nothing_of_a_request_that_was_not_served(ge, ends, want)
 
 
 def test_a_commit_with_a_step_of_other_requests_is_refused(ge):
-    pages = _Pages()
+    pages = ge.paged.PageTable(2, 8, 4, 4, device="cpu")
     with pytest.raises(ValueError, match="3 requests"):
         _chains(ge, (1, 2)).commit(pages, [1, 1], step=NS(status=_i32(0, 0, 0)))
-    assert not pages.calls
 
 
 def test_why_a_request_that_was_not_served_keeps_nothing():
@@ -69,8 +69,11 @@ def test_why_a_request_that_was_not_served_keeps_nothing():
     g.step([20, 32])
     g.step([0, 0], [20, 32])
     assert g.step([16, 0])["status"] == [1, 0]
+    h = copy.deepcopy(g)
     m = g.step([1, 0], [5, 0])
     assert m["status"] == [0, 0] and m["pos"] == [25]  # (20 to 24 were never written)
+    m = h.step([1, 0], [5, 0], laid=[1, 0])
+    assert m["status"] == [0, 0] and m["pos"] == [20]
 
 
 def test_a_refused_commit_moves_nothing(ge):

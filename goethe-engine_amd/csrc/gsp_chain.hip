@@ -293,8 +293,9 @@ __device__ __forceinline__ int chain_draw(const ChainRow &w, const double *sum, 
   return segment_search<PT, QT, VEC, S, HQ>(w, lst, lst == nseg - 1, V, lb, thr, found);
 }
 
-// The same from p alone, nothing summed yet: where p is nowhere above q. One wave over the row twice; only rounding (of p and
-// q to their types, of the product with the coin) leads here.
+// The same from p alone, nothing summed yet: where p is nowhere above q. One wave over the row twice (a row of
+// 128256 fp32 tokens 206 us, of 262144 bf16 112, of 151936 fp64 339; with something left 6.2, 6.6, 7.4): with rows that sum to
+// one only rounding (of p and q to their types, of the product with the coin) leads here.
 template <int PT, int QT, int VEC, int S>
 __device__ __noinline__ int chain_draw_again(const char *p, int nseg, int V, double u) {
   const ChainRow w{p, nullptr, -1};
@@ -406,7 +407,8 @@ hipError_t launch_chains(const RowsWs &w, const gsp_chains &c, hipStream_t s) {
     // Rows that together pass the last-level cache are read around it. Bytes of one row of p and q a request, us a call over
     // inputs in turn / the same input, cached and around: 134 MB (bf16 128 x 262144) 24.4 / 24.2 and 24.4 / 23.6; 233 MB (fp32
     // 192 x 151936) 41.2 / 31.1 and 37.7 / 35.3; 268 MB (bf16 256 x 262144) 44.7 / 37.0 and 40.5 / 37.5; 311 MB (fp32 256) 53.4 /
-    // 44.3 and 48.6 / 46.6; 537 MB (bf16 512) 78.3 / 68.7 and 71.4 / 68.4. Smaller calls lose: 64 fp32 rows 15.0 -> 15.5.
+    // 44.3 and 48.6 / 46.6; 537 MB (bf16 512) 78.3 / 68.7 and 71.4 / 68.4. Smaller calls lose: 64 fp32 rows 15.0 -> 15.5. So do
+    // fp64 rows: 525 MB (256 x 128256) 83.2 / 80.2 and 90.4 / 86.9.
     const bool past = (int64_t)c.requests * c.vocab * (PS + QS) >= (int64_t)256 << 20;
     a.tstride = (int)min((int64_t)w.ticks / per, (int64_t)64);
     for (int64_t r0 = 0; r0 < (int64_t)c.requests; r0 += per) {

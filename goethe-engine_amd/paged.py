@@ -106,7 +106,8 @@ class PageTable:
     def step(self, add, keep=None, depth=None, max_tokens=None, into=None, of=None):
         """One step on the current stream, asynchronously (a graph can capture it): request r's length grows by keep[r]
         tokens that an earlier step added (keep[r] < 0: it ends and gives back its pages, also where its new tokens then
-        do not fit), then add[r] new tokens get pages and slots. Pages are taken in request order; those given back are free from the next step on. depth [max_tokens]:
+        do not fit), then add[r] new tokens get pages and slots. Pages are taken in request order; those given back are free
+        from the next step on. depth [max_tokens]:
         each new token's distance from its request's first (a tree node's depth; default: its index). max_tokens: entries of
         the map (default: the sum of add, which then has to be on the host). into: counters of the same size that receive
         the new state; this table's own then stay as they were (pages taken are the same if the step is made again).

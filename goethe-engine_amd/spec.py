@@ -545,7 +545,9 @@ def verify_chains(target, tokens, begin, coins, u, draft=None, max_drafts=None):
     u [R], or [D + R] (one per target row: the row drawn from says which): numbers in [0, 1) (fp64). Draft x is accepted
     while coin * q(x) < p(x); at the first that is not, the token is drawn with u from max(p - q, 0), after the last one
     from the row that follows. Coin i = uniform(mix(seed, SALT_ACC), nout + i) and u of row i = uniform(mix(seed, SALT_RES),
-    nout + i) make a strict request's decisions (engine.py:278-283).
+    nout + i) make a strict request's decisions at its drafts (engine.py:278-283): which are accepted, and the token in a
+    rejected one's place. The token after the last draft is another draw than engine.py's there, which samples it with
+    the request's own stream in descending order of probability; here every draw goes in vocabulary order.
     max_drafts: the longest chain a request may have (default: from begin, which then has to be on the host)."""
     if max_drafts is None:
         if isinstance(begin, torch.Tensor) and begin.device.type != "cpu":

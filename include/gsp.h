@@ -45,8 +45,9 @@ typedef struct gsp_chains {
   int32_t *emit_tokens;     /* [requests][emit_ld]: columns [0, max_drafts] written, -1 past the emitted tokens */
   float *emit_probs;        /* [requests][emit_ld] the target's weight of each emitted token; 0 past them; or NULL */
   int64_t emit_ld;          /* >= max_drafts + 1 */
-  uint32_t *status;         /* [requests] GSE_WALK_OK, or GSE_WALK_ERROR: the row to draw from holds a NaN or an infinity
-                             * or no positive weight (or sums to an infinity), or begin is not in order (nothing emitted) */
+  uint32_t *status;         /* [requests] GSE_WALK_OK, or GSE_WALK_ERROR: the weights to draw from hold a NaN or an
+                             * infinity or none above zero (or sum to an infinity), or begin is not in order (nothing
+                             * emitted). A rejected one-hot draft's own entry is a weight only where no other is above zero */
   void *stream;
 } gsp_chains;
 
@@ -126,9 +127,11 @@ typedef struct gsp_path {
   void *stream;
 } gsp_path;
 
-/* Verifies every chain in one launch. With a the first draft that is not accepted (its distributions p, q): the token is
- * drawn from max(p - q, 0), one-hot: p without the draft; where that leaves nothing, from p. After n accepted drafts it is
- * drawn from the last row. The draw takes the first token with a positive weight whose inclusive sum in vocabulary order
+/* Verifies every chain, in one launch where the handle's workspace holds the call: up to 4096 requests (or the handle's
+ * rows, if more) whose rows' segment sums fit it (fp64 rows of 128256 tokens through a handle of 64 such rows: 1040
+ * requests); in as many as that takes otherwise. With a the first draft that is not accepted (its distributions p, q): the
+ * token is drawn from max(p - q, 0), one-hot: p without the draft; where that leaves nothing, from p. After n accepted drafts
+ * it is drawn from the last row. The draw takes the first token with a positive weight whose inclusive sum in vocabulary order
  * reaches u times the row's sum (negative weights count as 0). One chain of one draft is gse_mss with a single kid.
  * Replaces: dist + mss per node of a chain, goethe_engine/engine.py:278-283, spec.py:88-103, on rows already computed. */
 GSE_API int gsp_verify_chains(gse_handle *h, const gsp_chains *in);
@@ -138,8 +141,8 @@ GSE_API int gsp_verify_chains(gse_handle *h, const gsp_chains *in);
  * counters_out is counters. Replaces: goethe_engine/kv.py:287-303's commit on the host, for lengths on the device. */
 GSE_API int gsp_pages_step(gse_handle *h, const gsp_pages *pages, const gsp_step *step);
 
-/* Moves the accepted paths, in one launch. Replaces: goethe_engine/engine.py:299-305's commit of each path one request at a
- * time (gc_c.py:302-303, gc_commit of abi/gc.h:212), for a cache whose arrays are the caller's. */
+/* Moves the accepted paths, in one launch for up to 65535 requests. Replaces: goethe_engine/engine.py:299-305's commit of
+ * each path one request at a time (gc_c.py:302-303, gc_commit of abi/gc.h:212), for a cache whose arrays are the caller's. */
 GSE_API int gsp_keep_path(gse_handle *h, const gsp_path *in);
 
 #ifdef __cplusplus

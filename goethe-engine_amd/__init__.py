@@ -12,6 +12,6 @@ works too.
 """
 import sys
 
-from . import _lib, grammar, paged, sampling, spec, workloads  # noqa: F401
+from . import _lib, beam, grammar, kv, paged, sampling, spec, workloads  # noqa: F401
 
 sys.modules.setdefault("goethe_engine_amd", sys.modules[__name__])

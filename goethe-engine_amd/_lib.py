@@ -1,4 +1,4 @@
-"""ctypes binding of libgse.so (include/gse.h, include/gsp.h), in the style of goethe_engine/gc_c.py:58-77 (bind with an ABI
+"""ctypes binding of libgse.so (include/gse.h, gsp.h and gsk.h), in the style of goethe_engine/gc_c.py:58-77 (bind with an ABI
 check, size-first structs) and gc_c.py:222-227 (a negative return code becomes RuntimeError with the library's last error).
 
 torch is imported before the library is loaded so that libgse.so binds to the HIP runtime torch already mapped (both
@@ -12,7 +12,7 @@ from collections import OrderedDict
 import numpy as np
 import torch
 
-ABI_MAJOR, ABI_MINOR = 1, 6
+ABI_MAJOR, ABI_MINOR = 1, 7
 PATH_MAIN, PATH_DEEP, PATH_EXACT = 0, 1, 2  # gse_row_paths codes
 OK, E_ARG, E_DEVICE, E_UNSUPPORTED, E_CAPACITY = 0, -1, -4, -5, -7
 F32, BF16 = 0, 1
@@ -30,6 +30,8 @@ BATCH_SUBBIN_FINISH = 16  # (ABI 1.4, testing)
 MAX_LOGPROBS = 64
 P_F64, P_F32, P_BF16, P_F16 = 0, 1, 2, 3  # types of probability rows (gsp.h)
 STEP_OK, STEP_FULL, STEP_BAD = 0, 1, 2
+K_BF16, K_F16, K_F32, K_E4M3, K_I8 = 0, 1, 2, 3, 4  # types of cached rows (gsk.h)
+MAX_DIM, MAX_TREE, MAX_BEAMS, MAX_KEEP = 256, 64, 32, 64
 P_ = C.POINTER
 
 PATH = os.environ.get("GSE_LIB", os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgse.so"))
@@ -123,6 +125,52 @@ class Path(C.Structure):
                 ("token_stride", C.c_int64), ("chunk_stride", C.c_int64), ("stream", C.c_void_p)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("type", C.c_uint32), ("pages", C.c_uint32), ("page", C.c_uint32), ("heads", C.c_uint32),
+                ("dim", C.c_uint32), ("keys", C.c_void_p), ("values", C.c_void_p), ("page_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("key_scales", C.c_void_p),
+                ("value_scales", C.c_void_p), ("scale_page_stride", C.c_int64), ("scale_token_stride", C.c_int64),
+                ("scale_head_stride", C.c_int64)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("tokens", C.c_uint32), ("type", C.c_uint32), ("reserved", C.c_uint32),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64), ("slot", C.c_void_p), ("stream", C.c_void_p)]
+
+
+class KvRead(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("requests", C.c_uint32), ("rows", C.c_uint32), ("type", C.c_uint32),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_int64),
+                ("max_pages", C.c_uint32), ("reserved", C.c_uint32), ("begin", C.c_void_p), ("first", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+class Attention(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("requests", C.c_uint32), ("tokens", C.c_uint32), ("heads", C.c_uint32),
+                ("type", C.c_uint32), ("max_new", C.c_uint32), ("q", C.c_void_p), ("q_token_stride", C.c_int64),
+                ("q_head_stride", C.c_int64), ("out", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_int64),
+                ("max_pages", C.c_uint32), ("scale", C.c_float), ("begin", C.c_void_p), ("seq_len", C.c_void_p),
+                ("status", C.c_void_p), ("parent", C.c_void_p), ("work", C.c_void_p), ("work_bytes", C.c_int64),
+                ("stream", C.c_void_p)]
+
+
+class Beams(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("requests", C.c_uint32), ("beams", C.c_uint32), ("n", C.c_uint32),
+                ("vocab", C.c_uint32), ("type", C.c_uint32), ("logits", C.c_void_p), ("ld", C.c_int64),
+                ("scores", C.c_void_p), ("tokens", C.c_void_p), ("parents", C.c_void_p), ("out_scores", C.c_void_p),
+                ("work", C.c_void_p), ("work_bytes", C.c_int64), ("stream", C.c_void_p)]
+
+
+class Reorder(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("groups", C.c_uint32), ("beams", C.c_uint32), ("caches", C.c_uint32),
+                ("table", C.c_void_p), ("table_ld", C.c_int64), ("max_pages", C.c_uint32), ("page", C.c_uint32),
+                ("seq_len", C.c_void_p), ("parent", C.c_void_p), ("first", C.c_void_p), ("cache", C.c_void_p),
+                ("cache_stride", C.c_int64), ("cache_ptrs", C.c_void_p), ("align", C.c_uint32), ("pages", C.c_uint32),
+                ("chunks", C.c_uint32), ("chunk_bytes", C.c_uint32), ("page_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("chunk_stride", C.c_int64), ("stream", C.c_void_p)]
+
+
 SIGNATURES = dict(
     gse_abi_version=(C.c_uint32, []),
     gse_open=(C.c_int, [P_(OpenParams), P_(C.c_void_p)]),
@@ -147,10 +195,19 @@ ROUND_SIGNATURES = dict(  # include/gsp.h
     gsp_pages_step=(C.c_int, [C.c_void_p, P_(Pages), P_(Step)]),
     gsp_keep_path=(C.c_int, [C.c_void_p, P_(Path)]),
 )
+KV_SIGNATURES = dict(  # include/gsk.h
+    gsk_write=(C.c_int, [C.c_void_p, P_(KvCache), P_(KvRows)]),
+    gsk_read=(C.c_int, [C.c_void_p, P_(KvCache), P_(KvRead)]),
+    gsk_attention_work=(C.c_int64, [C.c_void_p, P_(KvCache), P_(Attention)]),
+    gsk_attend=(C.c_int, [C.c_void_p, P_(KvCache), P_(Attention)]),
+    gsk_beams_work=(C.c_int64, [C.c_void_p, P_(Beams)]),
+    gsk_beam=(C.c_int, [C.c_void_p, P_(Beams)]),
+    gsk_reorder=(C.c_int, [C.c_void_p, P_(Reorder)]),
+)
 
 
 def bind(path=PATH):
-    """The library at path with its gse.h and gsp.h signatures; refuses a different ABI major or an older minor."""
+    """The library at path with its gse.h, gsp.h and gsk.h signatures; refuses a different ABI major or an older minor."""
     if not os.path.exists(path):
         raise RuntimeError(f"{path} is not built: run __graft_entry__.build() (hipcc --offload-arch=gfx950)")
     L = C.CDLL(path)
@@ -160,7 +217,7 @@ def bind(path=PATH):
     v = L.gse_abi_version()
     if v >> 16 != ABI_MAJOR or (v & 0xFFFF) < ABI_MINOR:
         raise RuntimeError(f"{path}: C ABI {v >> 16}.{v & 0xFFFF}, this module needs {ABI_MAJOR}.{ABI_MINOR}+")
-    for n, (res, args) in ROUND_SIGNATURES.items():
+    for n, (res, args) in (*ROUND_SIGNATURES.items(), *KV_SIGNATURES.items()):
         f = getattr(L, n)
         f.restype, f.argtypes = res, args
     return L

@@ -1,4 +1,4 @@
-// Host side of the C ABI in include/gse.h and include/gsp.h: handle, device workspace, argument checks, launches.
+// Host side of the C ABI in include/gse.h, include/gsp.h and include/gsk.h: handle, device workspace, argument checks, launches.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -11,6 +11,7 @@
 
 #include "gse_dev.h"
 #include "gse_int.h"
+#include "gsk_int.h"
 #include "gsp_int.h"
 
 struct gse_handle {
@@ -724,3 +725,179 @@ GSE_API void gse_close(gse_handle *h) {
 }
 
 }  // extern "C"
+
+// ---- the paged cache's operators and beam search (include/gsk.h) --------------------------------------------------------
+
+namespace {
+
+uint32_t type_bytes(uint32_t t) { return t == GSK_F32 ? 4 : t == GSK_BF16 || t == GSK_F16 ? 2 : 1; }
+
+// A cache description's numbers and, where the call reads it, its arrays.
+int check_cache(gse_handle *h, const gsk_cache &c, bool arrays) {
+  const bool bits8 = c.type == GSK_E4M3 || c.type == GSK_I8;
+  if (!bits8 && c.type != GSK_BF16 && c.type != GSK_F16) return fail(h, GSE_E_ARG, "cache type %u", c.type);
+  if (c.pages == 0 || c.page == 0 || c.heads == 0) return fail(h, GSE_E_ARG, "pages, page and heads must be > 0");
+  if (c.dim == 0 || c.dim % 8 || c.dim > GSK_MAX_DIM)
+    return fail(h, GSE_E_UNSUPPORTED, "dim %u is no multiple of 8 in [8, %d]", c.dim, GSK_MAX_DIM);
+  if ((uint64_t)c.pages * c.page > UINT32_MAX || c.heads > (1u << 16))
+    return fail(h, GSE_E_UNSUPPORTED, "%u pages of %u tokens, %u heads: at most 2^32 - 1 slots and 2^16 heads", c.pages, c.page, c.heads);
+  if (!arrays) return GSE_OK;
+  if (!c.keys || !c.values || (bits8 && (!c.key_scales || !c.value_scales)))
+    return fail(h, GSE_E_ARG, "keys, values and, in 8 bits, their scales are required");
+  if (c.page_stride < 0 || c.token_stride < 0 || c.head_stride < 0 || c.scale_page_stride < 0 || c.scale_token_stride < 0 ||
+      c.scale_head_stride < 0)
+    return fail(h, GSE_E_ARG, "strides must be >= 0");
+  if ((c.page_stride | c.token_stride | c.head_stride) % 8 || ((uint64_t)c.keys | (uint64_t)c.values) % (8 * type_bytes(c.type)))
+    return fail(h, GSE_E_UNSUPPORTED, "the cache's addresses and strides must be multiples of 8 elements");
+  return GSE_OK;
+}
+
+int check_attention(gse_handle *h, const gsk_cache &c, const gsk_attention &a) {
+  if (a.type != GSK_BF16 && a.type != GSK_F16) return fail(h, GSE_E_ARG, "type %u of q", a.type);
+  if (type_bytes(c.type) == 2 && c.type != a.type) return fail(h, GSE_E_ARG, "q of type %u over a cache of type %u", a.type, c.type);
+  if (a.heads == 0 || a.heads % c.heads || a.heads > (1u << 16))
+    return fail(h, GSE_E_ARG, "%u query heads over %u cache heads", a.heads, c.heads);
+  if (a.max_pages == 0) return fail(h, GSE_E_ARG, "max_pages must be > 0");
+  if (a.max_new == 0 && a.tokens > 0) return fail(h, GSE_E_ARG, "max_new must be > 0");
+  if ((uint64_t)a.max_pages * c.page > (uint64_t)INT32_MAX)
+    return fail(h, GSE_E_UNSUPPORTED, "%u pages of %u tokens a request: at most 2^31 - 1 tokens", a.max_pages, c.page);
+  if (a.requests > (1u << 30) || a.tokens > (1u << 30) || a.max_new > (1u << 24))
+    return fail(h, GSE_E_UNSUPPORTED, "%u requests, %u tokens, %u a request: at most 2^30, 2^30 and 2^24", a.requests, a.tokens,
+                a.max_new);
+  if (a.parent && a.max_new > GSK_MAX_TREE)
+    return fail(h, GSE_E_UNSUPPORTED, "trees of %u new tokens: at most %d", a.max_new, GSK_MAX_TREE);
+  return GSE_OK;
+}
+
+int check_beams(gse_handle *h, const gsk_beams &b) {
+  if (b.type > GSK_F32) return fail(h, GSE_E_ARG, "type %u of the logits", b.type);
+  if (b.beams == 0 || b.beams > GSK_MAX_BEAMS || b.n == 0 || b.n > GSK_MAX_KEEP)
+    return fail(h, GSE_E_UNSUPPORTED, "%u beams, %u kept: 1 to %d and 1 to %d", b.beams, b.n, GSK_MAX_BEAMS, GSK_MAX_KEEP);
+  if (b.vocab == 0 || b.vocab > (1u << 30) || b.requests > (1u << 24))
+    return fail(h, GSE_E_UNSUPPORTED, "vocab %u, %u requests: 1 to 2^30 and at most 2^24", b.vocab, b.requests);
+  return GSE_OK;
+}
+
+}  // namespace
+
+GSE_API int gsk_write(gse_handle *h, const gsk_cache *cache, const gsk_rows *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsk_cache c;
+  gsk_rows a;
+  if (!take(cache, c) || !take(in, a)) return fail(h, GSE_E_ARG, "null or short gsk_cache / gsk_rows");
+  if (int rc = check_cache(h, c, true)) return rc;
+  if (a.type > GSK_F32) return fail(h, GSE_E_ARG, "type %u of the rows", a.type);
+  if (a.tokens == 0) return GSE_OK;
+  if (!a.k || !a.v || !a.slot) return fail(h, GSE_E_ARG, "k, v and slot are required");
+  if (a.k_token_stride < 0 || a.k_head_stride < 0 || a.v_token_stride < 0 || a.v_head_stride < 0)
+    return fail(h, GSE_E_ARG, "strides must be >= 0");
+  if ((a.k_token_stride | a.k_head_stride | a.v_token_stride | a.v_head_stride) % 8 || ((uint64_t)a.k | (uint64_t)a.v) % 16)
+    return fail(h, GSE_E_UNSUPPORTED, "the rows' addresses must be multiples of 16 bytes, their strides of 8 elements");
+  if ((uint64_t)a.tokens * c.heads > (1u << 26)) return fail(h, GSE_E_UNSUPPORTED, "%u tokens of %u heads: at most 2^26", a.tokens, c.heads);
+  DeviceGuard g(h->device);
+  hipError_t e = gse::launch_write(c, a, (hipStream_t)a.stream);
+  return e == hipSuccess ? GSE_OK : hip_fail(h, e, "cache write launch");
+}
+
+GSE_API int gsk_read(gse_handle *h, const gsk_cache *cache, const gsk_read_rows *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsk_cache c;
+  gsk_read_rows a;
+  if (!take(cache, c) || !take(in, a)) return fail(h, GSE_E_ARG, "null or short gsk_cache / gsk_read_rows");
+  if (int rc = check_cache(h, c, true)) return rc;
+  if (a.type > GSK_F32) return fail(h, GSE_E_ARG, "type %u of the rows", a.type);
+  if (a.rows == 0 || a.requests == 0) return GSE_OK;
+  if (!a.k || !a.v || !a.table || !a.begin) return fail(h, GSE_E_ARG, "k, v, table and begin are required");
+  if (((uint64_t)a.k | (uint64_t)a.v) % 16) return fail(h, GSE_E_UNSUPPORTED, "the rows' addresses must be multiples of 16 bytes");
+  if (a.max_pages == 0 || a.table_ld < 0) return fail(h, GSE_E_ARG, "max_pages must be > 0, table_ld >= 0");
+  if ((uint64_t)a.max_pages * c.page > (uint64_t)INT32_MAX || a.requests > (1u << 30))
+    return fail(h, GSE_E_UNSUPPORTED, "%u requests, %u pages of %u tokens each: at most 2^30, and 2^31 - 1 tokens", a.requests,
+                a.max_pages, c.page);
+  if ((uint64_t)a.rows * c.heads > (1u << 26)) return fail(h, GSE_E_UNSUPPORTED, "%u rows of %u heads: at most 2^26", a.rows, c.heads);
+  DeviceGuard g(h->device);
+  hipError_t e = gse::launch_read(c, a, (hipStream_t)a.stream);
+  return e == hipSuccess ? GSE_OK : hip_fail(h, e, "cache read launch");
+}
+
+GSE_API int64_t gsk_attention_work(gse_handle *h, const gsk_cache *cache, const gsk_attention *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsk_cache c;
+  gsk_attention a;
+  if (!take(cache, c) || !take(in, a)) return fail(h, GSE_E_ARG, "null or short gsk_cache / gsk_attention");
+  if (int rc = check_cache(h, c, false)) return rc;
+  if (int rc = check_attention(h, c, a)) return rc;
+  if (a.requests == 0 || a.tokens == 0) return 0;
+  return gse::attend_plan(c, a, std::max(h->max_rows, gse::TICKS), (int)h->target).work;
+}
+
+GSE_API int gsk_attend(gse_handle *h, const gsk_cache *cache, const gsk_attention *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsk_cache c;
+  gsk_attention a;
+  if (!take(cache, c) || !take(in, a)) return fail(h, GSE_E_ARG, "null or short gsk_cache / gsk_attention");
+  if (int rc = check_cache(h, c, true)) return rc;
+  if (int rc = check_attention(h, c, a)) return rc;
+  if (a.requests == 0 || a.tokens == 0) return GSE_OK;
+  if (!a.q || !a.out || !a.table || !a.seq_len) return fail(h, GSE_E_ARG, "q, out, table and seq_len are required");
+  if (!a.begin && (a.tokens != a.requests || a.max_new != 1 || a.parent))
+    return fail(h, GSE_E_ARG, "without begin: one new token a request");
+  if (a.q_token_stride < 0 || a.q_head_stride < 0 || a.table_ld < 0) return fail(h, GSE_E_ARG, "strides must be >= 0");
+  if ((a.q_token_stride | a.q_head_stride) % 8 || ((uint64_t)a.q | (uint64_t)a.out) % 16)
+    return fail(h, GSE_E_UNSUPPORTED, "q's and out's addresses must be multiples of 16 bytes, q's strides of 8 elements");
+  const gse::AttendPlan p = gse::attend_plan(c, a, std::max(h->max_rows, gse::TICKS), (int)h->target);
+  if (a.work_bytes < p.work || (p.work > 0 && (!a.work || (uint64_t)a.work % 16)))
+    return fail(h, GSE_E_CAPACITY, "%lld bytes of scratch, %lld are needed", (long long)a.work_bytes, (long long)p.work);
+  DeviceGuard g(h->device);
+  hipError_t e = gse::launch_attend(c, a, p, h->ptick, (hipStream_t)a.stream);
+  return e == hipSuccess ? GSE_OK : hip_fail(h, e, "attention launch");
+}
+
+GSE_API int64_t gsk_beams_work(gse_handle *h, const gsk_beams *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsk_beams b;
+  if (!take(in, b)) return fail(h, GSE_E_ARG, "null or short gsk_beams");
+  if (int rc = check_beams(h, b)) return rc;
+  return gse::beam_work(b);
+}
+
+GSE_API int gsk_beam(gse_handle *h, const gsk_beams *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsk_beams b;
+  if (!take(in, b)) return fail(h, GSE_E_ARG, "null or short gsk_beams");
+  if (int rc = check_beams(h, b)) return rc;
+  if (b.requests == 0) return GSE_OK;
+  if (!b.logits || !b.scores || !b.tokens || !b.parents || !b.out_scores)
+    return fail(h, GSE_E_ARG, "logits, scores, tokens, parents and out_scores are required");
+  if (b.ld < (int64_t)b.vocab) return fail(h, GSE_E_ARG, "ld < vocab");
+  const int64_t need = gse::beam_work(b);
+  if (b.work_bytes < need || !b.work || (uint64_t)b.work % 16)
+    return fail(h, GSE_E_CAPACITY, "%lld bytes of scratch, %lld are needed", (long long)b.work_bytes, (long long)need);
+  DeviceGuard g(h->device);
+  hipError_t e = gse::launch_beam(b, h->ptick, std::max(h->max_rows, gse::TICKS), (hipStream_t)b.stream);
+  return e == hipSuccess ? GSE_OK : hip_fail(h, e, "beam launch");
+}
+
+GSE_API int gsk_reorder(gse_handle *h, const gsk_reorder_beams *in) {
+  if (!h) return fail(nullptr, GSE_E_ARG, "null handle");
+  gsk_reorder_beams p;
+  if (!take(in, p)) return fail(h, GSE_E_ARG, "null or short gsk_reorder_beams");
+  if (p.groups == 0 || p.caches == 0) return GSE_OK;
+  if (!p.table || !p.seq_len || !p.parent || (!p.cache && !p.cache_ptrs))
+    return fail(h, GSE_E_ARG, "table, seq_len, parent and cache or cache_ptrs are required");
+  if (p.beams == 0 || p.beams > GSK_MAX_BEAMS) return fail(h, GSE_E_UNSUPPORTED, "%u beams: 1 to %d", p.beams, GSK_MAX_BEAMS);
+  if (p.page == 0 || p.pages == 0 || p.chunks == 0 || p.chunk_bytes == 0 || p.max_pages == 0)
+    return fail(h, GSE_E_ARG, "page, pages, chunks, chunk_bytes and max_pages must be > 0");
+  if (p.page_stride < 0 || p.token_stride < 0 || p.chunk_stride < 0 || p.table_ld < 0)
+    return fail(h, GSE_E_ARG, "page_stride, token_stride, chunk_stride and table_ld must be >= 0");
+  if (p.cache_ptrs && (p.align == 0 || (p.align & (p.align - 1))))
+    return fail(h, GSE_E_ARG, "align %u is no power of two", p.align);
+  if ((uint64_t)p.chunks * p.chunk_bytes > (1u << 25) || (uint64_t)p.chunks * p.chunk_bytes * p.caches > (1u << 25))
+    return fail(h, GSE_E_UNSUPPORTED, "%u caches of %llu bytes a token: at most 2^25 bytes in all", p.caches,
+                (unsigned long long)p.chunks * p.chunk_bytes);
+  if ((uint64_t)p.pages * p.page > UINT32_MAX || (uint64_t)p.max_pages * p.page > (uint64_t)INT32_MAX || p.groups > (1u << 24))
+    return fail(h, GSE_E_UNSUPPORTED, "%u pages of %u tokens, %u a row, %u groups: at most 2^32 - 1 slots, 2^31 - 1 tokens and 2^24",
+                p.pages, p.page, p.max_pages, p.groups);
+  DeviceGuard g(h->device);
+  hipError_t e = gse::launch_reorder(p, (hipStream_t)p.stream);
+  return e == hipSuccess ? GSE_OK : hip_fail(h, e, "reorder launch");
+}

@@ -1,0 +1,228 @@
+// The paged cache's rows (include/gsk.h): written (gsk_write), read back (gsk_read), moved between beams (gsk_reorder).
+#include "gsk_dev.h"
+#include "gsk_int.h"
+
+namespace gse {
+
+namespace {
+
+// ---- write and read -------------------------------------------------------------------------------------------------------
+// A group of 8, 16 or 32 lanes owns one token's head of the keys or of the values, a lane eight elements of it; in 8 bits the
+// group finds the row's largest magnitude by exchanges within it. Rows with a NaN or an infinity are found with it: as unsigned
+// integers their magnitudes are the largest.
+constexpr int CT = 256;
+
+struct Place {
+  int64_t at, scale;  // element offsets of the row and of its scale
+};
+__device__ __forceinline__ Place place(const gsk_cache &c, uint32_t pg, uint32_t off, uint32_t head) {
+  return {(int64_t)pg * c.page_stride + (int64_t)off * c.token_stride + (int64_t)head * c.head_stride,
+          (int64_t)pg * c.scale_page_stride + (int64_t)off * c.scale_token_stride + (int64_t)head * c.scale_head_stride};
+}
+
+template <uint32_t SRC, uint32_t DST, int GL>
+__global__ __launch_bounds__(CT) void write_kernel(gsk_cache c, gsk_rows a) {
+  const uint32_t id = (blockIdx.x * CT + threadIdx.x) / GL, j = threadIdx.x % GL, t = id / c.heads, h = id - t * c.heads;
+  if (t >= a.tokens) return;
+  const bool values = blockIdx.y != 0, mine = j * 8 < c.dim;
+  const uint64_t slot = (uint64_t)a.slot[t];
+  const char *src = values ? (const char *)a.v + ((int64_t)t * a.v_token_stride + (int64_t)h * a.v_head_stride) * type_size<SRC>
+                           : (const char *)a.k + ((int64_t)t * a.k_token_stride + (int64_t)h * a.k_head_stride) * type_size<SRC>;
+  float x[8] = {};
+  if (mine) to_f32(load_raw8<SRC>(src + j * 8 * type_size<SRC>), x);
+  if (slot >= (uint64_t)c.pages * c.page) return;  // (negative ones are past it; the group as a whole)
+  const uint32_t pg = (uint32_t)slot / c.page;
+  const Place p = place(c, pg, (uint32_t)slot - pg * c.page, h);
+  if constexpr (type_is_8bit<DST>) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+#pragma unroll
+    for (int k = GL / 2; k > 0; k /= 2) m = max(m, shfl_xor_u32(m, k));
+    const bool bad = m >= 0x7F800000u;
+    const float most = DST == GSK_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f;
+    const float scale = fmaxf(__fmul_rn(__uint_as_float(m), most), 0x1p-126f), inv = __fdiv_rn(1.0f, scale);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = bad ? 0.0f : __fmul_rn(x[i], inv);
+    if (j == 0) (values ? c.value_scales : c.key_scales)[p.scale] = bad ? __uint_as_float(0x7FC00000u) : scale;
+  }
+  if (mine) store_raw8<DST>((char *)(values ? c.values : c.keys) + (p.at + j * 8) * type_size<DST>, from_f32<DST>(x));
+}
+
+template <uint32_t SRC, uint32_t DST, int GL>
+__global__ __launch_bounds__(CT) void read_kernel(gsk_cache c, gsk_read_rows a) {
+  const uint32_t id = (blockIdx.x * CT + threadIdx.x) / GL, j = threadIdx.x % GL, row = id / c.heads, h = id - row * c.heads;
+  const uint32_t first_row = __builtin_amdgcn_readfirstlane(row);
+  if (first_row >= a.rows) return;
+  uint32_t r = wave_find(a.begin, a.requests, first_row);
+  if (row >= a.rows || j * 8 >= c.dim) return;
+  while (r + 1 < a.requests && (int64_t)a.begin[r + 1] <= (int64_t)row) ++r;
+  const int64_t b = a.begin[r];
+  if ((int64_t)row < b || (int64_t)row >= (int64_t)a.begin[r + 1]) return;
+  const int64_t t = (a.first ? a.first[r] : 0) + ((int64_t)row - b);
+  const bool values = blockIdx.y != 0;
+  float x[8] = {};
+  if (t >= 0 && t < (int64_t)a.max_pages * c.page) {
+    const uint32_t pi = (uint32_t)t / c.page;
+    const uint32_t pg = (uint32_t)a.table[(int64_t)r * a.table_ld + pi];
+    if (pg < c.pages) {
+      const Place p = place(c, pg, (uint32_t)t - pi * c.page, h);
+      to_f32(load_raw8<SRC>((const char *)(values ? c.values : c.keys) + (p.at + j * 8) * type_size<SRC>), x);
+      if constexpr (type_is_8bit<SRC>) {
+        const float scale = (values ? c.value_scales : c.key_scales)[p.scale];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], scale);
+      }
+    }
+  }
+  store_raw8<DST>((char *)(values ? a.v : a.k) + ((int64_t)id * c.dim + j * 8) * type_size<DST>, from_f32<DST>(x));
+}
+
+// ---- reorder --------------------------------------------------------------------------------------------------------------
+// A thread owns one vector of one token of one cache, in every beam of a group: it loads the vectors of all beams that move
+// before it stores any, so that the beams are permuted in place without a copy; no vector belongs to two threads. A workgroup
+// finds the offsets of TB tokens (a thread a token's beam) and leaves them in LDS, the moving beams of a token one after the
+// other; then its threads walk the (cache, chunk, token, place) of the block: neighbouring tokens of a chunk lie together
+// where the heads come first.
+struct ReorderShared {
+  int64_t src[CT], dst[CT];
+  uint32_t n[CT];
+};
+
+template <typename VEC, int MB>
+__global__ __launch_bounds__(CT) void reorder_kernel(gsk_reorder_beams a, uint32_t vecs) {
+  __shared__ ReorderShared sh;
+  constexpr uint32_t TB = CT / MB;  // tokens of a block
+  const uint32_t g = blockIdx.z, tid = threadIdx.x, beam = tid % MB, tok = tid / MB;
+  const uint32_t row = g * a.beams + beam;
+  const int64_t first = a.first ? a.first[g] : 0;
+  int64_t len = 0;
+  uint32_t from = row;
+  if (beam < a.beams) {
+    const uint32_t p = (uint32_t)a.parent[row];
+    if (p < a.beams) from = g * a.beams + p;
+    len = min(a.seq_len[row], a.seq_len[from]);
+  }
+  const bool moves = from != row && first >= 0;
+  const int64_t most = min((int64_t)wave_max_u64(moves && len > 0 ? (uint64_t)len : 0), (int64_t)a.max_pages * a.page);
+  const uint32_t columns = a.caches * a.chunks * TB * vecs;
+  for (int64_t t0 = first + (int64_t)blockIdx.y * TB; t0 < most; t0 += (int64_t)gridDim.y * TB) {
+    const int64_t t = t0 + tok;
+    uint32_t ps = 0, pd = 0, off = 0;
+    bool go = moves && t < len && t < most;
+    if (go) {
+      const uint32_t pi = (uint32_t)t / a.page;
+      off = (uint32_t)t - pi * a.page;
+      ps = (uint32_t)a.table[(int64_t)from * a.table_ld + pi];
+      pd = (uint32_t)a.table[(int64_t)row * a.table_ld + pi];
+      go = ps < a.pages && pd < a.pages;
+    }
+    const uint64_t all = ballot64(go), mine = MB == 64 ? all : (all >> (lane_id() / MB * MB)) & ((1ull << MB) - 1);
+    __syncthreads();  // (the block before is done)
+    if (go) {
+      const uint32_t k = tok * MB + (uint32_t)__popcll(mine & ((1ull << beam) - 1));
+      sh.src[k] = (int64_t)ps * a.page_stride + (int64_t)off * a.token_stride;
+      sh.dst[k] = (int64_t)pd * a.page_stride + (int64_t)off * a.token_stride;
+    }
+    if (beam == 0) sh.n[tok] = (uint32_t)__popcll(mine);
+    __syncthreads();
+    for (uint32_t id = blockIdx.x * CT + tid; id < columns; id += gridDim.x * CT) {
+      const uint32_t x = id / vecs, place = id - x * vecs, cc = x / TB, to = x - cc * TB, n = sh.n[to];
+      if (n == 0) continue;
+      const uint32_t k = cc / a.chunks;
+      char *base = a.cache_ptrs ? (char *)a.cache_ptrs[k] : (char *)a.cache + k * a.cache_stride;
+      base += (int64_t)(cc - k * a.chunks) * a.chunk_stride + (int64_t)place * sizeof(VEC);
+      VEC v[MB];
+#pragma unroll
+      for (uint32_t e = 0; e < MB; ++e)
+        if (e < n) v[e] = *(const VEC *)(base + sh.src[to * MB + e]);
+#pragma unroll
+      for (uint32_t e = 0; e < MB; ++e)
+        if (e < n) *(VEC *)(base + sh.dst[to * MB + e]) = v[e];
+    }
+  }
+}
+
+template <typename F>
+void by_lanes(uint32_t dim, F f) {
+  if (dim <= 64) f(std::integral_constant<int, 8>{});
+  else if (dim <= 128) f(std::integral_constant<int, 16>{});
+  else f(std::integral_constant<int, 32>{});
+}
+template <typename F>
+void by_type(uint32_t t, F f) {
+  switch (t) {
+    case GSK_BF16: return f(std::integral_constant<uint32_t, GSK_BF16>{});
+    case GSK_F16: return f(std::integral_constant<uint32_t, GSK_F16>{});
+    case GSK_F32: return f(std::integral_constant<uint32_t, GSK_F32>{});
+    case GSK_E4M3: return f(std::integral_constant<uint32_t, GSK_E4M3>{});
+    default: return f(std::integral_constant<uint32_t, GSK_I8>{});
+  }
+}
+
+}  // namespace
+
+hipError_t launch_write(const gsk_cache &c, const gsk_rows &a, hipStream_t s) {
+  by_type(a.type, [&](auto src) {
+    by_type(c.type, [&](auto dst) {
+      if constexpr (!type_is_8bit<src()> && dst() != GSK_F32) {
+        by_lanes(c.dim, [&](auto gl) {
+          const uint64_t threads = (uint64_t)a.tokens * c.heads * gl();
+          hipLaunchKernelGGL((write_kernel<src(), dst(), gl()>), dim3((uint32_t)((threads + CT - 1) / CT), 2), dim3(CT), 0, s, c, a);
+        });
+      }
+    });
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s) {
+  by_type(c.type, [&](auto src) {
+    by_type(a.type, [&](auto dst) {
+      if constexpr (src() != GSK_F32 && !type_is_8bit<dst()>) {
+        by_lanes(c.dim, [&](auto gl) {
+          const uint64_t threads = (uint64_t)a.rows * c.heads * gl();
+          hipLaunchKernelGGL((read_kernel<src(), dst(), gl()>), dim3((uint32_t)((threads + CT - 1) / CT), 2), dim3(CT), 0, s, c, a);
+        });
+      }
+    });
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_reorder(const gsk_reorder_beams &in, hipStream_t s) {
+  constexpr int64_t WGS = 4096;  // workgroups of a launch to aim for
+  auto go = [&](auto v, auto mb) {
+    using V = decltype(v);
+    constexpr int MB = mb();
+    const uint32_t vecs = (uint32_t)(in.chunk_bytes / sizeof(V));
+    const int64_t columns = (int64_t)in.caches * in.chunks * (CT / MB) * vecs;  // (below 2^32)
+    const int64_t blocks = ((int64_t)in.max_pages * in.page + CT / MB - 1) / (CT / MB);
+    for (uint32_t g0 = 0; g0 < in.groups; g0 += 65535) {
+      gsk_reorder_beams a = in;
+      a.groups = min(in.groups - g0, 65535u);
+      a.table += (int64_t)g0 * in.beams * in.table_ld;
+      a.seq_len += (int64_t)g0 * in.beams;
+      a.parent += (int64_t)g0 * in.beams;
+      if (a.first) a.first += g0;
+      const int64_t x = min((columns + CT - 1) / CT, max((int64_t)1, WGS / a.groups));
+      const int64_t y = min(min(blocks, (int64_t)65535), max((int64_t)1, WGS / (a.groups * x)));
+      hipLaunchKernelGGL((reorder_kernel<V, MB>), dim3((uint32_t)x, (uint32_t)y, a.groups), dim3(CT), 0, s, a, vecs);
+    }
+  };
+  auto by_beams = [&](auto v) {
+    if (in.beams <= 4) go(v, std::integral_constant<int, 4>{});
+    else if (in.beams <= 8) go(v, std::integral_constant<int, 8>{});
+    else if (in.beams <= 16) go(v, std::integral_constant<int, 16>{});
+    else go(v, std::integral_constant<int, 32>{});
+  };
+  // the widest vector that every address is a multiple of
+  const uint64_t all = (uint64_t)in.chunk_bytes | (uint64_t)in.page_stride | (uint64_t)in.token_stride | (uint64_t)in.chunk_stride |
+                       (in.cache_ptrs ? (uint64_t)in.align : (uint64_t)in.cache | (uint64_t)in.cache_stride);
+  if (all % 16 == 0) by_beams(uint4{});
+  else if (all % 4 == 0) by_beams(uint32_t{});
+  else by_beams(uint8_t{});
+  return hipGetLastError();
+}
+
+}  // namespace gse

@@ -1,0 +1,280 @@
+"""The keys and values of a paged cache (paged.PageTable keeps its books): written, read back, attended to, and moved between
+beams, on the device and on the current stream (include/gsk.h).
+
+  write    a step's new keys and values to their slots, as they are or in 8 bits with a scale per token and head
+  read     cached tokens as contiguous rows
+  attend   attention of a step's new tokens (one a request, a chain, a draft tree) over the cache
+  reorder  the cached tokens of beams moved to the beams that continue them (beam.select's parents)
+
+A layer of a model's step over the cache, then the round's end:
+
+    step = pages.step(add=nodes, depth=depth, max_tokens=n)
+    kv.write(step.slot, k, v, keys, values, scales=scales)
+    o = kv.attend(q, keys, values, pages.table, step.seq_len, begin=step.begin, status=step.status, parents=parents,
+                  max_new=most, scales=scales)
+    ...
+    step = call.commit(step, pages, caches, ...)          # spec.VerifyCall; 8-bit scales move as caches of their own
+
+keys and values are one layer's: tensors [pages, page, heads, dim] or, heads first, [pages, heads, page, dim], of one shape and
+layout, bfloat16, float16, float8_e4m3fn or int8; dim is a multiple of 8 up to 256. In 8 bits scales is a pair of float32 tensors
+[pages, page, heads] ([pages, heads, page]): an element stands for its value times its token's and head's scale. No call computes
+gradients. Calls on one stream follow one another; none waits for the host, and a graph can capture them (attend once its
+stream's handle is open: after one call on it).
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+from .paged import Caches, _layout
+from .spec import _count, _vec
+
+_TYPES = {torch.bfloat16: _lib.K_BF16, torch.float16: _lib.K_F16, torch.float8_e4m3fn: _lib.K_E4M3, torch.int8: _lib.K_I8}
+_ROWS = {torch.bfloat16: _lib.K_BF16, torch.float16: _lib.K_F16, torch.float32: _lib.K_F32}
+_CACHE, _WRITE, _READ, _ATTEND, _REORDER = (C.sizeof(t) for t in (_lib.KvCache, _lib.KvRows, _lib.KvRead, _lib.Attention,
+                                                                  _lib.Reorder))
+
+
+def _cache(keys, values, scales, heads_first, writes=False):
+    """The cache as the library takes it; what is not in order is refused here."""
+    shape, stride = keys.shape, keys.stride()
+    if keys.dtype not in _TYPES:
+        raise ValueError(f"a cache of {keys.dtype}: bfloat16, float16, float8_e4m3fn or int8 is wanted")
+    if len(shape) != 4 or 0 in shape:
+        raise ValueError(f"a cache of shape {tuple(shape)}: [pages, page, heads, dim] (heads first: [pages, heads, page, dim]) is wanted")
+    if values.shape != shape or values.stride() != stride or values.dtype != keys.dtype or values.device != keys.device:
+        raise ValueError("keys and values must have one shape, layout, type and device")
+    kind, dim, size = _TYPES[keys.dtype], shape[3], keys.element_size()
+    pages, (heads, page) = shape[0], shape[1:3] if heads_first else shape[2:0:-1]
+    ps, (hs, ts) = stride[0], stride[1:3] if heads_first else stride[2:0:-1]
+    if dim % 8 or dim > _lib.MAX_DIM:
+        raise ValueError(f"dim {dim} is no multiple of 8 up to {_lib.MAX_DIM}")
+    k, v = keys.data_ptr(), values.data_ptr()
+    if stride[3] != 1 or (ps | ts | hs) % 8 or (k | v) % (8 * size):
+        raise ValueError("a token's head must lie together, at a multiple of 8 elements")
+    if pages * page >= 1 << 32:
+        raise ValueError(f"{pages} pages of {page} tokens: at most 2^32 - 1 slots")
+    if writes and (k == v or (ps == 0 and pages > 1) or (ts == 0 and page > 1) or (hs == 0 and heads > 1)):
+        raise ValueError("the cache written to must not be expanded, nor be keys and values at once")
+    c = _lib.KvCache(_CACHE, kind, pages, page, heads, dim, k, v, ps, ts, hs)
+    if kind >= _lib.K_E4M3:
+        if scales is None:
+            raise ValueError("an 8-bit cache needs its scales")
+        a, b = scales
+        if a.dtype is not torch.float32 or b.dtype is not torch.float32 or a.shape != shape[:3] or b.shape != shape[:3] \
+                or a.stride() != b.stride():
+            raise ValueError(f"scales must be two float32 tensors of shape {tuple(shape[:3])} and one layout")
+        if a.device != keys.device or b.device != keys.device:
+            raise ValueError(f"scales on {a.device} and {b.device}, the cache on {keys.device}")
+        sp, (sh, st) = a.stride(0), a.stride()[1:] if heads_first else a.stride()[:0:-1]
+        if writes and (a.data_ptr() == b.data_ptr() or (sp == 0 and pages > 1) or (st == 0 and page > 1) or (sh == 0 and heads > 1)):
+            raise ValueError("the scales written to must not be expanded, nor the keys' and the values' at once")
+        c.key_scales, c.value_scales = a.data_ptr(), b.data_ptr()
+        c.scale_page_stride, c.scale_token_stride, c.scale_head_stride = sp, st, sh
+    elif scales is not None:
+        raise ValueError(f"a cache of {keys.dtype} has no scales")
+    return c
+
+
+def _on_device(dev, **tensors):
+    if dev.type != "cuda":
+        raise RuntimeError("goethe-engine_amd needs a HIP device (the cache is on the host)")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} on {t.device}, the cache on {dev}")
+
+
+def _rows(t, name, heads, dim):
+    """[tokens, heads, dim] rows as the kernels read them (rows that do not start at 16 bytes are copied)."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 3 or (heads and t.shape[1] != heads) or t.shape[2] != dim:
+        raise ValueError(f"{name} must be a tensor [tokens, {heads or 'heads'}, {dim}]")
+    s = t.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _table(table):
+    if not isinstance(table, torch.Tensor) or table.dtype is not torch.int32 or table.dim() != 2 or 0 in table.shape:
+        raise ValueError("table must be an int32 tensor [requests, pages]")
+    if table.stride(1) != 1 and table.shape[1] > 1:
+        raise ValueError("table must have unit stride")
+    return table
+
+
+def write(slot, k, v, keys, values, scales=None, heads_first=False):
+    """Writes the rows k, v [tokens, heads, dim] (bfloat16, float16, float32) to the cache slots slot (int64 [tokens], page * tokens
+    per page + offset: paged.StepMap.slot), in place; negative slots and those past the cache are skipped, a slot belongs to one
+    token of the call. In 8 bits, in fp32: scale = max(max |row| * (1 / M), 2^-126), M = 448 (float8_e4m3fn) or 127 (int8), the
+    elements row * (1 / scale) rounded to nearest even; a row with a NaN or an infinity then reads as NaN."""
+    c = _cache(keys, values, scales, heads_first, writes=True)
+    k, v = _rows(k, "k", c.heads, c.dim), _rows(v, "v", c.heads, c.dim)
+    if k.dtype not in _ROWS or v.dtype != k.dtype:
+        raise ValueError(f"k of {k.dtype} and v of {v.dtype}: both bfloat16, float16 or float32 are wanted")
+    n = k.shape[0]
+    if v.shape[0] != n or not isinstance(slot, torch.Tensor) or slot.dtype is not torch.int64 or slot.dim() != 1 or slot.shape[0] != n:
+        raise ValueError("k, v and slot (int64) must have one entry per token")
+    if n * c.heads > 1 << 26:
+        raise ValueError(f"{n} tokens of {c.heads} heads: at most 2^26 in all")
+    dev = keys.device
+    _on_device(dev, slot=slot, k=k, v=v)
+    if n == 0:
+        return
+    slot = slot.contiguous()
+    a = _lib.KvRows(_WRITE, n, _ROWS[k.dtype], 0, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                    slot.data_ptr(), _lib.raw_stream(dev.index))
+    _lib.device_handle(dev.index).call("gsk_write", C.byref(c), C.byref(a))
+
+
+def read(keys, values, table, begin, first=None, max_tokens=None, scales=None, dtype=torch.bfloat16, heads_first=False, out=None):
+    """Cached tokens as rows: (k, v), [max_tokens, heads, dim] of dtype. Rows begin[r] .. begin[r + 1] - 1 are request r's tokens
+    first[r], first[r] + 1, ... (first: 0). table int32 [requests, pages]: each request's pages (PageTable.table). max_tokens:
+    the rows (default: the last of begin, which then has to be on the host). out: the two tensors to write to (contiguous).
+    Rows from begin[requests] on are left as they were (without out: not set); a row whose token or page is out of range is 0."""
+    c = _cache(keys, values, scales, heads_first)
+    r = _table(table).shape[0]
+    if _count(begin) != r + 1 or (first is not None and _count(first) != r):
+        raise ValueError(f"begin must have {r + 1} entries, first {r}")
+    if dtype not in _ROWS:
+        raise ValueError(f"rows of {dtype}: bfloat16, float16 or float32 is wanted")
+    if max_tokens is None:
+        if isinstance(begin, torch.Tensor) and begin.device.type != "cpu":
+            raise ValueError("begin is on the device: max_tokens is required")
+        max_tokens = max(int(begin[r]), 0)
+    n = int(max_tokens)
+    if n < 0 or n * c.heads > 1 << 26:
+        raise ValueError(f"{n} rows of {c.heads} heads: 0 to 2^26 in all")
+    if table.shape[1] * c.page >= 1 << 31:
+        raise ValueError(f"{table.shape[1]} pages of {c.page} tokens a request: at most 2^31 - 1 tokens")
+    dev, shape = keys.device, (n, c.heads, c.dim)
+    if out is not None:
+        for t in out:
+            if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"out must be two contiguous {dtype} tensors of shape {shape}, at multiples of 16 bytes")
+        if n and out[0].data_ptr() == out[1].data_ptr():
+            raise ValueError("out must be two tensors")
+    _on_device(dev, table=table, out=out[0] if out is not None else None)
+    k, v = out if out is not None else (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
+    if n == 0:
+        return k, v
+    begin = _vec(begin, torch.int32, dev)
+    first = _vec(first, torch.int32, dev) if first is not None else None
+    a = _lib.KvRead(_READ, r, n, _ROWS[dtype], k.data_ptr(), v.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], 0,
+                    begin.data_ptr(), first.data_ptr() if first is not None else None, _lib.raw_stream(dev.index))
+    _lib.device_handle(dev.index).call("gsk_read", C.byref(c), C.byref(a))
+    return k, v
+
+
+def attend(q, keys, values, table, seq_len, begin=None, status=None, parents=None, max_new=None, scale=None, scales=None,
+           heads_first=False, out=None):
+    """Attention of a step's new tokens: softmax(scale * q k) v, [tokens, query heads, dim] of q's type. Request r's new tokens are
+    rows begin[r] .. begin[r + 1] - 1 of q (paged.StepMap.begin; without begin: row r alone), the last of its seq_len[r] cached
+    tokens, written to the cache already. Each sees the tokens before its request's new ones, and of those itself and the earlier
+    ones; with parents (int32 [tokens], gse_tree.parent: a node's parent row, -1 an anchor) itself and its ancestors alone.
+
+    q [tokens, query heads, dim], bfloat16 or float16 (the cache's type, where that is not 8 bits); query head h reads the cache's
+    head h // (query heads / heads). table int32 [requests, pages]. max_new: the most new tokens of a request (default: from begin,
+    which then has to be on the host; with parents at most 64), later ones are left out. status: the step's (a request that it did
+    not serve gives zeros). scale: default dim ** -0.5. out: a contiguous tensor to write to. What sees nothing is 0; rows from
+    begin[requests] on are left as they were (without out: not set); numbers out of range give zeros, cached tokens whose page
+    is out of range are not seen."""
+    c = _cache(keys, values, scales, heads_first)
+    q = _rows(q, "q", None, c.dim)
+    n, hq = q.shape[0], q.shape[1]
+    kind = _TYPES.get(q.dtype, _lib.K_F32)
+    if kind > _lib.K_F16 or (c.type <= _lib.K_F16 and c.type != kind):
+        raise ValueError(f"q of {q.dtype} over a cache of {keys.dtype}")
+    if hq == 0 or hq % c.heads:
+        raise ValueError(f"{hq} query heads over {c.heads} heads of the cache")
+    r, width = _table(table).shape
+    if width * c.page >= 1 << 31:
+        raise ValueError(f"{width} pages of {c.page} tokens a request: at most 2^31 - 1 tokens")
+    if _count(seq_len) != r or (begin is not None and _count(begin) != r + 1) or (status is not None and _count(status) != r):
+        raise ValueError(f"seq_len and status must have {r} entries, begin {r + 1}")
+    if begin is None:
+        if n != r or parents is not None or (max_new is not None and int(max_new) != 1):
+            raise ValueError(f"without begin: one new token for each of the {r} requests, got {n}")
+        max_new = 1
+    elif max_new is None:
+        if isinstance(begin, torch.Tensor) and begin.device.type != "cpu":
+            raise ValueError("begin is on the device: max_new is required")
+        b = [int(x) for x in begin]
+        max_new = max([1, *(y - x for x, y in zip(b, b[1:]))])
+    max_new = int(max_new)
+    if not 0 < max_new <= 1 << 24:
+        raise ValueError(f"max_new {max_new} is not in [1, 2^24]")
+    if parents is not None and (_count(parents) < n or max_new > _lib.MAX_TREE):
+        raise ValueError(f"parents must have {n} entries, for trees of at most {_lib.MAX_TREE} new tokens")
+    scale = c.dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale {scale}")
+    dev = keys.device
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous tensor like q, at a multiple of 16 bytes")
+    _on_device(dev, q=q, table=table, out=out)
+    if out is None:
+        out = torch.empty((n, hq, c.dim), dtype=q.dtype, device=dev)
+    if n == 0:
+        return out
+    i32 = torch.int32
+    seq_len = _vec(seq_len, i32, dev)
+    begin = _vec(begin, i32, dev) if begin is not None else None
+    parents = _vec(parents, i32, dev) if parents is not None else None
+    status = _vec(status, i32, dev) if status is not None else None
+    a = _lib.Attention(_ATTEND, r, n, hq, kind, max_new, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), table.data_ptr(),
+                       table.stride(0), width, scale, begin.data_ptr() if begin is not None else None, seq_len.data_ptr(),
+                       status.data_ptr() if status is not None else None, parents.data_ptr() if parents is not None else None,
+                       None, 0, _lib.raw_stream(dev.index))
+    h = _lib.handle(dev.index, 1, 1)
+    pc, pa = C.byref(c), C.byref(a)
+    need = h.call("gsk_attention_work", pc, pa)
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.work, a.work_bytes = work.data_ptr(), need
+    h.call("gsk_attend", pc, pa)
+    return out
+
+
+def reorder(caches, table, seq_len, parents, first=None, heads_first=False):
+    """Moves the cached tokens of beams, in place: with parents int32 [groups, beams], beam b of group g is row g * beams + b of
+    table and seq_len, and gets the tokens first[g] <= t < seq_len of beam parents[g, b] as they were before the call (first: 0;
+    what comes before it, a prompt, is alike in a group's beams). caches: a paged.Caches, or one stacked tensor [n, pages, page,
+    ...] (heads_first: [n, pages, heads, page, ...]), of any type. table int32 [groups * beams, pages] (PageTable.table), a page in
+    one row. At most 32 beams; a parent out of range leaves its beam as it is, and tokens past either beam's length stay."""
+    stacked = not isinstance(caches, Caches)
+    if not stacked:
+        n, layout, dev = len(caches.tensors), caches.layout, caches.device
+    else:
+        if not isinstance(caches, torch.Tensor) or caches.dim() < 4:
+            raise ValueError("caches must be a Caches or a stacked tensor [n, pages, page, ...]")
+        if caches.shape[0] > 1 and caches.stride(0) == 0:
+            raise ValueError("a cache must not be an expanded tensor")
+        n, dev = caches.shape[0], caches.device
+        layout = _layout(caches.shape[1:], caches.stride()[1:], caches.element_size(), heads_first, caches.is_contiguous())
+    if not isinstance(parents, torch.Tensor) or parents.dim() != 2:
+        raise ValueError("parents must be a tensor [groups, beams]")
+    groups, beams = parents.shape
+    if groups == 0 or n == 0:
+        return
+    if not 1 <= beams <= _lib.MAX_BEAMS:
+        raise ValueError(f"{beams} beams: 1 to {_lib.MAX_BEAMS}")
+    if _table(table).shape[0] != groups * beams or _count(seq_len) != groups * beams or (first is not None and _count(first) != groups):
+        raise ValueError(f"table and seq_len must have {groups * beams} rows, first {groups} entries")
+    pages, page, chunks, size, page_stride, token_stride, chunk_stride = layout
+    if n * chunks * size > 1 << 25:
+        raise ValueError(f"{n} caches of {chunks * size} bytes a token: at most 2^25 bytes in all")
+    if table.shape[1] * page >= 1 << 31 or pages * page >= 1 << 32:
+        raise ValueError(f"{table.shape[1]} of {pages} pages of {page} tokens: at most 2^31 - 1 tokens of 2^32 - 1")
+    _on_device(dev, table=table)
+    i32 = torch.int32
+    parents, seq_len = _vec(parents, i32, dev), _vec(seq_len, i32, dev)
+    first = _vec(first, i32, dev) if first is not None else None
+    if stacked:
+        base, stride, ptrs, align = caches.data_ptr(), caches.stride(0) * caches.element_size(), None, 0
+    else:
+        base, stride, ptrs, align = None, 0, caches.ptrs.data_ptr(), caches.align
+    a = _lib.Reorder(_REORDER, groups, beams, n, table.data_ptr(), table.stride(0), table.shape[1], page, seq_len.data_ptr(),
+                     parents.data_ptr(), first.data_ptr() if first is not None else None, base, stride, ptrs, align, pages, chunks,
+                     size, page_stride, token_stride, chunk_stride, _lib.raw_stream(dev.index))
+    _lib.device_handle(dev.index).call("gsk_reorder", C.byref(a))

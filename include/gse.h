@@ -27,7 +27,7 @@ extern "C" {
 #endif
 
 #define GSE_ABI_MAJOR 1
-#define GSE_ABI_MINOR 6
+#define GSE_ABI_MINOR 7
 #define GSE_ABI_VERSION ((GSE_ABI_MAJOR << 16) | GSE_ABI_MINOR)
 
 #if defined(__GNUC__)

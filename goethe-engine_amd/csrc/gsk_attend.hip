@@ -7,7 +7,7 @@ namespace {
 
 int row_tiles(const gsk_cache &c, const gsk_attention &a) {  // MT of the kernel
   const uint64_t rows = (uint64_t)a.max_new * (a.heads / c.heads);
-  return rows <= 16 ? 1 : rows <= 32 || c.dim > 128 ? 2 : 4;
+  return rows <= 16 ? 1 : rows <= 32 || c.dim > 128 ? 2 : 3;
 }
 
 }  // namespace
@@ -37,7 +37,7 @@ hipError_t launch_attend(const gsk_cache &c, const gsk_attention &a, const Atten
   const int mt = row_tiles(c, a);
   p.rows = (uint32_t)min((uint64_t)a.max_new * p.group, (uint64_t)(16 * mt));
   p.tick = tick;
-  const uint64_t units = (uint64_t)p.items * c.heads, blocks = (units + 7) / 8 * 8 * p.tiles;
+  const uint64_t blocks = ((uint64_t)p.items + 7) / 8 * 8 * c.heads * p.tiles;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks);
   const bool half = a.type == GSK_F16;

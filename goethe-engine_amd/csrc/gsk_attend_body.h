@@ -24,6 +24,7 @@ namespace gse {
 
 constexpr int AT = 256, AW = AT / WAVE;
 constexpr uint32_t AB = 64;  // tokens of a block
+constexpr uint32_t PART_MIN = AB * AW;
 
 struct AttendArgs {
   gsk_cache c;
@@ -34,7 +35,7 @@ struct AttendArgs {
 
 template <int KD>
 struct AttendShared {
-  static constexpr int VB = KD / 4, LD = 132;
+  static constexpr int VB = (KD + 3) / 4, LD = 132;
   float o[AW][16][LD];       // a wave's O of 16 rows and 128 elements (padded by a bank row)
   float m[AW][16], l[AW][16];
   int64_t at[AW][AB];        // byte offsets of the block's tokens
@@ -112,7 +113,7 @@ __device__ __forceinline__ float weight_of(float m, float l, float top) {
 }
 
 struct Span {       // a request's rows and cached tokens
-  int64_t begin;    // -1: nothing to write
+  int32_t begin;    // -1: nothing to write
   int32_t n, len;   // new tokens; cached ones, 0 where the request is not served
 };
 __device__ __forceinline__ Span span_of(const gsk_cache &c, const gsk_attention &a, uint32_t r) {
@@ -120,11 +121,11 @@ __device__ __forceinline__ Span span_of(const gsk_cache &c, const gsk_attention 
   const uint32_t st = a.status ? a.status[r] : 0;
   if (b < 0 || e > (int64_t)a.tokens || e <= b) return {-1, 0, 0};
   const bool ok = st == 0 && len >= e - b && len <= (int64_t)a.max_pages * c.page;
-  return {b, (int32_t)(e - b), ok ? (int32_t)len : 0};
+  return {(int32_t)b, (int32_t)(e - b), ok ? (int32_t)len : 0};
 }
 
 template <uint32_t Q, uint32_t C, int KD, int MT>
-__global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
+__global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void attend_kernel(AttendArgs p) {
   using Sh = AttendShared<KD>;
   constexpr uint32_t VT = type_is_8bit<C> ? (uint32_t)GSK_BF16 : Q;  // type of the second product
   constexpr int VB = Sh::VB, SZ = type_size<C>;
@@ -134,15 +135,34 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
   const gsk_attention &a = p.a;
   const uint32_t tid = threadIdx.x, lane = lane_id(), lc = lane % 16, lg = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  // the tiles of an (item, head) run on one XCD (workgroups go round the eight of them)
-  const uint32_t x8 = blockIdx.x / 8, unit = x8 / p.tiles * 8 + blockIdx.x % 8, tile = x8 % p.tiles;
-  if (unit >= p.items * c.heads) return;
-  const uint32_t item = unit / c.heads, head = unit - item * c.heads;
+  // The heads and tiles of an item run on one XCD (workgroups go round the eight of them): a token's heads lie together.
+  const uint32_t x8 = blockIdx.x / 8, each = c.heads * p.tiles, x = x8 % each, item = x8 / each * 8 + blockIdx.x % 8;
+  const uint32_t head = x / p.tiles, tile = x - head * p.tiles;
+  if (item >= p.items) return;
 
   // ---- which request and part this is ------------------------------------------------------------------------------------
+  // Parts are of one size, such that all requests' come to at most `items`: more of them than requests by items - requests.
   uint32_t r = item, part = 0, parts = 1, first_item = item, size = 0x7FFFFFC0u;
-  if (p.items > a.requests) {
-    // parts of one size, so that all requests' come to at most items: more of them than requests by items - requests
+  Span sp;
+  auto part_size_of = [&](int64_t total) {
+    const int64_t extra = p.items - a.requests, need = (total + extra - 1) / extra;
+    return ((uint32_t)max(need, (int64_t)PART_MIN) + AB - 1) / AB * AB;
+  };
+  if (p.items == a.requests) {
+    sp = span_of(c, a, r);
+  } else if (a.requests <= WAVE) {  // every wave for itself, a lane a request
+    const Span mine = span_of(c, a, min(lane, a.requests - 1));
+    size = part_size_of((int64_t)wave_sum_u64(lane < a.requests ? (uint64_t)mine.len : 0));
+    const uint32_t n = lane < a.requests ? max(((uint32_t)mine.len + size - 1) / size, 1u) : 0, inc = wave_incl_scan_u32(n);
+    r = (uint32_t)__popcll(ballot64(lane < a.requests && inc <= item));
+    if (r >= a.requests) return;
+    parts = __builtin_amdgcn_readlane(n, r);
+    first_item = __builtin_amdgcn_readlane(inc, r) - parts;
+    part = item - first_item;
+    sp.begin = __builtin_amdgcn_readlane(mine.begin, r);
+    sp.n = __builtin_amdgcn_readlane(mine.n, r);
+    sp.len = __builtin_amdgcn_readlane(mine.len, r);
+  } else {
     int64_t total = 0;
     for (uint32_t i = tid; i < a.requests; i += AT) total += span_of(c, a, i).len;
     total = (int64_t)wave_sum_u64((uint64_t)total);
@@ -151,9 +171,7 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
     __syncthreads();
     total = 0;
     for (int w = 0; w < AW; ++w) total += sh.red[w];
-    const int64_t extra = p.items - a.requests;
-    size = (uint32_t)max((total + extra - 1) / extra, (int64_t)(AB * AW));
-    size = (size + AB - 1) / AB * AB;
+    size = part_size_of(total);
     uint32_t before = 0;
     for (uint32_t i0 = 0; i0 < a.requests; i0 += AT) {
       const uint32_t i = i0 + tid;
@@ -182,8 +200,8 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
     part = __builtin_amdgcn_readfirstlane(sh.item[1]);
     parts = __builtin_amdgcn_readfirstlane(sh.item[2]);
     first_item = __builtin_amdgcn_readfirstlane(sh.item[3]);
+    sp = span_of(c, a, r);
   }
-  const Span sp = span_of(c, a, r);
   if (sp.begin < 0) return;
   const uint32_t rows = min((uint32_t)sp.n, a.max_new) * p.group, row0 = tile * 16 * MT;
   if (row0 >= rows) return;
@@ -194,28 +212,30 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
   if (k1 - min(k0, k1) > size) k1 = k0 + size;
 
   // ---- the rows -----------------------------------------------------------------------------------------------------------
+  const uint32_t sign = a.scale < 0 ? 0x80008000u : 0;  // (the scale's own, so that the largest score is the largest product)
   Frag<Q> q[MT][KD];
   uint32_t sees[MT];   // chains: the first cached token that the lane's row does not see
   uint64_t path[MT];   // trees: which new tokens it sees
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const uint32_t row = row0 + m * 16 + lc, i = min(row, rows - 1) / p.group, gi = min(row, rows - 1) - i * p.group;
-    const char *at = (const char *)a.q + ((sp.begin + i) * a.q_token_stride + (int64_t)(head * p.group + gi) * a.q_head_stride) * 2;
+    const char *at = (const char *)a.q + ((int64_t)(sp.begin + i) * a.q_token_stride + (int64_t)(head * p.group + gi) * a.q_head_stride) * 2;
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
       uint4 w = {0, 0, 0, 0};
       if (k * 32 + lg * 8 < c.dim) w = *(const uint4 *)(at + (k * 32 + lg * 8) * 2);
+      w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
       q[m][k] = __builtin_bit_cast(Frag<Q>, w);
     }
     sees[m] = ctx + i + 1;
     path[m] = 0;
     if (a.parent) {
-      int64_t at_ = sp.begin + i;
+      int32_t node = sp.begin + (int32_t)i;
       for (;;) {  // (at most 64 steps: an ancestor is an earlier row)
-        path[m] |= 1ull << (at_ - sp.begin);
-        const int64_t up = a.parent[at_];
-        if (up < sp.begin || up >= at_) break;
-        at_ = up;
+        path[m] |= 1ull << (node - sp.begin);
+        const int32_t up = a.parent[node];
+        if (up < sp.begin || up >= node) break;
+        node = up;
       }
     }
   }
@@ -232,70 +252,77 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
   }
 
   // ---- the tokens ---------------------------------------------------------------------------------------------------------
-  const float scale = a.scale * 1.44269504f;
-  const char *keys = (const char *)c.keys + (int64_t)head * c.head_stride * SZ;
-  const char *values = (const char *)c.values + (int64_t)head * c.head_stride * SZ;
+  // The loads of a block are in one straight line, the next tile's keys and the next block's offsets ahead of what is worked on:
+  // a load behind a branch would make every later wait one for all loads. Tokens that do not exist read slot 0 and are masked.
+  const float scale = fabsf(a.scale) * 1.44269504f;
   const int32_t *table = a.table + (int64_t)r * a.table_ld;
-  uint32_t v_at[VB];  // (a lane past dim reads the row's start, into output elements that do not exist)
-#pragma unroll
-  for (int b = 0; b < VB; ++b) v_at[b] = b * 128 + lc * 8 < c.dim ? (b * 128 + lc * 8) * SZ : 0;
-
-  auto page_of = [&](uint32_t t) -> uint32_t { return t < k1 ? (uint32_t)table[t / c.page] : ~0u; };
-  uint64_t there = 0;  // the block's tokens that exist
-  // A block's offsets and scales, from its tokens' pages, to LDS.
-  auto place_block = [&](uint32_t t, uint32_t pg) {
+  const uint32_t pages_on = AW * AB / c.page, tokens_on = AW * AB % c.page;  // from a block of the wave to its next one
+  uint32_t pi = (k0 + wave * AB + lane) / c.page, off = (k0 + wave * AB + lane) % c.page;  // the lane's token of the next block
+  auto next_page = [&] { return (uint32_t)table[min(pi, (k1 - 1) / c.page)]; };
+  uint64_t there;  // the tokens of the block that sh.at has
+  float ks = 0, vs = 0;
+  auto place_block = [&](uint32_t t, uint32_t pg) {  // the offsets of a block to LDS, from its tokens' pages; a lane a token
     const bool ok = t < k1 && pg < c.pages;
     there = ballot64(ok);
-    const uint32_t off = ok ? t % c.page : 0;
+    const uint32_t o = ok ? off : 0;
     if (!ok) pg = 0;
-    sh.at[wave][lane] = ((int64_t)pg * c.page_stride + (int64_t)off * c.token_stride) * SZ;
+    sh.at[wave][lane] = ((int64_t)pg * c.page_stride + (int64_t)o * c.token_stride) * SZ;
     if constexpr (type_is_8bit<C>) {
-      const int64_t s = (int64_t)pg * c.scale_page_stride + (int64_t)off * c.scale_token_stride + (int64_t)head * c.scale_head_stride;
-      sh.ks[wave][lane] = c.key_scales[s];
-      sh.vs[wave][lane] = c.value_scales[s];
+      const int64_t s = (int64_t)pg * c.scale_page_stride + (int64_t)o * c.scale_token_stride + (int64_t)head * c.scale_head_stride;
+      ks = c.key_scales[s];
+      vs = c.value_scales[s];
     }
+    pi += pages_on;
+    off += tokens_on;
+    if (off >= c.page) off -= c.page, ++pi;
     __builtin_amdgcn_wave_barrier();
   };
+  // A lane's part of a row: eight elements at 32k + 8g of a key, at 128b + 8c of a value. Past dim it reads what is there anyway:
+  // keys are zeroed then, values go into output elements that do not exist. WHOLE: the key chunks that are never past it.
+  constexpr int WHOLE = KD == 8 ? 4 : KD >= 3 ? KD - 1 : 0;
+  const char *keys = (const char *)c.keys + ((int64_t)head * c.head_stride + lg * 8) * SZ;
+  const char *values = (const char *)c.values + (int64_t)head * c.head_stride * SZ + (lc * 8 < c.dim ? lc * 8 * SZ : 0);
+  int32_t k_at[KD - WHOLE], v_at = 0;
+#pragma unroll
+  for (int k = WHOLE; k < KD; ++k) k_at[k - WHOLE] = (k * 32 + lg * 8 < c.dim ? k * 32 : -(int)lg * 8) * SZ;
+  if (VB > 1) v_at = (128 + lc * 8 < c.dim ? 128 : -(int)lc * 8) * SZ;
+  const bool whole = c.dim == KD * 32;
   Raw8<C> kr[2][KD];
   auto load_keys = [&](uint32_t half) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const char *row = keys + sh.at[wave][half * 32 + s * 16 + lc];
 #pragma unroll
-      for (int k = 0; k < KD; ++k) {
-        if (k * 32 >= (int)c.dim) continue;
-        const bool in = k * 32 + lg * 8 < c.dim;
-        kr[s][k] = load_raw8<C>(row + (in ? (k * 32 + lg * 8) * SZ : 0));
-        if ((k + 1) * 32 > (int)c.dim && !in) kr[s][k] = Raw8<C>{};
-      }
+      for (int k = 0; k < KD; ++k) kr[s][k] = load_raw8<C>(k < WHOLE ? row + k * 32 * SZ : row + k_at[k < WHOLE ? 0 : k - WHOLE]);
     }
   };
 
   uint32_t t0 = k0 + wave * AB;
   if (t0 < k1) {
-    uint32_t pg = page_of(t0 + lane);
-    place_block(t0 + lane, pg);
+    place_block(t0 + lane, next_page());
     load_keys(0);
     for (; t0 < k1; t0 += AW * AB) {
-      const uint32_t next = t0 + AW * AB;
-      pg = page_of(next + lane < next ? k1 : next + lane);
+      const uint32_t next = t0 + AW * AB, page = next_page();
       const uint64_t now = there;
+      if constexpr (type_is_8bit<C>) {
+        sh.ks[wave][lane] = ks * scale;
+        sh.vs[wave][lane] = vs;
+        __builtin_amdgcn_wave_barrier();
+      }
 #pragma unroll
       for (uint32_t half = 0; half < 2; ++half) {
         const uint32_t t = t0 + half * 32;
-        if (t >= k1) break;
         Raw8<C> vr[VB][8];
-        float kscale[8], vscale[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint32_t k = half * 32 + (j / 4) * 16 + lg * 4 + j % 4;
-          const char *row = values + sh.at[wave][k];
+          const char *row = values + sh.at[wave][half * 32 + (j / 4) * 16 + lg * 4 + j % 4];
 #pragma unroll
-          for (int b = 0; b < VB; ++b) vr[b][j] = load_raw8<C>(row + v_at[b]);
-          if constexpr (type_is_8bit<C>) {
-            kscale[j] = sh.ks[wave][k];
-            vscale[j] = sh.vs[wave][k];
-          }
+          for (int b = 0; b < VB; ++b) vr[b][j] = load_raw8<C>(b ? row + v_at : row);
+        }
+        if (!whole) {  // (what a lane past dim has read)
+#pragma unroll
+          for (int k = WHOLE; k < KD; ++k)
+            if (k_at[k - WHOLE] < 0 || (k == 0 && lg * 8 >= c.dim)) kr[0][k] = kr[1][k] = Raw8<C>{};
         }
         f32x4 s[MT][2];
 #pragma unroll
@@ -304,58 +331,70 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
           for (int m = 0; m < MT; ++m) s[m][u] = f32x4{0, 0, 0, 0};
 #pragma unroll
           for (int k = 0; k < KD; ++k) {
-            if (k * 32 >= (int)c.dim) continue;
             const Frag<Q> kf = operand<C, Q>(kr[u][k]);
 #pragma unroll
             for (int m = 0; m < MT; ++m) s[m][u] = mma<Q>(kf, q[m][k], s[m][u]);
           }
         }
-        // the next tile's keys
-        if (half == 0) {
-          if (t + 32 < k1) load_keys(1);
-        } else if (next < k1) {
-          place_block(next + lane, pg);
-          load_keys(0);
+        if (half == 1) place_block(next + lane, page);
+        load_keys(half ^ 1);
+        f32x4 kscale[2], vscale[2];
+        if constexpr (type_is_8bit<C>) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            kscale[u] = *(const f32x4 *)&sh.ks[wave][half * 32 + u * 16 + lg * 4];
+            vscale[u] = *(const f32x4 *)&sh.vs[wave][half * 32 + u * 16 + lg * 4];
+          }
         }
         const uint32_t real = (uint32_t)(now >> (half * 32));
         const bool masked = real != ~0u || t + 32 > ctx;
-        if (real != ~0u) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1))
-#pragma unroll
-              for (int b = 0; b < VB; ++b) vr[b][j] = Raw8<C>{};
-        }
         Frag<VT> pf[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           float z[8], top = -INF;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            z[j] = s[m][j / 4][j % 4] * scale;
-            if constexpr (type_is_8bit<C>) z[j] *= kscale[j];
+            z[j] = s[m][j / 4][j % 4];
+            if constexpr (type_is_8bit<C>) z[j] *= kscale[j / 4][j % 4];
           }
           if (masked) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const uint32_t k = (j / 4) * 16 + lg * 4 + j % 4, at = t + k;
-              bool see = real >> k & 1;
-              if (at >= ctx) see = see && (a.parent ? (path[m] >> min(at - ctx, 63u) & 1) && at - ctx < 64 : at < sees[m]);
-              if (!see) z[j] = -INF;
+              const uint32_t k = (j / 4) * 16 + lg * 4 + j % 4, at = t + k, d = at - ctx;  // (past ctx: the new token's index)
+              const uint32_t in_new = a.parent ? (uint32_t)(path[m] >> (d & 63)) & (uint32_t)(d < 64) : (uint32_t)(at < sees[m]);
+              const uint32_t see = (real >> k) & ((uint32_t)(at < ctx) | in_new) & 1;
+              z[j] = see ? z[j] : -INF;
             }
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) top = fmaxf(top, z[j]);
-          top = fmaxf(mx[m], over_groups(top, [](float x, float y) { return fmaxf(x, y); }));
-          const float base = top == -INF ? 0.0f : top, f = __builtin_amdgcn_exp2f(mx[m] - base);
-          mx[m] = top;
-          float sum = 0;
+          top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
+          if constexpr (!type_is_8bit<C>) top = top == -INF ? -INF : top * scale;  // (a scale of 0)
+          // The maximum follows once it is 2^8 behind: the weights are up to that, and what it saves is the output's rescaling.
+          if (ballot64(top > mx[m] + 8.0f)) {
+            top = fmaxf(top, mx[m]);
+            const float f = __builtin_amdgcn_exp2f(mx[m] - (top == -INF ? 0.0f : top));
+            mx[m] = top;
+            l[m] *= f;
+#pragma unroll
+            for (int b = 0; b < VB; ++b)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) acc[m][b][e] *= f;
+          }
+          const float base = mx[m] == -INF ? 0.0f : mx[m];
           uint32_t w[4];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            z[j] = __builtin_amdgcn_exp2f(z[j] - base);
-            sum += z[j];
-            if constexpr (type_is_8bit<C>) z[j] *= vscale[j];
+            if constexpr (type_is_8bit<C>) z[j] = __builtin_amdgcn_exp2f(z[j] - base);
+            else z[j] = __builtin_amdgcn_exp2f(z[j] == -INF ? -INF : __builtin_fmaf(z[j], scale, -base));
+            l[m] += z[j];
+            if constexpr (type_is_8bit<C>) z[j] *= vscale[j / 4][j % 4];
+          }
+          if constexpr (type_is_8bit<C>) {
+            if (real != ~0u) {  // (the scale of a token that does not exist is anything)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) z[j] = real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1 ? z[j] : 0.0f;
+            }
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -363,13 +402,13 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
             else w[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)z[2 * j], (__bf16)z[2 * j + 1]});
           }
           pf[m] = __builtin_bit_cast(Frag<VT>, uint4{w[0], w[1], w[2], w[3]});
-          l[m] = l[m] * f + sum;
-          if (ballot64(f != 1.0f)) {
+        }
+        if (real != ~0u) {  // (0 times what does not exist may be NaN)
 #pragma unroll
-            for (int b = 0; b < VB; ++b)
+          for (int j = 0; j < 8; ++j)
+            if (!(real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1))
 #pragma unroll
-              for (int e = 0; e < 8; ++e) acc[m][b][e] *= f;
-          }
+              for (int b = 0; b < VB; ++b) vr[b][j] = Raw8<C>{};
         }
 #pragma unroll
         for (int b = 0; b < VB; ++b) {
@@ -403,7 +442,7 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
     float y[8];
 #pragma unroll
     for (int d = 0; d < 8; ++d) y[d] = sum == 0 ? 0.0f : sum > 0 ? x[d] * inv : x[d] / sum;
-    store_raw8<Q>((char *)a.out + (((sp.begin + i) * a.heads + head * p.group + gi) * (int64_t)c.dim + e) * 2, from_f32<Q>(y));
+    store_raw8<Q>((char *)a.out + (((int64_t)(sp.begin + i) * a.heads + head * p.group + gi) * c.dim + e) * 2, from_f32<Q>(y));
   };
 #pragma unroll 1
   for (int m = 0; m < MT; ++m) {
@@ -466,31 +505,67 @@ __global__ __launch_bounds__(AT) void attend_kernel(AttendArgs p) {
   __syncthreads();
   if (!sh.last) return;
   if (tid == 0) st_ag(tick, 0u);
-  for (uint32_t i = tr; i < min(rows - row0, 16u * MT); i += 16) {
+  // 16 threads a row again; with few rows, several such groups share a row's parts. A thread finds the factors of 16 parts at
+  // a time with its group (a part a thread), then adds its eight elements of them, eight parts' loads at once.
+#pragma unroll 1
+  for (int m = 0; m < MT; ++m) {
+    if (row0 + m * 16 >= rows) break;
+    const uint32_t count = min(rows - row0 - m * 16, 16u), wide = count <= 1 ? 1 : 1u << (32 - __builtin_clz(count - 1));
+    const uint32_t i = m * 16 + tr % wide, share = tr / wide, shares = 16 / wide, j = tid % 16;
+    const bool real = tr % wide < count;
+    const int64_t ml_at = (int64_t)p.rows * c.dim + 2 * i;
     float top = -INF;
-    for (uint32_t s = 0; s < parts; ++s)
-      top = fmaxf(top, __uint_as_float((uint32_t)ld_ag((const uint64_t *)(scratch(first_item + s) + (int64_t)p.rows * c.dim + 2 * i))));
-#pragma unroll
+    if (real)
+      for (uint32_t s = j; s < parts; s += 16) top = fmaxf(top, __uint_as_float((uint32_t)ld_ag((const uint64_t *)(scratch(first_item + s) + ml_at))));
+    for (int k = 8; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, WAVE));
+#pragma unroll 1
     for (int b = 0; b < VB; ++b) {
       const uint32_t e = b * 128 + te;
-      if (e >= c.dim) continue;
+      const bool in = real && e < c.dim;
       float sum = 0, x[8] = {};
-      for (uint32_t s = 0; s < parts; ++s) {
-        const float *o = scratch(first_item + s);
-        const uint64_t ml = ld_ag((const uint64_t *)(o + (int64_t)p.rows * c.dim + 2 * i));
-        uint64_t w[4];
+      for (uint32_t s0 = share * 16; s0 < parts; s0 += 16 * shares) {
+        float f = 0;
+        if (real && s0 + j < parts) {
+          const uint64_t ml = ld_ag((const uint64_t *)(scratch(first_item + s0 + j) + ml_at));
+          const float part_l = __uint_as_float((uint32_t)(ml >> 32));
+          f = weight_of(__uint_as_float((uint32_t)ml), part_l, top);
+          sum += f == 0.0f ? 0.0f : f * part_l;
+        }
 #pragma unroll
-        for (int d = 0; d < 4; ++d) w[d] = ld_ag((const uint64_t *)(o + (int64_t)i * c.dim + e + 2 * d));
-        const float part_l = __uint_as_float((uint32_t)(ml >> 32)), f = weight_of(__uint_as_float((uint32_t)ml), part_l, top);
-        if (f == 0.0f) continue;
-        sum += f * part_l;
+        for (uint32_t k0_ = 0; k0_ < 16; k0_ += 8) {
+          uint64_t w[8][4];
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          x[2 * d] += f * __uint_as_float((uint32_t)w[d]);
-          x[2 * d + 1] += f * __uint_as_float((uint32_t)(w[d] >> 32));
+          for (uint32_t k = 0; k < 8; ++k) {
+            const float *o = scratch(first_item + min(s0 + k0_ + k, parts - 1)) + (int64_t)i * c.dim + e;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) w[k][d] = in ? ld_ag((const uint64_t *)o + d) : 0;
+          }
+#pragma unroll
+          for (uint32_t k = 0; k < 8; ++k) {
+            const float g = __shfl(f, (int)(lane / 16 * 16 + k0_ + k), WAVE);
+            if (g == 0.0f) continue;  // (nothing of this row in the part, or no such part)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              x[2 * d] += g * __uint_as_float((uint32_t)w[k][d]);
+              x[2 * d + 1] += g * __uint_as_float((uint32_t)(w[k][d] >> 32));
+            }
+          }
         }
       }
-      finish(row0 + i, e, x, sum);
+      for (int k = 8; k > 0; k /= 2) sum += __shfl_xor(sum, k, WAVE);
+      if (shares > 1) {
+        __syncthreads();
+        *(f32x4 *)&sh.o[0][tr][te] = f32x4{x[0], x[1], x[2], x[3]};
+        *(f32x4 *)&sh.o[0][tr][te + 4] = f32x4{x[4], x[5], x[6], x[7]};
+        if (j == 0) sh.l[0][tr] = sum;
+        __syncthreads();
+        for (uint32_t k = 1; share == 0 && k < shares; ++k) {
+          sum += sh.l[0][tr + k * wide];
+#pragma unroll
+          for (int d = 0; d < 8; ++d) x[d] += sh.o[0][tr + k * wide][te + d];
+        }
+      }
+      if (in && share == 0) finish(row0 + i, e, x, sum);
     }
   }
 }
@@ -501,9 +576,11 @@ void launch_attend_types(const AttendArgs &p, int mt, dim3 grid, hipStream_t s) 
   auto by = [&](auto kd) {
     if (mt == 1) go(kd, std::integral_constant<int, 1>{});
     else if (mt == 2) go(kd, std::integral_constant<int, 2>{});
-    else if constexpr (kd() == 4) go(kd, std::integral_constant<int, 4>{});
+    else if constexpr (kd() <= 4) go(kd, std::integral_constant<int, 3>{});
   };
-  if (p.c.dim <= 128) by(std::integral_constant<int, 4>{});
+  if (p.c.dim <= 64) by(std::integral_constant<int, 2>{});
+  else if (p.c.dim <= 96) by(std::integral_constant<int, 3>{});
+  else if (p.c.dim <= 128) by(std::integral_constant<int, 4>{});
   else by(std::integral_constant<int, 8>{});
 }
 

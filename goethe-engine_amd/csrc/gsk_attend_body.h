@@ -2,7 +2,7 @@
 //
 // A workgroup takes one part of one request's cached tokens, one head of the cache and one tile of up to 16 MT rows: a row is a
 // (new token, query head of the group), so that every query head that reads a cached row shares its load. Its four waves take
-// blocks of 64 tokens in turn, each with its own running maximum m, sum l and output O of every row (one pass: a tile's scores
+// blocks of 32 tokens in turn, each with its own running maximum m, sum l and output O of every row (one pass: a tile's scores
 // S, m' = max(m, S), p = 2^(S - m'), l = l 2^(m - m') + sum p, O = O 2^(m - m') + p V), joined through LDS at the end; the parts
 // of a request are joined, in their order, by the last workgroup of a (request, head, tile) to end.
 //
@@ -23,8 +23,8 @@
 namespace gse {
 
 constexpr int AT = 256, AW = AT / WAVE;
-constexpr uint32_t AB = 64;  // tokens of a block
-constexpr uint32_t PART_MIN = AB * AW;
+constexpr uint32_t AB = 32;  // tokens of a block
+constexpr uint32_t PART_MIN = 256;  // tokens of a part, at least
 
 struct AttendArgs {
   gsk_cache c;
@@ -39,7 +39,7 @@ struct AttendShared {
   float o[AW][16][LD];       // a wave's O of 16 rows and 128 elements (padded by a bank row)
   float m[AW][16], l[AW][16];
   int64_t at[AW][AB];        // byte offsets of the block's tokens
-  float ks[AW][AB], vs[AW][AB];
+  float scale[AW][2][AB];    // and their keys' and values' scales
   int64_t red[AW];
   uint32_t item[4];          // request, part, parts, first item
   uint32_t last;
@@ -142,11 +142,11 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
 
   // ---- which request and part this is ------------------------------------------------------------------------------------
   // Parts are of one size, such that all requests' come to at most `items`: more of them than requests by items - requests.
-  uint32_t r = item, part = 0, parts = 1, first_item = item, size = 0x7FFFFFC0u;
+  uint32_t r = item, part = 0, parts = 1, first_item = item, size = 0x7FFFFF80u;
   Span sp;
   auto part_size_of = [&](int64_t total) {
     const int64_t extra = p.items - a.requests, need = (total + extra - 1) / extra;
-    return ((uint32_t)max(need, (int64_t)PART_MIN) + AB - 1) / AB * AB;
+    return ((uint32_t)max(need, (int64_t)PART_MIN) + AB * AW - 1) / (AB * AW) * (AB * AW);
   };
   if (p.items == a.requests) {
     sp = span_of(c, a, r);
@@ -216,6 +216,7 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
   Frag<Q> q[MT][KD];
   uint32_t sees[MT];   // chains: the first cached token that the lane's row does not see
   uint64_t path[MT];   // trees: which new tokens it sees
+  const int32_t parent = a.parent ? a.parent[sp.begin + (int32_t)min(lane, (uint32_t)sp.n - 1)] : 0;  // of new token `lane`
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const uint32_t row = row0 + m * 16 + lc, i = min(row, rows - 1) / p.group, gi = min(row, rows - 1) - i * p.group;
@@ -229,13 +230,14 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
     }
     sees[m] = ctx + i + 1;
     path[m] = 0;
-    if (a.parent) {
-      int32_t node = sp.begin + (int32_t)i;
-      for (;;) {  // (at most 64 steps: an ancestor is an earlier row)
-        path[m] |= 1ull << (node - sp.begin);
-        const int32_t up = a.parent[node];
-        if (up < sp.begin || up >= node) break;
-        node = up;
+    if (a.parent) {  // (uniform; at most 64 steps: an ancestor is an earlier row)
+      uint32_t node = i;
+      bool on = true;
+      while (ballot64(on)) {
+        if (on) path[m] |= 1ull << node;
+        const int32_t up = __shfl(parent, (int)node, WAVE) - sp.begin;
+        on = on && up >= 0 && (uint32_t)up < node;
+        if (on) node = (uint32_t)up;
       }
     }
   }
@@ -252,26 +254,27 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
   }
 
   // ---- the tokens ---------------------------------------------------------------------------------------------------------
-  // The loads of a block are in one straight line, the next tile's keys and the next block's offsets ahead of what is worked on:
-  // a load behind a branch would make every later wait one for all loads. Tokens that do not exist read slot 0 and are masked.
+  // The loads of a block are in one straight line, the next block's keys and the offsets of the one after ahead of what is worked
+  // on: a load behind a branch would make every later wait one for all loads. Tokens that do not exist read slot 0 and are
+  // masked. Lanes l and l + 32 find the same token.
   const float scale = fabsf(a.scale) * 1.44269504f;
   const int32_t *table = a.table + (int64_t)r * a.table_ld;
   const uint32_t pages_on = AW * AB / c.page, tokens_on = AW * AB % c.page;  // from a block of the wave to its next one
-  uint32_t pi = (k0 + wave * AB + lane) / c.page, off = (k0 + wave * AB + lane) % c.page;  // the lane's token of the next block
-  auto next_page = [&] { return (uint32_t)table[min(pi, (k1 - 1) / c.page)]; };
-  uint64_t there;  // the tokens of the block that sh.at has
-  float ks = 0, vs = 0;
-  auto place_block = [&](uint32_t t, uint32_t pg) {  // the offsets of a block to LDS, from its tokens' pages; a lane a token
+  const uint32_t l32 = lane % 32;
+  uint32_t pi = (k0 + wave * AB + l32) / c.page, off = (k0 + wave * AB + l32) % c.page;  // the lane's token of the next block
+  const uint32_t last_page = (max(k1, 1u) - 1) / c.page;
+  auto next_page = [&] { return (uint32_t)table[min(pi, last_page)]; };
+  uint32_t there = 0;  // the tokens of the block that sh.at has
+  float scale_of = 0;  // 8 bits: the token's, of its key in the lower lanes and of its value in the upper ones
+  const float *scales = lane < 32 ? c.key_scales : c.value_scales;
+  auto place_block = [&](uint32_t t, uint32_t pg) {  // the offsets of a block to LDS, from its tokens' pages
     const bool ok = t < k1 && pg < c.pages;
-    there = ballot64(ok);
+    there = (uint32_t)ballot64(ok);
     const uint32_t o = ok ? off : 0;
     if (!ok) pg = 0;
-    sh.at[wave][lane] = ((int64_t)pg * c.page_stride + (int64_t)o * c.token_stride) * SZ;
-    if constexpr (type_is_8bit<C>) {
-      const int64_t s = (int64_t)pg * c.scale_page_stride + (int64_t)o * c.scale_token_stride + (int64_t)head * c.scale_head_stride;
-      ks = c.key_scales[s];
-      vs = c.value_scales[s];
-    }
+    sh.at[wave][l32] = ((int64_t)pg * c.page_stride + (int64_t)o * c.token_stride) * SZ;
+    if constexpr (type_is_8bit<C>)
+      scale_of = scales[(int64_t)pg * c.scale_page_stride + (int64_t)o * c.scale_token_stride + (int64_t)head * c.scale_head_stride];
     pi += pages_on;
     off += tokens_on;
     if (off >= c.page) off -= c.page, ++pi;
@@ -288,144 +291,134 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
   if (VB > 1) v_at = (128 + lc * 8 < c.dim ? 128 : -(int)lc * 8) * SZ;
   const bool whole = c.dim == KD * 32;
   Raw8<C> kr[2][KD];
-  auto load_keys = [&](uint32_t half) {
+  auto load_keys = [&] {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const char *row = keys + sh.at[wave][half * 32 + s * 16 + lc];
+      const char *row = keys + sh.at[wave][s * 16 + lc];
 #pragma unroll
       for (int k = 0; k < KD; ++k) kr[s][k] = load_raw8<C>(k < WHOLE ? row + k * 32 * SZ : row + k_at[k < WHOLE ? 0 : k - WHOLE]);
     }
   };
 
-  uint32_t t0 = k0 + wave * AB;
-  if (t0 < k1) {
-    place_block(t0 + lane, next_page());
-    load_keys(0);
-    for (; t0 < k1; t0 += AW * AB) {
-      const uint32_t next = t0 + AW * AB, page = next_page();
-      const uint64_t now = there;
-      if constexpr (type_is_8bit<C>) {
-        sh.ks[wave][lane] = ks * scale;
-        sh.vs[wave][lane] = vs;
-        __builtin_amdgcn_wave_barrier();
+  uint32_t t = k0 + wave * AB;
+  if (t < k1) {
+    place_block(t + l32, next_page());
+    load_keys();
+    for (; t < k1; t += AW * AB) {
+      const uint32_t page = next_page(), real = there;
+      if constexpr (type_is_8bit<C>) sh.scale[wave][lane / 32][l32] = lane < 32 ? scale_of * scale : scale_of;
+      Raw8<C> vr[VB][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const char *row = values + sh.at[wave][(j / 4) * 16 + lg * 4 + j % 4];
+#pragma unroll
+        for (int b = 0; b < VB; ++b) vr[b][j] = load_raw8<C>(b ? row + v_at : row);
       }
+      if (!whole) {  // (what a lane past dim has read)
 #pragma unroll
-      for (uint32_t half = 0; half < 2; ++half) {
-        const uint32_t t = t0 + half * 32;
-        Raw8<C> vr[VB][8];
+        for (int k = WHOLE; k < KD; ++k)
+          if (k_at[k - WHOLE] < 0 || (k == 0 && lg * 8 >= c.dim)) kr[0][k] = kr[1][k] = Raw8<C>{};
+      }
+      f32x4 s[MT][2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const char *row = values + sh.at[wave][half * 32 + (j / 4) * 16 + lg * 4 + j % 4];
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int b = 0; b < VB; ++b) vr[b][j] = load_raw8<C>(b ? row + v_at : row);
+        for (int m = 0; m < MT; ++m) s[m][u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < KD; ++k) {
+          const Frag<Q> kf = operand<C, Q>(kr[u][k]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) s[m][u] = mma<Q>(kf, q[m][k], s[m][u]);
         }
-        if (!whole) {  // (what a lane past dim has read)
-#pragma unroll
-          for (int k = WHOLE; k < KD; ++k)
-            if (k_at[k - WHOLE] < 0 || (k == 0 && lg * 8 >= c.dim)) kr[0][k] = kr[1][k] = Raw8<C>{};
-        }
-        f32x4 s[MT][2];
+      }
+      place_block(t + AW * AB + l32, page);
+      load_keys();
+      f32x4 kscale[2], vscale[2];
+      if constexpr (type_is_8bit<C>) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+          kscale[u] = *(const f32x4 *)&sh.scale[wave][0][u * 16 + lg * 4];
+          vscale[u] = *(const f32x4 *)&sh.scale[wave][1][u * 16 + lg * 4];
+        }
+      }
+      const bool masked = real != ~0u || t + 32 > ctx;
+      Frag<VT> pf[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) s[m][u] = f32x4{0, 0, 0, 0};
+      for (int m = 0; m < MT; ++m) {
+        float z[8], top = -INF;
 #pragma unroll
-          for (int k = 0; k < KD; ++k) {
-            const Frag<Q> kf = operand<C, Q>(kr[u][k]);
+        for (int j = 0; j < 8; ++j) {
+          z[j] = s[m][j / 4][j % 4];
+          if constexpr (type_is_8bit<C>) z[j] *= kscale[j / 4][j % 4];
+        }
+        if (masked) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) s[m][u] = mma<Q>(kf, q[m][k], s[m][u]);
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t k = (j / 4) * 16 + lg * 4 + j % 4, at = t + k, d = at - ctx;  // (past ctx: the new token's index)
+            const uint32_t in_new = a.parent ? (uint32_t)(path[m] >> (d & 63)) & (uint32_t)(d < 64) : (uint32_t)(at < sees[m]);
+            const uint32_t see = (real >> k) & ((uint32_t)(at < ctx) | in_new) & 1;
+            z[j] = see ? z[j] : -INF;
           }
         }
-        if (half == 1) place_block(next + lane, page);
-        load_keys(half ^ 1);
-        f32x4 kscale[2], vscale[2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, z[j]);
+        top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
+        if constexpr (!type_is_8bit<C>) top = top == -INF ? -INF : top * scale;  // (a scale of 0)
+        // The maximum follows once it is 2^8 behind: the weights are up to that, and what it saves is the output's rescaling.
+        if (ballot64(top > mx[m] + 8.0f)) {
+          top = fmaxf(top, mx[m]);
+          const float f = __builtin_amdgcn_exp2f(mx[m] - (top == -INF ? 0.0f : top));
+          mx[m] = top;
+          l[m] *= f;
+#pragma unroll
+          for (int b = 0; b < VB; ++b)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[m][b][e] *= f;
+        }
+        const float base = mx[m] == -INF ? 0.0f : mx[m];
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (type_is_8bit<C>) z[j] = __builtin_amdgcn_exp2f(z[j] - base);
+          else z[j] = __builtin_amdgcn_exp2f(z[j] == -INF ? -INF : __builtin_fmaf(z[j], scale, -base));
+          l[m] += z[j];
+          if constexpr (type_is_8bit<C>) z[j] *= vscale[j / 4][j % 4];
+        }
         if constexpr (type_is_8bit<C>) {
+          if (real != ~0u) {  // (the scale of a token that does not exist is anything)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            kscale[u] = *(const f32x4 *)&sh.ks[wave][half * 32 + u * 16 + lg * 4];
-            vscale[u] = *(const f32x4 *)&sh.vs[wave][half * 32 + u * 16 + lg * 4];
+            for (int j = 0; j < 8; ++j) z[j] = real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1 ? z[j] : 0.0f;
           }
         }
-        const uint32_t real = (uint32_t)(now >> (half * 32));
-        const bool masked = real != ~0u || t + 32 > ctx;
-        Frag<VT> pf[MT];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          float z[8], top = -INF;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            z[j] = s[m][j / 4][j % 4];
-            if constexpr (type_is_8bit<C>) z[j] *= kscale[j / 4][j % 4];
-          }
-          if (masked) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t k = (j / 4) * 16 + lg * 4 + j % 4, at = t + k, d = at - ctx;  // (past ctx: the new token's index)
-              const uint32_t in_new = a.parent ? (uint32_t)(path[m] >> (d & 63)) & (uint32_t)(d < 64) : (uint32_t)(at < sees[m]);
-              const uint32_t see = (real >> k) & ((uint32_t)(at < ctx) | in_new) & 1;
-              z[j] = see ? z[j] : -INF;
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = fmaxf(top, z[j]);
-          top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
-          if constexpr (!type_is_8bit<C>) top = top == -INF ? -INF : top * scale;  // (a scale of 0)
-          // The maximum follows once it is 2^8 behind: the weights are up to that, and what it saves is the output's rescaling.
-          if (ballot64(top > mx[m] + 8.0f)) {
-            top = fmaxf(top, mx[m]);
-            const float f = __builtin_amdgcn_exp2f(mx[m] - (top == -INF ? 0.0f : top));
-            mx[m] = top;
-            l[m] *= f;
-#pragma unroll
-            for (int b = 0; b < VB; ++b)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) acc[m][b][e] *= f;
-          }
-          const float base = mx[m] == -INF ? 0.0f : mx[m];
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if constexpr (type_is_8bit<C>) z[j] = __builtin_amdgcn_exp2f(z[j] - base);
-            else z[j] = __builtin_amdgcn_exp2f(z[j] == -INF ? -INF : __builtin_fmaf(z[j], scale, -base));
-            l[m] += z[j];
-            if constexpr (type_is_8bit<C>) z[j] *= vscale[j / 4][j % 4];
-          }
-          if constexpr (type_is_8bit<C>) {
-            if (real != ~0u) {  // (the scale of a token that does not exist is anything)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) z[j] = real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1 ? z[j] : 0.0f;
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (VT == GSK_F16) w[j] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)z[2 * j], (_Float16)z[2 * j + 1]});
-            else w[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)z[2 * j], (__bf16)z[2 * j + 1]});
-          }
-          pf[m] = __builtin_bit_cast(Frag<VT>, uint4{w[0], w[1], w[2], w[3]});
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (VT == GSK_F16) w[j] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)z[2 * j], (_Float16)z[2 * j + 1]});
+          else w[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)z[2 * j], (__bf16)z[2 * j + 1]});
         }
-        if (real != ~0u) {  // (0 times what does not exist may be NaN)
+        pf[m] = __builtin_bit_cast(Frag<VT>, uint4{w[0], w[1], w[2], w[3]});
+      }
+      if (real != ~0u) {  // (0 times what does not exist may be NaN)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1))
+        for (int j = 0; j < 8; ++j)
+          if (!(real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1))
 #pragma unroll
-              for (int b = 0; b < VB; ++b) vr[b][j] = Raw8<C>{};
-        }
+            for (int b = 0; b < VB; ++b) vr[b][j] = Raw8<C>{};
+      }
 #pragma unroll
-        for (int b = 0; b < VB; ++b) {
-          auto step = [&]<int E>(std::integral_constant<int, E>) {
-            const Frag<VT> vf = turned<C, VT, E>(vr[b]);
+      for (int b = 0; b < VB; ++b) {
+        auto step = [&]<int E>(std::integral_constant<int, E>) {
+          const Frag<VT> vf = turned<C, VT, E>(vr[b]);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][b][E] = mma<VT>(vf, pf[m], acc[m][b][E]);
-          };
-          step(std::integral_constant<int, 0>{});
-          step(std::integral_constant<int, 1>{});
-          step(std::integral_constant<int, 2>{});
-          step(std::integral_constant<int, 3>{});
-          step(std::integral_constant<int, 4>{});
-          step(std::integral_constant<int, 5>{});
-          step(std::integral_constant<int, 6>{});
-          step(std::integral_constant<int, 7>{});
-        }
+          for (int m = 0; m < MT; ++m) acc[m][b][E] = mma<VT>(vf, pf[m], acc[m][b][E]);
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
+        step(std::integral_constant<int, 4>{});
+        step(std::integral_constant<int, 5>{});
+        step(std::integral_constant<int, 6>{});
+        step(std::integral_constant<int, 7>{});
       }
     }
   }

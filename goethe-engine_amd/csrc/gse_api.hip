@@ -827,7 +827,7 @@ GSE_API int64_t gsk_attention_work(gse_handle *h, const gsk_cache *cache, const 
   if (int rc = check_cache(h, c, false)) return rc;
   if (int rc = check_attention(h, c, a)) return rc;
   if (a.requests == 0 || a.tokens == 0) return 0;
-  return gse::attend_plan(c, a, std::max(h->max_rows, gse::TICKS), (int)h->target).work;
+  return gse::attend_plan(c, a, std::max(h->max_rows, gse::TICKS), (int)h->target / 4).work;
 }
 
 GSE_API int gsk_attend(gse_handle *h, const gsk_cache *cache, const gsk_attention *in) {
@@ -844,7 +844,7 @@ GSE_API int gsk_attend(gse_handle *h, const gsk_cache *cache, const gsk_attentio
   if (a.q_token_stride < 0 || a.q_head_stride < 0 || a.table_ld < 0) return fail(h, GSE_E_ARG, "strides must be >= 0");
   if ((a.q_token_stride | a.q_head_stride) % 8 || ((uint64_t)a.q | (uint64_t)a.out) % 16)
     return fail(h, GSE_E_UNSUPPORTED, "q's and out's addresses must be multiples of 16 bytes, q's strides of 8 elements");
-  const gse::AttendPlan p = gse::attend_plan(c, a, std::max(h->max_rows, gse::TICKS), (int)h->target);
+  const gse::AttendPlan p = gse::attend_plan(c, a, std::max(h->max_rows, gse::TICKS), (int)h->target / 4);
   if (a.work_bytes < p.work || (p.work > 0 && (!a.work || (uint64_t)a.work % 16)))
     return fail(h, GSE_E_CAPACITY, "%lld bytes of scratch, %lld are needed", (long long)a.work_bytes, (long long)p.work);
   DeviceGuard g(h->device);

@@ -12,18 +12,16 @@ int row_tiles(const gsk_cache &c, const gsk_attention &a) {  // MT of the kernel
 
 }  // namespace
 
-AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tickets, int round) {
+AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tickets, int cus) {
   const uint64_t rows = (uint64_t)a.max_new * (a.heads / c.heads), most = 16 * row_tiles(c, a);
   AttendPlan p;
   p.tiles = (uint32_t)((rows + most - 1) / most);
-  p.items = a.requests;
-  p.work = 0;
-  const uint64_t units = (uint64_t)a.requests * c.heads * p.tiles;
-  // A join takes a ticket per (request, head, tile).
-  if (units <= tickets && a.max_pages * (uint64_t)c.page > AB * AW) {
-    p.items += (uint32_t)((round + c.heads * p.tiles - 1) / (c.heads * p.tiles));
-    p.work = (int64_t)p.items * c.heads * p.tiles * (int64_t)min(rows, most) * (c.dim + 2) * sizeof(float);
-  }
+  // One round of workgroups, if the requests' longest tables fill it.
+  const uint64_t each = (uint64_t)c.heads * p.tiles;
+  const uint64_t round = (uint64_t)cus * attend_resident(c.dim <= 128 ? 4 : 8, row_tiles(c, a)) / each;
+  const uint64_t blocks = (uint64_t)a.requests * (((uint64_t)a.max_pages * c.page + AB - 1) / AB);
+  p.items = (uint32_t)max(min(min(round, (uint64_t)tickets / each), (blocks + SHARE_MIN - 1) / SHARE_MIN), (uint64_t)1);
+  p.work = p.items == 1 ? 0 : (int64_t)(p.items * 2 * each * min(rows, most) * (c.dim + 2) * sizeof(float));
   return p;
 }
 

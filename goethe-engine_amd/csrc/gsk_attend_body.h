@@ -1,10 +1,12 @@
 // The attention kernel of gsk_attend (gsk_attend.hip has the plan and the launches; one source per cache type instantiates it).
 //
-// A workgroup takes one part of one request's cached tokens, one head of the cache and one tile of up to 16 MT rows: a row is a
-// (new token, query head of the group), so that every query head that reads a cached row shares its load. Its four waves take
-// blocks of 32 tokens in turn, each with its own running maximum m, sum l and output O of every row (one pass: a tile's scores
-// S, m' = max(m, S), p = 2^(S - m'), l = l 2^(m - m') + sum p, O = O 2^(m - m') + p V), joined through LDS at the end; the parts
-// of a request are joined, in their order, by the last workgroup of a (request, head, tile) to end.
+// The cached tokens of all requests, one after the other, are cut into equal shares of whole blocks, as many as workgroups run at
+// once (at most p.items): a workgroup takes one share, one head of the cache and one tile of up to 16 MT rows, and works on the
+// requests (or parts of them) in its share in turn. A row is a (new token, query head of the group), so that every query head
+// that reads a cached row shares its load. The four waves take blocks of 32 tokens in turn, each with its own running maximum m,
+// sum l and output O of every row (one pass: a block's scores S, m' = max(m, S), p = 2^(S - m'), l = l 2^(m - m') + sum p, O =
+// O 2^(m - m') + p V), joined through LDS at the end; the parts of a request are joined, in their order, by the last workgroup
+// of a (request, head, tile) to end.
 //
 // Both products are 16x16x32 matrix instructions. S^T = K Q^T: a lane (c, g) = (lane % 16, lane / 16) holds eight elements of
 // token c and of row c, and gets the scores of row c for tokens 4g .. 4g + 3 of each 16; O^T = V^T P^T over 32 tokens then takes
@@ -24,26 +26,29 @@ namespace gse {
 
 constexpr int AT = 256, AW = AT / WAVE;
 constexpr uint32_t AB = 32;  // tokens of a block
-constexpr uint32_t PART_MIN = 256;  // tokens of a part, at least
+constexpr uint32_t SHARE_MIN = 8;   // blocks of a share, at least
 
 struct AttendArgs {
   gsk_cache c;
   gsk_attention a;
-  uint32_t items, tiles, group, rows;  // rows: of a tile's scratch
+  uint32_t items, tiles, group, rows;  // shares; tiles of a request's rows; query heads of a head; rows of a tile's scratch
   uint32_t *tick;
 };
 
-template <int KD>
+template <int KD, int MT>
 struct AttendShared {
   static constexpr int VB = (KD + 3) / 4, LD = 132;
+  static constexpr bool QL = MT > 1;  // the rows' operands are read from LDS (registers have no room)
   float o[AW][16][LD];       // a wave's O of 16 rows and 128 elements (padded by a bank row)
   float m[AW][16], l[AW][16];
   int64_t at[AW][AB];        // byte offsets of the block's tokens
   float scale[AW][2][AB];    // and their keys' and values' scales
-  int64_t red[AW];
-  uint32_t item[4];          // request, part, parts, first item
+  uint4 q[QL ? MT : 1][QL ? 16 : 1][QL ? KD * 4 + 1 : 1];
   uint32_t last;
 };
+
+// Workgroups of a CU at once (what their registers allow).
+constexpr int attend_resident(int kd, int mt) { return kd > 4 ? 1 : mt == 1 ? 3 : 2; }
 
 template <uint32_t T>
 using Frag = std::conditional_t<T == GSK_F16, f16x8, bf16x8>;
@@ -125,8 +130,8 @@ __device__ __forceinline__ Span span_of(const gsk_cache &c, const gsk_attention 
 }
 
 template <uint32_t Q, uint32_t C, int KD, int MT>
-__global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void attend_kernel(AttendArgs p) {
-  using Sh = AttendShared<KD>;
+__global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(AttendArgs p) {
+  using Sh = AttendShared<KD, MT>;
   constexpr uint32_t VT = type_is_8bit<C> ? (uint32_t)GSK_BF16 : Q;  // type of the second product
   constexpr int VB = Sh::VB, SZ = type_size<C>;
   constexpr float INF = INFINITY;
@@ -140,80 +145,86 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
   const uint32_t head = x / p.tiles, tile = x - head * p.tiles;
   if (item >= p.items) return;
 
-  // ---- which request and part this is ------------------------------------------------------------------------------------
-  // Parts are of one size, such that all requests' come to at most `items`: more of them than requests by items - requests.
-  uint32_t r = item, part = 0, parts = 1, first_item = item, size = 0x7FFFFF80u;
-  Span sp;
-  auto part_size_of = [&](int64_t total) {
-    const int64_t extra = p.items - a.requests, need = (total + extra - 1) / extra;
-    return ((uint32_t)max(need, (int64_t)PART_MIN) + AB * AW - 1) / (AB * AW) * (AB * AW);
+  // ---- the share ----------------------------------------------------------------------------------------------------------
+  // Every wave for itself, a lane four requests at a time: a request's blocks, one at least if it has rows to write.
+  auto blocks_of = [&](uint32_t i) -> uint32_t {
+    const Span x = span_of(c, a, min(i, a.requests - 1));
+    return i < a.requests && x.begin >= 0 ? max(((uint32_t)x.len + AB - 1) / AB, 1u) : 0u;
   };
-  if (p.items == a.requests) {
-    sp = span_of(c, a, r);
-  } else if (a.requests <= WAVE) {  // every wave for itself, a lane a request
-    const Span mine = span_of(c, a, min(lane, a.requests - 1));
-    size = part_size_of((int64_t)wave_sum_u64(lane < a.requests ? (uint64_t)mine.len : 0));
-    const uint32_t n = lane < a.requests ? max(((uint32_t)mine.len + size - 1) / size, 1u) : 0, inc = wave_incl_scan_u32(n);
-    r = (uint32_t)__popcll(ballot64(lane < a.requests && inc <= item));
-    if (r >= a.requests) return;
-    parts = __builtin_amdgcn_readlane(n, r);
-    first_item = __builtin_amdgcn_readlane(inc, r) - parts;
-    part = item - first_item;
-    sp.begin = __builtin_amdgcn_readlane(mine.begin, r);
-    sp.n = __builtin_amdgcn_readlane(mine.n, r);
-    sp.len = __builtin_amdgcn_readlane(mine.len, r);
-  } else {
-    int64_t total = 0;
-    for (uint32_t i = tid; i < a.requests; i += AT) total += span_of(c, a, i).len;
-    total = (int64_t)wave_sum_u64((uint64_t)total);
-    if (lane == 0) sh.red[wave] = total;
-    if (tid == 0) sh.item[0] = ~0u;
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < AW; ++w) total += sh.red[w];
-    size = part_size_of(total);
-    uint32_t before = 0;
-    for (uint32_t i0 = 0; i0 < a.requests; i0 += AT) {
-      const uint32_t i = i0 + tid;
-      uint32_t n = 0;
-      if (i < a.requests) n = max(((uint32_t)span_of(c, a, i).len + size - 1) / size, 1u);
-      const uint32_t inc = wave_incl_scan_u32(n);
-      __syncthreads();
-      if (lane == WAVE - 1) sh.red[wave] = inc;
-      __syncthreads();
-      uint32_t at = before + inc - n;
-      for (uint32_t w = 0; w < AW; ++w) {
-        if (w < wave) at += (uint32_t)sh.red[w];
-        before += (uint32_t)sh.red[w];
-      }
-      if (n > 0 && item >= at && item < at + n) {
-        sh.item[0] = i;
-        sh.item[1] = item - at;
-        sh.item[2] = n;
-        sh.item[3] = at;
-      }
-      if (before > item) break;
-    }
-    __syncthreads();
-    r = __builtin_amdgcn_readfirstlane(sh.item[0]);
-    if (r == ~0u) return;
-    part = __builtin_amdgcn_readfirstlane(sh.item[1]);
-    parts = __builtin_amdgcn_readfirstlane(sh.item[2]);
-    first_item = __builtin_amdgcn_readfirstlane(sh.item[3]);
-    sp = span_of(c, a, r);
+  uint32_t u[4];
+  uint64_t total = 0;
+  for (uint32_t i0 = 0; i0 < a.requests; i0 += 4 * WAVE) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = blocks_of(i0 + lane * 4 + k);
+    total += (uint64_t)u[0] + u[1] + u[2] + u[3];
   }
-  if (sp.begin < 0) return;
+  total = wave_sum_u64(total);
+  const uint64_t share = max((total + p.items - 1) / p.items, (uint64_t)SHARE_MIN);
+  uint64_t pos = item * share, start = 0;  // the share's first block; the first block of request r
+  const uint64_t stop = min(pos + share, total);
+  uint32_t r = 0;
+  if (pos >= stop) return;
+  for (uint32_t i0 = 0;; i0 += 4 * WAVE) {
+    if (a.requests > 4 * WAVE) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = blocks_of(i0 + lane * 4 + k);
+    }
+    const uint64_t mine = (uint64_t)u[0] + u[1] + u[2] + u[3], inc = wave_incl_scan_u64(mine);
+    const uint64_t past = ballot64(start + inc > pos);
+    if (!past) {
+      start += lane63(inc);
+      continue;
+    }
+    const int at = __builtin_ctzll(past);
+    start += shfl_u64(inc - mine, at);
+    r = i0 + at * 4;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const uint32_t n = __builtin_amdgcn_readlane(u[k], at);
+      if (r == i0 + at * 4 + k && start + n <= pos) {
+        start += n;
+        ++r;
+      }
+    }
+    break;
+  }
+  start = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)start) | (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(start >> 32)) << 32;
+  r = __builtin_amdgcn_readfirstlane(r);
+
+  Span ahead = span_of(c, a, r);
+  for (; pos < stop; ++r) {
+  const Span sp = ahead;
+  ahead = span_of(c, a, min(r + 1, a.requests - 1));
+  if (sp.begin < 0) continue;
+  const uint64_t first = start, end = start + max(((uint32_t)sp.len + AB - 1) / AB, 1u);  // the request's blocks
+  const uint32_t k0 = (uint32_t)(pos - first) * AB, k_end = (uint32_t)(min(stop, end) - first) * AB;
+  const uint32_t first_item = (uint32_t)(first / share), parts = (uint32_t)((end - 1) / share) - first_item + 1;
+  start = end;
+  pos = min(stop, end);
   const uint32_t rows = min((uint32_t)sp.n, a.max_new) * p.group, row0 = tile * 16 * MT;
-  if (row0 >= rows) return;
+  if (row0 >= rows) continue;
   const uint32_t len = (uint32_t)sp.len, ctx = len >= (uint32_t)sp.n ? len - (uint32_t)sp.n : 0;
   const uint32_t last_new = (min(rows, row0 + 16 * MT) - 1) / p.group;
-  const uint32_t k0 = part * size;  // (below 2^32: parts are at most the length's)
-  uint32_t k1 = min(len, a.parent ? len : ctx + last_new + 1);
-  if (k1 - min(k0, k1) > size) k1 = k0 + size;
+  const uint32_t k1 = min(k_end, a.parent ? len : min(len, ctx + last_new + 1));
 
   // ---- the rows -----------------------------------------------------------------------------------------------------------
   const uint32_t sign = a.scale < 0 ? 0x80008000u : 0;  // (the scale's own, so that the largest score is the largest product)
-  Frag<Q> q[MT][KD];
+  Frag<Q> q[Sh::QL ? 1 : MT][KD];
+  if constexpr (Sh::QL) {
+    for (uint32_t i = tid; i < MT * 16 * KD * 4; i += AT) {
+      const uint32_t w = i / (KD * 4), e = i % (KD * 4), row = min(row0 + w, rows - 1), n = row / p.group, gi = row - n * p.group;
+      const char *at = (const char *)a.q + ((int64_t)(sp.begin + n) * a.q_token_stride + (int64_t)(head * p.group + gi) * a.q_head_stride) * 2;
+      uint4 v = {0, 0, 0, 0};
+      if (e * 8 < c.dim) v = *(const uint4 *)(at + e * 16);
+      v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
+      sh.q[w / 16][w % 16][e] = v;
+    }
+    __syncthreads();
+  }
+  auto q_of = [&](int m, int k) {
+    if constexpr (Sh::QL) return __builtin_bit_cast(Frag<Q>, sh.q[m][lc][k * 4 + lg]);
+    else return q[m][k];
+  };
   uint32_t sees[MT];   // chains: the first cached token that the lane's row does not see
   uint64_t path[MT];   // trees: which new tokens it sees
   const int32_t parent = a.parent ? a.parent[sp.begin + (int32_t)min(lane, (uint32_t)sp.n - 1)] : 0;  // of new token `lane`
@@ -222,11 +233,11 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
     const uint32_t row = row0 + m * 16 + lc, i = min(row, rows - 1) / p.group, gi = min(row, rows - 1) - i * p.group;
     const char *at = (const char *)a.q + ((int64_t)(sp.begin + i) * a.q_token_stride + (int64_t)(head * p.group + gi) * a.q_head_stride) * 2;
 #pragma unroll
-    for (int k = 0; k < KD; ++k) {
+    for (int k = 0; !Sh::QL && k < KD; ++k) {
       uint4 w = {0, 0, 0, 0};
       if (k * 32 + lg * 8 < c.dim) w = *(const uint4 *)(at + (k * 32 + lg * 8) * 2);
       w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
-      q[m][k] = __builtin_bit_cast(Frag<Q>, w);
+      q[Sh::QL ? 0 : m][k] = __builtin_bit_cast(Frag<Q>, w);
     }
     sees[m] = ctx + i + 1;
     path[m] = 0;
@@ -328,7 +339,7 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
         for (int k = 0; k < KD; ++k) {
           const Frag<Q> kf = operand<C, Q>(kr[u][k]);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) s[m][u] = mma<Q>(kf, q[m][k], s[m][u]);
+          for (int m = 0; m < MT; ++m) s[m][u] = mma<Q>(kf, q_of(m, k), s[m][u]);
         }
       }
       place_block(t + AW * AB + l32, page);
@@ -427,7 +438,8 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
   // A thread has eight elements of one of 16 rows. A part's scratch: rows x dim of O, then rows x (m, l).
   float *work = (float *)a.work;
   const int64_t part_size = (int64_t)p.rows * (c.dim + 2);
-  auto scratch = [&](uint32_t it) { return work + ((int64_t)(it * c.heads + head) * p.tiles + tile) * part_size; };
+  // A share has two of them: of the request that it goes on with, and of the one that goes on after it.
+  auto scratch = [&](uint32_t it) { return work + (((int64_t)it * 2 + (it == first_item)) * each + x) * part_size; };
   const uint32_t tr = tid / 16, te = tid % 16 * 8;
   auto finish = [&](uint32_t row, uint32_t e, const float (&x)[8], float sum) {
     const uint32_t i = row / p.group, gi = row - i * p.group;
@@ -488,78 +500,93 @@ __global__ __launch_bounds__(AT, KD > 4 || MT > 2 ? 1 : MT == 2 ? 2 : 3) void at
               (uint64_t)__float_as_uint(top) | (uint64_t)__float_as_uint(sum) << 32);
     }
   }
-  if (parts == 1) return;
+  if (parts == 1) {
+    __syncthreads();
+    continue;
+  }
 
   // ---- the parts joined ---------------------------------------------------------------------------------------------------
   store_wait();
   __syncthreads();
-  uint32_t *tick = p.tick + ((int64_t)r * c.heads + head) * p.tiles + tile;
+  uint32_t *tick = p.tick + (int64_t)first_item * each + x;  // (one request at most goes on after a share)
   if (tid == 0) sh.last = ticket_add(tick) == parts - 1;
   __syncthreads();
-  if (!sh.last) return;
+  const bool last = sh.last;
+  __syncthreads();
+  if (!last) continue;
   if (tid == 0) st_ag(tick, 0u);
-  // 16 threads a row again; with few rows, several such groups share a row's parts. A thread finds the factors of 16 parts at
-  // a time with its group (a part a thread), then adds its eight elements of them, eight parts' loads at once.
+  // 16 threads a row again; with few rows, several such groups share a row's parts. A thread takes eight of its parts' loads at
+  // once: a round trip, in most calls the only one.
 #pragma unroll 1
   for (int m = 0; m < MT; ++m) {
     if (row0 + m * 16 >= rows) break;
     const uint32_t count = min(rows - row0 - m * 16, 16u), wide = count <= 1 ? 1 : 1u << (32 - __builtin_clz(count - 1));
-    const uint32_t i = m * 16 + tr % wide, share = tr / wide, shares = 16 / wide, j = tid % 16;
+    const uint32_t i = m * 16 + tr % wide, mine = tr / wide, shares = 16 / wide;
     const bool real = tr % wide < count;
-    const int64_t ml_at = (int64_t)p.rows * c.dim + 2 * i;
-    float top = -INF;
-    if (real)
-      for (uint32_t s = j; s < parts; s += 16) top = fmaxf(top, __uint_as_float((uint32_t)ld_ag((const uint64_t *)(scratch(first_item + s) + ml_at))));
-    for (int k = 8; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, WAVE));
 #pragma unroll 1
     for (int b = 0; b < VB; ++b) {
       const uint32_t e = b * 128 + te;
       const bool in = real && e < c.dim;
-      float sum = 0, x[8] = {};
-      for (uint32_t s0 = share * 16; s0 < parts; s0 += 16 * shares) {
-        float f = 0;
-        if (real && s0 + j < parts) {
-          const uint64_t ml = ld_ag((const uint64_t *)(scratch(first_item + s0 + j) + ml_at));
-          const float part_l = __uint_as_float((uint32_t)(ml >> 32));
-          f = weight_of(__uint_as_float((uint32_t)ml), part_l, top);
-          sum += f == 0.0f ? 0.0f : f * part_l;
+      float top = -INF, sum = 0, y[8] = {};
+      for (uint32_t s0 = mine; in && s0 < parts; s0 += 8 * shares) {
+        uint64_t ml[8], w[8][4];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+          const float *o = scratch(first_item + min(s0 + k * shares, parts - 1));
+          ml[k] = ld_ag((const uint64_t *)(o + (int64_t)p.rows * c.dim + 2 * i));
+#pragma unroll
+          for (int d = 0; d < 4; ++d) w[k][d] = ld_ag((const uint64_t *)(o + (int64_t)i * c.dim + e) + d);
         }
+        float next = top;
 #pragma unroll
-        for (uint32_t k0_ = 0; k0_ < 16; k0_ += 8) {
-          uint64_t w[8][4];
+        for (uint32_t k = 0; k < 8; ++k) next = fmaxf(next, __uint_as_float((uint32_t)ml[k]));
+        const float f = weight_of(top, sum, next);
+        top = next;
+        sum *= f;
 #pragma unroll
-          for (uint32_t k = 0; k < 8; ++k) {
-            const float *o = scratch(first_item + min(s0 + k0_ + k, parts - 1)) + (int64_t)i * c.dim + e;
+        for (int d = 0; d < 8; ++d) y[d] *= f;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) w[k][d] = in ? ld_ag((const uint64_t *)o + d) : 0;
-          }
+        for (uint32_t k = 0; k < 8; ++k) {
+          const float part_l = __uint_as_float((uint32_t)(ml[k] >> 32));
+          const float g = s0 + k * shares < parts ? weight_of(__uint_as_float((uint32_t)ml[k]), part_l, top) : 0.0f;
+          if (g == 0.0f) continue;  // (nothing of this row in the part, or no such part)
+          sum += g * part_l;
 #pragma unroll
-          for (uint32_t k = 0; k < 8; ++k) {
-            const float g = __shfl(f, (int)(lane / 16 * 16 + k0_ + k), WAVE);
-            if (g == 0.0f) continue;  // (nothing of this row in the part, or no such part)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              x[2 * d] += g * __uint_as_float((uint32_t)w[k][d]);
-              x[2 * d + 1] += g * __uint_as_float((uint32_t)(w[k][d] >> 32));
-            }
+          for (int d = 0; d < 4; ++d) {
+            y[2 * d] += g * __uint_as_float((uint32_t)w[k][d]);
+            y[2 * d + 1] += g * __uint_as_float((uint32_t)(w[k][d] >> 32));
           }
         }
       }
-      for (int k = 8; k > 0; k /= 2) sum += __shfl_xor(sum, k, WAVE);
       if (shares > 1) {
         __syncthreads();
-        *(f32x4 *)&sh.o[0][tr][te] = f32x4{x[0], x[1], x[2], x[3]};
-        *(f32x4 *)&sh.o[0][tr][te + 4] = f32x4{x[4], x[5], x[6], x[7]};
-        if (j == 0) sh.l[0][tr] = sum;
+        *(f32x4 *)&sh.o[0][tr][te] = f32x4{y[0], y[1], y[2], y[3]};
+        *(f32x4 *)&sh.o[0][tr][te + 4] = f32x4{y[4], y[5], y[6], y[7]};
+        if (te == 0) {
+          sh.m[0][tr] = top;
+          sh.l[0][tr] = sum;
+        }
         __syncthreads();
-        for (uint32_t k = 1; share == 0 && k < shares; ++k) {
-          sum += sh.l[0][tr + k * wide];
+        if (in && mine == 0) {
+          const float was = top;
+          for (uint32_t k = 1; k < shares; ++k) top = fmaxf(top, sh.m[0][tr + k * wide]);
+          const float f = weight_of(was, sum, top);
+          sum *= f;
 #pragma unroll
-          for (int d = 0; d < 8; ++d) x[d] += sh.o[0][tr + k * wide][te + d];
+          for (int d = 0; d < 8; ++d) y[d] *= f;
+          for (uint32_t k = 1; k < shares; ++k) {
+            const float part_l = sh.l[0][tr + k * wide], g = weight_of(sh.m[0][tr + k * wide], part_l, top);
+            if (g == 0.0f) continue;
+            sum += g * part_l;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) y[d] += g * sh.o[0][tr + k * wide][te + d];
+          }
         }
       }
-      if (in && share == 0) finish(row0 + i, e, x, sum);
+      if (in && mine == 0) finish(row0 + i, e, y, sum);
     }
+  }
+  __syncthreads();
   }
 }
 

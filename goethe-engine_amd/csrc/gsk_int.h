@@ -12,10 +12,10 @@ hipError_t launch_reorder(const gsk_reorder_beams &a, hipStream_t s);
 // How a call of gsk_attend is cut (gsk_attend.hip); tick: the tickets that it may use.
 struct AttendPlan {
   uint32_t tiles;  // of a request's (new token, query head of the group) rows
-  uint32_t items;  // (request, part of its cached tokens): workgroups per cache head and tile
+  uint32_t items;  // equal shares of the requests' cached tokens: workgroups per cache head and tile, at most
   int64_t work;    // scratch bytes
 };
-AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tickets, int round);
+AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tickets, int cus);
 hipError_t launch_attend(const gsk_cache &c, const gsk_attention &a, const AttendPlan &p, uint32_t *tick, hipStream_t s);
 
 uint32_t beam_slices(const gsk_beams &a);

@@ -38,17 +38,22 @@ struct AttendArgs {
 template <int KD, int MT>
 struct AttendShared {
   static constexpr int VB = (KD + 3) / 4, LD = 132;
-  static constexpr bool QL = MT > 1;  // the rows' operands are read from LDS (registers have no room)
-  float o[AW][16][LD];       // a wave's O of 16 rows and 128 elements (padded by a bank row)
-  float m[AW][16], l[AW][16];
-  int64_t at[AW][AB];        // byte offsets of the block's tokens
-  float scale[AW][2][AB];    // and their keys' and values' scales
-  uint4 q[QL ? MT : 1][QL ? 16 : 1][QL ? KD * 4 + 1 : 1];
+  union {
+    struct {                       // the tokens' loop
+      uint4 q[MT][16][KD * 4 + 1]; // the rows' operands (a piece of padding: the rows' pieces lie in different banks)
+      int64_t at[AW][AB];          // byte offsets of the block's tokens
+      float scale[AW][2][AB];      // and their keys' and values' scales
+    };
+    struct {                       // the joins
+      float o[AW][16][LD];         // a wave's O of 16 rows and 128 elements
+      float m[AW][16], l[AW][16];
+    };
+  };
   uint32_t last;
 };
 
 // Workgroups of a CU at once (what their registers allow).
-constexpr int attend_resident(int kd, int mt) { return kd > 4 ? 1 : mt == 1 ? 3 : 2; }
+constexpr int attend_resident(int kd, int mt) { return kd > 4 ? 1 : mt > 1 ? 2 : 3; }
 
 template <uint32_t T>
 using Frag = std::conditional_t<T == GSK_F16, f16x8, bf16x8>;
@@ -117,17 +122,27 @@ __device__ __forceinline__ float weight_of(float m, float l, float top) {
   return l == 0.0f ? 0.0f : m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
 }
 
+struct Raw {        // a request's numbers as they are
+  int32_t begin, end, len;
+  uint32_t status;
+};
+__device__ __forceinline__ Raw raw_of(const gsk_attention &a, uint32_t r) {
+  Raw x{(int32_t)r, (int32_t)r + 1, a.seq_len[r], 0};
+  if (a.begin) x.begin = a.begin[r], x.end = a.begin[r + 1];
+  if (a.status) x.status = a.status[r];
+  return x;
+}
 struct Span {       // a request's rows and cached tokens
   int32_t begin;    // -1: nothing to write
   int32_t n, len;   // new tokens; cached ones, 0 where the request is not served
 };
-__device__ __forceinline__ Span span_of(const gsk_cache &c, const gsk_attention &a, uint32_t r) {
-  const int64_t b = a.begin ? a.begin[r] : (int64_t)r, e = a.begin ? a.begin[r + 1] : (int64_t)r + 1, len = a.seq_len[r];
-  const uint32_t st = a.status ? a.status[r] : 0;
-  if (b < 0 || e > (int64_t)a.tokens || e <= b) return {-1, 0, 0};
-  const bool ok = st == 0 && len >= e - b && len <= (int64_t)a.max_pages * c.page;
-  return {(int32_t)b, (int32_t)(e - b), ok ? (int32_t)len : 0};
+__device__ __forceinline__ Span span_of(const gsk_cache &c, const gsk_attention &a, Raw x) {
+  if (x.begin < 0 || x.end < 0 || (uint32_t)x.end > a.tokens || x.end <= x.begin) return {-1, 0, 0};
+  const int32_t n = x.end - x.begin;
+  const bool ok = x.status == 0 && x.len >= n && (int64_t)x.len <= (int64_t)a.max_pages * c.page;
+  return {x.begin, n, ok ? x.len : 0};
 }
+__device__ __forceinline__ uint32_t blocks_of(Span x) { return x.begin < 0 ? 0u : max(((uint32_t)x.len + AB - 1) / AB, 1u); }
 
 template <uint32_t Q, uint32_t C, int KD, int MT>
 __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(AttendArgs p) {
@@ -147,30 +162,33 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
 
   // ---- the share ----------------------------------------------------------------------------------------------------------
   // Every wave for itself, a lane four requests at a time: a request's blocks, one at least if it has rows to write.
-  auto blocks_of = [&](uint32_t i) -> uint32_t {
-    const Span x = span_of(c, a, min(i, a.requests - 1));
-    return i < a.requests && x.begin >= 0 ? max(((uint32_t)x.len + AB - 1) / AB, 1u) : 0u;
-  };
+  Span own[4];
   uint32_t u[4];
-  uint64_t total = 0;
-  for (uint32_t i0 = 0; i0 < a.requests; i0 += 4 * WAVE) {
+  auto take = [&](uint32_t i0) {  // returns the lane's blocks
+    Raw raw[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) u[k] = blocks_of(i0 + lane * 4 + k);
-    total += (uint64_t)u[0] + u[1] + u[2] + u[3];
-  }
+    for (int k = 0; k < 4; ++k) raw[k] = raw_of(a, min(i0 + lane * 4 + k, a.requests - 1));
+    uint64_t n = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      own[k] = span_of(c, a, raw[k]);
+      u[k] = i0 + lane * 4 + k < a.requests ? blocks_of(own[k]) : 0;
+      n += u[k];
+    }
+    return n;
+  };
+  uint64_t mine = take(0), total = mine;
+  for (uint32_t i0 = 4 * WAVE; i0 < a.requests; i0 += 4 * WAVE) total += take(i0);
   total = wave_sum_u64(total);
   const uint64_t share = max((total + p.items - 1) / p.items, (uint64_t)SHARE_MIN);
   uint64_t pos = item * share, start = 0;  // the share's first block; the first block of request r
   const uint64_t stop = min(pos + share, total);
-  uint32_t r = 0;
   if (pos >= stop) return;
+  uint32_t r = 0;
+  Span sp;
   for (uint32_t i0 = 0;; i0 += 4 * WAVE) {
-    if (a.requests > 4 * WAVE) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = blocks_of(i0 + lane * 4 + k);
-    }
-    const uint64_t mine = (uint64_t)u[0] + u[1] + u[2] + u[3], inc = wave_incl_scan_u64(mine);
-    const uint64_t past = ballot64(start + inc > pos);
+    if (a.requests > 4 * WAVE) mine = take(i0);
+    const uint64_t inc = wave_incl_scan_u64(mine), past = ballot64(start + inc > pos);
     if (!past) {
       start += lane63(inc);
       continue;
@@ -179,9 +197,13 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     start += shfl_u64(inc - mine, at);
     r = i0 + at * 4;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
+    for (int k = 0; k < 4; ++k) {
+      if (r != i0 + at * 4 + k) continue;
+      sp.begin = __builtin_amdgcn_readlane(own[k].begin, at);
+      sp.n = __builtin_amdgcn_readlane(own[k].n, at);
+      sp.len = __builtin_amdgcn_readlane(own[k].len, at);
       const uint32_t n = __builtin_amdgcn_readlane(u[k], at);
-      if (r == i0 + at * 4 + k && start + n <= pos) {
+      if (k < 3 && start + n <= pos) {
         start += n;
         ++r;
       }
@@ -191,12 +213,11 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   start = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)start) | (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(start >> 32)) << 32;
   r = __builtin_amdgcn_readfirstlane(r);
 
-  Span ahead = span_of(c, a, r);
-  for (; pos < stop; ++r) {
-  const Span sp = ahead;
-  ahead = span_of(c, a, min(r + 1, a.requests - 1));
+  for (Raw ahead;; sp = span_of(c, a, ahead), ++r) {
+  if (pos >= stop) break;
+  ahead = raw_of(a, min(r + 1, a.requests - 1));  // (the next request's, for the next turn)
   if (sp.begin < 0) continue;
-  const uint64_t first = start, end = start + max(((uint32_t)sp.len + AB - 1) / AB, 1u);  // the request's blocks
+  const uint64_t first = start, end = start + blocks_of(sp);  // the request's blocks
   const uint32_t k0 = (uint32_t)(pos - first) * AB, k_end = (uint32_t)(min(stop, end) - first) * AB;
   const uint32_t first_item = (uint32_t)(first / share), parts = (uint32_t)((end - 1) / share) - first_item + 1;
   start = end;
@@ -209,36 +230,21 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
 
   // ---- the rows -----------------------------------------------------------------------------------------------------------
   const uint32_t sign = a.scale < 0 ? 0x80008000u : 0;  // (the scale's own, so that the largest score is the largest product)
-  Frag<Q> q[Sh::QL ? 1 : MT][KD];
-  if constexpr (Sh::QL) {
-    for (uint32_t i = tid; i < MT * 16 * KD * 4; i += AT) {
-      const uint32_t w = i / (KD * 4), e = i % (KD * 4), row = min(row0 + w, rows - 1), n = row / p.group, gi = row - n * p.group;
-      const char *at = (const char *)a.q + ((int64_t)(sp.begin + n) * a.q_token_stride + (int64_t)(head * p.group + gi) * a.q_head_stride) * 2;
-      uint4 v = {0, 0, 0, 0};
-      if (e * 8 < c.dim) v = *(const uint4 *)(at + e * 16);
-      v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
-      sh.q[w / 16][w % 16][e] = v;
-    }
-    __syncthreads();
+  for (uint32_t i = tid; i < MT * 16 * KD * 4; i += AT) {
+    const uint32_t w = i / (KD * 4), e = i % (KD * 4), row = min(row0 + w, rows - 1), n = row / p.group, gi = row - n * p.group;
+    const char *at = (const char *)a.q + ((int64_t)(sp.begin + n) * a.q_token_stride + (int64_t)(head * p.group + gi) * a.q_head_stride) * 2;
+    uint4 v = {0, 0, 0, 0};
+    if (e * 8 < c.dim) v = *(const uint4 *)(at + e * 16);
+    v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
+    sh.q[w / 16][w % 16][e] = v;
   }
-  auto q_of = [&](int m, int k) {
-    if constexpr (Sh::QL) return __builtin_bit_cast(Frag<Q>, sh.q[m][lc][k * 4 + lg]);
-    else return q[m][k];
-  };
+  auto q_of = [&](int m, int k) { return __builtin_bit_cast(Frag<Q>, sh.q[m][lc][k * 4 + lg]); };
   uint32_t sees[MT];   // chains: the first cached token that the lane's row does not see
   uint64_t path[MT];   // trees: which new tokens it sees
   const int32_t parent = a.parent ? a.parent[sp.begin + (int32_t)min(lane, (uint32_t)sp.n - 1)] : 0;  // of new token `lane`
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const uint32_t row = row0 + m * 16 + lc, i = min(row, rows - 1) / p.group, gi = min(row, rows - 1) - i * p.group;
-    const char *at = (const char *)a.q + ((int64_t)(sp.begin + i) * a.q_token_stride + (int64_t)(head * p.group + gi) * a.q_head_stride) * 2;
-#pragma unroll
-    for (int k = 0; !Sh::QL && k < KD; ++k) {
-      uint4 w = {0, 0, 0, 0};
-      if (k * 32 + lg * 8 < c.dim) w = *(const uint4 *)(at + (k * 32 + lg * 8) * 2);
-      w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
-      q[Sh::QL ? 0 : m][k] = __builtin_bit_cast(Frag<Q>, w);
-    }
+    const uint32_t i = min(row0 + m * 16 + lc, rows - 1) / p.group;
     sees[m] = ctx + i + 1;
     path[m] = 0;
     if (a.parent) {  // (uniform; at most 64 steps: an ancestor is an earlier row)
@@ -315,6 +321,9 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   if (t < k1) {
     place_block(t + l32, next_page());
     load_keys();
+  }
+  __syncthreads();  // (the rows' operands)
+  if (t < k1) {
     for (; t < k1; t += AW * AB) {
       const uint32_t page = next_page(), real = there;
       if constexpr (type_is_8bit<C>) sh.scale[wave][lane / 32][l32] = lane < 32 ? scale_of * scale : scale_of;
@@ -454,7 +463,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     if (row0 + m * 16 >= rows) break;
 #pragma unroll 1
     for (int b = 0; b < VB; ++b) {
-      if (m || b) __syncthreads();
+      __syncthreads();  // (the last use of what lies there)
       // (the accumulators are picked with constant indexes)
 #pragma unroll
       for (int mm = 0; mm < MT; ++mm) {

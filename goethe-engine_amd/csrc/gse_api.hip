@@ -739,8 +739,8 @@ int check_cache(gse_handle *h, const gsk_cache &c, bool arrays) {
   if (c.pages == 0 || c.page == 0 || c.heads == 0) return fail(h, GSE_E_ARG, "pages, page and heads must be > 0");
   if (c.dim == 0 || c.dim % 8 || c.dim > GSK_MAX_DIM)
     return fail(h, GSE_E_UNSUPPORTED, "dim %u is no multiple of 8 in [8, %d]", c.dim, GSK_MAX_DIM);
-  if ((uint64_t)c.pages * c.page > UINT32_MAX || c.heads > (1u << 16))
-    return fail(h, GSE_E_UNSUPPORTED, "%u pages of %u tokens, %u heads: at most 2^32 - 1 slots and 2^16 heads", c.pages, c.page, c.heads);
+  if ((uint64_t)c.pages * c.page > UINT32_MAX || c.heads > (1u << 12))
+    return fail(h, GSE_E_UNSUPPORTED, "%u pages of %u tokens, %u heads: at most 2^32 - 1 slots and 2^12 heads", c.pages, c.page, c.heads);
   if (!arrays) return GSE_OK;
   if (!c.keys || !c.values || (bits8 && (!c.key_scales || !c.value_scales)))
     return fail(h, GSE_E_ARG, "keys, values and, in 8 bits, their scales are required");

@@ -6,10 +6,10 @@ namespace gse {
 
 namespace {
 
-// ---- write and read -------------------------------------------------------------------------------------------------------
+// ---- write ---------------------------------------------------------------------------------------------------------------
 // A group of 8, 16 or 32 lanes owns one token's head of the keys or of the values, a lane eight elements of it; in 8 bits the
 // group finds the row's largest magnitude by exchanges within it. Rows with a NaN or an infinity are found with it: as unsigned
-// integers their magnitudes are the largest.
+// integers their magnitudes are the largest. ROWS: a group's rows, all loaded before the first is worked on.
 constexpr int CT = 256;
 
 struct Place {
@@ -20,62 +20,134 @@ __device__ __forceinline__ Place place(const gsk_cache &c, uint32_t pg, uint32_t
           (int64_t)pg * c.scale_page_stride + (int64_t)off * c.scale_token_stride + (int64_t)head * c.scale_head_stride};
 }
 
-template <uint32_t SRC, uint32_t DST, int GL>
+template <uint32_t SRC, uint32_t DST, int GL, int ROWS>
 __global__ __launch_bounds__(CT) void write_kernel(gsk_cache c, gsk_rows a) {
-  const uint32_t id = (blockIdx.x * CT + threadIdx.x) / GL, j = threadIdx.x % GL, t = id / c.heads, h = id - t * c.heads;
-  if (t >= a.tokens) return;
+  const uint32_t j = threadIdx.x % GL, rows = a.tokens * c.heads;
+  const uint32_t first = blockIdx.x * (CT / GL * ROWS) + threadIdx.x / GL;
   const bool values = blockIdx.y != 0, mine = j * 8 < c.dim;
-  const uint64_t slot = (uint64_t)a.slot[t];
-  const char *src = values ? (const char *)a.v + ((int64_t)t * a.v_token_stride + (int64_t)h * a.v_head_stride) * type_size<SRC>
-                           : (const char *)a.k + ((int64_t)t * a.k_token_stride + (int64_t)h * a.k_head_stride) * type_size<SRC>;
-  float x[8] = {};
-  if (mine) to_f32(load_raw8<SRC>(src + j * 8 * type_size<SRC>), x);
-  if (slot >= (uint64_t)c.pages * c.page) return;  // (negative ones are past it; the group as a whole)
-  const uint32_t pg = (uint32_t)slot / c.page;
-  const Place p = place(c, pg, (uint32_t)slot - pg * c.page, h);
-  if constexpr (type_is_8bit<DST>) {
-    uint32_t m = 0;
+  const char *src = (const char *)(values ? a.v : a.k) + j * 8 * type_size<SRC>;
+  const int64_t ts = (values ? a.v_token_stride : a.k_token_stride) * type_size<SRC>;
+  const int64_t hs = (values ? a.v_head_stride : a.k_head_stride) * type_size<SRC>;
+  char *dst = (char *)(values ? c.values : c.keys) + j * 8 * type_size<DST>;
+  float *scales = values ? c.value_scales : c.key_scales;
+  Raw8<SRC> raw[ROWS];
+  uint64_t slot[ROWS];
+  uint32_t head[ROWS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-#pragma unroll
-    for (int k = GL / 2; k > 0; k /= 2) m = max(m, shfl_xor_u32(m, k));
-    const bool bad = m >= 0x7F800000u;
-    const float most = DST == GSK_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f;
-    const float scale = fmaxf(__fmul_rn(__uint_as_float(m), most), 0x1p-126f), inv = __fdiv_rn(1.0f, scale);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = bad ? 0.0f : __fmul_rn(x[i], inv);
-    if (j == 0) (values ? c.value_scales : c.key_scales)[p.scale] = bad ? __uint_as_float(0x7FC00000u) : scale;
+  for (int i = 0; i < ROWS; ++i) {
+    const uint32_t id = first + i * (CT / GL), t = min(id, rows - 1) / c.heads;
+    head[i] = min(id, rows - 1) - t * c.heads;
+    slot[i] = id < rows ? (uint64_t)a.slot[t] : ~0ull;
+    raw[i] = Raw8<SRC>{};
+    if (mine) raw[i] = load_raw8<SRC>(src + (int64_t)t * ts + (int64_t)head[i] * hs);
   }
-  if (mine) store_raw8<DST>((char *)(values ? c.values : c.keys) + (p.at + j * 8) * type_size<DST>, from_f32<DST>(x));
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    if (slot[i] >= (uint64_t)c.pages * c.page) continue;  // (negative ones are past it; the group as a whole)
+    const uint32_t pg = (uint32_t)slot[i] / c.page;
+    const Place p = place(c, pg, (uint32_t)slot[i] - pg * c.page, head[i]);
+    float x[8];
+    to_f32(raw[i], x);
+    if constexpr (type_is_8bit<DST>) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int k = GL / 2; k > 0; k /= 2) m = max(m, shfl_xor_u32(m, k));
+      const bool bad = m >= 0x7F800000u;
+      const float most = DST == GSK_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f;
+      const float scale = fmaxf(__fmul_rn(__uint_as_float(m), most), 0x1p-126f), inv = __fdiv_rn(1.0f, scale);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = bad ? 0.0f : __fmul_rn(x[e], inv);
+      if (j == 0) scales[p.scale] = bad ? __uint_as_float(0x7FC00000u) : scale;
+    }
+    if (mine) store_raw8<DST>(dst + p.at * type_size<DST>, from_f32<DST>(x));
+  }
 }
 
-template <uint32_t SRC, uint32_t DST, int GL>
-__global__ __launch_bounds__(CT) void read_kernel(gsk_cache c, gsk_read_rows a) {
-  const uint32_t id = (blockIdx.x * CT + threadIdx.x) / GL, j = threadIdx.x % GL, row = id / c.heads, h = id - row * c.heads;
-  const uint32_t first_row = __builtin_amdgcn_readfirstlane(row);
-  if (first_row >= a.rows) return;
-  uint32_t r = wave_find(a.begin, a.requests, first_row);
-  if (row >= a.rows || j * 8 >= c.dim) return;
-  while (r + 1 < a.requests && (int64_t)a.begin[r + 1] <= (int64_t)row) ++r;
-  const int64_t b = a.begin[r];
-  if ((int64_t)row < b || (int64_t)row >= (int64_t)a.begin[r + 1]) return;
-  const int64_t t = (a.first ? a.first[r] : 0) + ((int64_t)row - b);
-  const bool values = blockIdx.y != 0;
-  float x[8] = {};
-  if (t >= 0 && t < (int64_t)a.max_pages * c.page) {
-    const uint32_t pi = (uint32_t)t / c.page;
-    const uint32_t pg = (uint32_t)a.table[(int64_t)r * a.table_ld + pi];
-    if (pg < c.pages) {
-      const Place p = place(c, pg, (uint32_t)t - pi * c.page, h);
-      to_f32(load_raw8<SRC>((const char *)(values ? c.values : c.keys) + (p.at + j * 8) * type_size<SRC>), x);
-      if constexpr (type_is_8bit<SRC>) {
-        const float scale = (values ? c.value_scales : c.key_scales)[p.scale];
+// ---- read ----------------------------------------------------------------------------------------------------------------
+// A workgroup takes `tokens` rows, every head of them, keys and values. Its first wave finds their places (a lane a token: the
+// request by a search of the whole wave for the first, from there on step by step; then the page) and leaves them in LDS; the
+// threads then walk the rows' pieces of eight elements, which lie together in the output.
+constexpr uint32_t RTOK = 32;  // tokens of a workgroup, at most
+
+struct ReadShared {
+  int64_t at[RTOK], scale[RTOK];
+  int32_t kind[RTOK];  // 1: a cached token, 0: zeros, -1: left as it is
+};
+
+template <uint32_t SRC, uint32_t DST, int U>
+__global__ __launch_bounds__(CT) void read_kernel(gsk_cache c, gsk_read_rows a, uint32_t tokens, uint32_t by_pieces, uint32_t by_heads) {
+  __shared__ ReadShared sh;
+  const uint32_t tid = threadIdx.x, row0 = blockIdx.x * tokens, pieces = c.dim / 8;
+  if (tid < WAVE) {
+    uint32_t r = wave_find(a.begin, a.requests, row0);
+    const uint32_t row = row0 + tid;
+    if (tid < tokens) {
+      int32_t kind = -1;
+      Place p = {0, 0};
+      if (row < a.rows) {
+        int64_t b = a.begin[r], e = a.begin[r + 1];
+        while (e <= (int64_t)row && r + 1 < a.requests) {
+          ++r;
+          b = e;
+          e = a.begin[r + 1];
+        }
+        if ((int64_t)row >= b && (int64_t)row < e) {
+          const int64_t t = (a.first ? a.first[r] : 0) + ((int64_t)row - b);
+          kind = 0;
+          if (t >= 0 && t < (int64_t)a.max_pages * c.page) {
+            const uint32_t pi = (uint32_t)t / c.page, pg = (uint32_t)a.table[(int64_t)r * a.table_ld + pi];
+            if (pg < c.pages) {
+              kind = 1;
+              p = place(c, pg, (uint32_t)t - pi * c.page, 0);
+            }
+          }
+        }
+      }
+      sh.kind[tid] = kind;
+      sh.at[tid] = p.at;
+      sh.scale[tid] = p.scale;
+    }
+  }
+  __syncthreads();
+  const uint32_t n = min(tokens, a.rows - row0) * c.heads * pieces;
+  const int64_t out = (int64_t)row0 * c.heads * pieces;
+  for (uint32_t i0 = tid; i0 < n; i0 += U * CT) {
+    Raw8<SRC> raw[U][2];
+    float scale[U][2];
+    int32_t kind[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], scale);
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = min(i0 + u * CT, n - 1);
+      const uint32_t hr = pieces == 1 ? i : __umulhi(i, by_pieces), t = c.heads == 1 ? hr : __umulhi(hr, by_heads);
+      const uint32_t piece = i - hr * pieces, head = hr - t * c.heads;
+      kind[u] = i0 + u * CT < n ? sh.kind[t] : -1;  // (a token without a place reads slot 0)
+      const int64_t at = sh.at[t] + (int64_t)head * c.head_stride + piece * 8;
+      raw[u][0] = load_raw8<SRC>((const char *)c.keys + at * type_size<SRC>);
+      raw[u][1] = load_raw8<SRC>((const char *)c.values + at * type_size<SRC>);
+      if constexpr (type_is_8bit<SRC>) {
+        const int64_t sc = sh.scale[t] + (int64_t)head * c.scale_head_stride;
+        scale[u][0] = c.key_scales[sc];
+        scale[u][1] = c.value_scales[sc];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (kind[u] < 0) continue;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        float x[8];
+        to_f32(raw[u][v], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (type_is_8bit<SRC>) x[e] = __fmul_rn(x[e], scale[u][v]);
+          x[e] = kind[u] ? x[e] : 0.0f;
+        }
+        store_raw8<DST>((char *)(v ? a.v : a.k) + (out + i0 + u * CT) * 8 * type_size<DST>, from_f32<DST>(x));
       }
     }
   }
-  store_raw8<DST>((char *)(values ? a.v : a.k) + ((int64_t)id * c.dim + j * 8) * type_size<DST>, from_f32<DST>(x));
 }
 
 // ---- reorder --------------------------------------------------------------------------------------------------------------
@@ -167,8 +239,14 @@ hipError_t launch_write(const gsk_cache &c, const gsk_rows &a, hipStream_t s) {
     by_type(c.type, [&](auto dst) {
       if constexpr (!type_is_8bit<src()> && dst() != GSK_F32) {
         by_lanes(c.dim, [&](auto gl) {
-          const uint64_t threads = (uint64_t)a.tokens * c.heads * gl();
-          hipLaunchKernelGGL((write_kernel<src(), dst(), gl()>), dim3((uint32_t)((threads + CT - 1) / CT), 2), dim3(CT), 0, s, c, a);
+          const uint64_t rows = (uint64_t)a.tokens * c.heads, each = CT / gl();
+          auto go = [&](auto n) {
+            const dim3 grid((uint32_t)((rows + each * n() - 1) / (each * n())), 2);
+            hipLaunchKernelGGL((write_kernel<src(), dst(), gl(), n()>), grid, dim3(CT), 0, s, c, a);
+          };
+          // rows one after the other pay once every CU has workgroups to spare
+          if (rows >= each * 4096) go(std::integral_constant<int, 4>{});
+          else go(std::integral_constant<int, 1>{});
         });
       }
     });
@@ -177,13 +255,20 @@ hipError_t launch_write(const gsk_cache &c, const gsk_rows &a, hipStream_t s) {
 }
 
 hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s) {
+  // tokens of a workgroup: as many as leave the launch 2048 of them
+  uint32_t tokens = 1;
+  while (tokens < RTOK && a.rows / tokens >= 4096) tokens *= 2;
+  const uint32_t pieces = c.dim / 8;
+  auto inverse = [](uint32_t d) { return (uint32_t)(((1ull << 32) + d - 1) / d); };  // x / d = umulhi(x, it), x d < 2^32, d > 1
   by_type(c.type, [&](auto src) {
     by_type(a.type, [&](auto dst) {
       if constexpr (src() != GSK_F32 && !type_is_8bit<dst()>) {
-        by_lanes(c.dim, [&](auto gl) {
-          const uint64_t threads = (uint64_t)a.rows * c.heads * gl();
-          hipLaunchKernelGGL((read_kernel<src(), dst(), gl()>), dim3((uint32_t)((threads + CT - 1) / CT), 2), dim3(CT), 0, s, c, a);
-        });
+        auto go = [&](auto u) {
+          hipLaunchKernelGGL((read_kernel<src(), dst(), u()>), dim3((a.rows + tokens - 1) / tokens), dim3(CT), 0, s, c, a, tokens,
+                             inverse(pieces), inverse(c.heads));
+        };
+        if ((uint64_t)tokens * c.heads * pieces >= 4 * CT) go(std::integral_constant<int, 4>{});
+        else go(std::integral_constant<int, 1>{});
       }
     });
   });

@@ -1,15 +1,18 @@
 // Beam search's selection (gsk_beam, include/gsk.h): for each request the n best of score + log softmax over its beams and the
 // vocabulary.
 //
-// One pass over the logits. A row is cut into slices of BS tokens, one a workgroup, held in registers. The slice's n largest: the
-// n-th largest of the 256 threads' maxima is a bound that n elements reach, so the elements that reach it are listed (about n
-// of them in an unordered row) and ranked by counting; where more tie with the bound than the list holds, the n-th largest
-// (value, token) is found digit by digit instead. The slice leaves its maximum m, its sum of exp(x - m) and its list. The sum decides
-// the order of tokens of different beams, so the large terms, the listed ones, are fp64; the many small ones are fp32 in each
-// thread (their errors average out: about 1e-9 of the sum) and fp64 from there on. The last workgroup of a request (a ticket)
-// joins its beams' slices: log of each beam's sum, then the n best of all lists by the same two steps over the lists' heads.
+// One pass over the logits. A row is cut into slices of BS tokens, one a workgroup, held in registers. The slice's n largest: in
+// each of the four waves, a quarter of n lanes' maxima (rounded up) reach some value, so n elements reach the least of the four;
+// the elements that reach it are listed (a few more than n in an unordered row) and ranked by counting; where more tie with the
+// bound than the list holds, the n-th largest (value, token) is found digit by digit instead. The slice leaves its maximum m, its
+// sum of exp(x - m) and its list. The sum decides the order of tokens of different beams, so the large terms, the listed ones,
+// are fp64; the many small ones are fp32 in each thread (their errors average out: about 1e-9 of the sum) and fp64 from there on.
+// The last workgroup of a request (a ticket) joins its beams' slices: log of each beam's sum, then the n best of all lists by the
+// same two steps over the lists' heads.
 #include "gsk_dev.h"
 #include "gsk_int.h"
+
+#include <float.h>
 
 namespace gse {
 
@@ -96,48 +99,49 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
   const int64_t lists = (int64_t)a.requests * a.beams * slices;
   SliceSum *sums = (SliceSum *)a.work;
   uint64_t *tops = (uint64_t *)(sums + lists);
-  // the slice's elements as order-preserving keys: 0 for NaN, KEY_NEGINF for what is past the row
-  uint32_t key[BE];
+  // the slice's elements, -inf for NaN and past the row
+  float v[BE];
   const char *x = (const char *)a.logits + (int64_t)row * a.ld * type_size<T>;
   const uint32_t t0 = slice * BS;
   constexpr int VE = WIDE ? 8 : 1;  // elements of a load
   auto token = [&](int e) { return t0 + (uint32_t)(e / VE) * (BT * VE) + tid * VE + (uint32_t)(e % VE); };
+  if (WIDE && t0 + BS <= a.vocab) {
 #pragma unroll
-  for (int e = 0; e < BE; e += VE) {
-    const uint32_t t = token(e);
-    if constexpr (WIDE) {
-      float f[8];
-      if (t + 8 <= a.vocab) {
-        to_f32(load_raw8<T>(x + (int64_t)t * type_size<T>), f);
-      } else {
+    for (int e = 0; e < BE; e += 8) to_f32(load_raw8<T>(x + (int64_t)token(e) * type_size<T>), *(float(*)[8])(v + e));
+  } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = t + i < a.vocab ? load_logit(x, T, t + i) : -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) key[e + i] = fkey(f[i]);
-    } else {
-      key[e] = fkey(t < a.vocab ? load_logit(x, T, t) : -INFINITY);
-    }
+    for (int e = 0; e < BE; ++e) v[e] = token(e) < a.vocab ? load_logit(x, T, token(e)) : -INFINITY;
   }
-  uint32_t top = 0;
+  float top = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < BE; ++e) top = max(top, key[e]);
-  const uint32_t most = (uint32_t)block_max_u64(top, sh.redu);
-  const float m = fkey_inv(most);
-  const bool some = most > KEY_NEGINF && most < KEY_POSINF;  // (+inf: the row gives nothing)
-  const uint32_t bound = max(block_kth_u32(top, n, (uint32_t *)sh.list), KEY_NEGINF + 1);
+  for (int e = 0; e < BE; ++e) {
+    v[e] = fmaxf(v[e], -INFINITY);
+    top = fmaxf(top, v[e]);
+  }
+  // each wave's bound, of the values' upper 16 bits; the slice's maximum
+  const uint32_t own = fkey(top) >> 16, kth = wave_kth_largest_u16(own, (int)(n + 3) / 4) << 16, most = wave_max_u32(fkey(top));
+  if (lane_id() == 0) sh.redu[tid / WAVE] = (uint64_t)most << 32 | kth;
   if (tid == 0) sh.n = 0;
   __syncthreads();
+  uint32_t best = 0, bound_key = ~0u;
+#pragma unroll
+  for (int i = 0; i < BT / WAVE; ++i) {
+    best = max(best, (uint32_t)(sh.redu[i] >> 32));
+    bound_key = min(bound_key, (uint32_t)sh.redu[i]);
+  }
+  const float m = fkey_inv(best);
+  const bool some = best > KEY_NEGINF && best < KEY_POSINF;  // (+inf: the row gives nothing)
+  const float bound = bound_key > KEY_NEGINF ? fkey_inv(bound_key) : -FLT_MAX;
+  auto term = [&](float y) { return __builtin_amdgcn_exp2f((y - m) * 1.44269504f); };
   double sum = 0;
   if (some) {
     float rest = 0;
 #pragma unroll
     for (int e = 0; e < BE; ++e) {
-      if (key[e] >= bound) {
+      rest += term(v[e]);
+      if (v[e] >= bound) {
         const uint32_t k = atomicAdd(&sh.n, 1u);
-        if (k < BL) sh.list[k] = pack(key[e], token(e));
-      } else if (key[e] > KEY_NEGINF) {
-        rest += __builtin_amdgcn_exp2f((fkey_inv(key[e]) - m) * 1.44269504f);
+        if (k < BL) sh.list[k] = pack(fkey(v[e]), token(e));
       }
     }
     sum = rest;
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
   __syncthreads();
   uint32_t count = sh.n;
   if (count > BL) {
-    // the n-th largest (key, token), 8 bits at a time; the terms between it and the bound are summed here
+    // the n-th largest (value, token), 8 bits at a time
     uint64_t prefix = 0;
     uint32_t want = n;
     for (int shift = 56; shift >= 0; shift -= 8) {
@@ -154,8 +158,8 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < BE; ++e) {
-        const uint64_t p = pack(key[e], token(e));
-        if (key[e] >= bound && (shift == 56 || (p >> (shift + 8)) == (prefix >> (shift + 8))))
+        const uint64_t p = pack(fkey(v[e]), token(e));
+        if (v[e] >= bound && (shift == 56 || (p >> (shift + 8)) == (prefix >> (shift + 8))))
           atomicAdd(&sh.hist[(p >> shift) & 255], 1u);
       }
       __syncthreads();
@@ -172,22 +176,18 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
     }
     if (tid == 0) sh.n = 0;
     __syncthreads();
-    float rest = 0;
 #pragma unroll
     for (int e = 0; e < BE; ++e) {
-      const uint64_t p = pack(key[e], token(e));
-      if (key[e] < bound) continue;
-      if (p >= prefix) sh.list[atomicAdd(&sh.n, 1u)] = p;
-      else rest += __builtin_amdgcn_exp2f((fkey_inv(key[e]) - m) * 1.44269504f);
+      const uint64_t p = pack(fkey(v[e]), token(e));
+      if (v[e] >= bound && p >= prefix) sh.list[atomicAdd(&sh.n, 1u)] = p;
     }
-    sum += rest;
     __syncthreads();
     count = sh.n;
   }
   uint64_t *out = tops + ((int64_t)row * slices + slice) * n;
   for (uint32_t i = tid; i < count; i += BT) {
     const uint64_t p = sh.list[i];
-    sum += exp((double)fkey_inv(pk_key(p)) - (double)m);
+    sum += exp((double)fkey_inv(pk_key(p)) - (double)m) - (double)term(fkey_inv(pk_key(p)));
     uint32_t rank = 0;
     for (uint32_t k = 0; k < count; ++k) rank += sh.list[k] > p;
     if (rank < n) st_ag(out + rank, p);
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
   if (tid == 0) {
     SliceSum *o = sums + (int64_t)row * slices + slice;
     st_ag((uint64_t *)&o->sum, (uint64_t)__double_as_longlong(some ? sum : 0.0));
-    st_ag((uint64_t *)&o->max, (uint64_t)__float_as_uint(some ? m : -INFINITY) | (uint64_t)(most >= KEY_POSINF) << 32);
+    st_ag((uint64_t *)&o->max, (uint64_t)__float_as_uint(some ? m : -INFINITY) | (uint64_t)(best >= KEY_POSINF) << 32);
   }
   store_wait();
   __syncthreads();
@@ -242,9 +242,9 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
     return dkey(((double)fkey_inv(pk_key(p)) - sh.base[b]) - sh.shift[b] + sh.score[b]);
   };
   // a bound that n entries reach: the n-th largest of the threads' largest heads, by its upper 32 bits
-  uint64_t best = 0;
-  for (uint32_t i = tid; i < total; i += BT) best = max(best, value(i, ld_ag(heads + (int64_t)i * n)));
-  const uint64_t from = max((uint64_t)block_kth_u32((uint32_t)(best >> 32), n, (uint32_t *)sh.list) << 32, (uint64_t)1);
+  uint64_t lead = 0;
+  for (uint32_t i = tid; i < total; i += BT) lead = max(lead, value(i, ld_ag(heads + (int64_t)i * n)));
+  const uint64_t from = max((uint64_t)block_kth_u32((uint32_t)(lead >> 32), n, (uint32_t *)sh.list) << 32, (uint64_t)1);
   if (tid == 0) sh.n = 0;
   __syncthreads();
   for (uint32_t i = tid; i < total; i += BT) {

@@ -21,7 +21,7 @@ __device__ __forceinline__ Place place(const gsk_cache &c, uint32_t pg, uint32_t
 }
 
 template <uint32_t SRC, uint32_t DST, int GL, int ROWS>
-__global__ __launch_bounds__(CT) void write_kernel(gsk_cache c, gsk_rows a) {
+__global__ __launch_bounds__(CT) void write_kernel(gsk_cache c, gsk_rows a, Div heads, Div page) {
   const uint32_t j = threadIdx.x % GL, rows = a.tokens * c.heads;
   const uint32_t first = blockIdx.x * (CT / GL * ROWS) + threadIdx.x / GL;
   const bool values = blockIdx.y != 0, mine = j * 8 < c.dim;
@@ -35,8 +35,7 @@ __global__ __launch_bounds__(CT) void write_kernel(gsk_cache c, gsk_rows a) {
   uint32_t head[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const uint32_t id = first + i * (CT / GL), t = min(id, rows - 1) / c.heads;
-    head[i] = min(id, rows - 1) - t * c.heads;
+    const uint32_t id = first + i * (CT / GL), t = quotient(min(id, rows - 1), heads, head[i]);
     slot[i] = id < rows ? (uint64_t)a.slot[t] : ~0ull;
     raw[i] = Raw8<SRC>{};
     if (mine) raw[i] = load_raw8<SRC>(src + (int64_t)t * ts + (int64_t)head[i] * hs);
@@ -44,16 +43,16 @@ __global__ __launch_bounds__(CT) void write_kernel(gsk_cache c, gsk_rows a) {
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     if (slot[i] >= (uint64_t)c.pages * c.page) continue;  // (negative ones are past it; the group as a whole)
-    const uint32_t pg = (uint32_t)slot[i] / c.page;
-    const Place p = place(c, pg, (uint32_t)slot[i] - pg * c.page, head[i]);
+    uint32_t off;
+    const uint32_t pg = quotient((uint32_t)slot[i], page, off);
+    const Place p = place(c, pg, off, head[i]);
     float x[8];
     to_f32(raw[i], x);
     if constexpr (type_is_8bit<DST>) {
       uint32_t m = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-#pragma unroll
-      for (int k = GL / 2; k > 0; k /= 2) m = max(m, shfl_xor_u32(m, k));
+      m = group_max<GL>(m);
       const bool bad = m >= 0x7F800000u;
       const float most = DST == GSK_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f;
       const float scale = fmaxf(__fmul_rn(__uint_as_float(m), most), 0x1p-126f), inv = __fdiv_rn(1.0f, scale);
@@ -77,7 +76,7 @@ struct ReadShared {
 };
 
 template <uint32_t SRC, uint32_t DST, int U>
-__global__ __launch_bounds__(CT) void read_kernel(gsk_cache c, gsk_read_rows a, uint32_t tokens, uint32_t by_pieces, uint32_t by_heads) {
+__global__ __launch_bounds__(CT) void read_kernel(gsk_cache c, gsk_read_rows a, uint32_t tokens, Div by_pieces, Div by_heads) {
   __shared__ ReadShared sh;
   const uint32_t tid = threadIdx.x, row0 = blockIdx.x * tokens, pieces = c.dim / 8;
   if (tid < WAVE) {
@@ -120,8 +119,8 @@ __global__ __launch_bounds__(CT) void read_kernel(gsk_cache c, gsk_read_rows a, 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t i = min(i0 + u * CT, n - 1);
-      const uint32_t hr = pieces == 1 ? i : __umulhi(i, by_pieces), t = c.heads == 1 ? hr : __umulhi(hr, by_heads);
-      const uint32_t piece = i - hr * pieces, head = hr - t * c.heads;
+      uint32_t piece, head;
+      const uint32_t t = quotient(quotient(i, by_pieces, piece), by_heads, head);
       kind[u] = i0 + u * CT < n ? sh.kind[t] : -1;  // (a token without a place reads slot 0)
       const int64_t at = sh.at[t] + (int64_t)head * c.head_stride + piece * 8;
       raw[u][0] = load_raw8<SRC>((const char *)c.keys + at * type_size<SRC>);
@@ -150,6 +149,8 @@ __global__ __launch_bounds__(CT) void read_kernel(gsk_cache c, gsk_read_rows a, 
   }
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // ---- reorder --------------------------------------------------------------------------------------------------------------
 // A thread owns one vector of one token of one cache, in every beam of a group: it loads the vectors of all beams that move
 // before it stores any, so that the beams are permuted in place without a copy; no vector belongs to two threads. A workgroup
@@ -162,7 +163,7 @@ struct ReorderShared {
 };
 
 template <typename VEC, int MB>
-__global__ __launch_bounds__(CT) void reorder_kernel(gsk_reorder_beams a, uint32_t vecs) {
+__global__ __launch_bounds__(CT) void reorder_kernel(gsk_reorder_beams a, Div vecs, Div chunks) {
   __shared__ ReorderShared sh;
   constexpr uint32_t TB = CT / MB;  // tokens of a block
   const uint32_t g = blockIdx.z, tid = threadIdx.x, beam = tid % MB, tok = tid / MB;
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(CT) void reorder_kernel(gsk_reorder_beams a, uint32
   }
   const bool moves = from != row && first >= 0;
   const int64_t most = min((int64_t)wave_max_u64(moves && len > 0 ? (uint64_t)len : 0), (int64_t)a.max_pages * a.page);
-  const uint32_t columns = a.caches * a.chunks * TB * vecs;
+  const uint32_t columns = a.caches * a.chunks * TB * vecs.d;
   for (int64_t t0 = first + (int64_t)blockIdx.y * TB; t0 < most; t0 += (int64_t)gridDim.y * TB) {
     const int64_t t = t0 + tok;
     uint32_t ps = 0, pd = 0, off = 0;
@@ -199,11 +200,11 @@ __global__ __launch_bounds__(CT) void reorder_kernel(gsk_reorder_beams a, uint32
     if (beam == 0) sh.n[tok] = (uint32_t)__popcll(mine);
     __syncthreads();
     for (uint32_t id = blockIdx.x * CT + tid; id < columns; id += gridDim.x * CT) {
-      const uint32_t x = id / vecs, place = id - x * vecs, cc = x / TB, to = x - cc * TB, n = sh.n[to];
+      uint32_t place, chunk;
+      const uint32_t x = quotient(id, vecs, place), k = quotient(x / TB, chunks, chunk), to = x % TB, n = sh.n[to];
       if (n == 0) continue;
-      const uint32_t k = cc / a.chunks;
       char *base = a.cache_ptrs ? (char *)a.cache_ptrs[k] : (char *)a.cache + k * a.cache_stride;
-      base += (int64_t)(cc - k * a.chunks) * a.chunk_stride + (int64_t)place * sizeof(VEC);
+      base += (int64_t)chunk * a.chunk_stride + (int64_t)place * sizeof(VEC);
       VEC v[MB];
 #pragma unroll
       for (uint32_t e = 0; e < MB; ++e)
@@ -242,7 +243,7 @@ hipError_t launch_write(const gsk_cache &c, const gsk_rows &a, hipStream_t s) {
           const uint64_t rows = (uint64_t)a.tokens * c.heads, each = CT / gl();
           auto go = [&](auto n) {
             const dim3 grid((uint32_t)((rows + each * n() - 1) / (each * n())), 2);
-            hipLaunchKernelGGL((write_kernel<src(), dst(), gl(), n()>), grid, dim3(CT), 0, s, c, a);
+            hipLaunchKernelGGL((write_kernel<src(), dst(), gl(), n()>), grid, dim3(CT), 0, s, c, a, div_by(c.heads), div_by(c.page));
           };
           // rows one after the other pay once every CU has workgroups to spare
           if (rows >= each * 4096) go(std::integral_constant<int, 4>{});
@@ -259,13 +260,12 @@ hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s
   uint32_t tokens = 1;
   while (tokens < RTOK && a.rows / tokens >= 4096) tokens *= 2;
   const uint32_t pieces = c.dim / 8;
-  auto inverse = [](uint32_t d) { return (uint32_t)(((1ull << 32) + d - 1) / d); };  // x / d = umulhi(x, it), x d < 2^32, d > 1
   by_type(c.type, [&](auto src) {
     by_type(a.type, [&](auto dst) {
       if constexpr (src() != GSK_F32 && !type_is_8bit<dst()>) {
         auto go = [&](auto u) {
           hipLaunchKernelGGL((read_kernel<src(), dst(), u()>), dim3((a.rows + tokens - 1) / tokens), dim3(CT), 0, s, c, a, tokens,
-                             inverse(pieces), inverse(c.heads));
+                             div_by(pieces), div_by(c.heads));
         };
         if ((uint64_t)tokens * c.heads * pieces >= 4 * CT) go(std::integral_constant<int, 4>{});
         else go(std::integral_constant<int, 1>{});
@@ -276,7 +276,7 @@ hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s
 }
 
 hipError_t launch_reorder(const gsk_reorder_beams &in, hipStream_t s) {
-  constexpr int64_t WGS = 4096;  // workgroups of a launch to aim for
+  constexpr int64_t WGS = 4096, EACH = 4;  // workgroups of a launch to aim for, a thread's vectors of a block of tokens
   auto go = [&](auto v, auto mb) {
     using V = decltype(v);
     constexpr int MB = mb();
@@ -290,9 +290,10 @@ hipError_t launch_reorder(const gsk_reorder_beams &in, hipStream_t s) {
       a.seq_len += (int64_t)g0 * in.beams;
       a.parent += (int64_t)g0 * in.beams;
       if (a.first) a.first += g0;
-      const int64_t x = min((columns + CT - 1) / CT, max((int64_t)1, WGS / a.groups));
+      const int64_t x = max(min((columns + EACH * CT - 1) / (EACH * CT), WGS / a.groups), (int64_t)1);
       const int64_t y = min(min(blocks, (int64_t)65535), max((int64_t)1, WGS / (a.groups * x)));
-      hipLaunchKernelGGL((reorder_kernel<V, MB>), dim3((uint32_t)x, (uint32_t)y, a.groups), dim3(CT), 0, s, a, vecs);
+      hipLaunchKernelGGL((reorder_kernel<V, MB>), dim3((uint32_t)x, (uint32_t)y, a.groups), dim3(CT), 0, s, a, div_by(vecs),
+                         div_by(in.chunks));
     }
   };
   auto by_beams = [&](auto v) {
@@ -304,7 +305,7 @@ hipError_t launch_reorder(const gsk_reorder_beams &in, hipStream_t s) {
   // the widest vector that every address is a multiple of
   const uint64_t all = (uint64_t)in.chunk_bytes | (uint64_t)in.page_stride | (uint64_t)in.token_stride | (uint64_t)in.chunk_stride |
                        (in.cache_ptrs ? (uint64_t)in.align : (uint64_t)in.cache | (uint64_t)in.cache_stride);
-  if (all % 16 == 0) by_beams(uint4{});
+  if (all % 16 == 0) by_beams(u32x4{});
   else if (all % 4 == 0) by_beams(uint32_t{});
   else by_beams(uint8_t{});
   return hipGetLastError();

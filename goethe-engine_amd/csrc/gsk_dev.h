@@ -81,13 +81,14 @@ __device__ __forceinline__ Raw8<T> from_f32(const float (&x)[8]) {
       r.w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w, true);
     }
   }
-  if constexpr (T == GSK_I8) {
+  if constexpr (T == GSK_I8) {  // (added to 1.5 * 2^23, a number's lowest byte is its nearest whole number)
+    uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      r.w[i] = 0;
+    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(x[i] + 12582912.0f);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) r.w[i] |= ((uint32_t)(int32_t)rintf(x[4 * i + k]) & 0xFFu) << (8 * k);
-    }
+    for (int i = 0; i < 2; ++i)
+      r.w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * i + 3], b[4 * i + 2], 0x0C0C0400u),
+                                     __builtin_amdgcn_perm(b[4 * i + 1], b[4 * i], 0x0C0C0400u), 0x05040100u);
   }
   return r;
 }
@@ -100,6 +101,29 @@ __device__ __forceinline__ void store_raw8(void *p, const Raw8<T> &r) {
 #pragma unroll
     for (int i = 0; i < Raw8<T>::N; i += 4) ((uint4 *)p)[i / 4] = *(const uint4 *)(r.w + i);
   }
+}
+
+// Division by a number of the host's choice: the quotient by its inverse is the one wanted or one less.
+struct Div {
+  uint32_t d, inverse;
+};
+inline Div div_by(uint32_t d) { return {d, d > 1 ? (uint32_t)((1ull << 32) / d) : ~0u}; }
+__device__ __forceinline__ uint32_t quotient(uint32_t x, Div v, uint32_t &rest) {
+  uint32_t q = __umulhi(x, v.inverse);
+  rest = x - q * v.d;
+  if (rest >= v.d) rest -= v.d, ++q;
+  return q;
+}
+
+// The largest of a group of 8, 16 or 32 lanes, in each of them.
+template <int GL>
+__device__ __forceinline__ uint32_t group_max(uint32_t m) {
+  m = max(m, dpp32<0xB1, 0xF>(0u, m));   // lane ^ 1
+  m = max(m, dpp32<0x4E, 0xF>(0u, m));   // lane ^ 2
+  m = max(m, dpp32<0x141, 0xF>(0u, m));  // mirrored in eight
+  if constexpr (GL > 8) m = max(m, dpp32<0x140, 0xF>(0u, m));  // mirrored in sixteen
+  if constexpr (GL > 16) m = max(m, shfl_xor_u32(m, 16));
+  return m;
 }
 
 // The last r in [0, n) with first[r] <= x (first ascends), 0 where there is none: found by the whole wave, 64 entries a step.

@@ -857,7 +857,7 @@ GSE_API int64_t gsk_beams_work(gse_handle *h, const gsk_beams *in) {
   gsk_beams b;
   if (!take(in, b)) return fail(h, GSE_E_ARG, "null or short gsk_beams");
   if (int rc = check_beams(h, b)) return rc;
-  return gse::beam_work(b);
+  return gse::beam_work(b, (int)h->target / 4);
 }
 
 GSE_API int gsk_beam(gse_handle *h, const gsk_beams *in) {
@@ -869,11 +869,11 @@ GSE_API int gsk_beam(gse_handle *h, const gsk_beams *in) {
   if (!b.logits || !b.scores || !b.tokens || !b.parents || !b.out_scores)
     return fail(h, GSE_E_ARG, "logits, scores, tokens, parents and out_scores are required");
   if (b.ld < (int64_t)b.vocab) return fail(h, GSE_E_ARG, "ld < vocab");
-  const int64_t need = gse::beam_work(b);
+  const int64_t need = gse::beam_work(b, (int)h->target / 4);
   if (b.work_bytes < need || !b.work || (uint64_t)b.work % 16)
     return fail(h, GSE_E_CAPACITY, "%lld bytes of scratch, %lld are needed", (long long)b.work_bytes, (long long)need);
   DeviceGuard g(h->device);
-  hipError_t e = gse::launch_beam(b, h->ptick, std::max(h->max_rows, gse::TICKS), (hipStream_t)b.stream);
+  hipError_t e = gse::launch_beam(b, (int)h->target / 4, h->ptick, std::max(h->max_rows, gse::TICKS), (hipStream_t)b.stream);
   return e == hipSuccess ? GSE_OK : hip_fail(h, e, "beam launch");
 }
 

@@ -1,14 +1,18 @@
 // Beam search's selection (gsk_beam, include/gsk.h): for each request the n best of score + log softmax over its beams and the
 // vocabulary.
 //
-// One pass over the logits. A row is cut into slices of BS tokens, one a workgroup, held in registers. The slice's n largest: in
-// each of the four waves, a quarter of n lanes' maxima (rounded up) reach some value, so n elements reach the least of the four;
-// the elements that reach it are listed (a few more than n in an unordered row) and ranked by counting; where more tie with the
-// bound than the list holds, the n-th largest (value, token) is found digit by digit instead. The slice leaves its maximum m, its
-// sum of exp(x - m) and its list. The sum decides the order of tokens of different beams, so the large terms, the listed ones,
-// are fp64; the many small ones are fp32 in each thread (their errors average out: about 1e-9 of the sum) and fp64 from there on.
-// The last workgroup of a request (a ticket) joins its beams' slices: log of each beam's sum, then the n best of all lists by the
-// same two steps over the lists' heads.
+// One pass over the logits. A row is cut into slices of BS tokens, held in registers; a workgroup takes one or more slices of a
+// row in turn (the next one's loads in flight) and keeps the n largest so far. A slice's n largest: in each of the four waves, a
+// quarter of n lanes' maxima (rounded up) reach some value, so n elements reach the least of the four; the elements that reach
+// it, and the n-th largest of the slices before, are listed (a few more than n in an unordered row) and ranked by counting; where
+// more tie with the bound than the list holds, the n-th largest (value, token) is found digit by digit instead. The workgroup
+// leaves its maximum m, its sum of exp(x - m) and its list. The sum decides the order of tokens of different beams, so the large
+// terms, the listed ones, are fp64 (their differences from the fp32 ones added up as whole multiples of 2^-62: in any order the
+// same, so that equal rows have equal sums); the many small ones are fp32 in each thread (their errors average out: about 1e-9 of
+// the sum) and fp64 from there on. The last workgroup of a request (a ticket) joins its beams' lists: log of each beam's sum, then
+// the n best of all entries by the same two steps.
+//
+// A workgroup lives 8 us for one slice and the device starts about 94 of them a us, so a large call has one round of them.
 #include "gsk_dev.h"
 #include "gsk_int.h"
 
@@ -22,9 +26,10 @@ constexpr int BT = 256;
 constexpr uint32_t BS = 8192;      // tokens of a slice
 constexpr int BE = BS / BT;        // a thread's elements
 constexpr uint32_t BL = 1024;      // entries of the list
-constexpr uint32_t BLISTS = GSK_MAX_BEAMS;
+constexpr uint32_t LISTS = 1024;   // a request's lists, at most
+constexpr int AHEAD = 8;           // entries of its request's lists that a thread reads at once in the join
 
-struct SliceSum {  // a slice's part of its row's sum
+struct ListSum {  // a workgroup's part of its row's sum
   double sum;
   float max;
   uint32_t bad;  // a +inf among the logits
@@ -32,13 +37,18 @@ struct SliceSum {  // a slice's part of its row's sum
 
 struct BeamShared {
   uint64_t list[BL];
-  uint64_t sub[BL];  // (the join: the entries' places)
+  union {
+    uint64_t sub[BL];                 // (the join: the entries' places)
+    double sums[LISTS];               // (before that: the lists' sums)
+  };
+  uint64_t best[GSK_MAX_KEEP];        // the n largest so far
+  float maxs[LISTS];                  // the join: the lists' maxima (NaN: a +inf in the row)
   double red[BT / WAVE];
   uint64_t redu[BT / WAVE];
   uint32_t hist[256];
+  unsigned long long fix;             // the listed terms' fp64 values less their fp32 ones, in units of 2^-62
   uint32_t n, last, rank;
-  double base[BLISTS], shift[BLISTS];  // a beam's maximum; log of its sum
-  double score[BLISTS];
+  double base[GSK_MAX_BEAMS], shift[GSK_MAX_BEAMS], score[GSK_MAX_BEAMS];  // a beam's maximum, log of its sum, score
 };
 
 __device__ __forceinline__ float load_logit(const void *p, uint32_t type, int64_t i) {
@@ -92,142 +102,186 @@ __device__ __forceinline__ double dkey_inv(uint64_t k) {
 }
 
 template <uint32_t T, bool WIDE>
-__global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, uint32_t *tick, uint32_t r0) {
+__global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts, uint32_t *tick, uint32_t r0) {
   __shared__ BeamShared sh;
-  const uint32_t tid = threadIdx.x, slice = blockIdx.x, beam = blockIdx.y % a.beams, r = r0 + blockIdx.y / a.beams;
-  const uint32_t row = r * a.beams + beam, n = a.n;
-  const int64_t lists = (int64_t)a.requests * a.beams * slices;
-  SliceSum *sums = (SliceSum *)a.work;
-  uint64_t *tops = (uint64_t *)(sums + lists);
-  // the slice's elements, -inf for NaN and past the row
-  float v[BE];
+  const uint32_t tid = threadIdx.x, part = blockIdx.x, beam = blockIdx.y % a.beams, r = r0 + blockIdx.y / a.beams;
+  const uint32_t row = r * a.beams + beam, n = a.n, lane = lane_id(), wave = tid / WAVE;
+  ListSum *sums = (ListSum *)a.work;
+  uint64_t *tops = (uint64_t *)(sums + (int64_t)a.requests * a.beams * parts);
   const char *x = (const char *)a.logits + (int64_t)row * a.ld * type_size<T>;
-  const uint32_t t0 = slice * BS;
+  const uint32_t slices = (a.vocab + BS - 1) / BS, first = (uint32_t)((uint64_t)slices * part / parts);
+  const uint32_t end = (uint32_t)((uint64_t)slices * (part + 1) / parts);
   constexpr int VE = WIDE ? 8 : 1;  // elements of a load
-  auto token = [&](int e) { return t0 + (uint32_t)(e / VE) * (BT * VE) + tid * VE + (uint32_t)(e % VE); };
-  if (WIDE && t0 + BS <= a.vocab) {
+  // a slice's elements as they are (16 bytes a load), or one by one where a row or its end is not aligned
+  Raw8<T> raw[BE / 8];
+  float v[BE];
+  auto token = [&](uint32_t slice, int e) { return slice * BS + (uint32_t)(e / VE) * (BT * VE) + tid * VE + (uint32_t)(e % VE); };
+  auto whole = [&](uint32_t slice) { return WIDE && (slice + 1) * BS <= a.vocab; };
+  auto load = [&](uint32_t slice) {
 #pragma unroll
-    for (int e = 0; e < BE; e += 8) to_f32(load_raw8<T>(x + (int64_t)token(e) * type_size<T>), *(float(*)[8])(v + e));
-  } else {
-#pragma unroll
-    for (int e = 0; e < BE; ++e) v[e] = token(e) < a.vocab ? load_logit(x, T, token(e)) : -INFINITY;
-  }
+    for (int e = 0; e < BE; e += 8) raw[e / 8] = load_raw8<T>(x + (int64_t)token(slice, e) * type_size<T>);
+  };
+  if (whole(first)) load(first);
+  uint32_t kept = 0;          // entries of sh.best
+  uint32_t top_key = 0;       // of the slices before: their largest value ...
   float top = -INFINITY;
+  double sum = 0;             // ... and the thread's part of the sum of exp(x - it)
+  auto settle = [&] {         // the listed terms of the slice before (thread 0; after a barrier)
+    sum += (double)(long long)sh.fix * 0x1p-62;
+    sh.fix = 0;
+  };
+  if (tid == 0) sh.fix = 0;
+  for (uint32_t slice = first; slice < end; ++slice) {
+    if (whole(slice)) {
 #pragma unroll
-  for (int e = 0; e < BE; ++e) {
-    v[e] = fmaxf(v[e], -INFINITY);
-    top = fmaxf(top, v[e]);
-  }
-  // each wave's bound, of the values' upper 16 bits; the slice's maximum
-  const uint32_t own = fkey(top) >> 16, kth = wave_kth_largest_u16(own, (int)(n + 3) / 4) << 16, most = wave_max_u32(fkey(top));
-  if (lane_id() == 0) sh.redu[tid / WAVE] = (uint64_t)most << 32 | kth;
-  if (tid == 0) sh.n = 0;
-  __syncthreads();
-  uint32_t best = 0, bound_key = ~0u;
+      for (int e = 0; e < BE; e += 8) to_f32(raw[e / 8], *(float(*)[8])(v + e));
+    } else {
 #pragma unroll
-  for (int i = 0; i < BT / WAVE; ++i) {
-    best = max(best, (uint32_t)(sh.redu[i] >> 32));
-    bound_key = min(bound_key, (uint32_t)sh.redu[i]);
-  }
-  const float m = fkey_inv(best);
-  const bool some = best > KEY_NEGINF && best < KEY_POSINF;  // (+inf: the row gives nothing)
-  const float bound = bound_key > KEY_NEGINF ? fkey_inv(bound_key) : -FLT_MAX;
-  auto term = [&](float y) { return __builtin_amdgcn_exp2f((y - m) * 1.44269504f); };
-  double sum = 0;
-  if (some) {
+      for (int e = 0; e < BE; ++e) v[e] = token(slice, e) < a.vocab ? load_logit(x, T, token(slice, e)) : -INFINITY;
+    }
+    if (slice + 1 < end && whole(slice + 1)) load(slice + 1);
+    float most = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < BE; ++e) {
+      v[e] = fmaxf(v[e], -INFINITY);  // (NaN counts as -inf)
+      most = fmaxf(most, v[e]);
+    }
+    // each wave's bound, of the values' upper 16 bits; the slice's maximum
+    const uint32_t kth = wave_kth_largest_u16(fkey(most) >> 16, (int)(n + 3) / 4) << 16, wave_most = wave_max_u32(fkey(most));
+    __syncthreads();  // (the slice before is done with the list)
+    if (lane == 0) sh.redu[wave] = (uint64_t)wave_most << 32 | kth;
+    if (tid < kept) sh.list[tid] = sh.best[tid];
+    if (tid == 0) {
+      sh.n = kept;
+      settle();
+    }
+    __syncthreads();
+    uint32_t bound_key = ~0u, now_key = top_key;
+#pragma unroll
+    for (int i = 0; i < BT / WAVE; ++i) {
+      now_key = max(now_key, (uint32_t)(sh.redu[i] >> 32));
+      bound_key = min(bound_key, (uint32_t)sh.redu[i]);
+    }
+    if (kept == n) bound_key = max(bound_key, pk_key(sh.best[n - 1]));
+    const float now = fkey_inv(now_key);
+    if (now_key > top_key && top_key > KEY_NEGINF) sum *= exp((double)top - (double)now);
+    top_key = now_key;
+    top = now;
+    if (now_key <= KEY_NEGINF || now_key >= KEY_POSINF) continue;  // (nothing yet; or +inf: the row gives nothing)
+    const float bound = bound_key > KEY_NEGINF ? fkey_inv(bound_key) : -FLT_MAX;
+    auto term = [&](float y) { return __builtin_amdgcn_exp2f((y - now) * 1.44269504f); };
     float rest = 0;
 #pragma unroll
     for (int e = 0; e < BE; ++e) {
       rest += term(v[e]);
       if (v[e] >= bound) {
         const uint32_t k = atomicAdd(&sh.n, 1u);
-        if (k < BL) sh.list[k] = pack(fkey(v[e]), token(e));
+        if (k < BL) sh.list[k] = pack(fkey(v[e]), token(slice, e));
       }
     }
-    sum = rest;
+    sum += (double)rest;
+    __syncthreads();
+    uint32_t count = sh.n;
+    if (count > BL) {
+      // the slice's n-th largest (value, token), 8 bits at a time; read again, so that the rare path needs no registers
+      auto entry = [&](int e) {
+        const uint32_t t = slice * BS + e * BT + tid;
+        const float y = t < a.vocab ? fmaxf(load_logit(x, T, t), -INFINITY) : -INFINITY;
+        return y >= bound ? pack(fkey(y), t) : (uint64_t)0;
+      };
+      uint64_t prefix = 0;
+      uint32_t want = n;
+      for (int shift = 56; shift >= 0; shift -= 8) {
+        __syncthreads();
+        sh.hist[tid] = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int e = 0; e < BE; ++e) {
+          const uint64_t p = entry(e);
+          if (p && (shift == 56 || (p >> (shift + 8)) == (prefix >> (shift + 8)))) atomicAdd(&sh.hist[(p >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        if (tid == 0) {
+          uint32_t above = 0;
+          int d = 255;
+          while (d > 0 && above + sh.hist[d] < want) above += sh.hist[d--];
+          sh.rank = want - above;
+          sh.last = (uint32_t)d;
+        }
+        __syncthreads();
+        want = sh.rank;
+        prefix |= (uint64_t)sh.last << shift;
+      }
+      if (tid == 0) sh.n = kept;
+      __syncthreads();
+#pragma unroll 1
+      for (int e = 0; e < BE; ++e) {
+        const uint64_t p = entry(e);
+        if (p >= prefix) sh.list[atomicAdd(&sh.n, 1u)] = p;
+      }
+      __syncthreads();
+      count = sh.n;
+    }
+    for (uint32_t i = tid; i < count; i += BT) {
+      const uint64_t p = sh.list[i];
+      const float y = fkey_inv(pk_key(p));
+      if (i >= kept)
+        atomicAdd(&sh.fix, (unsigned long long)(long long)((exp((double)y - (double)now) - (double)term(y)) * 0x1p62));
+      uint32_t rank = 0;
+#pragma unroll 8
+      for (uint32_t k = 0; k < count; ++k) rank += sh.list[k] > p;
+      if (rank < n) sh.best[rank] = p;
+    }
+    kept = min(count, n);
   }
   __syncthreads();
-  uint32_t count = sh.n;
-  if (count > BL) {
-    // the n-th largest (value, token), 8 bits at a time
-    uint64_t prefix = 0;
-    uint32_t want = n;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      __syncthreads();
-      sh.hist[tid] = 0;
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < BE; ++e) {
-        const uint64_t p = pack(fkey(v[e]), token(e));
-        if (v[e] >= bound && (shift == 56 || (p >> (shift + 8)) == (prefix >> (shift + 8))))
-          atomicAdd(&sh.hist[(p >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t above = 0;
-        int d = 255;
-        while (d > 0 && above + sh.hist[d] < want) above += sh.hist[d--];
-        sh.rank = want - above;
-        sh.last = (uint32_t)d;
-      }
-      __syncthreads();
-      want = sh.rank;
-      prefix |= (uint64_t)sh.last << shift;
-    }
-    if (tid == 0) sh.n = 0;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < BE; ++e) {
-      const uint64_t p = pack(fkey(v[e]), token(e));
-      if (v[e] >= bound && p >= prefix) sh.list[atomicAdd(&sh.n, 1u)] = p;
-    }
-    __syncthreads();
-    count = sh.n;
-  }
-  uint64_t *out = tops + ((int64_t)row * slices + slice) * n;
-  for (uint32_t i = tid; i < count; i += BT) {
-    const uint64_t p = sh.list[i];
-    sum += exp((double)fkey_inv(pk_key(p)) - (double)m) - (double)term(fkey_inv(pk_key(p)));
-    uint32_t rank = 0;
-    for (uint32_t k = 0; k < count; ++k) rank += sh.list[k] > p;
-    if (rank < n) st_ag(out + rank, p);
-  }
-  for (uint32_t i = count + tid; i < n; i += BT) st_ag(out + i, (uint64_t)0);
+  if (tid == 0) settle();
+  uint64_t *out = tops + ((int64_t)row * parts + part) * n;
+  if (tid < n) st_ag(out + tid, tid < kept ? sh.best[tid] : (uint64_t)0);
   sum = block_sum_f64(sum, sh.red);
   if (tid == 0) {
-    SliceSum *o = sums + (int64_t)row * slices + slice;
-    st_ag((uint64_t *)&o->sum, (uint64_t)__double_as_longlong(some ? sum : 0.0));
-    st_ag((uint64_t *)&o->max, (uint64_t)__float_as_uint(some ? m : -INFINITY) | (uint64_t)(best >= KEY_POSINF) << 32);
+    ListSum *o = sums + (int64_t)row * parts + part;
+    st_ag((uint64_t *)&o->sum, (uint64_t)__double_as_longlong(top_key > KEY_NEGINF ? sum : 0.0));
+    st_ag((uint64_t *)&o->max, (uint64_t)__float_as_uint(top_key > KEY_NEGINF ? top : -INFINITY) | (uint64_t)(top_key >= KEY_POSINF) << 32);
   }
   store_wait();
   __syncthreads();
-  if (tid == 0) sh.last = ticket_add(tick + blockIdx.y / a.beams) == a.beams * slices - 1;
+  if (tid == 0) sh.last = ticket_add(tick + blockIdx.y / a.beams) == a.beams * parts - 1;
   __syncthreads();
   if (!sh.last) return;
   if (tid == 0) st_ag(tick + blockIdx.y / a.beams, 0u);
 
-  // ---- the join: a thread a list (a slice of a beam), in turn -------------------------------------------------------------
-  const uint32_t total = a.beams * slices, lane = lane_id(), wave = tid / WAVE;
-  const SliceSum *my = sums + (int64_t)r * total;
-  const uint64_t *heads = tops + (int64_t)r * total * n;
+  // ---- the join -----------------------------------------------------------------------------------------------------------
+  const uint32_t total = a.beams * parts, entries = total * n;  // (lists, and what they hold)
+  const ListSum *my = sums + (int64_t)r * total;
+  const uint64_t *lists = tops + (int64_t)r * entries;
+  uint64_t ahead[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) ahead[j] = j * BT + tid < entries ? ld_ag(lists + j * BT + tid) : 0;
+  for (uint32_t i = tid; i < total; i += BT) {
+    const uint64_t most = ld_ag((const uint64_t *)&my[i].max);
+    sh.sums[i] = __longlong_as_double((long long)ld_ag((const uint64_t *)&my[i].sum));
+    sh.maxs[i] = most >> 32 ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)most);
+  }
+  const float my_score = lane < a.beams ? a.scores[(int64_t)r * a.beams + lane] : 0;
+  __syncthreads();
   for (uint32_t b = wave; b < a.beams; b += BT / WAVE) {
     float bm = -INFINITY;
-    uint32_t bad = 0;
-    for (uint32_t i = lane; i < slices; i += WAVE) {
-      const uint64_t v = ld_ag((const uint64_t *)&my[b * slices + i].max);
-      bm = fmaxf(bm, __uint_as_float((uint32_t)v));
-      bad |= (uint32_t)(v >> 32);
+    bool bad = false;
+    for (uint32_t i = lane; i < parts; i += WAVE) {
+      const float y = sh.maxs[b * parts + i];
+      bad = bad || y != y;
+      bm = fmaxf(bm, y);
     }
     bm = wave_max_f32(bm);
-    bad = ballot64(bad != 0) != 0;
+    bad = ballot64(bad) != 0;
     double s = 0;
-    for (uint32_t i = lane; i < slices; i += WAVE) {
-      const double part = __longlong_as_double((long long)ld_ag((const uint64_t *)&my[b * slices + i].sum));
-      const float pm = __uint_as_float((uint32_t)ld_ag((const uint64_t *)&my[b * slices + i].max));
-      if (part > 0) s += part * exp((double)pm - (double)bm);
+    for (uint32_t i = lane; i < parts; i += WAVE) {
+      const double part_sum = sh.sums[b * parts + i];
+      if (part_sum > 0) s += part_sum * exp((double)sh.maxs[b * parts + i] - (double)bm);
     }
     s = wave_sum_f64(s);
-    const float score = a.scores[(int64_t)r * a.beams + b];
+    const float score = __shfl(my_score, (int)b, WAVE);
     if (lane == 0) {
       const bool ok = !bad && bm > -INFINITY && isfinite(score);
       sh.base[b] = ok ? (double)bm : -INFINITY;  // (-inf: the beam gives nothing)
@@ -236,30 +290,36 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
     }
   }
   __syncthreads();
-  auto value = [&](uint32_t list, uint64_t p) -> uint64_t {  // 0: none
-    const uint32_t b = list / slices;
+  const uint32_t of_beam = parts * n;
+  auto value = [&](uint32_t i, uint64_t p) -> uint64_t {  // of entry i; 0: none
+    const uint32_t b = i / of_beam;
     if (p == 0 || sh.base[b] == -INFINITY) return 0;
     return dkey(((double)fkey_inv(pk_key(p)) - sh.base[b]) - sh.shift[b] + sh.score[b]);
   };
-  // a bound that n entries reach: the n-th largest of the threads' largest heads, by its upper 32 bits
+  // a bound that n entries reach: the n-th largest of the threads' largest so far, by its upper 32 bits
   uint64_t lead = 0;
-  for (uint32_t i = tid; i < total; i += BT) lead = max(lead, value(i, ld_ag(heads + (int64_t)i * n)));
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (j * BT < entries) lead = max(lead, value(min(j * BT + tid, entries - 1), ahead[j]));
   const uint64_t from = max((uint64_t)block_kth_u32((uint32_t)(lead >> 32), n, (uint32_t *)sh.list) << 32, (uint64_t)1);
   if (tid == 0) sh.n = 0;
   __syncthreads();
-  for (uint32_t i = tid; i < total; i += BT) {
-    for (uint32_t k = 0; k < n; ++k) {
-      const uint64_t p = ld_ag(heads + (int64_t)i * n + k), v = value(i, p);
-      if (v < from) break;  // (a list descends)
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < BL) {
-        sh.list[at] = v;
-        sh.sub[at] = (uint64_t)(i / slices) << 32 | pk_id(p);
-      }
+  auto take = [&](uint32_t i, uint64_t p) {
+    const uint64_t y = value(i, p);
+    if (y < from) return;
+    const uint32_t at = atomicAdd(&sh.n, 1u);
+    if (at < BL) {
+      sh.list[at] = y;
+      sh.sub[at] = (uint64_t)(i / of_beam) << 32 | pk_id(p);
     }
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (j * BT + tid < entries) take(j * BT + tid, ahead[j]);
+#pragma unroll 4
+  for (uint32_t i = AHEAD * BT + tid; i < entries; i += BT) take(i, ld_ag(lists + i));
   __syncthreads();
-  count = sh.n;
+  const uint32_t count = sh.n;
   int32_t *tokens = a.tokens + (int64_t)r * n, *parents = a.parents + (int64_t)r * n;
   float *scores = a.out_scores + (int64_t)r * n;
   auto emit = [&](uint32_t rank, uint64_t v, uint64_t place) {
@@ -271,6 +331,7 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
     for (uint32_t i = tid; i < count; i += BT) {
       const uint64_t v = sh.list[i], p = sh.sub[i];
       uint32_t rank = 0;
+#pragma unroll 8
       for (uint32_t k = 0; k < count; ++k) rank += sh.list[k] > v || (sh.list[k] == v && sh.sub[k] < p);
       if (rank < n) emit(rank, v, p);
     }
@@ -281,15 +342,13 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
   uint64_t lv = ~0ull, lp = 0;
   for (uint32_t k = 0; k < n; ++k) {
     uint64_t bv = 0, bp = ~0ull;
-    for (uint32_t i = tid; i < total; i += BT) {
-      for (uint32_t e = 0; e < n; ++e) {
-        const uint64_t p = ld_ag(heads + (int64_t)i * n + e), v = value(i, p);
-        if (v == 0 || v < bv) break;
-        const uint64_t place = (uint64_t)(i / slices) << 32 | pk_id(p);
-        if ((v < lv || (v == lv && k > 0 && place > lp)) && (v > bv || place < bp)) {
-          bv = v;
-          bp = place;
-        }
+    for (uint32_t i = tid; i < entries; i += BT) {
+      const uint64_t p = ld_ag(lists + i), v = value(i, p);
+      if (v == 0) continue;
+      const uint64_t place = (uint64_t)(i / of_beam) << 32 | pk_id(p);
+      if ((v < lv || (v == lv && k > 0 && place > lp)) && (v > bv || (v == bv && place < bp))) {
+        bv = v;
+        bp = place;
       }
     }
     const uint64_t v = block_max_u64(bv, sh.redu), p = ~block_max_u64(bv == v && v ? ~bp : 0, sh.redu);
@@ -305,19 +364,24 @@ __global__ __launch_bounds__(BT) void beam_kernel(gsk_beams a, uint32_t slices, 
 
 }  // namespace
 
-uint32_t beam_slices(const gsk_beams &a) { return (a.vocab + BS - 1) / BS; }
-
-int64_t beam_work(const gsk_beams &a) {
-  return (int64_t)a.requests * a.beams * beam_slices(a) * (int64_t)(sizeof(SliceSum) + a.n * sizeof(uint64_t));
+// Workgroups of a row: a slice each while all of them run at once (four a CU), else as many as do.
+static uint32_t beam_parts(const gsk_beams &a, int cus) {
+  const uint64_t slices = (a.vocab + BS - 1) / BS, rows = (uint64_t)a.requests * a.beams;
+  const uint64_t most = max((uint64_t)4 * cus / max(rows, (uint64_t)1), (uint64_t)1);
+  return (uint32_t)min(min(slices, most), (uint64_t)(LISTS / a.beams));
 }
 
-hipError_t launch_beam(const gsk_beams &a, uint32_t *tick, uint32_t tickets, hipStream_t s) {
-  const uint32_t slices = beam_slices(a);
+int64_t beam_work(const gsk_beams &a, int cus) {
+  return (int64_t)a.requests * a.beams * beam_parts(a, cus) * (int64_t)(sizeof(ListSum) + a.n * sizeof(uint64_t));
+}
+
+hipError_t launch_beam(const gsk_beams &a, int cus, uint32_t *tick, uint32_t tickets, hipStream_t s) {
+  const uint32_t parts = beam_parts(a, cus);
   // a launch takes a ticket per request, and 65535 rows at most
   const uint32_t most = min(tickets, 65535u / a.beams);
   auto go = [&](auto type, auto wide) {
     for (uint32_t r0 = 0; r0 < a.requests; r0 += most)
-      hipLaunchKernelGGL((beam_kernel<type(), wide()>), dim3(slices, min(most, a.requests - r0) * a.beams), dim3(BT), 0, s, a, slices,
+      hipLaunchKernelGGL((beam_kernel<type(), wide()>), dim3(parts, min(most, a.requests - r0) * a.beams), dim3(BT), 0, s, a, parts,
                          tick, r0);
   };
   const uint64_t size = a.type == GSK_F32 ? 4 : 2;

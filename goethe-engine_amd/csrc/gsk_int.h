@@ -18,8 +18,7 @@ struct AttendPlan {
 AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tickets, int cus);
 hipError_t launch_attend(const gsk_cache &c, const gsk_attention &a, const AttendPlan &p, uint32_t *tick, hipStream_t s);
 
-uint32_t beam_slices(const gsk_beams &a);
-int64_t beam_work(const gsk_beams &a);
-hipError_t launch_beam(const gsk_beams &a, uint32_t *tick, uint32_t tickets, hipStream_t s);
+int64_t beam_work(const gsk_beams &a, int cus);
+hipError_t launch_beam(const gsk_beams &a, int cus, uint32_t *tick, uint32_t tickets, hipStream_t s);
 
 }  // namespace gse

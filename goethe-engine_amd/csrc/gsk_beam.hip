@@ -102,7 +102,7 @@ __device__ __forceinline__ double dkey_inv(uint64_t k) {
 }
 
 template <uint32_t T, bool WIDE>
-__global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts, uint32_t *tick, uint32_t r0) {
+__global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts, Div by_beam, uint32_t *tick, uint32_t r0) {
   __shared__ BeamShared sh;
   const uint32_t tid = threadIdx.x, part = blockIdx.x, beam = blockIdx.y % a.beams, r = r0 + blockIdx.y / a.beams;
   const uint32_t row = r * a.beams + beam, n = a.n, lane = lane_id(), wave = tid / WAVE;
@@ -112,16 +112,20 @@ __global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts
   const uint32_t slices = (a.vocab + BS - 1) / BS, first = (uint32_t)((uint64_t)slices * part / parts);
   const uint32_t end = (uint32_t)((uint64_t)slices * (part + 1) / parts);
   constexpr int VE = WIDE ? 8 : 1;  // elements of a load
-  // a slice's elements as they are (16 bytes a load), or one by one where a row or its end is not aligned
+  // a slice's elements as they are, 16 bytes a load (unaligned rows: one by one), -inf past the row
   Raw8<T> raw[BE / 8];
   float v[BE];
   auto token = [&](uint32_t slice, int e) { return slice * BS + (uint32_t)(e / VE) * (BT * VE) + tid * VE + (uint32_t)(e % VE); };
-  auto whole = [&](uint32_t slice) { return WIDE && (slice + 1) * BS <= a.vocab; };
+  constexpr uint32_t NOTHING = T == GSK_F32 ? 0xFF800000u : T == GSK_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
   auto load = [&](uint32_t slice) {
 #pragma unroll
-    for (int e = 0; e < BE; e += 8) raw[e / 8] = load_raw8<T>(x + (int64_t)token(slice, e) * type_size<T>);
+    for (int e = 0; WIDE && e < BE; e += 8) {
+#pragma unroll
+      for (int i = 0; i < Raw8<T>::N; ++i) raw[e / 8].w[i] = NOTHING;
+      if (token(slice, e) + 8 <= a.vocab) raw[e / 8] = load_raw8<T>(x + (int64_t)token(slice, e) * type_size<T>);
+    }
   };
-  if (whole(first)) load(first);
+  load(first);
   uint32_t kept = 0;          // entries of sh.best
   uint32_t top_key = 0;       // of the slices before: their largest value ...
   float top = -INFINITY;
@@ -132,14 +136,16 @@ __global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts
   };
   if (tid == 0) sh.fix = 0;
   for (uint32_t slice = first; slice < end; ++slice) {
-    if (whole(slice)) {
 #pragma unroll
-      for (int e = 0; e < BE; e += 8) to_f32(raw[e / 8], *(float(*)[8])(v + e));
-    } else {
+    for (int e = 0; e < BE; e += 8) {
+      if constexpr (WIDE) to_f32(raw[e / 8], *(float(*)[8])(v + e));
+      const bool some = WIDE ? token(slice, e) < a.vocab && token(slice, e) + 8 > a.vocab : true;  // (the row's ragged end)
+      if (some) {
 #pragma unroll
-      for (int e = 0; e < BE; ++e) v[e] = token(slice, e) < a.vocab ? load_logit(x, T, token(slice, e)) : -INFINITY;
+        for (int i = e; i < e + 8; ++i) v[i] = token(slice, i) < a.vocab ? load_logit(x, T, token(slice, i)) : -INFINITY;
+      }
     }
-    if (slice + 1 < end && whole(slice + 1)) load(slice + 1);
+    if (slice + 1 < end) load(slice + 1);
     float most = -INFINITY;
 #pragma unroll
     for (int e = 0; e < BE; ++e) {
@@ -290,34 +296,41 @@ __global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts
     }
   }
   __syncthreads();
-  const uint32_t of_beam = parts * n;
-  auto value = [&](uint32_t i, uint64_t p) -> uint64_t {  // of entry i; 0: none
-    const uint32_t b = i / of_beam;
+  auto value = [&](uint32_t i, uint64_t p, uint32_t &b) -> uint64_t {  // of entry i, of beam b; 0: none
+    uint32_t rest;
+    b = quotient(i, by_beam, rest);
     if (p == 0 || sh.base[b] == -INFINITY) return 0;
     return dkey(((double)fkey_inv(pk_key(p)) - sh.base[b]) - sh.shift[b] + sh.score[b]);
   };
   // a bound that n entries reach: the n-th largest of the threads' largest so far, by its upper 32 bits
-  uint64_t lead = 0;
+  uint64_t lead = 0, val[AHEAD];
+  uint32_t of[AHEAD];
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j)
-    if (j * BT < entries) lead = max(lead, value(min(j * BT + tid, entries - 1), ahead[j]));
+  for (int j = 0; j < AHEAD; ++j) {
+    val[j] = 0;
+    if (j * BT < entries) val[j] = value(min(j * BT + tid, entries - 1), ahead[j], of[j]);
+    lead = max(lead, val[j]);
+  }
   const uint64_t from = max((uint64_t)block_kth_u32((uint32_t)(lead >> 32), n, (uint32_t *)sh.list) << 32, (uint64_t)1);
   if (tid == 0) sh.n = 0;
   __syncthreads();
-  auto take = [&](uint32_t i, uint64_t p) {
-    const uint64_t y = value(i, p);
+  auto take = [&](uint64_t y, uint32_t b, uint64_t p) {
     if (y < from) return;
     const uint32_t at = atomicAdd(&sh.n, 1u);
     if (at < BL) {
       sh.list[at] = y;
-      sh.sub[at] = (uint64_t)(i / of_beam) << 32 | pk_id(p);
+      sh.sub[at] = (uint64_t)b << 32 | pk_id(p);
     }
   };
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j)
-    if (j * BT + tid < entries) take(j * BT + tid, ahead[j]);
+  for (int j = 0; j < AHEAD; ++j) take(val[j], of[j], ahead[j]);
 #pragma unroll 4
-  for (uint32_t i = AHEAD * BT + tid; i < entries; i += BT) take(i, ld_ag(lists + i));
+  for (uint32_t i = AHEAD * BT + tid; i < entries; i += BT) {
+    const uint64_t p = ld_ag(lists + i);
+    uint32_t b;
+    const uint64_t y = value(i, p, b);
+    take(y, b, p);
+  }
   __syncthreads();
   const uint32_t count = sh.n;
   int32_t *tokens = a.tokens + (int64_t)r * n, *parents = a.parents + (int64_t)r * n;
@@ -343,9 +356,10 @@ __global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts
   for (uint32_t k = 0; k < n; ++k) {
     uint64_t bv = 0, bp = ~0ull;
     for (uint32_t i = tid; i < entries; i += BT) {
-      const uint64_t p = ld_ag(lists + i), v = value(i, p);
+      uint32_t b;
+      const uint64_t p = ld_ag(lists + i), v = value(i, p, b);
       if (v == 0) continue;
-      const uint64_t place = (uint64_t)(i / of_beam) << 32 | pk_id(p);
+      const uint64_t place = (uint64_t)b << 32 | pk_id(p);
       if ((v < lv || (v == lv && k > 0 && place > lp)) && (v > bv || (v == bv && place < bp))) {
         bv = v;
         bp = place;
@@ -382,7 +396,7 @@ hipError_t launch_beam(const gsk_beams &a, int cus, uint32_t *tick, uint32_t tic
   auto go = [&](auto type, auto wide) {
     for (uint32_t r0 = 0; r0 < a.requests; r0 += most)
       hipLaunchKernelGGL((beam_kernel<type(), wide()>), dim3(parts, min(most, a.requests - r0) * a.beams), dim3(BT), 0, s, a, parts,
-                         tick, r0);
+                         div_by(parts * a.n), tick, r0);
   };
   const uint64_t size = a.type == GSK_F32 ? 4 : 2;
   const bool wide = ((uint64_t)a.logits | (uint64_t)a.ld * size) % 16 == 0;

@@ -49,10 +49,10 @@ def select(logits, scores, n):
         raise ValueError(f"scores on {scores.device}, the logits on {dev}")
     if (logits.stride(1) != 1 and vocab > 1) or (logits.shape[0] > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
-    scores = scores.to(torch.float32).contiguous()
-    ints = torch.empty((2, requests, n), dtype=torch.int32, device=dev)
+    if scores.dtype is not torch.float32 or not scores.is_contiguous():
+        scores = scores.to(torch.float32).contiguous()
+    tokens, parents = torch.empty((2, requests, n), dtype=torch.int32, device=dev).unbind()
     best = torch.empty((requests, n), dtype=torch.float32, device=dev)
-    tokens, parents = ints[0], ints[1]
     if requests:
         b = _lib.Beams(_SIZE, requests, beams, n, vocab, _TYPES[logits.dtype], logits.data_ptr(),
                        logits.stride(0) if logits.shape[0] > 1 else vocab, scores.data_ptr(), tokens.data_ptr(),

@@ -16,11 +16,11 @@ AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tick
   const uint64_t rows = (uint64_t)a.max_new * (a.heads / c.heads), most = 16 * row_tiles(c, a);
   AttendPlan p;
   p.tiles = (uint32_t)((rows + most - 1) / most);
-  // One round of workgroups, if the requests' longest tables fill it.
-  const uint64_t each = (uint64_t)c.heads * p.tiles;
-  const uint64_t round = (uint64_t)cus * attend_resident(c.dim <= 128 ? 4 : 8, row_tiles(c, a)) / each;
-  const uint64_t blocks = (uint64_t)a.requests * (((uint64_t)a.max_pages * c.page + AB - 1) / AB);
-  p.items = (uint32_t)max(min(min(round, (uint64_t)tickets / each), (blocks + SHARE_MIN - 1) / SHARE_MIN), (uint64_t)1);
+  // One round of workgroups, as many on each XCD, if the requests' longest tables fill it.
+  const uint64_t each = (uint64_t)c.heads * p.tiles, xcd = (uint64_t)cus / 8 * attend_resident(c.dim <= 128 ? 4 : 8, row_tiles(c, a));
+  const uint64_t round = each <= xcd ? xcd / each * 8 : xcd * 8 / each;
+  const uint64_t blocks = (uint64_t)a.requests * (TURN + ((uint64_t)a.max_pages * c.page + AB - 1) / AB);
+  p.items = (uint32_t)max(min(min(round, (uint64_t)tickets / each), blocks / SHARE_MIN), (uint64_t)1);
   p.work = p.items == 1 ? 0 : (int64_t)(p.items * 2 * each * min(rows, most) * (c.dim + 2) * sizeof(float));
   return p;
 }

@@ -27,6 +27,7 @@ namespace gse {
 constexpr int AT = 256, AW = AT / WAVE;
 constexpr uint32_t AB = 32;  // tokens of a block
 constexpr uint32_t SHARE_MIN = 8;   // blocks of a share, at least
+constexpr uint32_t TURN = 8;        // what a request's turn costs besides its tokens, in blocks: a share's requests count it
 
 struct AttendArgs {
   gsk_cache c;
@@ -142,7 +143,7 @@ __device__ __forceinline__ Span span_of(const gsk_cache &c, const gsk_attention 
   const bool ok = x.status == 0 && x.len >= n && (int64_t)x.len <= (int64_t)a.max_pages * c.page;
   return {x.begin, n, ok ? x.len : 0};
 }
-__device__ __forceinline__ uint32_t blocks_of(Span x) { return x.begin < 0 ? 0u : max(((uint32_t)x.len + AB - 1) / AB, 1u); }
+__device__ __forceinline__ uint32_t blocks_of(Span x) { return x.begin < 0 ? 0u : TURN + max(((uint32_t)x.len + AB - 1) / AB, 1u); }
 
 template <uint32_t Q, uint32_t C, int KD, int MT>
 __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(AttendArgs p) {
@@ -161,18 +162,22 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   if (item >= p.items) return;
 
   // ---- the share ----------------------------------------------------------------------------------------------------------
-  // Every wave for itself, a lane four requests at a time: a request's blocks, one at least if it has rows to write.
+  // Every wave for itself, a lane one request or, where there are more than lanes, four at a time: a request's blocks, one at
+  // least if it has rows to write, after TURN that stand for its turn. The shares are of one size, the first ones a block more.
+  const int per = a.requests <= WAVE ? 1 : 4;
   Span own[4];
-  uint32_t u[4];
+  uint32_t u[4] = {};
   auto take = [&](uint32_t i0) {  // returns the lane's blocks
+    uint64_t n = 0;
     Raw raw[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) raw[k] = raw_of(a, min(i0 + lane * 4 + k, a.requests - 1));
-    uint64_t n = 0;
+    for (int k = 0; k < 4; ++k)
+      if (k < per) raw[k] = raw_of(a, min(i0 + lane * per + k, a.requests - 1));
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      if (k >= per) continue;
       own[k] = span_of(c, a, raw[k]);
-      u[k] = i0 + lane * 4 + k < a.requests ? blocks_of(own[k]) : 0;
+      u[k] = i0 + lane * per + k < a.requests ? blocks_of(own[k]) : 0;
       n += u[k];
     }
     return n;
@@ -180,10 +185,18 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   uint64_t mine = take(0), total = mine;
   for (uint32_t i0 = 4 * WAVE; i0 < a.requests; i0 += 4 * WAVE) total += take(i0);
   total = wave_sum_u64(total);
-  const uint64_t share = max((total + p.items - 1) / p.items, (uint64_t)SHARE_MIN);
-  uint64_t pos = item * share, start = 0;  // the share's first block; the first block of request r
-  const uint64_t stop = min(pos + share, total);
-  if (pos >= stop) return;
+  const uint32_t shares = (uint32_t)min(max(total / SHARE_MIN, (uint64_t)1), (uint64_t)p.items);
+  if (item >= shares) return;
+  const bool fits = total >> 32 == 0;  // (64-bit divisions are long)
+  const uint64_t share = fits ? (uint32_t)total / shares : total / shares, longer = total - share * shares;
+  auto first_of = [&](uint64_t w) { return w * share + min(w, longer); };
+  auto share_of = [&](uint64_t block) -> uint32_t {
+    const uint64_t border = longer * (share + 1), x = block < border ? block : block - border, d = block < border ? share + 1 : share;
+    return (uint32_t)((fits ? (uint32_t)x / (uint32_t)d : x / d) + (block < border ? 0 : longer));
+  };
+  uint64_t pos = first_of(item), start = 0;  // the share's first block; the first block of request r
+  const uint64_t stop = first_of(item + 1);
+  if (pos >= stop) return;  // (nothing to write at all)
   uint32_t r = 0;
   Span sp;
   for (uint32_t i0 = 0;; i0 += 4 * WAVE) {
@@ -195,15 +208,17 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     }
     const int at = __builtin_ctzll(past);
     start += shfl_u64(inc - mine, at);
-    r = i0 + at * 4;
+    r = i0 + at * per;
+    bool found = false;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (r != i0 + at * 4 + k) continue;
+      if (found || k >= per) continue;
       sp.begin = __builtin_amdgcn_readlane(own[k].begin, at);
       sp.n = __builtin_amdgcn_readlane(own[k].n, at);
       sp.len = __builtin_amdgcn_readlane(own[k].len, at);
       const uint32_t n = __builtin_amdgcn_readlane(u[k], at);
-      if (k < 3 && start + n <= pos) {
+      found = k + 1 >= per || start + n > pos;
+      if (!found) {
         start += n;
         ++r;
       }
@@ -217,11 +232,12 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   if (pos >= stop) break;
   ahead = raw_of(a, min(r + 1, a.requests - 1));  // (the next request's, for the next turn)
   if (sp.begin < 0) continue;
-  const uint64_t first = start, end = start + blocks_of(sp);  // the request's blocks
-  const uint32_t k0 = (uint32_t)(pos - first) * AB, k_end = (uint32_t)(min(stop, end) - first) * AB;
-  const uint32_t first_item = (uint32_t)(first / share), parts = (uint32_t)((end - 1) / share) - first_item + 1;
+  const uint64_t first = start + TURN, end = start + blocks_of(sp), from = max(pos, first);  // the request's blocks
   start = end;
   pos = min(stop, end);
+  if (from >= pos) continue;  // (the share ends within its turn)
+  const uint32_t k0 = (uint32_t)(from - first) * AB, k_end = (uint32_t)(pos - first) * AB;
+  const uint32_t first_item = from == first ? item : share_of(first), parts = (end <= stop ? item : share_of(end - 1)) - first_item + 1;
   const uint32_t rows = min((uint32_t)sp.n, a.max_new) * p.group, row0 = tile * 16 * MT;
   if (row0 >= rows) continue;
   const uint32_t len = (uint32_t)sp.len, ctx = len >= (uint32_t)sp.n ? len - (uint32_t)sp.n : 0;
@@ -230,13 +246,15 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
 
   // ---- the rows -----------------------------------------------------------------------------------------------------------
   const uint32_t sign = a.scale < 0 ? 0x80008000u : 0;  // (the scale's own, so that the largest score is the largest product)
-  for (uint32_t i = tid; i < MT * 16 * KD * 4; i += AT) {
-    const uint32_t w = i / (KD * 4), e = i % (KD * 4), row = min(row0 + w, rows - 1), n = row / p.group, gi = row - n * p.group;
-    const char *at = (const char *)a.q + ((int64_t)(sp.begin + n) * a.q_token_stride + (int64_t)(head * p.group + gi) * a.q_head_stride) * 2;
-    uint4 v = {0, 0, 0, 0};
-    if (e * 8 < c.dim) v = *(const uint4 *)(at + e * 16);
-    v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
-    sh.q[w / 16][w % 16][e] = v;
+  constexpr int QN = (MT * 16 * KD * 4 + AT - 1) / AT;
+  uint4 rows_q[QN];  // (to LDS once the first block's loads are on their way)
+#pragma unroll
+  for (int j = 0; j < QN; ++j) {
+    const uint32_t at_q = j * AT + tid, w = at_q / (KD * 4), e = at_q % (KD * 4), row = min(row0 + w, rows - 1), n = row / p.group;
+    rows_q[j] = uint4{0, 0, 0, 0};
+    if (w < MT * 16 && e * 8 < c.dim)
+      rows_q[j] = *(const uint4 *)((const char *)a.q + ((int64_t)(sp.begin + n) * a.q_token_stride +
+                                                        (int64_t)(head * p.group + row - n * p.group) * a.q_head_stride + e * 8) * 2);
   }
   auto q_of = [&](int m, int k) { return __builtin_bit_cast(Frag<Q>, sh.q[m][lc][k * 4 + lg]); };
   uint32_t sees[MT];   // chains: the first cached token that the lane's row does not see
@@ -322,7 +340,14 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     place_block(t + l32, next_page());
     load_keys();
   }
-  __syncthreads();  // (the rows' operands)
+#pragma unroll
+  for (int j = 0; j < QN; ++j) {
+    const uint32_t at_q = j * AT + tid, w = at_q / (KD * 4);
+    uint4 v = rows_q[j];
+    v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
+    if (w < MT * 16) sh.q[w / 16][w % 16][at_q % (KD * 4)] = v;
+  }
+  __syncthreads();
   if (t < k1) {
     for (; t < k1; t += AW * AB) {
       const uint32_t page = next_page(), real = there;

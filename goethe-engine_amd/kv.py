@@ -22,6 +22,7 @@ gradients. Calls on one stream follow one another; none waits for the host, and 
 stream's handle is open: after one call on it).
 """
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -36,45 +37,66 @@ _CACHE, _WRITE, _READ, _ATTEND, _REORDER = (C.sizeof(t) for t in (_lib.KvCache, 
                                                                   _lib.Reorder))
 
 
-def _cache(keys, values, scales, heads_first, writes=False):
-    """The cache as the library takes it; what is not in order is refused here."""
-    shape, stride = keys.shape, keys.stride()
-    if keys.dtype not in _TYPES:
-        raise ValueError(f"a cache of {keys.dtype}: bfloat16, float16, float8_e4m3fn or int8 is wanted")
+@functools.lru_cache(maxsize=1024)
+def _layout_of(shape, stride, dtype, heads_first, scale_shape, scale_stride, writes):
+    """gsk_cache's numbers of a cache's shape and strides: (type, pages, page, heads, dim), (page, token, head strides), the same of
+    the scales or (), and what the addresses have to be multiples of. Refuses what is not in order."""
+    if dtype not in _TYPES:
+        raise ValueError(f"a cache of {dtype}: bfloat16, float16, float8_e4m3fn or int8 is wanted")
     if len(shape) != 4 or 0 in shape:
         raise ValueError(f"a cache of shape {tuple(shape)}: [pages, page, heads, dim] (heads first: [pages, heads, page, dim]) is wanted")
-    if values.shape != shape or values.stride() != stride or values.dtype != keys.dtype or values.device != keys.device:
-        raise ValueError("keys and values must have one shape, layout, type and device")
-    kind, dim, size = _TYPES[keys.dtype], shape[3], keys.element_size()
+    kind, dim = _TYPES[dtype], shape[3]
     pages, (heads, page) = shape[0], shape[1:3] if heads_first else shape[2:0:-1]
-    ps, (hs, ts) = stride[0], stride[1:3] if heads_first else stride[2:0:-1]
+
+    def strides(t):
+        ps, (hs, ts) = t[0], t[1:3] if heads_first else t[2:0:-1]
+        if writes and ((ps == 0 and pages > 1) or (ts == 0 and page > 1) or (hs == 0 and heads > 1)):
+            raise ValueError("the cache written to, and its scales, must not be expanded")
+        return ps, ts, hs
+
     if dim % 8 or dim > _lib.MAX_DIM:
         raise ValueError(f"dim {dim} is no multiple of 8 up to {_lib.MAX_DIM}")
-    k, v = keys.data_ptr(), values.data_ptr()
-    if stride[3] != 1 or (ps | ts | hs) % 8 or (k | v) % (8 * size):
+    at = strides(stride)
+    if stride[3] != 1 or (at[0] | at[1] | at[2]) % 8:
         raise ValueError("a token's head must lie together, at a multiple of 8 elements")
-    if pages * page >= 1 << 32:
-        raise ValueError(f"{pages} pages of {page} tokens: at most 2^32 - 1 slots")
-    if writes and (k == v or (ps == 0 and pages > 1) or (ts == 0 and page > 1) or (hs == 0 and heads > 1)):
-        raise ValueError("the cache written to must not be expanded, nor be keys and values at once")
-    c = _lib.KvCache(_CACHE, kind, pages, page, heads, dim, k, v, ps, ts, hs)
-    if kind >= _lib.K_E4M3:
-        if scales is None:
-            raise ValueError("an 8-bit cache needs its scales")
+    if pages * page >= 1 << 32 or heads > 1 << 12:
+        raise ValueError(f"{pages} pages of {page} tokens, {heads} heads: at most 2^32 - 1 slots and 2^12 heads")
+    if kind < _lib.K_E4M3:
+        if scale_shape is not None:
+            raise ValueError(f"a cache of {dtype} has no scales")
+        return (kind, pages, page, heads, dim), at, (), 16
+    if scale_shape is None:
+        raise ValueError("an 8-bit cache needs its scales")
+    if scale_shape != shape[:3]:
+        raise ValueError(f"scales must be of shape {tuple(shape[:3])}")
+    return (kind, pages, page, heads, dim), at, strides(scale_stride), 8
+
+
+def _cache(keys, values, scales, heads_first, writes=False):
+    """The cache as the library takes it; what is not in order is refused here."""
+    shape, stride, dtype, dev = keys.shape, keys.stride(), keys.dtype, keys.device
+    if values.shape != shape or values.stride() != stride or values.dtype is not dtype or values.device != dev:
+        raise ValueError("keys and values must have one shape, layout, type and device")
+    if scales is None:
+        size, at, _, align = _layout_of(shape, stride, dtype, heads_first, None, None, writes)
+        extra = ()
+    else:
         a, b = scales
-        if a.dtype is not torch.float32 or b.dtype is not torch.float32 or a.shape != shape[:3] or b.shape != shape[:3] \
-                or a.stride() != b.stride():
-            raise ValueError(f"scales must be two float32 tensors of shape {tuple(shape[:3])} and one layout")
-        if a.device != keys.device or b.device != keys.device:
-            raise ValueError(f"scales on {a.device} and {b.device}, the cache on {keys.device}")
-        sp, (sh, st) = a.stride(0), a.stride()[1:] if heads_first else a.stride()[:0:-1]
-        if writes and (a.data_ptr() == b.data_ptr() or (sp == 0 and pages > 1) or (st == 0 and page > 1) or (sh == 0 and heads > 1)):
-            raise ValueError("the scales written to must not be expanded, nor the keys' and the values' at once")
-        c.key_scales, c.value_scales = a.data_ptr(), b.data_ptr()
-        c.scale_page_stride, c.scale_token_stride, c.scale_head_stride = sp, st, sh
-    elif scales is not None:
-        raise ValueError(f"a cache of {keys.dtype} has no scales")
-    return c
+        s_shape, s_stride = a.shape, a.stride()
+        if a.dtype is not torch.float32 or b.dtype is not torch.float32 or b.shape != s_shape or b.stride() != s_stride:
+            raise ValueError("scales must be two float32 tensors of one shape and layout")
+        if a.device != dev or b.device != dev:
+            raise ValueError(f"scales on {a.device} and {b.device}, the cache on {dev}")
+        size, at, s_at, align = _layout_of(shape, stride, dtype, heads_first, s_shape, s_stride, writes)
+        extra = (a.data_ptr(), b.data_ptr(), *s_at)
+        if writes and extra[0] == extra[1]:
+            raise ValueError("the scales written to must not be the keys' and the values' at once")
+    k, v = keys.data_ptr(), values.data_ptr()
+    if (k | v) % align:
+        raise ValueError("a token's head must lie together, at a multiple of 8 elements")
+    if writes and k == v:
+        raise ValueError("the cache written to must not be keys and values at once")
+    return _lib.KvCache(_CACHE, *size, k, v, *at, *extra)
 
 
 def _on_device(dev, **tensors):
@@ -85,14 +107,28 @@ def _on_device(dev, **tensors):
             raise ValueError(f"{name} on {t.device}, the cache on {dev}")
 
 
+@functools.lru_cache(maxsize=1024)
+def _rows_in_order(shape, stride, name, heads, dim):
+    if len(shape) != 3 or (heads and shape[1] != heads) or shape[2] != dim:
+        raise ValueError(f"{name} must be a tensor [tokens, {heads or 'heads'}, {dim}]")
+    return stride[2] == 1 and stride[0] % 8 == 0 and stride[1] % 8 == 0
+
+
 def _rows(t, name, heads, dim):
     """[tokens, heads, dim] rows as the kernels read them (rows that do not start at 16 bytes are copied)."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 3 or (heads and t.shape[1] != heads) or t.shape[2] != dim:
+    if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor [tokens, {heads or 'heads'}, {dim}]")
-    s = t.stride()
-    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+    if not _rows_in_order(t.shape, t.stride(), name, heads, dim) or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
+
+
+@functools.lru_cache(maxsize=1024)
+def _work_bytes(device, handle_rows, cache, call):
+    """gsk_attention_work for sizes alone: cache (type .. dim of gsk_cache), call (requests .. max_new, max_pages, trees)."""
+    c, a = _lib.KvCache(_CACHE, *cache), _lib.Attention(_ATTEND, *call[:-1])
+    a.max_pages = call[-1]
+    return _lib.handle(device, 1, 1).call("gsk_attention_work", C.byref(c), C.byref(a))
 
 
 def _table(table):
@@ -214,7 +250,7 @@ def attend(q, keys, values, table, seq_len, begin=None, status=None, parents=Non
         raise ValueError("out must be a contiguous tensor like q, at a multiple of 16 bytes")
     _on_device(dev, q=q, table=table, out=out)
     if out is None:
-        out = torch.empty((n, hq, c.dim), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if n == 0:
         return out
     i32 = torch.int32
@@ -227,12 +263,11 @@ def attend(q, keys, values, table, seq_len, begin=None, status=None, parents=Non
                        status.data_ptr() if status is not None else None, parents.data_ptr() if parents is not None else None,
                        None, 0, _lib.raw_stream(dev.index))
     h = _lib.handle(dev.index, 1, 1)
-    pc, pa = C.byref(c), C.byref(a)
-    need = h.call("gsk_attention_work", pc, pa)
+    need = _work_bytes(dev.index, h.rows, (c.type, c.pages, c.page, c.heads, c.dim), (r, n, hq, kind, max_new, width))
     if need:
         work = torch.empty(need, dtype=torch.uint8, device=dev)
         a.work, a.work_bytes = work.data_ptr(), need
-    h.call("gsk_attend", pc, pa)
+    h.call("gsk_attend", C.byref(c), C.byref(a))
     return out
 
 

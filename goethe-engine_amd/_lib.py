@@ -195,14 +195,14 @@ ROUND_SIGNATURES = dict(  # include/gsp.h
     gsp_pages_step=(C.c_int, [C.c_void_p, P_(Pages), P_(Step)]),
     gsp_keep_path=(C.c_int, [C.c_void_p, P_(Path)]),
 )
-KV_SIGNATURES = dict(  # include/gsk.h
-    gsk_write=(C.c_int, [C.c_void_p, P_(KvCache), P_(KvRows)]),
-    gsk_read=(C.c_int, [C.c_void_p, P_(KvCache), P_(KvRead)]),
-    gsk_attention_work=(C.c_int64, [C.c_void_p, P_(KvCache), P_(Attention)]),
-    gsk_attend=(C.c_int, [C.c_void_p, P_(KvCache), P_(Attention)]),
-    gsk_beams_work=(C.c_int64, [C.c_void_p, P_(Beams)]),
-    gsk_beam=(C.c_int, [C.c_void_p, P_(Beams)]),
-    gsk_reorder=(C.c_int, [C.c_void_p, P_(Reorder)]),
+KV_SIGNATURES = dict(  # include/gsk.h (structs: the ctypes ones above, or their bytes)
+    gsk_write=(C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    gsk_read=(C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    gsk_attention_work=(C.c_int64, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    gsk_attend=(C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    gsk_beams_work=(C.c_int64, [C.c_void_p, C.c_void_p]),
+    gsk_beam=(C.c_int, [C.c_void_p, C.c_void_p]),
+    gsk_reorder=(C.c_int, [C.c_void_p, C.c_void_p]),
 )
 
 

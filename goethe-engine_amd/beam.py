@@ -6,14 +6,15 @@ paged cache then follows with kv.reorder.
     kv.reorder(caches, pages.table, step.seq_len, parents, first=prompt)
     step = pages.step(add=ones, keep=ones)
 """
-import ctypes as C
+import functools
+import struct
 
 import torch
 
 from . import _lib
 
 _TYPES = {torch.bfloat16: _lib.K_BF16, torch.float16: _lib.K_F16, torch.float32: _lib.K_F32}
-_SIZE = C.sizeof(_lib.Beams)
+_BEAMS = struct.Struct("6IQq5QqQ")  # gsk_beams
 
 
 class Choice:
@@ -54,12 +55,16 @@ def select(logits, scores, n):
     tokens, parents = torch.empty((2, requests, n), dtype=torch.int32, device=dev).unbind()
     best = torch.empty((requests, n), dtype=torch.float32, device=dev)
     if requests:
-        b = _lib.Beams(_SIZE, requests, beams, n, vocab, _TYPES[logits.dtype], logits.data_ptr(),
-                       logits.stride(0) if logits.shape[0] > 1 else vocab, scores.data_ptr(), tokens.data_ptr(),
-                       parents.data_ptr(), best.data_ptr(), None, 0, _lib.raw_stream(dev.index))
-        h, p = _lib.handle(dev.index, 1, 1), C.byref(b)
-        need = h.call("gsk_beams_work", p)
+        h = _lib.handle(dev.index, 1, 1)
+        kind, ld = _TYPES[logits.dtype], logits.stride(0) if logits.shape[0] > 1 else vocab
+        need = _work_bytes(dev.index, requests, beams, n, vocab, kind)
         work = torch.empty(need, dtype=torch.uint8, device=dev)
-        b.work, b.work_bytes = work.data_ptr(), need
-        h.call("gsk_beam", p)
+        h.call("gsk_beam", _BEAMS.pack(_BEAMS.size, requests, beams, n, vocab, kind, logits.data_ptr(), ld, scores.data_ptr(),
+                                       tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), work.data_ptr(), need,
+                                       _lib.raw_stream(dev.index)))
     return Choice(tokens, parents, best)
+
+
+@functools.lru_cache(maxsize=1024)
+def _work_bytes(device, *sizes):
+    return _lib.handle(device, 1, 1).call("gsk_beams_work", _BEAMS.pack(_BEAMS.size, *sizes, *[0] * 9))

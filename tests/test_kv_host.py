@@ -177,3 +177,15 @@ def test_select_refuses(ge):
     _refusals(ge.beam.select, dict(logits=x, scores=s, n=4),
               [dict(logits=x[:5]), dict(logits=x.double()), dict(logits=x[0]), dict(logits=x[:, :0]), dict(scores=s[0]), dict(scores=s.int()),
                dict(n=0), dict(n=65), dict(logits=torch.zeros(66, 5), scores=torch.zeros(2, 33)), dict(scores=s.tolist())])
+
+
+def test_packed_structs_are_the_headers(ge):
+    """The structs that kv and beam pack have the fields, sizes and places of the ctypes ones (which the header pins)."""
+    lib, kinds = ge._lib, {4: {C.c_uint32: "I", C.c_float: "f"}, 8: {C.c_int64: "q", C.c_void_p: "Q"}}
+    for packed, cls in ((ge.kv._CACHE, lib.KvCache), (ge.kv._WRITE, lib.KvRows), (ge.kv._READ, lib.KvRead), (ge.kv._ATTEND, lib.Attention),
+                        (ge.kv._REORDER, lib.Reorder), (ge.beam._BEAMS, lib.Beams)):
+        flat = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([IfqQ])", packed.format))
+        assert packed.size == C.sizeof(cls) and len(flat) == len(cls._fields_)
+        assert [kinds[C.sizeof(t)][t] for _, t in cls._fields_] == list(flat)
+        raw = cls.from_buffer_copy(packed.pack(*range(1, len(flat) + 1)))
+        assert [getattr(raw, f) for f, _ in cls._fields_] == list(range(1, len(flat) + 1))

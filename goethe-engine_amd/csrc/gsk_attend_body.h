@@ -50,7 +50,7 @@ struct AttendShared {
       float m[AW][16], l[AW][16];
     };
   };
-  uint32_t last;
+  uint32_t last, bad[AW];
 };
 
 // Workgroups of a CU at once (what their registers allow).
@@ -107,6 +107,22 @@ __device__ __forceinline__ Frag<T> turned(const Raw8<C> (&v)[8]) {
     }
   }
   return __builtin_bit_cast(Frag<T>, uint4{w[0], w[1], w[2], w[3]});
+}
+
+// Makes finite numbers of the NaNs and infinities of eight elements (their exponents' upper bit cleared); nonzero if it has any.
+template <uint32_t C>
+__device__ __forceinline__ uint32_t tame(Raw8<C> &r) {
+  constexpr uint32_t ALL = C == GSK_BF16 ? 0x7F807F80u : C == GSK_F16 ? 0x7C007C00u : 0x7F7F7F7Fu;
+  constexpr uint32_t ONE = C == GSK_BF16 ? 0x00800080u : C == GSK_F16 ? 0x04000400u : 0x01010101u;
+  constexpr uint32_t TOP = type_is_8bit<C> ? 0x80808080u : 0x80008000u;
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; C != GSK_I8 && i < Raw8<C>::N; ++i) {
+    const uint32_t bad = ((r.w[i] & ALL) + ONE) & TOP;  // (8 bits: the one magnitude that is no number)
+    r.w[i] &= ~(bad >> 1);
+    any |= bad;
+  }
+  return any;
 }
 
 // The value over the lanes of the same lane % 16.
@@ -168,7 +184,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   Span own[4];
   uint32_t u[4] = {};
   auto take = [&](uint32_t i0) {  // returns the lane's blocks
-    uint64_t n = 0;
+    uint32_t n = 0;
     Raw raw[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -182,32 +198,32 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     }
     return n;
   };
-  uint64_t mine = take(0), total = mine;
+  uint32_t mine = take(0), total = mine;  // (below 2^32 by the host's check)
   for (uint32_t i0 = 4 * WAVE; i0 < a.requests; i0 += 4 * WAVE) total += take(i0);
-  total = wave_sum_u64(total);
-  const uint32_t shares = (uint32_t)min(max(total / SHARE_MIN, (uint64_t)1), (uint64_t)p.items);
+  total = wave_sum_u32(total);
+  const uint32_t shares = min(max(total / SHARE_MIN, 1u), p.items);
   if (item >= shares) return;
-  const bool fits = total >> 32 == 0;  // (64-bit divisions are long)
-  const uint64_t share = fits ? (uint32_t)total / shares : total / shares, longer = total - share * shares;
-  auto first_of = [&](uint64_t w) { return w * share + min(w, longer); };
-  auto share_of = [&](uint64_t block) -> uint32_t {
-    const uint64_t border = longer * (share + 1), x = block < border ? block : block - border, d = block < border ? share + 1 : share;
-    return (uint32_t)((fits ? (uint32_t)x / (uint32_t)d : x / d) + (block < border ? 0 : longer));
+  const uint32_t share = total / shares, longer = total - share * shares;
+  auto first_of = [&](uint32_t w) { return w * share + min(w, longer); };
+  auto share_of = [&](uint32_t block) {
+    const uint32_t border = longer * (share + 1);
+    return block < border ? block / (share + 1) : longer + (block - border) / share;
   };
-  uint64_t pos = first_of(item), start = 0;  // the share's first block; the first block of request r
-  const uint64_t stop = first_of(item + 1);
+  uint32_t pos = first_of(item), start = 0;  // the share's first block; the first block of request r
+  const uint32_t stop = first_of(item + 1);
   if (pos >= stop) return;  // (nothing to write at all)
   uint32_t r = 0;
   Span sp;
   for (uint32_t i0 = 0;; i0 += 4 * WAVE) {
     if (a.requests > 4 * WAVE) mine = take(i0);
-    const uint64_t inc = wave_incl_scan_u64(mine), past = ballot64(start + inc > pos);
+    const uint32_t inc = wave_incl_scan_u32(mine);
+    const uint64_t past = ballot64(start + inc > pos);
     if (!past) {
       start += lane63(inc);
       continue;
     }
     const int at = __builtin_ctzll(past);
-    start += shfl_u64(inc - mine, at);
+    start += __builtin_amdgcn_readlane(inc - mine, at);
     r = i0 + at * per;
     bool found = false;
 #pragma unroll
@@ -225,18 +241,18 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     }
     break;
   }
-  start = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)start) | (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(start >> 32)) << 32;
+  start = __builtin_amdgcn_readfirstlane(start);
   r = __builtin_amdgcn_readfirstlane(r);
 
   for (Raw ahead;; sp = span_of(c, a, ahead), ++r) {
   if (pos >= stop) break;
   ahead = raw_of(a, min(r + 1, a.requests - 1));  // (the next request's, for the next turn)
   if (sp.begin < 0) continue;
-  const uint64_t first = start + TURN, end = start + blocks_of(sp), from = max(pos, first);  // the request's blocks
+  const uint32_t first = start + TURN, end = start + blocks_of(sp), from = max(pos, first);  // the request's blocks
   start = end;
   pos = min(stop, end);
   if (from >= pos) continue;  // (the share ends within its turn)
-  const uint32_t k0 = (uint32_t)(from - first) * AB, k_end = (uint32_t)(pos - first) * AB;
+  const uint32_t k0 = (from - first) * AB, k_end = (pos - first) * AB;
   const uint32_t first_item = from == first ? item : share_of(first), parts = (end <= stop ? item : share_of(end - 1)) - first_item + 1;
   const uint32_t rows = min((uint32_t)sp.n, a.max_new) * p.group, row0 = tile * 16 * MT;
   if (row0 >= rows) continue;
@@ -300,6 +316,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   const uint32_t last_page = (max(k1, 1u) - 1) / c.page;
   auto next_page = [&] { return (uint32_t)table[min(pi, last_page)]; };
   uint32_t there = 0;  // the tokens of the block that sh.at has
+  uint32_t bad = 0;    // NaNs or infinities among values that some rows do not see
   float scale_of = 0;  // 8 bits: the token's, of its key in the lower lanes and of its value in the upper ones
   const float *scales = lane < 32 ? c.key_scales : c.value_scales;
   auto place_block = [&](uint32_t t, uint32_t pg) {  // the offsets of a block to LDS, from its tokens' pages
@@ -411,7 +428,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         if constexpr (!type_is_8bit<C>) top = top == -INF ? -INF : top * scale;  // (a scale of 0)
         // The maximum follows once it is 2^8 behind: the weights are up to that, and what it saves is the output's rescaling.
         if (ballot64(top > mx[m] + 8.0f)) {
-          top = fmaxf(top, mx[m]);
+          top = top > mx[m] + 8.0f ? top : mx[m];  // (a row's own: what others see does not change it)
           const float f = __builtin_amdgcn_exp2f(mx[m] - (top == -INF ? 0.0f : top));
           mx[m] = top;
           l[m] *= f;
@@ -427,12 +444,9 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
           if constexpr (type_is_8bit<C>) z[j] = __builtin_amdgcn_exp2f(z[j] - base);
           else z[j] = __builtin_amdgcn_exp2f(z[j] == -INF ? -INF : __builtin_fmaf(z[j], scale, -base));
           l[m] += z[j];
-          if constexpr (type_is_8bit<C>) z[j] *= vscale[j / 4][j % 4];
-        }
-        if constexpr (type_is_8bit<C>) {
-          if (real != ~0u) {  // (the scale of a token that does not exist is anything)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1 ? z[j] : 0.0f;
+          if constexpr (type_is_8bit<C>) {
+            const float v = z[j] * vscale[j / 4][j % 4];
+            z[j] = masked && z[j] == 0.0f ? 0.0f : v;  // (the scale of a token that is not seen may be NaN)
           }
         }
 #pragma unroll
@@ -442,12 +456,14 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         }
         pf[m] = __builtin_bit_cast(Frag<VT>, uint4{w[0], w[1], w[2], w[3]});
       }
-      if (real != ~0u) {  // (0 times what does not exist may be NaN)
+      if (masked) {  // (0 times what does not exist, or is not seen, may be NaN; what is seen of that is added at the end)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (!(real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1))
 #pragma unroll
-            for (int b = 0; b < VB; ++b) vr[b][j] = Raw8<C>{};
+          for (int b = 0; b < VB; ++b) {
+            if (!(real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1)) vr[b][j] = Raw8<C>{};
+            bad |= tame<C>(vr[b][j]);
+          }
       }
 #pragma unroll
       for (int b = 0; b < VB; ++b) {
@@ -467,6 +483,30 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
       }
     }
   }
+
+  if (C != GSK_I8) {
+    const bool any = ballot64(bad != 0) != 0;
+    if (lane == 0) sh.bad[wave] = any;
+  }
+  // What a row sees of the NaNs and infinities that were taken out, of the new tokens in this part, one by one.
+  auto add_bad = [&](uint32_t row, uint32_t e, float(&y)[8]) {
+    const uint32_t i = row / p.group;
+    int32_t node = sp.begin + (int32_t)i;
+    for (uint32_t t = min(k1, a.parent ? len : ctx + i + 1); t-- > max(k0, ctx);) {  // (backwards: a tree's path, from its node)
+      if (a.parent) {
+        if (t - ctx != (uint32_t)(node - sp.begin)) continue;
+        const int32_t up = a.parent[node];
+        node = up >= sp.begin && up < node ? up : sp.begin - 1;
+      }
+      const uint32_t pg = (uint32_t)a.table[(int64_t)r * a.table_ld + t / c.page];
+      if (pg >= c.pages) continue;
+      const int64_t at = (int64_t)pg * c.page_stride + (int64_t)(t % c.page) * c.token_stride + (int64_t)head * c.head_stride + e;
+      float x[8];
+      to_f32(load_raw8<C>((const char *)c.values + at * SZ), x);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) y[d] += fabsf(x[d]) < INF ? 0.0f : x[d];
+    }
+  };
 
   // ---- the waves' results joined ------------------------------------------------------------------------------------------
   // A thread has eight elements of one of 16 rows. A part's scratch: rows x dim of O, then rows x (m, l).
@@ -522,6 +562,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
 #pragma unroll
         for (int d = 0; d < 8; ++d) x[d] += f * sh.o[w][tr][te + d];
       }
+      if (C != GSK_I8 && (sh.bad[0] | sh.bad[1] | sh.bad[2] | sh.bad[3])) add_bad(row, e, x);
       if (parts == 1) {
         finish(row, e, x, sum);
         continue;

@@ -241,8 +241,8 @@ def attend(q, keys, values, table, seq_len, begin=None, status=None, parents=Non
     if hq == 0 or hq % heads:
         raise ValueError(f"{hq} query heads over {heads} heads of the cache")
     r, width, ld = _table(table)
-    if width * page >= 1 << 31:
-        raise ValueError(f"{width} pages of {page} tokens a request: at most 2^31 - 1 tokens")
+    if width * page >= 1 << 31 or r * (16 + width * page // 32) >= 1 << 32:
+        raise ValueError(f"{width} pages of {page} tokens for {r} requests: at most 2^31 - 1 tokens each, 2^37 in all")
     if _count(seq_len) != r or (begin is not None and _count(begin) != r + 1) or (status is not None and _count(status) != r):
         raise ValueError(f"seq_len and status must have {r} entries, begin {r + 1}")
     if begin is None:

@@ -461,3 +461,46 @@ def test_reorder_bad_pages(ge, gpu):
         c = caches.clone()
         ge.kv.reorder(c, table, lengths, torch.from_numpy(parents).to(gpu), first=prompt)
         assert np.array_equal(c.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("query,cache", [(BF, BF), (HF, HF), (BF, E4), (HF, I8)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attend_bad_values_of_unseen_tokens(ge, gpu, query, cache, tree):
+    """NaN and infinities in the keys and values of new tokens reach the tokens that see them and no others; a row written with a
+    NaN (whose 8-bit scale is NaN) likewise."""
+    g = _gen(gpu, 21)
+    lengths, news, group, page = [50, 9, 300], [9, 9, 20], 4, 16
+    table, pages = _pages(g, lengths, page)
+    keys, values, scales = _cache(g, cache, pages, page, 2, 80, False)
+    q = _rand(g, sum(news), 2 * group, 80).to(query)
+    begin = np.concatenate([[0], np.cumsum(news)])
+    par = None
+    if tree:
+        par = np.concatenate([begin[r] + np.array([-1 - begin[r]] + [(i - 1) // 2 for i in range(1, n)]) for r, n in enumerate(news)])
+    clean = ge.kv.attend(q, keys, values, table, lengths, begin=begin.tolist(), parents=par, scales=scales)
+    for r, i, what, value in [(0, 5, "v", float("nan")), (1, 0, "v", float("inf")), (2, 12, "v", -float("inf")), (0, 7, "k", float("nan")),
+                              (2, 19, "both", float("inf"))]:
+        t = lengths[r] - news[r] + i
+        at = (table[r, t // page].long(), t % page)
+        was = [x[at].clone() for x in (keys, values, *(scales or ()))]
+        row = torch.ones((1, 2, 80), device=gpu)
+        row[0, 1, 3] = value
+        kk = row if what in ("k", "both") else torch.ones_like(row)
+        vv = row if what in ("v", "both") else torch.ones_like(row)
+        ge.kv.write((at[0] * page + at[1]).reshape(1), kk, vv, keys, values, scales=scales)
+        got = ge.kv.attend(q, keys, values, table, lengths, begin=begin.tolist(), parents=par, scales=scales)
+        for rr, n in enumerate(news):
+            sees = kr.sees(n, 0, None if par is None else par, begin[rr])
+            for k in range(n):
+                a, b = got[begin[rr] + k].float(), clean[begin[rr] + k].float()
+                if rr != r or not sees[k, i]:
+                    assert torch.equal(a, b), (r, i, what, rr, k)
+                elif what == "v":
+                    assert torch.isfinite(a[:group]).all()  # (the first head's row is fine)
+                    if cache in (BF, HF):
+                        assert torch.isfinite(a[group:]).sum() == group * 79 and (
+                            torch.isnan(a[group:, 3]).all() if value != value else (a[group:, 3] == value).all())
+                    else:
+                        assert torch.isnan(a[group:]).all()
+        for x, w in zip((keys, values, *(scales or ())), was):
+            x[at] = w

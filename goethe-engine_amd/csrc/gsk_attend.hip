@@ -17,11 +17,16 @@ AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tick
   AttendPlan p;
   p.tiles = (uint32_t)((rows + most - 1) / most);
   // One round of workgroups, as many on each XCD, if the requests' longest tables fill it.
-  const uint64_t each = (uint64_t)c.heads * p.tiles, xcd = (uint64_t)cus / 8 * attend_resident(c.dim <= 128 ? 4 : 8, row_tiles(c, a));
-  const uint64_t round = each <= xcd ? xcd / each * 8 : xcd * 8 / each;
+  const uint64_t xcd = (uint64_t)cus / 8 * attend_resident(c.dim <= 128 ? 4 : 8, row_tiles(c, a));
   const uint64_t blocks = (uint64_t)a.requests * (TURN + ((uint64_t)a.max_pages * c.page + AB - 1) / AB);
-  p.items = (uint32_t)max(min(min(round, (uint64_t)tickets / each), blocks / SHARE_MIN), (uint64_t)1);
-  p.work = p.items == 1 ? 0 : (int64_t)(p.items * 2 * each * min(rows, most) * (c.dim + 2) * sizeof(float));
+  auto round = [&](uint64_t each) { return min(each <= xcd ? xcd / each * 8 : xcd * 8 / each, (uint64_t)tickets / each); };
+  p.items = (uint32_t)max(min(round((uint64_t)c.heads * p.tiles), blocks / SHARE_MIN), (uint64_t)1);
+  // (four heads of a token lie together: no more than the row of one, or its strides, between them)
+  const bool together = c.heads % AW == 0 && most == 16 && c.head_stride < c.token_stride;
+  p.items4 = together ? (uint32_t)round((uint64_t)c.heads / AW * p.tiles) : 0;
+  if (blocks < (uint64_t)p.items4 * FOUR_MIN) p.items4 = 0;
+  const uint64_t shares = max(p.items, p.items4);
+  p.work = shares == 1 ? 0 : (int64_t)(shares * 2 * c.heads * p.tiles * min(rows, most) * (c.dim + 2) * sizeof(float));
   return p;
 }
 
@@ -30,12 +35,13 @@ hipError_t launch_attend(const gsk_cache &c, const gsk_attention &a, const Atten
   p.c = c;
   p.a = a;
   p.items = plan.items;
+  p.items4 = plan.items4;
   p.tiles = plan.tiles;
   p.group = a.heads / c.heads;
   const int mt = row_tiles(c, a);
   p.rows = (uint32_t)min((uint64_t)a.max_new * p.group, (uint64_t)(16 * mt));
   p.tick = tick;
-  const uint64_t blocks = ((uint64_t)p.items + 7) / 8 * 8 * c.heads * p.tiles;
+  const uint64_t blocks = max(((uint64_t)p.items + 7) / 8 * 8 * c.heads, ((uint64_t)p.items4 + 7) / 8 * 8 * (c.heads / AW)) * p.tiles;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks);
   const bool half = a.type == GSK_F16;

@@ -27,6 +27,7 @@ namespace gse {
 constexpr int AT = 256, AW = AT / WAVE;
 constexpr uint32_t AB = 32;  // tokens of a block
 constexpr uint32_t SHARE_MIN = 8;   // blocks of a share, at least
+constexpr uint32_t FOUR_MIN = 16;   // blocks of a share, at least, where the waves take four heads
 constexpr uint32_t TURN = 8;        // what a request's turn costs besides its tokens, in blocks: a share's requests count it
 
 struct AttendArgs {
@@ -34,6 +35,7 @@ struct AttendArgs {
   gsk_attention a;
   uint32_t items, tiles, group, rows;  // shares; tiles of a request's rows; query heads of a head; rows of a tile's scratch
   uint32_t *tick;
+  uint32_t items4;  // shares where the waves take four heads (0: never)
 };
 
 template <int KD, int MT>
@@ -41,7 +43,7 @@ struct AttendShared {
   static constexpr int VB = (KD + 3) / 4, LD = 132;
   union {
     struct {                       // the tokens' loop
-      uint4 q[MT][16][KD * 4 + 1]; // the rows' operands (a piece of padding: the rows' pieces lie in different banks)
+      uint4 q[MT == 1 ? AW : MT][16][KD * 4 + 1]; // the rows' operands (a piece of padding: the rows' pieces lie in different banks)
       int64_t at[AW][AB];          // byte offsets of the block's tokens
       float scale[AW][2][AB];      // and their keys' and values' scales
     };
@@ -172,11 +174,6 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   const gsk_attention &a = p.a;
   const uint32_t tid = threadIdx.x, lane = lane_id(), lc = lane % 16, lg = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  // The heads and tiles of an item run on one XCD (workgroups go round the eight of them): a token's heads lie together.
-  const uint32_t x8 = blockIdx.x / 8, each = c.heads * p.tiles, x = x8 % each, item = x8 / each * 8 + blockIdx.x % 8;
-  const uint32_t head = x / p.tiles, tile = x - head * p.tiles;
-  if (item >= p.items) return;
-
   // ---- the share ----------------------------------------------------------------------------------------------------------
   // Every wave for itself, a lane one request or, where there are more than lanes, four at a time: a request's blocks, one at
   // least if it has rows to write, after TURN that stand for its turn. The shares are of one size, the first ones a block more.
@@ -201,7 +198,15 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   uint32_t mine = take(0), total = mine;  // (below 2^32 by the host's check)
   for (uint32_t i0 = 4 * WAVE; i0 < a.requests; i0 += 4 * WAVE) total += take(i0);
   total = wave_sum_u32(total);
-  const uint32_t shares = min(max(total / SHARE_MIN, 1u), p.items);
+  // Four heads: where a token's heads lie together and there are tokens enough, a wave takes every block of the share for one of
+  // four heads (a workgroup's loads are then 512 bytes or 1 KB together, not a quarter of that; 128 requests of up to 16384
+  // tokens of 8 heads of 128 bytes: 637 -> FOUR us), and nothing is joined between waves.
+  const bool four = MT == 1 && p.items4 && total >= p.items4 * FOUR_MIN;
+  const uint32_t shares = four ? p.items4 : min(max(total / SHARE_MIN, 1u), p.items);
+  // The heads and tiles of an item run on one XCD (workgroups go round the eight of them): a token's heads lie together.
+  const uint32_t x8 = blockIdx.x / 8, each = (four ? c.heads / AW : c.heads) * p.tiles, x = x8 % each;
+  const uint32_t item = x8 / each * 8 + blockIdx.x % 8, head0 = x / p.tiles * (four ? AW : 1), tile = x % p.tiles;
+  const uint32_t head = four ? head0 + wave : head0, heads_here = four ? AW : 1;
   if (item >= shares) return;
   const uint32_t share = total / shares, longer = total - share * shares;
   auto first_of = [&](uint32_t w) { return w * share + min(w, longer); };
@@ -262,17 +267,18 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
 
   // ---- the rows -----------------------------------------------------------------------------------------------------------
   const uint32_t sign = a.scale < 0 ? 0x80008000u : 0;  // (the scale's own, so that the largest score is the largest product)
-  constexpr int QN = (MT * 16 * KD * 4 + AT - 1) / AT;
+  constexpr int QN = ((MT == 1 ? AW : MT) * 16 * KD * 4 + AT - 1) / AT;
   uint4 rows_q[QN];  // (to LDS once the first block's loads are on their way)
 #pragma unroll
   for (int j = 0; j < QN; ++j) {
-    const uint32_t at_q = j * AT + tid, w = at_q / (KD * 4), e = at_q % (KD * 4), row = min(row0 + w, rows - 1), n = row / p.group;
+    const uint32_t at_q = j * AT + tid, w = at_q / (KD * 4), e = at_q % (KD * 4);
+    const uint32_t row = min(row0 + (four ? w % 16 : w), rows - 1), n = row / p.group, h = head0 + (four ? w / 16 : 0);
     rows_q[j] = uint4{0, 0, 0, 0};
-    if (w < MT * 16 && e * 8 < c.dim)
+    if (w < (four ? AW : MT) * 16 && e * 8 < c.dim)
       rows_q[j] = *(const uint4 *)((const char *)a.q + ((int64_t)(sp.begin + n) * a.q_token_stride +
-                                                        (int64_t)(head * p.group + row - n * p.group) * a.q_head_stride + e * 8) * 2);
+                                                        (int64_t)(h * p.group + row - n * p.group) * a.q_head_stride + e * 8) * 2);
   }
-  auto q_of = [&](int m, int k) { return __builtin_bit_cast(Frag<Q>, sh.q[m][lc][k * 4 + lg]); };
+  auto q_of = [&](int m, int k) { return __builtin_bit_cast(Frag<Q>, sh.q[four ? wave : m][lc][k * 4 + lg]); };
   uint32_t sees[MT];   // chains: the first cached token that the lane's row does not see
   uint64_t path[MT];   // trees: which new tokens it sees
   const int32_t parent = a.parent ? a.parent[sp.begin + (int32_t)min(lane, (uint32_t)sp.n - 1)] : 0;  // of new token `lane`
@@ -310,9 +316,10 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   // masked. Lanes l and l + 32 find the same token.
   const float scale = fabsf(a.scale) * 1.44269504f;
   const int32_t *table = a.table + (int64_t)r * a.table_ld;
-  const uint32_t pages_on = AW * AB / c.page, tokens_on = AW * AB % c.page;  // from a block of the wave to its next one
+  const uint32_t hop = four ? AB : AW * AB, pages_on = hop / c.page, tokens_on = hop % c.page;  // to the wave's next block
   const uint32_t l32 = lane % 32;
-  uint32_t pi = (k0 + wave * AB + l32) / c.page, off = (k0 + wave * AB + l32) % c.page;  // the lane's token of the next block
+  uint32_t t = k0 + (four ? 0 : wave * AB);
+  uint32_t pi = (t + l32) / c.page, off = (t + l32) % c.page;  // the lane's token of the next block
   const uint32_t last_page = (max(k1, 1u) - 1) / c.page;
   auto next_page = [&] { return (uint32_t)table[min(pi, last_page)]; };
   uint32_t there = 0;  // the tokens of the block that sh.at has
@@ -352,7 +359,6 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     }
   };
 
-  uint32_t t = k0 + wave * AB;
   if (t < k1) {
     place_block(t + l32, next_page());
     load_keys();
@@ -362,11 +368,11 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     const uint32_t at_q = j * AT + tid, w = at_q / (KD * 4);
     uint4 v = rows_q[j];
     v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
-    if (w < MT * 16) sh.q[w / 16][w % 16][at_q % (KD * 4)] = v;
+    if (w < (four ? AW : MT) * 16) sh.q[w / 16][w % 16][at_q % (KD * 4)] = v;
   }
   __syncthreads();
   if (t < k1) {
-    for (; t < k1; t += AW * AB) {
+    for (; t < k1; t += hop) {
       const uint32_t page = next_page(), real = there;
       if constexpr (type_is_8bit<C>) sh.scale[wave][lane / 32][l32] = lane < 32 ? scale_of * scale : scale_of;
       Raw8<C> vr[VB][8];
@@ -393,7 +399,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
           for (int m = 0; m < MT; ++m) s[m][u] = mma<Q>(kf, q_of(m, k), s[m][u]);
         }
       }
-      place_block(t + AW * AB + l32, page);
+      place_block(t + hop + l32, page);
       load_keys();
       f32x4 kscale[2], vscale[2];
       if constexpr (type_is_8bit<C>) {
@@ -489,7 +495,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     if (lane == 0) sh.bad[wave] = any;
   }
   // What a row sees of the NaNs and infinities that were taken out, of the new tokens in this part, one by one.
-  auto add_bad = [&](uint32_t row, uint32_t e, float(&y)[8]) {
+  auto add_bad = [&](uint32_t h, uint32_t row, uint32_t e, float(&y)[8]) {
     const uint32_t i = row / p.group;
     int32_t node = sp.begin + (int32_t)i;
     for (uint32_t t = min(k1, a.parent ? len : ctx + i + 1); t-- > max(k0, ctx);) {  // (backwards: a tree's path, from its node)
@@ -500,7 +506,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
       }
       const uint32_t pg = (uint32_t)a.table[(int64_t)r * a.table_ld + t / c.page];
       if (pg >= c.pages) continue;
-      const int64_t at = (int64_t)pg * c.page_stride + (int64_t)(t % c.page) * c.token_stride + (int64_t)head * c.head_stride + e;
+      const int64_t at = (int64_t)pg * c.page_stride + (int64_t)(t % c.page) * c.token_stride + (int64_t)h * c.head_stride + e;
       float x[8];
       to_f32(load_raw8<C>((const char *)c.values + at * SZ), x);
 #pragma unroll
@@ -513,15 +519,17 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   float *work = (float *)a.work;
   const int64_t part_size = (int64_t)p.rows * (c.dim + 2);
   // A share has two of them: of the request that it goes on with, and of the one that goes on after it.
-  auto scratch = [&](uint32_t it) { return work + (((int64_t)it * 2 + (it == first_item)) * each + x) * part_size; };
+  auto scratch = [&](uint32_t it, uint32_t h) {
+    return work + ((((int64_t)it * 2 + (it == first_item)) * c.heads + h) * p.tiles + tile) * part_size;
+  };
   const uint32_t tr = tid / 16, te = tid % 16 * 8;
-  auto finish = [&](uint32_t row, uint32_t e, const float (&x)[8], float sum) {
+  auto finish = [&](uint32_t h, uint32_t row, uint32_t e, const float (&x)[8], float sum) {
     const uint32_t i = row / p.group, gi = row - i * p.group;
     const float inv = sum > 0 ? 1.0f / sum : 0.0f;
     float y[8];
 #pragma unroll
     for (int d = 0; d < 8; ++d) y[d] = sum == 0 ? 0.0f : sum > 0 ? x[d] * inv : x[d] / sum;
-    store_raw8<Q>((char *)a.out + (((int64_t)(sp.begin + i) * a.heads + head * p.group + gi) * c.dim + e) * 2, from_f32<Q>(y));
+    store_raw8<Q>((char *)a.out + (((int64_t)(sp.begin + i) * a.heads + h * p.group + gi) * c.dim + e) * 2, from_f32<Q>(y));
   };
 #pragma unroll 1
   for (int m = 0; m < MT; ++m) {
@@ -551,28 +559,31 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
       __syncthreads();
       const uint32_t row = row0 + m * 16 + tr, e = b * 128 + te;
       if (row >= rows || e >= c.dim) continue;
-      float top = -INF, sum = 0, x[8] = {};
+#pragma unroll 1
+      for (uint32_t hh = 0; hh < heads_here; ++hh) {  // (four heads: a wave has all of one)
+        float top = -INF, sum = 0, x[8] = {};
+        const uint32_t w0 = four ? hh : 0, w1 = four ? hh + 1 : AW;
+        for (uint32_t w = w0; w < w1; ++w) top = fmaxf(top, sh.m[w][tr]);
+        for (uint32_t w = w0; w < w1; ++w) {
+          const float f = weight_of(sh.m[w][tr], sh.l[w][tr], top);
+          if (f == 0.0f) continue;
+          sum += f * sh.l[w][tr];
 #pragma unroll
-      for (int w = 0; w < AW; ++w) top = fmaxf(top, sh.m[w][tr]);
+          for (int d = 0; d < 8; ++d) x[d] += f * sh.o[w][tr][te + d];
+        }
+        if (C != GSK_I8 && (sh.bad[0] | sh.bad[1] | sh.bad[2] | sh.bad[3])) add_bad(head0 + hh, row, e, x);
+        if (parts == 1) {
+          finish(head0 + hh, row, e, x, sum);
+          continue;
+        }
+        float *o = scratch(item, head0 + hh) + (int64_t)(row - row0) * c.dim + e;
 #pragma unroll
-      for (int w = 0; w < AW; ++w) {
-        const float f = weight_of(sh.m[w][tr], sh.l[w][tr], top);
-        if (f == 0.0f) continue;
-        sum += f * sh.l[w][tr];
-#pragma unroll
-        for (int d = 0; d < 8; ++d) x[d] += f * sh.o[w][tr][te + d];
+        for (int d = 0; d < 8; d += 2)
+          st_ag((uint64_t *)(o + d), (uint64_t)__float_as_uint(x[d]) | (uint64_t)__float_as_uint(x[d + 1]) << 32);
+        if (e == 0)
+          st_ag((uint64_t *)(scratch(item, head0 + hh) + (int64_t)p.rows * c.dim + 2 * (row - row0)),
+                (uint64_t)__float_as_uint(top) | (uint64_t)__float_as_uint(sum) << 32);
       }
-      if (C != GSK_I8 && (sh.bad[0] | sh.bad[1] | sh.bad[2] | sh.bad[3])) add_bad(row, e, x);
-      if (parts == 1) {
-        finish(row, e, x, sum);
-        continue;
-      }
-      float *o = scratch(item) + (int64_t)(row - row0) * c.dim + e;
-#pragma unroll
-      for (int d = 0; d < 8; d += 2) st_ag((uint64_t *)(o + d), (uint64_t)__float_as_uint(x[d]) | (uint64_t)__float_as_uint(x[d + 1]) << 32);
-      if (e == 0)
-        st_ag((uint64_t *)(scratch(item) + (int64_t)p.rows * c.dim + 2 * (row - row0)),
-              (uint64_t)__float_as_uint(top) | (uint64_t)__float_as_uint(sum) << 32);
     }
   }
   if (parts == 1) {
@@ -593,7 +604,8 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   // 16 threads a row again; with few rows, several such groups share a row's parts. A thread takes eight of its parts' loads at
   // once: a round trip, in most calls the only one.
 #pragma unroll 1
-  for (int m = 0; m < MT; ++m) {
+  for (uint32_t mh = 0; mh < MT * heads_here; ++mh) {
+    const uint32_t m = four ? 0 : mh, h = head0 + (four ? mh : 0);
     if (row0 + m * 16 >= rows) break;
     const uint32_t count = min(rows - row0 - m * 16, 16u), wide = count <= 1 ? 1 : 1u << (32 - __builtin_clz(count - 1));
     const uint32_t i = m * 16 + tr % wide, mine = tr / wide, shares = 16 / wide;
@@ -607,7 +619,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         uint64_t ml[8], w[8][4];
 #pragma unroll
         for (uint32_t k = 0; k < 8; ++k) {
-          const float *o = scratch(first_item + min(s0 + k * shares, parts - 1));
+          const float *o = scratch(first_item + min(s0 + k * shares, parts - 1), h);
           ml[k] = ld_ag((const uint64_t *)(o + (int64_t)p.rows * c.dim + 2 * i));
 #pragma unroll
           for (int d = 0; d < 4; ++d) w[k][d] = ld_ag((const uint64_t *)(o + (int64_t)i * c.dim + e) + d);
@@ -658,7 +670,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
           }
         }
       }
-      if (in && mine == 0) finish(row0 + i, e, y, sum);
+      if (in && mine == 0) finish(h, row0 + i, e, y, sum);
     }
   }
   __syncthreads();

@@ -13,6 +13,7 @@ hipError_t launch_reorder(const gsk_reorder_beams &a, hipStream_t s);
 struct AttendPlan {
   uint32_t tiles;  // of a request's (new token, query head of the group) rows
   uint32_t items;  // equal shares of the requests' cached tokens: workgroups per cache head and tile, at most
+  uint32_t items4; // shares where a workgroup takes four heads (0: it never does)
   int64_t work;    // scratch bytes
 };
 AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tickets, int cus);

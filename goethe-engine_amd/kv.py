@@ -74,7 +74,8 @@ def _layout_of(shape, stride, dtype, heads_first, scale_shape, scale_stride, wri
 
 
 def _cache(keys, values, scales, heads_first, writes=False):
-    """The cache as the library takes it, and its (size, type, pages, page, heads, dim); what is not in order is refused here."""
+    """The cache as the library takes it, its (size, type, pages, page, heads, dim), its strides and its device; what is not in
+    order is refused here."""
     shape, stride, dtype, dev = keys.shape, keys.stride(), keys.dtype, keys.device
     if values.shape != shape or values.stride() != stride or values.dtype is not dtype or values.device != dev:
         raise ValueError("keys and values must have one shape, layout, type and device")
@@ -96,7 +97,7 @@ def _cache(keys, values, scales, heads_first, writes=False):
         raise ValueError("a token's head must lie together, at a multiple of 8 elements")
     if writes and k == v:
         raise ValueError("the cache written to must not be keys and values at once")
-    return _CACHE.pack(*size, k, v, *at, ks, vs, *s_at), size, dev
+    return _CACHE.pack(*size, k, v, *at, ks, vs, *s_at), size, at, dev
 
 
 def _same_device(dev, name, t):
@@ -129,9 +130,9 @@ def _rows(t, name, heads, dim):
 
 
 @functools.lru_cache(maxsize=1024)
-def _work_bytes(device, handle_rows, cache, call):
-    """gsk_attention_work for sizes alone: cache: (size .. dim) of gsk_cache, call: (requests .. max_new, max_pages)."""
-    c = _CACHE.pack(*cache, *[0] * 10)
+def _work_bytes(device, handle_rows, size, at, call):
+    """gsk_attention_work for sizes alone: (size .. dim) and strides of gsk_cache, call: (requests .. max_new, max_pages)."""
+    c = _CACHE.pack(*size, 0, 0, *at, *[0] * 5)
     a = _ATTEND.pack(_ATTEND.size, *call[:-1], *[0] * 6, call[-1], 0.0, *[0] * 7)
     return _lib.handle(device, 1, 1).call("gsk_attention_work", c, a)
 
@@ -151,7 +152,7 @@ def write(slot, k, v, keys, values, scales=None, heads_first=False):
     per page + offset: paged.StepMap.slot), in place; negative slots and those past the cache are skipped, a slot belongs to one
     token of the call. In 8 bits, in fp32: scale = max(max |row| * (1 / M), 2^-126), M = 448 (float8_e4m3fn) or 127 (int8), the
     elements row * (1 / scale) rounded to nearest even; a row with a NaN or an infinity then reads as NaN."""
-    c, (_, _, _, _, heads, dim), dev = _cache(keys, values, scales, heads_first, writes=True)
+    c, (_, _, _, _, heads, dim), _, dev = _cache(keys, values, scales, heads_first, writes=True)
     k, k_at, shape, k_stride = _rows(k, "k", heads, dim)
     v, v_at, v_shape, v_stride = _rows(v, "v", heads, dim)
     kind, n = _ROWS.get(k.dtype), shape[0]
@@ -180,7 +181,7 @@ def read(keys, values, table, begin, first=None, max_tokens=None, scales=None, d
     first[r], first[r] + 1, ... (first: 0). table int32 [requests, pages]: each request's pages (PageTable.table). max_tokens:
     the rows (default: the last of begin, which then has to be on the host). out: the two tensors to write to (contiguous).
     Rows from begin[requests] on are left as they were (without out: not set); a row whose token or page is out of range is 0."""
-    c, (_, _, _, page, heads, dim), dev = _cache(keys, values, scales, heads_first)
+    c, (_, _, _, page, heads, dim), _, dev = _cache(keys, values, scales, heads_first)
     r, width, ld = _table(table)
     if _count(begin) != r + 1 or (first is not None and _count(first) != r):
         raise ValueError(f"begin must have {r + 1} entries, first {r}")
@@ -232,7 +233,7 @@ def attend(q, keys, values, table, seq_len, begin=None, status=None, parents=Non
     not serve gives zeros). scale: default dim ** -0.5. out: a contiguous tensor to write to. What sees nothing is 0; rows from
     begin[requests] on are left as they were (without out: not set); numbers out of range give zeros, cached tokens whose page
     is out of range are not seen."""
-    c, size, dev = _cache(keys, values, scales, heads_first)
+    c, size, at, dev = _cache(keys, values, scales, heads_first)
     _, cache_kind, _, page, heads, dim = size
     q, q_at, (n, hq, _), q_stride = _rows(q, "q", None, dim)
     kind = _TYPES.get(q.dtype, _lib.K_F32)
@@ -279,7 +280,7 @@ def attend(q, keys, values, table, seq_len, begin=None, status=None, parents=Non
     parents = _vec(parents, i32, dev) if parents is not None else None
     status = _vec(status, i32, dev) if status is not None else None
     h, work = _lib.handle(index, 1, 1), None
-    need = _work_bytes(index, h.rows, size, (r, n, hq, kind, max_new, width))
+    need = _work_bytes(index, h.rows, size, at, (r, n, hq, kind, max_new, width))
     if need:
         work = torch.empty(need, dtype=torch.uint8, device=dev)
     a = _ATTEND.pack(_ATTEND.size, r, n, hq, kind, max_new, q_at, q_stride[0], q_stride[1], out.data_ptr(), table.data_ptr(), ld,

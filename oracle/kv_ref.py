@@ -63,15 +63,17 @@ def tokens(cache, scale, ids, first, n, heads_first):
     rows are NaN-free zeros, and False in the mask returned beside)."""
     page, pages = cache.shape[2 if heads_first else 1], cache.shape[0]
     heads, dim = cache.shape[1 if heads_first else 2], cache.shape[3]
-    x, there = np.zeros((n, heads, dim)), np.zeros(n, bool)
-    for i in range(n):
-        p, o = divmod(first + i, page)
-        if first + i < 0 or p >= len(ids) or not 0 <= ids[p] < pages:
-            continue
-        at = (ids[p], slice(None), o) if heads_first else (ids[p], o)
-        x[i], there[i] = _np(cache[at]), True
-        if scale is not None:
-            x[i] *= scale[at].cpu().numpy().astype(np.float64)[:, None]
+    at = first + np.arange(n)
+    held = np.concatenate([np.asarray(ids, np.int64), [-1]])
+    page_of = held[np.clip(at // page, 0, len(ids))]
+    there = (at >= 0) & (at // page < len(ids)) & (page_of >= 0) & (page_of < pages)
+    x = np.zeros((n, heads, dim))
+    p, o = (torch.from_numpy(i[there]).to(cache.device) for i in (page_of, at % page))
+    where = (p, slice(None), o) if heads_first else (p, o)
+    rows = _np(cache[where])
+    if scale is not None:
+        rows = rows * scale[where].cpu().numpy().astype(np.float64)[..., None]
+    x[there] = rows
     return x, there
 
 

@@ -504,3 +504,24 @@ def test_attend_bad_values_of_unseen_tokens(ge, gpu, query, cache, tree):
                         assert torch.isnan(a[group:]).all()
         for x, w in zip((keys, values, *(scales or ())), was):
             x[at] = w
+
+
+@pytest.mark.parametrize("query,cache", KINDS)
+@pytest.mark.parametrize("dim,heads,group", [(128, 8, 4), (80, 4, 16), (256, 4, 2), (64, 12, 1)])
+def test_attend_heads_together(ge, gpu, query, cache, dim, heads, group):
+    """Long ragged contexts whose heads lie together in a token (a wave then takes a head of its own), chains and a tree among
+    them, and the same caches with the heads ahead."""
+    g = _gen(gpu, dim + heads)
+    news, lengths = [1, 1, 0, 1, 1, 1, 1], [30000, 17, 0, 9000, 1, 12345, 60001]
+    if group <= 2:
+        news = [3, 1, 0, 5, 1, 2, 8]
+    par = None
+    if group == 1:
+        begin = np.concatenate([[0], np.cumsum(news)])
+        par = [-1 if i == 0 else int(begin[r] + (i - 1) // 2) for r, n in enumerate(news) for i in range(n)]
+    table, pages = _pages(g, lengths, 16)
+    keys, values, scales = _cache(g, cache, pages, 16, heads, dim, False)
+    q = _rand(g, sum(news), heads * group, dim).to(query)
+    _check(ge, q, keys, values, scales, table, lengths, news, False, parents=par)
+    turned = [x.transpose(1, 2).contiguous() for x in (keys, values, *(scales or ()))]
+    _check(ge, q, turned[0], turned[1], tuple(turned[2:]) or None, table, lengths, news, True, parents=par)

@@ -27,7 +27,7 @@ namespace gse {
 constexpr int AT = 256, AW = AT / WAVE;
 constexpr uint32_t AB = 32;  // tokens of a block
 constexpr uint32_t SHARE_MIN = 8;   // blocks of a share, at least
-constexpr uint32_t FOUR_MIN = 16;   // blocks of a share, at least, where the waves take four heads
+constexpr uint32_t FOUR_MIN = 32;   // blocks of a share, at least, where the waves take four heads
 constexpr uint32_t TURN = 8;        // what a request's turn costs besides its tokens, in blocks: a share's requests count it
 
 struct AttendArgs {
@@ -198,9 +198,8 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   uint32_t mine = take(0), total = mine;  // (below 2^32 by the host's check)
   for (uint32_t i0 = 4 * WAVE; i0 < a.requests; i0 += 4 * WAVE) total += take(i0);
   total = wave_sum_u32(total);
-  // Four heads: where a token's heads lie together and there are tokens enough, a wave takes every block of the share for one of
-  // four heads (a workgroup's loads are then 512 bytes or 1 KB together, not a quarter of that; 128 requests of up to 16384
-  // tokens of 8 heads of 128 bytes: 637 -> FOUR us), and nothing is joined between waves.
+  // Four heads: where a token's heads lie together and the host finds it worth it (attend_plan), with tokens enough, a wave takes
+  // every block of the share for one of four heads, and nothing is joined between waves.
   const bool four = MT == 1 && p.items4 && total >= p.items4 * FOUR_MIN;
   const uint32_t shares = four ? p.items4 : min(max(total / SHARE_MIN, 1u), p.items);
   // The heads and tiles of an item run on one XCD (workgroups go round the eight of them): a token's heads lie together.

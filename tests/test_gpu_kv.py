@@ -507,21 +507,36 @@ def test_attend_bad_values_of_unseen_tokens(ge, gpu, query, cache, tree):
 
 
 @pytest.mark.parametrize("query,cache", KINDS)
-@pytest.mark.parametrize("dim,heads,group", [(128, 8, 4), (80, 4, 16), (256, 4, 2), (64, 12, 1)])
+@pytest.mark.parametrize("dim,heads,group", [(128, 8, 4), (80, 12, 3), (64, 4, 2)])
 def test_attend_heads_together(ge, gpu, query, cache, dim, heads, group):
-    """Long ragged contexts whose heads lie together in a token (a wave then takes a head of its own), chains and a tree among
-    them, and the same caches with the heads ahead."""
+    """Tokens enough that, their heads lying together, a wave takes a head of its own: requests that share their pages (a table
+    may name a page twice), chains or a tree, short and empty ones among them; and the same caches with the heads ahead."""
     g = _gen(gpu, dim + heads)
-    news, lengths = [1, 1, 0, 1, 1, 1, 1], [30000, 17, 0, 9000, 1, 12345, 60001]
-    if group <= 2:
-        news = [3, 1, 0, 5, 1, 2, 8]
+    many = 44 if heads > 8 else 68 if heads == 8 else 132
+    news = ([2, 1, 0, 3] if group < 4 else [1, 1, 0, 1]) * (many // 4)
+    lengths = [10000 - 13 * r if r % 4 else 17 for r in range(many)]
+    lengths[2] = 0
     par = None
-    if group == 1:
+    if group == 3:
         begin = np.concatenate([[0], np.cumsum(news)])
-        par = [-1 if i == 0 else int(begin[r] + (i - 1) // 2) for r, n in enumerate(news) for i in range(n)]
-    table, pages = _pages(g, lengths, 16)
+        par = [-1 if i == 0 else int(begin[r]) for r, n in enumerate(news) for i in range(n)]
+    one, pages = _pages(g, [10000], 16)
+    table = one.repeat(many, 1)
     keys, values, scales = _cache(g, cache, pages, 16, heads, dim, False)
     q = _rand(g, sum(news), heads * group, dim).to(query)
-    _check(ge, q, keys, values, scales, table, lengths, news, False, parents=par)
+    args = dict(begin=np.concatenate([[0], np.cumsum(news)]), parents=par, max_new=3)
+    got = ge.kv.attend(q, keys, values, table, lengths, scales=scales, **args)
     turned = [x.transpose(1, 2).contiguous() for x in (keys, values, *(scales or ()))]
-    _check(ge, q, turned[0], turned[1], tuple(turned[2:]) or None, table, lengths, news, True, parents=par)
+    ahead = ge.kv.attend(q, turned[0], turned[1], table, lengths, scales=tuple(turned[2:]) or None, heads_first=True, **args)
+    k, _ = kr.tokens(keys, scales and scales[0], one[0].tolist(), 0, 10000, False)
+    v, _ = kr.tokens(values, scales and scales[1], one[0].tolist(), 0, 10000, False)
+    begin, qn = args["begin"], kr._np(q)
+    for r in [0, 1, 3, 4, many // 2 + 1, many - 1]:
+        n, ln = news[r], lengths[r]
+        want, tol = kr.attend(qn[begin[r]:begin[r + 1]], k[:ln], v[:ln], kr.sees(n, ln - n, par, begin[r]), float(np.float32(dim ** -0.5)),
+                              query, cache in kr.MOST)
+        for x in (got, ahead):
+            assert (np.abs(kr._np(x[begin[r]:begin[r + 1]]) - want) <= tol).all(), r
+    # every row: what one order of the cache gives is what the other gives, to twice the bound's size
+    off = (got.float() - ahead.float()).abs()
+    assert (off <= 2 ** -6 * (ahead.float().abs() + ahead.float().abs().mean())).all()

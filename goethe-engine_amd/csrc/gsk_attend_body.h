@@ -111,16 +111,17 @@ __device__ __forceinline__ Frag<T> turned(const Raw8<C> (&v)[8]) {
   return __builtin_bit_cast(Frag<T>, uint4{w[0], w[1], w[2], w[3]});
 }
 
-// Makes finite numbers of the NaNs and infinities of eight elements (their exponents' upper bit cleared); nonzero if it has any.
+// Makes finite numbers of the NaNs and infinities of eight elements (their exponents' upper bit cleared), if `on`; nonzero if
+// there are any.
 template <uint32_t C>
-__device__ __forceinline__ uint32_t tame(Raw8<C> &r) {
+__device__ __forceinline__ uint32_t tame(Raw8<C> &r, bool on) {
   constexpr uint32_t ALL = C == GSK_BF16 ? 0x7F807F80u : C == GSK_F16 ? 0x7C007C00u : 0x7F7F7F7Fu;
   constexpr uint32_t ONE = C == GSK_BF16 ? 0x00800080u : C == GSK_F16 ? 0x04000400u : 0x01010101u;
-  constexpr uint32_t TOP = type_is_8bit<C> ? 0x80808080u : 0x80008000u;
+  const uint32_t top = on ? type_is_8bit<C> ? 0x80808080u : 0x80008000u : 0u;
   uint32_t any = 0;
 #pragma unroll
   for (int i = 0; C != GSK_I8 && i < Raw8<C>::N; ++i) {
-    const uint32_t bad = ((r.w[i] & ALL) + ONE) & TOP;  // (8 bits: the one magnitude that is no number)
+    const uint32_t bad = ((r.w[i] & ALL) + ONE) & top;  // (8 bits: the one magnitude that is no number)
     r.w[i] &= ~(bad >> 1);
     any |= bad;
   }
@@ -461,14 +462,16 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         }
         pf[m] = __builtin_bit_cast(Frag<VT>, uint4{w[0], w[1], w[2], w[3]});
       }
-      if (masked) {  // (0 times what does not exist, or is not seen, may be NaN; what is seen of that is added at the end)
+      if (masked) {  // (0 times what does not exist, or a new token that is not seen, may be NaN; what is seen is added at the end)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t k = (j / 4) * 16 + lg * 4 + j % 4;
 #pragma unroll
           for (int b = 0; b < VB; ++b) {
-            if (!(real >> ((j / 4) * 16 + lg * 4 + j % 4) & 1)) vr[b][j] = Raw8<C>{};
-            bad |= tame<C>(vr[b][j]);
+            if (!(real >> k & 1)) vr[b][j] = Raw8<C>{};
+            bad |= tame<C>(vr[b][j], t + k >= ctx);
           }
+        }
       }
 #pragma unroll
       for (int b = 0; b < VB; ++b) {

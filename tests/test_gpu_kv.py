@@ -540,3 +540,37 @@ def test_attend_heads_together(ge, gpu, query, cache, dim, heads, group):
     # every row: what one order of the cache gives is what the other gives, to twice the bound's size
     off = (got.float() - ahead.float()).abs()
     assert (off <= 2 ** -6 * (ahead.float().abs() + ahead.float().abs().mean())).all()
+
+
+@pytest.mark.parametrize("cache", [BF, HF, E4, I8])
+def test_attend_bad_values_of_older_tokens(ge, gpu, cache):
+    """A NaN or an infinity in an older token's value reaches every new token of its request, wherever it lies: beside the new
+    ones, in a block with a page that is out of range, far from both."""
+    g = _gen(gpu, 22)
+    lengths, news, page = [70, 70, 130], [6, 1, 4], 8
+    table, pages = _pages(g, lengths, page)
+    table[2, 3] = -1
+    keys, values, scales = _cache(g, cache, pages, page, 2, 64, False)
+    query = HF if cache is HF else BF
+    q = _rand(g, sum(news), 4, 64).to(query)
+    begin = [0, 6, 7, 11]
+    clean = ge.kv.attend(q, keys, values, table, lengths, begin=begin, scales=scales)
+    for r, t, value in [(0, 63, float("inf")), (0, 3, float("nan")), (1, 68, -float("inf")), (2, 33, float("inf")), (2, 20, float("nan")),
+                        (2, 120, float("inf"))]:
+        at = (table[r, t // page].long(), t % page)
+        was = [x[at].clone() for x in (keys, values, *(scales or ()))]
+        row = torch.ones((1, 2, 64), device=gpu)
+        row[0, 1, 3] = value
+        ge.kv.write((at[0] * page + at[1]).reshape(1), torch.ones_like(row), row, keys, values, scales=scales)
+        got = ge.kv.attend(q, keys, values, table, lengths, begin=begin, scales=scales).float()
+        for rr in range(3):
+            a = got[begin[rr]:begin[rr + 1]]
+            if rr != r:
+                assert torch.equal(a, clean[begin[rr]:begin[rr + 1]].float()), (r, t)
+            elif cache in (BF, HF):
+                assert torch.isfinite(a[:, :2]).all() and torch.isfinite(a[:, 2:]).sum() == news[r] * 2 * 63, (r, t)
+                assert torch.isnan(a[:, 2:, 3]).all() if value != value else (a[:, 2:, 3] == value).all(), (r, t)
+            else:
+                assert torch.isfinite(a[:, :2]).all() and torch.isnan(a[:, 2:]).all(), (r, t)
+        for x, w in zip((keys, values, *(scales or ())), was):
+            x[at] = w

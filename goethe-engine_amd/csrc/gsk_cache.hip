@@ -20,48 +20,38 @@ __device__ __forceinline__ Place place(const gsk_cache &c, uint32_t pg, uint32_t
           (int64_t)pg * c.scale_page_stride + (int64_t)off * c.scale_token_stride + (int64_t)head * c.scale_head_stride};
 }
 
-template <uint32_t SRC, uint32_t DST, int GL, int ROWS>
+template <uint32_t SRC, uint32_t DST, int GL>
 __global__ __launch_bounds__(CT) void write_kernel(gsk_cache c, gsk_rows a, Div heads, Div page) {
-  const uint32_t j = threadIdx.x % GL, rows = a.tokens * c.heads;
-  const uint32_t first = blockIdx.x * (CT / GL * ROWS) + threadIdx.x / GL;
+  const uint32_t j = threadIdx.x % GL, id = blockIdx.x * (CT / GL) + threadIdx.x / GL;
+  if (id >= a.tokens * c.heads) return;  // (the group as a whole)
   const bool values = blockIdx.y != 0, mine = j * 8 < c.dim;
   const char *src = (const char *)(values ? a.v : a.k) + j * 8 * type_size<SRC>;
-  const int64_t ts = (values ? a.v_token_stride : a.k_token_stride) * type_size<SRC>;
-  const int64_t hs = (values ? a.v_head_stride : a.k_head_stride) * type_size<SRC>;
+  const int64_t ts = values ? a.v_token_stride : a.k_token_stride, hs = values ? a.v_head_stride : a.k_head_stride;
   char *dst = (char *)(values ? c.values : c.keys) + j * 8 * type_size<DST>;
   float *scales = values ? c.value_scales : c.key_scales;
-  Raw8<SRC> raw[ROWS];
-  uint64_t slot[ROWS];
-  uint32_t head[ROWS];
+  uint32_t head, off;
+  const uint32_t t = quotient(id, heads, head);
+  const uint64_t slot = (uint64_t)a.slot[t];
+  Raw8<SRC> raw{};
+  if (mine) raw = load_raw8<SRC>(src + ((int64_t)t * ts + (int64_t)head * hs) * type_size<SRC>);
+  if (slot >= (uint64_t)c.pages * c.page) return;  // (negative ones are past it; the group as a whole)
+  const uint32_t pg = quotient((uint32_t)slot, page, off);
+  const Place p = place(c, pg, off, head);
+  float x[8];
+  to_f32(raw, x);
+  if constexpr (type_is_8bit<DST>) {
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const uint32_t id = first + i * (CT / GL), t = quotient(min(id, rows - 1), heads, head[i]);
-    slot[i] = id < rows ? (uint64_t)a.slot[t] : ~0ull;
-    raw[i] = Raw8<SRC>{};
-    if (mine) raw[i] = load_raw8<SRC>(src + (int64_t)t * ts + (int64_t)head[i] * hs);
+    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+    m = group_max<GL>(m);
+    const bool bad = m >= 0x7F800000u;
+    const float most = DST == GSK_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f;
+    const float scale = fmaxf(__fmul_rn(__uint_as_float(m), most), 0x1p-126f), inv = __fdiv_rn(1.0f, scale);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = bad ? 0.0f : __fmul_rn(x[e], inv);
+    if (j == 0) scales[p.scale] = bad ? __uint_as_float(0x7FC00000u) : scale;
   }
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    if (slot[i] >= (uint64_t)c.pages * c.page) continue;  // (negative ones are past it; the group as a whole)
-    uint32_t off;
-    const uint32_t pg = quotient((uint32_t)slot[i], page, off);
-    const Place p = place(c, pg, off, head[i]);
-    float x[8];
-    to_f32(raw[i], x);
-    if constexpr (type_is_8bit<DST>) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-      m = group_max<GL>(m);
-      const bool bad = m >= 0x7F800000u;
-      const float most = DST == GSK_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f;
-      const float scale = fmaxf(__fmul_rn(__uint_as_float(m), most), 0x1p-126f), inv = __fdiv_rn(1.0f, scale);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = bad ? 0.0f : __fmul_rn(x[e], inv);
-      if (j == 0) scales[p.scale] = bad ? __uint_as_float(0x7FC00000u) : scale;
-    }
-    if (mine) store_raw8<DST>(dst + p.at * type_size<DST>, from_f32<DST>(x));
-  }
+  if (mine) store_raw8<DST>(dst + p.at * type_size<DST>, from_f32<DST>(x));
 }
 
 // ---- read ----------------------------------------------------------------------------------------------------------------
@@ -241,13 +231,8 @@ hipError_t launch_write(const gsk_cache &c, const gsk_rows &a, hipStream_t s) {
       if constexpr (!type_is_8bit<src()> && dst() != GSK_F32) {
         by_lanes(c.dim, [&](auto gl) {
           const uint64_t rows = (uint64_t)a.tokens * c.heads, each = CT / gl();
-          auto go = [&](auto n) {
-            const dim3 grid((uint32_t)((rows + each * n() - 1) / (each * n())), 2);
-            hipLaunchKernelGGL((write_kernel<src(), dst(), gl(), n()>), grid, dim3(CT), 0, s, c, a, div_by(c.heads), div_by(c.page));
-          };
-          // rows one after the other pay once every CU has workgroups to spare
-          if (rows >= each * 4096) go(std::integral_constant<int, 4>{});
-          else go(std::integral_constant<int, 1>{});
+          hipLaunchKernelGGL((write_kernel<src(), dst(), gl()>), dim3((uint32_t)((rows + each - 1) / each), 2), dim3(CT), 0, s, c, a,
+                             div_by(c.heads), div_by(c.page));
         });
       }
     });
@@ -276,7 +261,7 @@ hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s
 }
 
 hipError_t launch_reorder(const gsk_reorder_beams &in, hipStream_t s) {
-  constexpr int64_t WGS = 4096, EACH = 4;  // workgroups of a launch to aim for, a thread's vectors of a block of tokens
+  constexpr int64_t WGS = 4096, EACH = 1;  // workgroups of a launch to aim for, a thread's vectors of a block of tokens
   auto go = [&](auto v, auto mb) {
     using V = decltype(v);
     constexpr int MB = mb();

@@ -15,9 +15,10 @@
 // instruction e of eight has element 8c + e as its row c. So nothing goes through LDS but the tokens' offsets (a lane finds one
 // token's, a block ahead) and 8-bit scales. 8-bit elements are exact in 16 bits; their scales multiply S and p in fp32.
 //
-// The weights p are rounded to 16 bits for the second product (half a step each, 2^-8 relative in bfloat16, 2^-11 in float16;
-// their sum l is of the unrounded ones). Over an 8-bit cache p times the token's scale is rounded, to bfloat16 whatever q's
-// type: the products would leave float16's range.
+// The weights p (up to 2^8: the maximum lags) are rounded to 16 bits for the second product, half a step each (2^-8 of the value in
+// bfloat16, 2^-11 in float16); their sum l is of the rounded ones, so that what they have in common divides out: where one token has
+// nearly all the weight the result has its value. Over an 8-bit cache a weight is p times the token's scale, which may leave
+// float16's range and has no such sum: it goes in as two bfloat16 numbers, rounded and the rest (2^-16), whatever q's type.
 #pragma once
 #include "gsk_dev.h"
 #include "gsk_int.h"
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         }
       }
       const bool masked = real != ~0u || t + 32 > ctx;
-      Frag<VT> pf[MT];
+      Frag<VT> pf[MT], rest[type_is_8bit<C> ? MT : 1];  // (8 bits: what the first rounding leaves)
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         float z[8], top = -INF;
@@ -455,23 +456,32 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
             for (int e = 0; e < 8; ++e) acc[m][b][e] *= f;
         }
         const float base = mx[m] == -INF ? 0.0f : mx[m];
-        uint32_t w[4];
+        uint32_t w[4], d[4];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if constexpr (type_is_8bit<C>) z[j] = __builtin_amdgcn_exp2f(z[j] - base);
           else z[j] = __builtin_amdgcn_exp2f(z[j] == -INF ? -INF : __builtin_fmaf(z[j], scale, -base));
-          l[m] += z[j];
           if constexpr (type_is_8bit<C>) {
+            l[m] += z[j];
             const float v = z[j] * vscale[j / 4][j % 4];
             z[j] = masked && z[j] == 0.0f ? 0.0f : v;  // (the scale of a token that is not seen may be NaN)
           }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if constexpr (VT == GSK_F16) w[j] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)z[2 * j], (_Float16)z[2 * j + 1]});
-          else w[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)z[2 * j], (__bf16)z[2 * j + 1]});
+          if constexpr (VT == GSK_F16) {
+            const f16x2 h = {(_Float16)z[2 * j], (_Float16)z[2 * j + 1]};
+            w[j] = __builtin_bit_cast(uint32_t, h);
+            l[m] += (float)h.x + (float)h.y;
+          } else {
+            w[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)z[2 * j], (__bf16)z[2 * j + 1]});
+            const float x = __uint_as_float(w[j] << 16), y = __uint_as_float(w[j] & 0xFFFF0000u);
+            if constexpr (type_is_8bit<C>) d[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)(z[2 * j] - x), (__bf16)(z[2 * j + 1] - y)});
+            else l[m] += x + y;
+          }
         }
         pf[m] = __builtin_bit_cast(Frag<VT>, uint4{w[0], w[1], w[2], w[3]});
+        if constexpr (type_is_8bit<C>) rest[m] = __builtin_bit_cast(Frag<VT>, uint4{d[0], d[1], d[2], d[3]});
       }
       if (masked) {  // (0 times what does not exist, or a new token that is not seen, may be NaN; what is seen is added at the end)
 #pragma unroll
@@ -489,7 +499,10 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         auto step = [&]<int E>(std::integral_constant<int, E>) {
           const Frag<VT> vf = turned<C, VT, E>(vr[b]);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) acc[m][b][E] = mma<VT>(vf, pf[m], acc[m][b][E]);
+          for (int m = 0; m < MT; ++m) {
+            acc[m][b][E] = mma<VT>(vf, pf[m], acc[m][b][E]);
+            if constexpr (type_is_8bit<C>) acc[m][b][E] = mma<VT>(vf, rest[m], acc[m][b][E]);
+          }
         };
         step(std::integral_constant<int, 0>{});
         step(std::integral_constant<int, 1>{});

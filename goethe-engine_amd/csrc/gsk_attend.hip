@@ -5,7 +5,10 @@ namespace gse {
 
 namespace {
 
-int row_tiles(const gsk_cache &c, const gsk_attention &a) {  // MT of the kernel
+// MT of the kernel: as many of a request's rows as share a tile's loads, up to 48. 96 trees of 36 rows a head: 250 us with 3, 283 with
+// tiles of 2 (which read the cache twice), 338 of 1; of 18 rows: 228 with 2, 239 with 3, 291 with 1; 24 chains of up to 18: 27.2 with 2,
+// 29.3 with 1, 32.5 with 3.
+int row_tiles(const gsk_cache &c, const gsk_attention &a) {
   const uint64_t rows = (uint64_t)a.max_new * (a.heads / c.heads);
   return rows <= 16 ? 1 : rows <= 32 || c.dim > 128 ? 2 : 3;
 }

@@ -19,6 +19,13 @@
 // bfloat16, 2^-11 in float16); their sum l is of the rounded ones, so that what they have in common divides out: where one token has
 // nearly all the weight the result has its value. Over an 8-bit cache a weight is p times the token's scale, which may leave
 // float16's range and has no such sum: it goes in as two bfloat16 numbers, rounded and the rest (2^-16), whatever q's type.
+//
+// Bound: memory, by how the rows lie and by how evenly the workgroups of a CU get on. 128 requests of up to 16384 tokens of 8 heads of
+// 128 8-bit elements (2.79 GB, 2.83 read by the counters), 8 rows a head: 534 us, 5.2 TB/s; with the heads ahead of a page's tokens 481 us,
+// 5.8 TB/s (one head's tokens are then one stretch of memory). 96 trees of 9 new tokens over up to 4096 tokens of 16 bits (1.03 GB, 36
+// rows a head): 249 us, 4.1 TB/s; of one new token 230. One request of 8192 tokens (34 MB): 20 to 22 us, a chain: lengths and table 4 us,
+// two blocks a wave 6, the waves' join 2, the ticket 1, the parts' join 6. More shares than workgroups that run at once, so that those
+// that end early take another, cost as the heads of an item fall apart (trees 285 us with two, 323 with four; batch 605, 653).
 #pragma once
 #include "gsk_dev.h"
 #include "gsk_int.h"
@@ -27,9 +34,11 @@ namespace gse {
 
 constexpr int AT = 256, AW = AT / WAVE;
 constexpr uint32_t AB = 32;  // tokens of a block
-constexpr uint32_t SHARE_MIN = 8;   // blocks of a share, at least
+// Blocks of a share, at least, and what a request's turn costs besides its tokens, in blocks (a share's requests count it). One request
+// of up to 2048 and 8192 tokens: 15.4 and 22.1 us; with shares of 4 blocks 15.5 and 27.8 (twice the parts to join), of 16 18.0 and
+// 20.2. 16 trees of up to 4096 tokens: 59.0 us, with a turn of 4 65.5, of 14 60.7.
+constexpr uint32_t SHARE_MIN = 8, TURN = 8;
 constexpr uint32_t FOUR_MIN = 32;   // blocks of a share, at least, where the waves take four heads
-constexpr uint32_t TURN = 8;        // what a request's turn costs besides its tokens, in blocks: a share's requests count it
 
 struct AttendArgs {
   gsk_cache c;
@@ -56,7 +65,7 @@ struct AttendShared {
   uint32_t last, bad[AW];
 };
 
-// Workgroups of a CU at once (what their registers allow).
+// Workgroups of a CU at once (what their registers allow; of MT = 1, four a CU left the loop spills and were slower).
 constexpr int attend_resident(int kd, int mt) { return kd > 4 ? 1 : mt > 1 ? 2 : 3; }
 
 template <uint32_t T>

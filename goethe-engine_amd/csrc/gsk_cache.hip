@@ -9,7 +9,11 @@ namespace {
 // ---- write ---------------------------------------------------------------------------------------------------------------
 // A group of 8, 16 or 32 lanes owns one token's head of the keys or of the values, a lane eight elements of it; in 8 bits the
 // group finds the row's largest magnitude by exchanges within it. Rows with a NaN or an infinity are found with it: as unsigned
-// integers their magnitudes are the largest. ROWS: a group's rows, all loaded before the first is worked on.
+// integers their magnitudes are the largest.
+//
+// Bound: up to some hundreds of tokens the launch and two dependent reads (64 tokens of 8 heads of 128: 2.4 us); from there memory:
+// 16384 tokens of 5 heads of 80, fp16 into 8-bit integers (39 MB), 12.5 us or 3.1 TB/s, 65536 of them 38.5 us or 4.1 TB/s. A group
+// with four rows in turn, all loaded first, took as long at both.
 constexpr int CT = 256;
 
 struct Place {
@@ -58,6 +62,9 @@ __global__ __launch_bounds__(CT) void write_kernel(gsk_cache c, gsk_rows a, Div 
 // A workgroup takes `tokens` rows, every head of them, keys and values. Its first wave finds their places (a lane a token: the
 // request by a search of the whole wave for the first, from there on step by step; then the page) and leaves them in LDS; the
 // threads then walk the rows' pieces of eight elements, which lie together in the output.
+//
+// Bound: memory. 32 requests of 4096 to 8192 tokens of 5 heads of 80, 8-bit integers to fp16 (168 MB read, 281 written by the
+// counters): 94 us, 4.4 TB/s. 4 requests of 256 to 512 tokens: 4.3 us, the search, the table and the rows one after the other.
 constexpr uint32_t RTOK = 32;  // tokens of a workgroup, at most
 
 struct ReadShared {
@@ -147,6 +154,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // finds the offsets of TB tokens (a thread a token's beam) and leaves them in LDS, the moving beams of a token one after the
 // other; then its threads walk the (cache, chunk, token, place) of the block: neighbouring tokens of a chunk lie together
 // where the heads come first.
+//
+// Bound: memory where there is enough to move (8 groups of 8 beams, 256 tokens in 48 caches of 400 bytes: 550 MB, 99 us, 5.6 TB/s);
+// else the launch, the table and the rows one after the other (4 beams, 16 tokens, 64 caches of 2 KB rows: 5.9 us).
 struct ReorderShared {
   int64_t src[CT], dst[CT];
   uint32_t n[CT];
@@ -241,7 +251,8 @@ hipError_t launch_write(const gsk_cache &c, const gsk_rows &a, hipStream_t s) {
 }
 
 hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s) {
-  // tokens of a workgroup: as many as leave the launch 2048 of them
+  // tokens of a workgroup: as many as leave the launch 2048 of them (8 requests of up to 1024 tokens: 8.7 us, with 8192 workgroups
+  // 10.1; up to 4096 tokens: 23.2, with 8192 workgroups 25.3, with 512 24.0)
   uint32_t tokens = 1;
   while (tokens < RTOK && a.rows / tokens >= 4096) tokens *= 2;
   const uint32_t pieces = c.dim / 8;
@@ -252,6 +263,8 @@ hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s
           hipLaunchKernelGGL((read_kernel<src(), dst(), u()>), dim3((a.rows + tokens - 1) / tokens), dim3(CT), 0, s, c, a, tokens,
                              div_by(pieces), div_by(c.heads));
         };
+        // four pieces a thread at once where its workgroup has them: 32 requests of up to 8192 tokens 97 us, one by one 101; with
+        // fewer the lanes past the end cost (8 of up to 1024: 8.7 us, 10.4 so)
         if ((uint64_t)tokens * c.heads * pieces >= 4 * CT) go(std::integral_constant<int, 4>{});
         else go(std::integral_constant<int, 1>{});
       }
@@ -261,7 +274,10 @@ hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s
 }
 
 hipError_t launch_reorder(const gsk_reorder_beams &in, hipStream_t s) {
-  constexpr int64_t WGS = 4096, EACH = 1;  // workgroups of a launch to aim for, a thread's vectors of a block of tokens
+  // Workgroups of a launch to aim for, a thread's vectors of a block of tokens (8 x 8 beams, 256 and 16 tokens: 98 and 8.9 us; with four
+  // vectors 107 and 13.2, with two 103 and 10.3; with 2048 workgroups 101 and 8.1, with 8192 95 and 9.9, and 4 beams of 16
+  // tokens 5.5, 5.8 and 7.2 with 2048, 4096 and 8192).
+  constexpr int64_t WGS = 4096, EACH = 1;
   auto go = [&](auto v, auto mb) {
     using V = decltype(v);
     constexpr int MB = mb();

@@ -31,7 +31,7 @@ typedef struct gsk_cache {
   uint32_t type;            /* GSK_BF16, GSK_F16, GSK_E4M3, GSK_I8 */
   uint32_t pages;
   uint32_t page;            /* tokens per page; pages * page < 2^32 */
-  uint32_t heads;
+  uint32_t heads;           /* at most 2^12 */
   uint32_t dim;
   void *keys;
   void *values;
@@ -86,7 +86,8 @@ typedef struct gsk_read_rows {
  * of those itself and the earlier ones; with parent: itself, parent[row], that one's parent and so on (entries that are no
  * earlier row of the request end the path). Query head h reads head h / (heads / cache heads). Where nothing is seen, or every
  * score is -inf, the result is 0, as it is for a request with status[r] != 0 or with numbers out of range; cached tokens
- * whose page is out of range are not seen. Rows from begin[requests] on are left as they were. */
+ * whose page is out of range are not seen. A NaN or an infinity reaches the rows that see its token, and no other. Rows from
+ * begin[requests] on are left as they were. */
 typedef struct gsk_attention {
   uint32_t size;
   uint32_t requests;
@@ -176,11 +177,13 @@ GSE_API int gsk_write(gse_handle *h, const gsk_cache *cache, const gsk_rows *in)
 GSE_API int gsk_read(gse_handle *h, const gsk_cache *cache, const gsk_read_rows *in);
 
 /* Attention of new tokens, in one launch. gsk_attention_work: the scratch bytes that it needs for these sizes on this device
- * (0: none; negative: an error); no pointer of the structs is read. */
+ * (0: none; negative: an error); of the structs no pointer is read, and neither q's strides nor the scales'. Up to 2^37 tokens in all:
+ * requests * (16 + max_pages * page / 32) < 2^32. */
 GSE_API int64_t gsk_attention_work(gse_handle *h, const gsk_cache *cache, const gsk_attention *in);
 GSE_API int gsk_attend(gse_handle *h, const gsk_cache *cache, const gsk_attention *in);
 
-/* One step of beam search, in one launch; its scratch bytes likewise. */
+/* One step of beam search, in one launch for up to 65535 rows and as many requests as the handle has tickets (its rows, 4096 at
+ * least), in as many as that takes otherwise; its scratch bytes likewise. */
 GSE_API int64_t gsk_beams_work(gse_handle *h, const gsk_beams *in);
 GSE_API int gsk_beam(gse_handle *h, const gsk_beams *in);
 

@@ -14,7 +14,7 @@
 //
 // Bound: 4 beams of 128256 fp32 logits, 14.1 us, are a chain: a slice's load, its maxima, bound, list and ranks (8 us), the ticket, the
 // join's reads, logs and ranks. 64 requests of 8 beams of 151936 bf16 logits (156 MB), 63.5 us or 2.4 TB/s (fp32: 79, 3.9), are bound
-// by the instructions on each element (8 x (load, compare, exp2, add) of 2 bytes), then by the join of the last request.
+// by instructions (15 on each element of 2 bytes by the counters: unpacking, maxima, exp2, compare), then by the last request's join.
 #include "gsk_dev.h"
 #include "gsk_int.h"
 

@@ -764,9 +764,14 @@ int check_attention(gse_handle *h, const gsk_cache &c, const gsk_attention &a) {
   if (a.requests > (1u << 30) || a.tokens > (1u << 30) || a.max_new > (1u << 24))
     return fail(h, GSE_E_UNSUPPORTED, "%u requests, %u tokens, %u a request: at most 2^30, 2^30 and 2^24", a.requests, a.tokens,
                 a.max_new);
-  if (a.requests * (16 + (uint64_t)a.max_pages * c.page / 32) > (uint64_t)UINT32_MAX)  // (blocks of 32 tokens are counted)
+  // blocks of 32 tokens are counted, for each tile of a request's rows
+  const uint64_t blocks = a.requests * (16 + (uint64_t)a.max_pages * c.page / 32), tiles = gse::attend_tiles(c, a);
+  if (blocks > (uint64_t)UINT32_MAX)
     return fail(h, GSE_E_UNSUPPORTED, "%u requests of up to %llu tokens: at most 2^37 in all", a.requests,
                 (unsigned long long)a.max_pages * c.page);
+  if (tiles > UINT32_MAX / std::max<uint64_t>(blocks, 16))
+    return fail(h, GSE_E_UNSUPPORTED, "%u requests of up to %u new tokens over up to %llu: fewer new ones a call", a.requests,
+                std::min(a.max_new, a.tokens), (unsigned long long)a.max_pages * c.page);
   if (a.parent && a.max_new > GSK_MAX_TREE)
     return fail(h, GSE_E_UNSUPPORTED, "trees of %u new tokens: at most %d", a.max_new, GSK_MAX_TREE);
   return GSE_OK;

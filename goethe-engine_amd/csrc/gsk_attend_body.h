@@ -1,12 +1,14 @@
 // The attention kernel of gsk_attend (gsk_attend.hip has the plan and the launches; one source per cache type instantiates it).
 //
-// The cached tokens of all requests, one after the other, are cut into equal shares of whole blocks, as many as workgroups run at
-// once (at most p.items): a workgroup takes one share, one head of the cache and one tile of up to 16 MT rows, and works on the
-// requests (or parts of them) in its share in turn. A row is a (new token, query head of the group), so that every query head
+// The work is a line of blocks of cached tokens: each request's tokens once for every tile of up to 16 MT of its rows, request after
+// request. It is cut into equal shares of whole blocks, as many as workgroups run at once (at most p.items): a workgroup takes one share
+// and one head of the cache, and works on the tiles (or parts of them) in its share in turn, so that requests with many new tokens and
+// with one, in one call, take what they need (24 requests of up to 400 new tokens, 260 us; 765 with workgroups for each tile of every
+// request). A row is a (new token, query head of the group), so that every query head
 // that reads a cached row shares its load. The four waves take blocks of 32 tokens in turn, each with its own running maximum m,
 // sum l and output O of every row (one pass: a block's scores S, m' = max(m, S), p = 2^(S - m'), l = l 2^(m - m') + sum p, O =
-// O 2^(m - m') + p V), joined through LDS at the end; the parts of a request are joined, in their order, by the last workgroup
-// of a (request, head, tile) to end.
+// O 2^(m - m') + p V), joined through LDS at the end; the parts of a tile are joined, in their order, by the last workgroup
+// of a (request, tile, head) to end.
 //
 // Both products are 16x16x32 matrix instructions. S^T = K Q^T: a lane (c, g) = (lane % 16, lane / 16) holds eight elements of
 // token c and of row c, and gets the scores of row c for tokens 4g .. 4g + 3 of each 16; O^T = V^T P^T over 32 tokens then takes
@@ -43,7 +45,7 @@ constexpr uint32_t FOUR_MIN = 32;   // blocks of a share, at least, where the wa
 struct AttendArgs {
   gsk_cache c;
   gsk_attention a;
-  uint32_t items, tiles, group, rows;  // shares; tiles of a request's rows; query heads of a head; rows of a tile's scratch
+  uint32_t items, group, rows;  // shares, at most; query heads of a head; rows of a tile's scratch
   uint32_t *tick;
   uint32_t items4;  // shares where the waves take four heads (0: never)
 };
@@ -172,7 +174,15 @@ __device__ __forceinline__ Span span_of(const gsk_cache &c, const gsk_attention 
   const bool ok = x.status == 0 && x.len >= n && (int64_t)x.len <= (int64_t)a.max_pages * c.page;
   return {x.begin, n, ok ? x.len : 0};
 }
-__device__ __forceinline__ uint32_t blocks_of(Span x) { return x.begin < 0 ? 0u : TURN + max(((uint32_t)x.len + AB - 1) / AB, 1u); }
+// A request's turns, one for each tile of its rows (of 16 MT), and the blocks that a turn counts.
+struct Turns {
+  uint32_t n, blocks;
+};
+template <int MT>
+__device__ __forceinline__ Turns turns_of(const gsk_attention &a, uint32_t group, Span x) {
+  if (x.begin < 0) return {0, 0};
+  return {(min((uint32_t)x.n, a.max_new) * group + 16 * MT - 1) / (16 * MT), TURN + max(((uint32_t)x.len + AB - 1) / AB, 1u)};
+}
 
 template <uint32_t Q, uint32_t C, int KD, int MT>
 __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(AttendArgs p) {
@@ -186,8 +196,8 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   const uint32_t tid = threadIdx.x, lane = lane_id(), lc = lane % 16, lg = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   // ---- the share ----------------------------------------------------------------------------------------------------------
-  // Every wave for itself, a lane one request or, where there are more than lanes, four at a time: a request's blocks, one at
-  // least if it has rows to write, after TURN that stand for its turn. The shares are of one size, the first ones a block more.
+  // Every wave for itself, a lane one request or, where there are more than lanes, four at a time: a tile's blocks, one at least if
+  // there are rows to write, after TURN that stand for its turn. The shares are of one size, the first ones a block more.
   const int per = a.requests <= WAVE ? 1 : 4;
   Span own[4];
   uint32_t u[4] = {};
@@ -201,7 +211,8 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     for (int k = 0; k < 4; ++k) {
       if (k >= per) continue;
       own[k] = span_of(c, a, raw[k]);
-      u[k] = i0 + lane * per + k < a.requests ? blocks_of(own[k]) : 0;
+      const Turns w = turns_of<MT>(a, p.group, own[k]);
+      u[k] = i0 + lane * per + k < a.requests ? w.n * w.blocks : 0;
       n += u[k];
     }
     return n;
@@ -213,9 +224,9 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   // every block of the share for one of four heads, and nothing is joined between waves.
   const bool four = MT == 1 && p.items4 && total >= p.items4 * FOUR_MIN;
   const uint32_t shares = four ? p.items4 : min(max(total / SHARE_MIN, 1u), p.items);
-  // The heads and tiles of an item run on one XCD (workgroups go round the eight of them): a token's heads lie together.
-  const uint32_t x8 = blockIdx.x / 8, each = (four ? c.heads / AW : c.heads) * p.tiles, x = x8 % each;
-  const uint32_t item = x8 / each * 8 + blockIdx.x % 8, head0 = x / p.tiles * (four ? AW : 1), tile = x % p.tiles;
+  // The heads of an item run on one XCD (workgroups go round the eight of them): a token's heads lie together.
+  const uint32_t x8 = blockIdx.x / 8, each = four ? c.heads / AW : c.heads, x = x8 % each;
+  const uint32_t item = x8 / each * 8 + blockIdx.x % 8, head0 = x * (four ? AW : 1);
   const uint32_t head = four ? head0 + wave : head0, heads_here = four ? AW : 1;
   if (item >= shares) return;
   const uint32_t share = total / shares, longer = total - share * shares;
@@ -259,19 +270,29 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   }
   start = __builtin_amdgcn_readfirstlane(start);
   r = __builtin_amdgcn_readfirstlane(r);
+  Turns turns = turns_of<MT>(a, p.group, sp);
+  uint32_t tile = turns.n ? (pos - start) / turns.blocks : 0;
+  start += tile * turns.blocks;
 
-  for (Raw ahead;; sp = span_of(c, a, ahead), ++r) {
+  Raw ahead;
+  auto next = [&] {  // the request's next tile, or the next request
+    if (++tile < turns.n) return;
+    tile = 0;
+    sp = span_of(c, a, ahead);
+    turns = turns_of<MT>(a, p.group, sp);
+    ++r;
+  };
+  for (;; next()) {
   if (pos >= stop) break;
   ahead = raw_of(a, min(r + 1, a.requests - 1));  // (the next request's, for the next turn)
   if (sp.begin < 0) continue;
-  const uint32_t first = start + TURN, end = start + blocks_of(sp), from = max(pos, first);  // the request's blocks
+  const uint32_t first = start + TURN, end = start + turns.blocks, from = max(pos, first);  // the request's blocks
   start = end;
   pos = min(stop, end);
   if (from >= pos) continue;  // (the share ends within its turn)
   const uint32_t k0 = (from - first) * AB, k_end = (pos - first) * AB;
   const uint32_t first_item = from == first ? item : share_of(first), parts = (end <= stop ? item : share_of(end - 1)) - first_item + 1;
   const uint32_t rows = min((uint32_t)sp.n, a.max_new) * p.group, row0 = tile * 16 * MT;
-  if (row0 >= rows) continue;
   const uint32_t len = (uint32_t)sp.len, ctx = len >= (uint32_t)sp.n ? len - (uint32_t)sp.n : 0;
   const uint32_t last_new = (min(rows, row0 + 16 * MT) - 1) / p.group;
   const uint32_t k1 = min(k_end, a.parent ? len : min(len, ctx + last_new + 1));
@@ -555,7 +576,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   const int64_t part_size = (int64_t)p.rows * (c.dim + 2);
   // A share has two of them: of the request that it goes on with, and of the one that goes on after it.
   auto scratch = [&](uint32_t it, uint32_t h) {
-    return work + ((((int64_t)it * 2 + (it == first_item)) * c.heads + h) * p.tiles + tile) * part_size;
+    return work + (((int64_t)it * 2 + (it == first_item)) * c.heads + h) * part_size;
   };
   const uint32_t tr = tid / 16, te = tid % 16 * 8;
   auto finish = [&](uint32_t h, uint32_t row, uint32_t e, const float (&x)[8], float sum) {
@@ -629,7 +650,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   // ---- the parts joined ---------------------------------------------------------------------------------------------------
   store_wait();
   __syncthreads();
-  uint32_t *tick = p.tick + (int64_t)first_item * each + x;  // (one request at most goes on after a share)
+  uint32_t *tick = p.tick + (int64_t)first_item * each + x;  // (one turn at most goes on after a share)
   if (tid == 0) sh.last = ticket_add(tick) == parts - 1;
   __syncthreads();
   const bool last = sh.last;

@@ -11,11 +11,11 @@ hipError_t launch_reorder(const gsk_reorder_beams &a, hipStream_t s);
 
 // How a call of gsk_attend is cut (gsk_attend.hip); tick: the tickets that it may use.
 struct AttendPlan {
-  uint32_t tiles;  // of a request's (new token, query head of the group) rows
-  uint32_t items;  // equal shares of the requests' cached tokens: workgroups per cache head and tile, at most
+  uint32_t items;  // equal shares of the work on the requests' cached tokens: workgroups per cache head, at most
   uint32_t items4; // shares where a workgroup takes four heads (0: it never does)
   int64_t work;    // scratch bytes
 };
+uint64_t attend_tiles(const gsk_cache &c, const gsk_attention &a);  // of a request's (new token, query head of the group) rows
 AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tickets, int cus);
 hipError_t launch_attend(const gsk_cache &c, const gsk_attention &a, const AttendPlan &p, uint32_t *tick, hipStream_t s);
 

@@ -574,3 +574,28 @@ def test_attend_bad_values_of_older_tokens(ge, gpu, cache):
                 assert torch.isfinite(a[:, :2]).all() and torch.isnan(a[:, 2:]).all(), (r, t)
         for x, w in zip((keys, values, *(scales or ())), was):
             x[at] = w
+
+
+@pytest.mark.parametrize("query,cache,dim,heads,group", [(BF, BF, 128, 2, 4), (HF, I8, 80, 3, 5), (BF, E4, 256, 1, 3)])
+def test_attend_prompts_beside_single_tokens(ge, gpu, query, cache, dim, heads, group):
+    """A step of a long prompt's chunk, short ones and single tokens; a wide max_new over the same rows changes no bit."""
+    g = _gen(gpu, dim + group)
+    news = [1, 1, 130, 0, 17, 1, 70, 1]
+    lengths = [900, 1, 333, 0, 17, 64, 71, 2000]
+    table, pages = _pages(g, lengths, 16)
+    keys, values, scales = _cache(g, cache, pages, 16, heads, dim, False)
+    q = _rand(g, sum(news) + 3, heads * group, dim).to(query)
+    _check(ge, q, keys, values, scales, table, lengths, news, False)
+    begin = torch.tensor(np.concatenate([[0], np.cumsum(news)]), dtype=torch.int32, device=gpu)
+    seq = torch.tensor(lengths, dtype=torch.int32, device=gpu)
+    a, b = (ge.kv.attend(q, keys, values, table, seq, begin=begin, scales=scales, max_new=m)[:sum(news)] for m in (130, 220))
+    assert torch.equal(a, b)
+
+
+def test_attend_new_tokens_past_what_is_counted(ge, gpu):
+    """More new tokens times cached ones than 2^32 blocks: refused."""
+    x = torch.zeros((1, 1, 1, 8), dtype=BF, device=gpu)
+    table = torch.zeros((1, (1 << 31) - 1), dtype=torch.int32, device="meta").expand(1, -1)
+    q = torch.zeros((1 << 12, 1, 8), dtype=BF, device=gpu)
+    with pytest.raises(ValueError, match="fewer new ones"):
+        ge.kv.attend(q, x, x, table, [1], begin=[0, 1 << 12], max_new=1 << 12)

@@ -31,8 +31,9 @@ AttendPlan attend_plan(const gsk_cache &c, const gsk_attention &a, uint32_t tick
   p.items = (uint32_t)max(min(round(c.heads), blocks / SHARE_MIN), (uint64_t)1);
   // Four heads a workgroup, where heads of at most 128 bytes lie next to each other in a token: its loads are then four times as
   // long a piece of memory (8-bit rows of 128 bytes, 128 requests of up to 16384 tokens: 637 -> 553 us, 534 since waves give way; 64:
-  // 337 -> 310; with the heads ahead 481 as it is; rows of 256 bytes: 529 -> 538). The parts of a request are then four times as many, joined by a quarter
-  // of the workgroups: not where a request has more than about six (32 such requests: 180 us, 212 so; 8 of 131072: 299, 428).
+  // 337 -> 310; with the heads ahead 481 as it is; rows of 256 bytes: 529 -> 538). The parts of a request are then four times as
+  // many, joined by a quarter of the workgroups: not where a request has more than about six (32 such requests: 180 us, 212 so; 8 of
+  // 131072: 299, 428).
   const bool together = c.heads % AW == 0 && most == 16 && c.head_stride < c.token_stride && c.dim * (c.type >= GSK_E4M3 ? 1 : 2) <= 128;
   p.items4 = together ? (uint32_t)round((uint64_t)c.heads / AW) : 0;
   if (p.items4 > 6 * (uint64_t)a.requests) p.items4 = 0;

@@ -17,10 +17,11 @@
 // instruction e of eight has element 8c + e as its row c. So nothing goes through LDS but the tokens' offsets (a lane finds one
 // token's, a block ahead) and 8-bit scales. 8-bit elements are exact in 16 bits; their scales multiply S and p in fp32.
 //
-// The weights p (up to 2^8: the maximum lags) are rounded to 16 bits for the second product, half a step each (2^-8 of the value in
-// bfloat16, 2^-11 in float16); their sum l is of the rounded ones, so that what they have in common divides out: where one token has
-// nearly all the weight the result has its value. Over an 8-bit cache a weight is p times the token's scale, which may leave
-// float16's range and has no such sum: it goes in as two bfloat16 numbers, rounded and the rest (2^-16), whatever q's type.
+// The weights p (up to 2^8: the maximum lags) go into the second product as two 16-bit numbers, so that results are off by little more than
+// their own rounding (with one, half a step of each weight, bfloat16's rms error was up to a seventh more). Over a 16-bit cache a weight is cut
+// off and its rest rounded, off by 2^-15 of it in bfloat16 and 2^-20 in float16: both above 0, so that an infinite value times them is the
+// same infinity. Over an 8-bit cache, whose values are finite or NaN, a weight is p times the token's scale, which may leave
+// float16's range: two bfloat16 numbers, rounded and the rest (2^-16), whatever q's type.
 //
 // Bound: memory, by how the rows lie and by how evenly the workgroups of a CU get on. 128 requests of up to 16384 tokens of 8 heads of
 // 128 8-bit elements (2.79 GB, 2.83 read by the counters), 8 rows a head: 534 us, 5.2 TB/s; with the heads ahead of a page's tokens 481 us,
@@ -190,6 +191,8 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   constexpr uint32_t VT = type_is_8bit<C> ? (uint32_t)GSK_BF16 : Q;  // type of the second product
   constexpr int VB = Sh::VB, SZ = type_size<C>;
   constexpr float INF = INFINITY;
+  // 16 bits: a weight times MORE goes into the second product, cut off and the rest, which then is above 0 (an infinite value stays one)
+  constexpr float MORE = type_is_8bit<C> ? 1.0f : VT == GSK_F16 ? 1.0f + 0x1p-12f : 1.0f + 0x1p-17f;
   __shared__ Sh sh;
   const gsk_cache &c = p.c;
   const gsk_attention &a = p.a;
@@ -452,7 +455,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         }
       }
       const bool masked = real != ~0u || t + 32 > ctx;
-      Frag<VT> pf[MT], rest[type_is_8bit<C> ? MT : 1];  // (8 bits: what the first rounding leaves)
+      Frag<VT> pf[MT], rest[MT];  // (what the first rounding leaves)
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         float z[8], top = -INF;
@@ -491,8 +494,8 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         for (int j = 0; j < 8; ++j) {
           if constexpr (type_is_8bit<C>) z[j] = __builtin_amdgcn_exp2f(z[j] - base);
           else z[j] = __builtin_amdgcn_exp2f(z[j] == -INF ? -INF : __builtin_fmaf(z[j], scale, -base));
+          l[m] += z[j];
           if constexpr (type_is_8bit<C>) {
-            l[m] += z[j];
             const float v = z[j] * vscale[j / 4][j % 4];
             z[j] = masked && z[j] == 0.0f ? 0.0f : v;  // (the scale of a token that is not seen may be NaN)
           }
@@ -500,18 +503,23 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if constexpr (VT == GSK_F16) {
-            const f16x2 h = {(_Float16)z[2 * j], (_Float16)z[2 * j + 1]};
+            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(z[2 * j], z[2 * j + 1]));
             w[j] = __builtin_bit_cast(uint32_t, h);
-            l[m] += (float)h.x + (float)h.y;
-          } else {
+            d[j] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)__builtin_fmaf(z[2 * j], MORE, -(float)h.x),
+                                                      (_Float16)__builtin_fmaf(z[2 * j + 1], MORE, -(float)h.y)});
+          } else if constexpr (type_is_8bit<C>) {
             w[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)z[2 * j], (__bf16)z[2 * j + 1]});
             const float x = __uint_as_float(w[j] << 16), y = __uint_as_float(w[j] & 0xFFFF0000u);
-            if constexpr (type_is_8bit<C>) d[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)(z[2 * j] - x), (__bf16)(z[2 * j + 1] - y)});
-            else l[m] += x + y;
+            d[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)(z[2 * j] - x), (__bf16)(z[2 * j + 1] - y)});
+          } else {
+            const uint32_t x = __float_as_uint(z[2 * j]), y = __float_as_uint(z[2 * j + 1]);
+            w[j] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+            d[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)__builtin_fmaf(z[2 * j], MORE, -__uint_as_float(x & 0xFFFF0000u)),
+                                                       (__bf16)__builtin_fmaf(z[2 * j + 1], MORE, -__uint_as_float(y & 0xFFFF0000u))});
           }
         }
         pf[m] = __builtin_bit_cast(Frag<VT>, uint4{w[0], w[1], w[2], w[3]});
-        if constexpr (type_is_8bit<C>) rest[m] = __builtin_bit_cast(Frag<VT>, uint4{d[0], d[1], d[2], d[3]});
+        rest[m] = __builtin_bit_cast(Frag<VT>, uint4{d[0], d[1], d[2], d[3]});
       }
       if (masked) {  // (0 times what does not exist, or a new token that is not seen, may be NaN; what is seen is added at the end)
 #pragma unroll
@@ -531,7 +539,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             acc[m][b][E] = mma<VT>(vf, pf[m], acc[m][b][E]);
-            if constexpr (type_is_8bit<C>) acc[m][b][E] = mma<VT>(vf, rest[m], acc[m][b][E]);
+            acc[m][b][E] = mma<VT>(vf, rest[m], acc[m][b][E]);
           }
         };
         step(std::integral_constant<int, 0>{});
@@ -605,7 +613,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
             *(f32x4 *)o = f32x4{acc[mm][bb][0][i], acc[mm][bb][1][i], acc[mm][bb][2][i], acc[mm][bb][3][i]};
             *(f32x4 *)(o + 4) = f32x4{acc[mm][bb][4][i], acc[mm][bb][5][i], acc[mm][bb][6][i], acc[mm][bb][7][i]};
           }
-          const float sum = over_groups(l[mm], [](float x, float y) { return x + y; });
+          const float sum = over_groups(l[mm], [](float x, float y) { return x + y; }) * MORE;
           if (lg == 0) {
             sh.m[wave][lc] = mx[mm];
             sh.l[wave][lc] = sum;

@@ -99,19 +99,17 @@ def attend(q, k, v, mask, scale, dtype, bits8):
     """One request: q [n, query heads, dim], k, v [tokens, heads, dim] float64, mask [n, tokens] -> (out, what a result of type
     dtype may be off by), both [n, query heads, dim].
 
-    The bound: out is rounded once (half a step of its size). The weights w are rounded to 16 bits for the product with v, half a
-    step of each: e = 2^-8 in bfloat16, 2^-11 in float16, whose weights below 2^-14 of the largest are off by up to 2^-25 of it; the
-    largest is at most the sum. They are divided by the sum of the rounded ones: sum w (1 + e_i) v / sum w (1 + e_i) is off from o =
-    sum w v / sum w by sum w e_i (v - o) / sum w (1 + e_i), at most e (sum w |v| / sum w + |o|) / (1 - e). Over 8 bits a weight goes in
-    as a bfloat16 number and what that leaves, at most 2^-8 of it, as another: off by 2^-16 of it, and divided by the unrounded sum. A score is a sum of dim products in fp32 and some products more: off by
-    (dim + 8) 2^-24 of the sum of its terms' magnitudes; that much, twice (the score's and the largest one's), is the relative
-    error of a weight, and again of their sum. exp, its argument's roundings (2^-23 of its size, at most 100 for a weight that
-    counts) and the fp32 sums' (2^-24 for each of a chain of at most 4096 terms and joins) come to 2^-11.5 at most, far less in
-    practice: 2^-13 is allowed for them."""
+    The bound: out is rounded once (half a step of its size). A weight goes into the product with v as two 16-bit numbers: cut off
+    (a step at most, 2^-7 of it in bfloat16, 2^-10 in float16) and the rest, rounded to half a step of that: off by 2^-15 of it, 2^-20
+    in float16 (whose rest is up to 2^-12 larger), where weights below 2^-14 of the largest are off by up to 2^-25 of it (the largest
+    is at most the sum). Over 8 bits the first is rounded: 2^-16. They are divided by the sum of the unrounded ones. A score is a sum of dim products in fp32 and some products more: off by (dim + 8) 2^-24 of the sum of its terms' magnitudes; that much, twice
+    (the score's and the largest one's), is the relative error of a weight, and again of their sum. exp, its argument's roundings
+    (2^-23 of its size, at most 100 for a weight that counts) and the fp32 sums' (2^-24 for each of a chain of at most 4096 terms
+    and joins) come to 2^-11.5 at most, far less in practice: 2^-13 is allowed for them."""
     n, hq, dim = q.shape
     group = hq // k.shape[1]
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
-    p16 = HALF[torch.bfloat16] ** 2 if bits8 else HALF[dtype]
+    p16 = 2.0 ** (-16 if bits8 else -20 if dtype is torch.float16 else -15)
     for h in range(hq):
         kk, vv = k[:, h // group], v[:, h // group]
         s = q[:, h] @ kk.T * scale
@@ -126,8 +124,6 @@ def attend(q, k, v, mask, scale, dtype, bits8):
         off = (dim + 8) * 2.0 ** -24 * np.where(mask, size, 0).max(1, initial=0, keepdims=True)
         rel = p16 + 4 * off + 2.0 ** -13
         tol[:, h] = HALF[dtype] * np.abs(out[:, h]) * (1 + rel) + rel * mag
-        if not bits8:
-            tol[:, h] += p16 * np.abs(out[:, h]) + 2 * p16 ** 2 * mag
         if not bits8 and dtype is torch.float16:
             tol[:, h] += 2.0 ** -25 * (mask @ np.abs(np.where(mask.any(0)[:, None], vv, 0.0)))
             tol[:, h] += 2.0 ** -25  # (and the result's own smallest step)

@@ -1,0 +1,63 @@
+"""How far attention's results are from the definition in 64 bits: little more than their own rounding, whatever the type of the
+cache, the spread of the weights and the size of the values."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_ref as kr
+from test_gpu_kv import KINDS, _cache, _gen, _pages, _rand
+
+pytestmark = pytest.mark.gpu
+
+
+def _both(ge, q, keys, values, scales, table, lengths, news, parents=None, rows=None, scale=None):
+    """kv.attend's and the oracle's outputs [rows, query heads, dim], float64, and the oracle's bound, of the requests `rows`."""
+    begin = np.concatenate([[0], np.cumsum(news)])
+    got = kr._np(ge.kv.attend(q, keys, values, table, lengths, begin=begin, scales=scales, parents=parents, scale=scale))
+    ks, vs = scales or (None, None)
+    out = []
+    for r in range(len(news)) if rows is None else rows:
+        ids, at = table[r].tolist(), slice(begin[r], begin[r + 1])
+        k, there = kr.tokens(keys, ks, ids, 0, lengths[r], False)
+        v, _ = kr.tokens(values, vs, ids, 0, lengths[r], False)
+        mask = kr.sees(news[r], lengths[r] - news[r], parents, begin[r]) & there
+        scale_of = float(np.float32(q.shape[2] ** -0.5 if scale is None else scale))
+        out.append((got[at], *kr.attend(kr._np(q[at]), k, v, mask, scale_of, q.dtype, keys.dtype in kr.MOST)))
+    return [np.concatenate(x) for x in zip(*out)]
+
+
+def _rms(x):
+    return float(np.sqrt(np.mean(np.square(x))))
+
+
+@pytest.mark.parametrize("query,cache", KINDS)
+@pytest.mark.parametrize("what", ["trees", "chains", "long", "one"])
+def test_attend_is_off_by_its_rounding(ge, gpu, query, cache, what):
+    """The rms error over a call is that of the results' own rounding: every weight goes into the product to 2^-15 of it (2^-20 in
+    a float16 cache, 2^-16 in 8 bits), a rounding whose rms is a quarter of that, independent of the other weights', so that the sum
+    is off by about 2^-17 of its size (2^-22, 2^-18); the results' own rounding is 2^-8 / sqrt(12) to twice that, 2^-9.8 at least, in
+    float16 2^-12.8. The scores' fp32 sums, 2^-20 at these sizes, add less. So at most sqrt(1 + 2^-10) of the rounding's rms is
+    expected, and 1.02 allowed. A block of 32 tokens left out of n alike moves the results by sqrt(32 / n) of their size: 2^-6 of it at
+    the longest here, ten times the rounding."""
+    g = _gen(gpu, 31)
+    parents, dim, group = None, 128, 4
+    if what == "trees":
+        news, lengths = [9] * 6, [900, 64, 9, 1500, 333, 2000]
+        begin = np.concatenate([[0], np.cumsum(news)])
+        parents = np.concatenate([begin[r] + np.array([-1 - begin[r]] + [(i - 1) // 2 for i in range(1, 9)]) for r in range(6)])
+    elif what == "chains":
+        news, lengths, dim, group = [6, 1, 3, 5, 2, 40], [700, 1, 60, 1300, 31, 40], 80, 3
+    elif what == "long":
+        news, lengths, dim = [1, 1, 2], [100003, 9, 30011], 64
+    else:
+        news, lengths, group = [1] * 8, [33, 64, 100, 1, 257, 1000, 3000, 31], 2
+    table, pages = _pages(g, lengths, 16)
+    keys, values, scales = _cache(g, cache, pages, 16, 2, dim, False)
+    q = _rand(g, sum(news), 2 * group, dim).to(query)
+    got, want, tol = _both(ge, q, keys, values, scales, table, lengths, news, parents)
+    assert (np.abs(got - want) <= tol).all()
+    rounded = kr._np(torch.from_numpy(want).to(query))
+    assert _rms(got - want) <= 1.02 * _rms(rounded - want), (_rms(got - want), _rms(rounded - want))
+    if what == "long":  # (each request by itself: the short one's results are large)
+        for i in (slice(0, 1), slice(2, 4)):
+            assert _rms(got[i] - want[i]) <= 1.02 * _rms(rounded[i] - want[i])

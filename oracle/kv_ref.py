@@ -101,11 +101,12 @@ def attend(q, k, v, mask, scale, dtype, bits8):
 
     The bound: out is rounded once (half a step of its size). A weight goes into the product with v as two 16-bit numbers: cut off
     (a step at most, 2^-7 of it in bfloat16, 2^-10 in float16) and the rest, rounded to half a step of that: off by 2^-15 of it, 2^-20
-    in float16 (whose rest is up to 2^-12 larger), where weights below 2^-14 of the largest are off by up to 2^-25 of it (the largest
-    is at most the sum). Over 8 bits the first is rounded: 2^-16. They are divided by the sum of the unrounded ones. A score is a sum of dim products in fp32 and some products more: off by (dim + 8) 2^-24 of the sum of its terms' magnitudes; that much, twice
-    (the score's and the largest one's), is the relative error of a weight, and again of their sum. exp, its argument's roundings
-    (2^-23 of its size, at most 100 for a weight that counts) and the fp32 sums' (2^-24 for each of a chain of at most 4096 terms
-    and joins) come to 2^-11.5 at most, far less in practice: 2^-13 is allowed for them."""
+    in float16 (whose rest is up to 2^-12 larger), where the smallest step is 2^-24 and the largest weight 2^7 at least: off by up to
+    2^-32 of that, which is at most the sum. Over 8 bits the first is rounded: 2^-16. They are divided by the sum of the unrounded
+    ones. A score is a sum of dim products in fp32 and some products more: off by (dim + 8) 2^-24 of the sum of its terms'
+    magnitudes; that much, twice (the score's and the largest one's), is the relative error of a weight, and again of their sum.
+    exp, its argument's roundings (2^-23 of its size, at most 100 for a weight that counts) and the fp32 sums' (2^-24 for each of a
+    chain of at most 4096 terms and joins) come to 2^-11.5 at most, far less in practice: 2^-13 is allowed for them."""
     n, hq, dim = q.shape
     group = hq // k.shape[1]
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
@@ -125,7 +126,7 @@ def attend(q, k, v, mask, scale, dtype, bits8):
         rel = p16 + 4 * off + 2.0 ** -13
         tol[:, h] = HALF[dtype] * np.abs(out[:, h]) * (1 + rel) + rel * mag
         if not bits8 and dtype is torch.float16:
-            tol[:, h] += 2.0 ** -25 * (mask @ np.abs(np.where(mask.any(0)[:, None], vv, 0.0)))
+            tol[:, h] += 2.0 ** -32 * (mask @ np.abs(np.where(mask.any(0)[:, None], vv, 0.0)))
             tol[:, h] += 2.0 ** -25  # (and the result's own smallest step)
     return out, tol
 

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import kv_ref as kr
-from test_gpu_kv import KINDS, _cache, _gen, _pages, _rand
+from test_gpu_kv import BF, E4, HF, I8, KINDS, _cache, _gen, _pages, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,24 @@ def test_attend_is_off_by_its_rounding(ge, gpu, query, cache, what):
     if what == "long":  # (each request by itself: the short one's results are large)
         for i in (slice(0, 1), slice(2, 4)):
             assert _rms(got[i] - want[i]) <= 1.02 * _rms(rounded[i] - want[i])
+
+
+@pytest.mark.parametrize("query,cache", [(HF, HF), (BF, BF), (HF, I8), (BF, E4)])
+def test_attend_a_sink_and_a_long_tail(ge, gpu, query, cache):
+    """One token of weight 1 and 131072 of 2^-25.1 each, together 2^-8.1, that share its wave's maximum: they count. As many
+    requests as workgroups run at once, so that a wave has a quarter of a request."""
+    n, many, dim = 131073, 768, 8
+    table = torch.randperm(n // 64 + 1, generator=_gen(gpu, 32), device=gpu).int()[None].repeat(many, 1)
+    pages = table.shape[1]
+    keys = torch.zeros((pages, 64, 1, dim), device=gpu)
+    values = torch.ones((pages, 64, 1, dim), device=gpu)
+    keys[table[0, 0].long(), 0], values[table[0, 0].long(), 0] = 25.1 * np.log(2) / dim, -1
+    scales = None
+    if cache in kr.MOST:
+        keys[table[0, 0].long(), 0] = 2
+        scales = tuple(torch.full((pages, 64, 1), x, device=gpu) for x in (float(25.1 * np.log(2) / dim / 2), 1.0))
+    keys, values = keys.to(cache), values.to(cache)
+    q = torch.ones((many, 1, dim), device=gpu).to(query)
+    got, want, tol = _both(ge, q, keys, values, scales, table, [n] * many, [1] * many, rows=[0, 1, 400, many - 1], scale=1.0)
+    assert -0.9935 < want[0, 0, 0] < -0.991
+    assert (np.abs(got - want) <= tol).all(), float(np.abs(got - want).max())

@@ -562,16 +562,19 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     const bool any = ballot64(bad != 0) != 0;
     if (lane == 0) sh.bad[wave] = any;
   }
-  // What a row sees of the NaNs and infinities that were taken out, of the new tokens in this part, one by one.
+  // What a row sees of the NaNs and infinities that were taken out, of the new tokens in this part, one by one: back from its own
+  // token, which may lie in a later part.
   auto add_bad = [&](uint32_t h, uint32_t row, uint32_t e, float(&y)[8]) {
-    const uint32_t i = row / p.group;
-    int32_t node = sp.begin + (int32_t)i;
-    for (uint32_t t = min(k1, a.parent ? len : ctx + i + 1); t-- > max(k0, ctx);) {  // (backwards: a tree's path, from its node)
+    const uint32_t i = row / p.group, low = max(k0, ctx);
+    if (k1 <= low) return;
+    for (uint32_t past = (a.parent ? ctx + i : min(ctx + i, k1 - 1)) + 1; past > low;) {
+      const uint32_t t = past - 1;
+      past = t;
       if (a.parent) {
-        if (t - ctx != (uint32_t)(node - sp.begin)) continue;
-        const int32_t up = a.parent[node];
-        node = up >= sp.begin && up < node ? up : sp.begin - 1;
+        const int32_t node = sp.begin + (int32_t)(t - ctx), up = a.parent[node];
+        past = up >= sp.begin && up < node ? ctx + (uint32_t)(up - sp.begin) + 1 : 0;
       }
+      if (t >= k1) continue;
       const uint32_t pg = (uint32_t)a.table[(int64_t)r * a.table_ld + t / c.page];
       if (pg >= c.pages) continue;
       const int64_t at = (int64_t)pg * c.page_stride + (int64_t)(t % c.page) * c.token_stride + (int64_t)h * c.head_stride + e;

@@ -1,0 +1,66 @@
+"""NaNs and infinities in attention: which results they reach, whatever the cut of the work and the weights of their tokens."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_ref as kr
+from test_gpu_kv import BF, E4, HF, I8, _cache, _gen, _pages, _rand
+
+pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
+
+
+def _poison(ge, keys, values, scales, table, r, t, value, first_head=1, element=3):
+    """Token t of request r written anew, with a value row of ones in all heads but `first_head`, that has `value` in it."""
+    page, heads, dim = keys.shape[1:]
+    row = torch.ones((1, heads, dim), device=keys.device)
+    row[0, first_head, element] = value
+    at = (table[r, t // page].long(), t % page)
+    was = values[at].clone(), None if scales is None else scales[1][at].clone()
+    if scales is None:
+        values[at] = row[0].to(values.dtype)
+    else:
+        slot = (at[0] * page + at[1]).reshape(1)
+        k, s = keys[at].clone(), scales[0][at].clone()
+        ge.kv.write(slot, row, row, keys, values, scales=scales)
+        keys[at], scales[0][at] = k, s
+    return at, was
+
+
+def _undo(values, scales, at, was):
+    values[at] = was[0]
+    if scales is not None:
+        scales[1][at] = was[1]
+
+
+@pytest.mark.parametrize("query,cache", [(BF, BF), (HF, HF), (BF, E4), (HF, I8)])
+@pytest.mark.parametrize("shape", ["chain", "star", "random"])
+def test_bad_values_of_a_tree_over_two_shares(ge, gpu, query, cache, shape):
+    """A request's new tokens lie on both sides of a border of the work's shares (35 blocks of 32 in four: a border at token 320): a
+    NaN or an infinity reaches the descendants on the other side too, and no other row."""
+    g = _gen(gpu, 41)
+    lengths, news = [330, 256], [20, 1]
+    rng = np.random.default_rng(3)
+    par = np.array([-1] + [i - 1 if shape == "chain" else 0 if shape == "star" else int(rng.integers(max(i - 4, 0), i)) for i in range(1, 20)]
+                   + [-1])
+    table, pages = _pages(g, lengths, 16)
+    keys, values, scales = _cache(g, cache, pages, 16, 2, 64, False)
+    q = _rand(g, 21, 2, 64).to(query)
+    run = lambda: ge.kv.attend(q, keys, values, table, lengths, begin=[0, 20, 21], parents=par, scales=scales)  # noqa: E731
+    clean, sees = run(), kr.sees(20, 0, par, 0)
+    for i, value in [(1, INF), (9, NAN), (0, -INF), (10, INF), (19, NAN)]:
+        at, was = _poison(ge, keys, values, scales, table, 0, 310 + i, value)
+        got = run()
+        assert torch.equal(got[20], clean[20])
+        for k in range(20):
+            a = got[k].float()
+            if not sees[k, i]:
+                assert torch.equal(got[k], clean[k]), (i, k)
+                continue
+            assert torch.isfinite(a[0]).all(), (i, k)
+            if scales is None:
+                assert torch.isfinite(a[1]).sum() == 63 and (torch.isnan(a[1, 3]) if value != value else a[1, 3] == value), (i, k)
+            else:
+                assert torch.isnan(a[1]).all(), (i, k)
+        _undo(values, scales, at, was)
+    assert torch.equal(run(), clean)

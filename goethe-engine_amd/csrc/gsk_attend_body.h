@@ -150,7 +150,8 @@ __device__ __forceinline__ float over_groups(float x, Op op) {
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// The factor of a part of maximum m and sum l in a whole of maximum top (NaN scores leave m at -inf and l NaN).
+// The factor of a part of maximum m and sum l in a whole of maximum top (NaN scores leave m at -inf and l NaN). A part that saw
+// nothing has l 0 and is left out; one whose factor is 0 is not: its NaNs and infinities count.
 __device__ __forceinline__ float weight_of(float m, float l, float top) {
   return l == 0.0f ? 0.0f : m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
 }
@@ -636,8 +637,8 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         const uint32_t w0 = four ? hh : 0, w1 = four ? hh + 1 : AW;
         for (uint32_t w = w0; w < w1; ++w) top = fmaxf(top, sh.m[w][tr]);
         for (uint32_t w = w0; w < w1; ++w) {
+          if (sh.l[w][tr] == 0.0f) continue;
           const float f = weight_of(sh.m[w][tr], sh.l[w][tr], top);
-          if (f == 0.0f) continue;
           sum += f * sh.l[w][tr];
 #pragma unroll
           for (int d = 0; d < 8; ++d) x[d] += f * sh.o[w][tr][te + d];
@@ -706,8 +707,8 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
 #pragma unroll
         for (uint32_t k = 0; k < 8; ++k) {
           const float part_l = __uint_as_float((uint32_t)(ml[k] >> 32));
-          const float g = s0 + k * shares < parts ? weight_of(__uint_as_float((uint32_t)ml[k]), part_l, top) : 0.0f;
-          if (g == 0.0f) continue;  // (nothing of this row in the part, or no such part)
+          if (part_l == 0.0f || s0 + k * shares >= parts) continue;  // (nothing of this row in the part, or no such part)
+          const float g = weight_of(__uint_as_float((uint32_t)ml[k]), part_l, top);
           sum += g * part_l;
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
@@ -734,7 +735,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
           for (int d = 0; d < 8; ++d) y[d] *= f;
           for (uint32_t k = 1; k < shares; ++k) {
             const float part_l = sh.l[0][tr + k * wide], g = weight_of(sh.m[0][tr + k * wide], part_l, top);
-            if (g == 0.0f) continue;
+            if (part_l == 0.0f) continue;
             sum += g * part_l;
 #pragma unroll
             for (int d = 0; d < 8; ++d) y[d] += g * sh.o[0][tr + k * wide][te + d];

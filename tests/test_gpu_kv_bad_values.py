@@ -64,3 +64,46 @@ def test_bad_values_of_a_tree_over_two_shares(ge, gpu, query, cache, shape):
                 assert torch.isnan(a[1]).all(), (i, k)
         _undo(values, scales, at, was)
     assert torch.equal(run(), clean)
+
+
+@pytest.mark.parametrize("query,cache", [(BF, BF), (HF, HF)])
+def test_bad_values_of_small_weight(ge, gpu, query, cache):
+    """A token whose weight is too small for fp32 (its score 320 below the largest) is seen all the same: a NaN or an infinity in
+    its value reaches the result, whichever wave or share has it; the other requests and heads have none."""
+    g = _gen(gpu, 42)
+    lengths, news = [64, 40, 5000, 700], [1, 3, 2, 4]
+    begin = np.concatenate([[0], np.cumsum(news)])
+    table, pages = _pages(g, lengths, 16)
+    keys, values, scales = _cache(g, cache, pages, 16, 2, 64, False)
+    if scales is None:
+        keys[..., 0] = 0
+    else:
+        keys.view(torch.int8)[..., 0] = 0
+        scales[0].fill_(0.01)
+    q = (_rand(g, sum(news), 4, 64) * 0.05).to(query)
+    q[..., 0] = 16
+    high, scale = (40.0, 0.5) if scales is None else (120.0, 17.0)  # (16 * 40 * 0.5 = 320; 8 bits: 16 * 1.2 * 17 = 326)
+    bits = torch.int16 if scales is None else torch.int8
+    high = torch.tensor(high, device=gpu).to(cache).view(bits)
+    tokens = [(0, 3, [40]), (0, 63, [0]), (1, 5, [33]), (1, 39, [3]), (2, 7, [4000]), (2, 4000, [7]), (3, 699, [2]), (3, 2, [600]),
+              (3, 698, [650])]
+    run = lambda: ge.kv.attend(q, keys, values, table, lengths, begin=begin, scales=scales, scale=scale)  # noqa: E731
+    for r, t, tops in tokens:
+        old = keys.clone()
+        for x in tops:
+            keys.view(bits)[table[r, x // 16].long(), x % 16, :, 0] = high
+        clean = run()
+        for value in (NAN, INF):
+            at, was = _poison(ge, keys, values, scales, table, r, t, value)
+            got = run().float()
+            for rr in range(4):
+                for k in range(begin[rr], begin[rr + 1]):
+                    n = lengths[rr] - news[rr] + k - begin[rr]  # (the last token that it sees)
+                    if rr != r or n < t:
+                        assert torch.equal(got[k], clean[k].float()), (r, t, rr, k)
+                    elif scales is None:
+                        assert not torch.isfinite(got[k, 2:, 3]).any() and torch.isfinite(got[k]).sum() == 4 * 64 - 2, (r, t, k, value)
+                    else:
+                        assert torch.isnan(got[k, 2:]).all() and torch.isfinite(got[k, :2]).all(), (r, t, k, value)
+            _undo(values, scales, at, was)
+        keys.copy_(old)

@@ -474,6 +474,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
             const uint32_t k = (j / 4) * 16 + lg * 4 + j % 4, at = t + k, d = at - ctx;  // (past ctx: the new token's index)
             const uint32_t in_new = a.parent ? (uint32_t)(path[m] >> (d & 63)) & (uint32_t)(d < 64) : (uint32_t)(at < sees[m]);
             const uint32_t see = (real >> k) & ((uint32_t)(at < ctx) | in_new) & 1;
+            if constexpr (type_is_8bit<C>) z[j] = __builtin_fmaf(vscale[j / 4][j % 4], 0.0f, z[j]);  // (a value's NaN, at any weight)
             z[j] = see ? z[j] : -INF;
           }
         }

@@ -66,7 +66,7 @@ def test_bad_values_of_a_tree_over_two_shares(ge, gpu, query, cache, shape):
     assert torch.equal(run(), clean)
 
 
-@pytest.mark.parametrize("query,cache", [(BF, BF), (HF, HF)])
+@pytest.mark.parametrize("query,cache", [(BF, BF), (HF, HF), (BF, E4), (HF, I8)])
 def test_bad_values_of_small_weight(ge, gpu, query, cache):
     """A token whose weight is too small for fp32 (its score 320 below the largest) is seen all the same: a NaN or an infinity in
     its value reaches the result, whichever wave or share has it; the other requests and heads have none."""
@@ -86,7 +86,7 @@ def test_bad_values_of_small_weight(ge, gpu, query, cache):
     bits = torch.int16 if scales is None else torch.int8
     high = torch.tensor(high, device=gpu).to(cache).view(bits)
     tokens = [(0, 3, [40]), (0, 63, [0]), (1, 5, [33]), (1, 39, [3]), (2, 7, [4000]), (2, 4000, [7]), (3, 699, [2]), (3, 2, [600]),
-              (3, 698, [650])]
+              (3, 698, [650]), (0, 63, [40]), (1, 33, [36]), (1, 39, [35]), (2, 4995, [4993]), (2, 4999, [4994]), (3, 680, [690])]
     run = lambda: ge.kv.attend(q, keys, values, table, lengths, begin=begin, scales=scales, scale=scale)  # noqa: E731
     for r, t, tops in tokens:
         old = keys.clone()

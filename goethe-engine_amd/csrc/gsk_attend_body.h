@@ -434,7 +434,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
       if (!whole) {  // (what a lane past dim has read)
 #pragma unroll
         for (int k = WHOLE; k < KD; ++k)
-          if (k_at[k - WHOLE] < 0 || (k == 0 && lg * 8 >= c.dim)) kr[0][k] = kr[1][k] = Raw8<C>{};
+          if (k * 32 + lg * 8 >= c.dim) kr[0][k] = kr[1][k] = Raw8<C>{};
       }
       f32x4 s[MT][2];
 #pragma unroll

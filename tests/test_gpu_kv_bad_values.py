@@ -107,3 +107,30 @@ def test_bad_values_of_small_weight(ge, gpu, query, cache):
                         assert torch.isnan(got[k, 2:]).all() and torch.isfinite(got[k, :2]).all(), (r, t, k, value)
             _undo(values, scales, at, was)
         keys.copy_(old)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [8, 16, 32, 40, 64, 72, 96, 104, 128, 136, 160, 192, 200, 224, 232, 256])
+def test_keys_of_minus_infinity(ge, gpu, dtype, dim):
+    """A key with -inf in any of its places has the score -inf (its queries are above 0 there): the token has no weight, as if it was
+    not there, whatever lies past dim in the registers; where every token is so, the result is 0."""
+    g = _gen(gpu, dim)
+    lengths, news = [70, 33, 5], [1, 2, 1]
+    table, pages = _pages(g, lengths, 16)
+    keys, values, _ = _cache(g, dtype, pages, 16, 1, dim, False)
+    q = _rand(g, 4, 2, dim).abs().to(dtype) + 0.125
+    begin, off = [0, 1, 3, 4], {0: [0, 1, 40, 69], 1: [3, 32], 2: [0, 1, 2, 3, 4]}
+    for place in sorted({0, 3, 7, dim // 2, dim - 1}):
+        k = keys.clone()
+        for r, ts in off.items():
+            for t in ts:
+                k[table[r, t // 16].long(), t % 16, 0, place] = -INF
+        got = kr._np(ge.kv.attend(q, k, values, table, lengths, begin=begin))
+        assert (got[3] == 0).all()
+        for r in (0, 1):
+            kk, there = kr.tokens(keys, None, table[r].tolist(), 0, lengths[r], False)
+            vv, _ = kr.tokens(values, None, table[r].tolist(), 0, lengths[r], False)
+            mask = kr.sees(news[r], lengths[r] - news[r]) & there
+            mask[:, off[r]] = False
+            want, tol = kr.attend(kr._np(q[begin[r]:begin[r + 1]]), kk, vv, mask, float(np.float32(dim ** -0.5)), dtype, False)
+            assert (np.abs(got[begin[r]:begin[r + 1]] - want) <= tol).all(), (place, r)

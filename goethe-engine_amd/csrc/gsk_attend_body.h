@@ -194,9 +194,6 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
   constexpr float INF = INFINITY;
   // 16 bits: a weight times MORE goes into the second product, cut off and the rest, which then is above 0 (an infinite value stays one)
   constexpr float MORE = type_is_8bit<C> ? 1.0f : VT == GSK_F16 ? 1.0f + 0x1p-12f : 1.0f + 0x1p-17f;
-  // What the running maximum has added to it: over float16 the weights are 2^7 as large, up to 2^15, so that those below 2^-14 of
-  // the largest, whose steps are 2^-24, count to 2^-32 of it (a long tail behind one token that outweighs each of them).
-  constexpr float DROP = VT == GSK_F16 ? -7.0f : 0.0f;
   __shared__ Sh sh;
   const gsk_cache &c = p.c;
   const gsk_attention &a = p.a;
@@ -338,6 +335,11 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
     }
   }
   f32x4 acc[MT][VB][8];
+  // What the running maximum has added to it. Over float16 the weights are 2^7 as large, up to 2^15, so that those below 2^-14 of the
+  // largest, whose steps are 2^-24, count to 2^-32 of it (a long tail behind one token that outweighs each of them). In bfloat16 the
+  // weights of all tokens add up to less than 1/2, so that no sum of values, or scale times weight, leaves fp32's range (what is lost
+  // at its other end is below 2^-126 times 2^9 and the tokens).
+  const float drop = VT == GSK_F16 ? -7.0f : (float)(9 + 32 - __builtin_clz(len | 1));
   float mx[MT], l[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -483,7 +485,7 @@ __global__ __launch_bounds__(AT, attend_resident(KD, MT)) void attend_kernel(Att
         top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
         if constexpr (!type_is_8bit<C>) top = top == -INF ? -INF : top * scale;  // (a scale of 0)
         // The maximum follows once it is 2^8 behind: the weights are up to that, and what it saves is the output's rescaling.
-        top += DROP;
+        top += drop;
         if (ballot64(top > mx[m] + 8.0f)) {
           top = top > mx[m] + 8.0f ? top : mx[m];  // (a row's own: what others see does not change it)
           const float f = __builtin_amdgcn_exp2f(mx[m] - (top == -INF ? 0.0f : top));

@@ -23,8 +23,8 @@ enum { GSK_BF16 = 0, GSK_F16 = 1, GSK_F32 = 2, GSK_E4M3 = 3, GSK_I8 = 4 };
 
 /* One layer's cache: keys and values of one type and layout, dim elements of a token's head lying together; strides in
  * elements. In 8 bits (GSK_E4M3: 8-bit floats of 4 exponent and 3 mantissa bits, largest 448, no infinities; GSK_I8: whole
- * numbers, -127 .. 127) a token's head has a scale, below 2^112, and stands for its elements times that. dim is a multiple of 8, at most
- * GSK_MAX_DIM; the arrays' addresses are multiples of 8 elements, as are the strides. */
+ * numbers, -127 .. 127) a token's head has a scale, finite or NaN, and stands for its elements times that. dim is a multiple of 8, at
+ * most GSK_MAX_DIM; the arrays' addresses are multiples of 8 elements, as are the strides. */
 #define GSK_MAX_DIM 256
 typedef struct gsk_cache {
   uint32_t size;

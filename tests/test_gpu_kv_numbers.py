@@ -82,3 +82,34 @@ def test_attend_a_sink_and_a_long_tail(ge, gpu, query, cache):
     got, want, tol = _both(ge, q, keys, values, scales, table, [n] * many, [1] * many, rows=[0, 1, 400, many - 1], scale=1.0)
     assert -0.9935 < want[0, 0, 0] < -0.991
     assert (np.abs(got - want) <= tol).all(), float(np.abs(got - want).max())
+
+
+@pytest.mark.parametrize("cache", [BF, E4, I8])
+def test_attend_values_of_every_size(ge, gpu, cache):
+    """Values near the end of fp32's range, and far below 1: sums over many tokens of one weight, over ones whose weight grows
+    up to 2^7.9 before the maximum follows, joined or not, are as exact as at any size."""
+    g = _gen(gpu, 33)
+    lengths = [1, 32, 300, 5000, 40000]
+    table, pages = _pages(g, lengths, 16)
+    keys, _, scales = _cache(g, cache, pages, 16, 1, 64, False)
+    held = {BF: [-1.75, 1.0, 1.25, 1.9375], E4: [-448.0, 256.0, 320.0, 384.0], I8: [-127.0, 64.0, 100.0, 126.0]}[cache]
+    end = {BF: 2.0 ** 127, E4: 2.0 ** 119, I8: 2.0 ** 121 * 0.98}[cache]  # (1.9375 * 2^127 = 3.3e38)
+    codes = torch.tensor(held, device=gpu)[torch.randint(0, 4, (pages, 16, 1, 64), generator=g, device=gpu)].double()
+    q = _rand(g, len(lengths), 4, 64).to(BF)
+    grow = torch.arange(40000, device=gpu) / 40000 * 5.4  # (natural: 2^7.8)
+    for rising in (False, True):
+        k = torch.zeros((pages, 16, 1, 64), device=gpu)
+        if rising:
+            k.view(-1, 1, 64)[(table[4].long()[:, None] * 16 + torch.arange(16, device=gpu)).reshape(-1)[:40000], 0, 0] = grow
+            q[:] = 0
+            q[..., 0] = 8
+        ks = None
+        if cache in kr.MOST:
+            ks = torch.full((pages, 16, 1), 5.4 / kr.MOST[cache], device=gpu)
+            k = torch.round(k / ks[..., None]) if cache is I8 else k / ks[..., None]
+        for size in (end, 1.0, 2.0 ** -70):
+            v, vs = (codes * size).to(BF) if cache is BF else codes.to(cache), torch.full((pages, 16, 1), size, device=gpu)
+            got, want, tol = _both(ge, q, k.to(cache), v, None if cache is BF else (ks, vs), table, lengths, [1] * 5)
+            assert np.isfinite(want).all() and np.abs(want).max() > 0
+            assert np.isfinite(got).all(), (rising, size)
+            assert (np.abs(got - want) <= tol).all(), (rising, size, float((np.abs(got - want) / tol).max()))

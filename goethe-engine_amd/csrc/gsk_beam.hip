@@ -6,13 +6,14 @@
 // quarter of n lanes' maxima (rounded up) reach some value, so n elements reach the least of the four; the elements that reach
 // it, and the n-th largest of the slices before, are listed (a few more than n in an unordered row) and ranked by counting; where
 // more tie with the bound than the list holds, the n-th largest (value, token) is found digit by digit instead. The workgroup
-// leaves its maximum m, its sum of exp(x - m) and its list. The sum decides the order of tokens of different beams, so the large
-// terms, the listed ones, are fp64 (their differences from the fp32 ones added up as whole multiples of 2^-62: in any order the
-// same, so that equal rows have equal sums); the many small ones are fp32 in each thread (their errors average out: about 1e-9 of
-// the sum) and fp64 from there on. The last workgroup of a request (a ticket) joins its beams' lists: log of each beam's sum, then
-// the n best of all entries by the same two steps.
+// leaves its maximum m, its sum of exp(x - m) and its list. The sum decides the order of tokens of different beams: a term is exp2 in
+// fp32, off by 2^-24 (2 |x - m| + 4) of it at most and by either sign, added up in fp64; the listed ones, the largest, are corrected to
+// fp64 (by whole multiples of 2^-62: in any order the same, so that equal rows have equal sums). Measured over rows of 128256 logits,
+// fp32, bfloat16 and float16, normal (sigma 1 to 5), uniform and with one peak: 5e-9 of the sum at most (a thread's terms of a slice added
+// up in fp32: 5e-8, beside a peak 1e-6; 64 x 8 rows took 64 us instead of 66). The last workgroup of a request (a ticket) joins its beams'
+// lists: log of each beam's sum, then the n best of all entries by the same two steps.
 //
-// Bound: 4 beams of 128256 fp32 logits, 14.1 us, are a chain: a slice's load, its maxima, bound, list and ranks (8 us), the ticket, the
+// Bound: 4 beams of 128256 fp32 logits, 14.4 us, are a chain: a slice's load, its maxima, bound, list and ranks (8 us), the ticket, the
 // join's reads, logs and ranks. 64 requests of 8 beams of 151936 bf16 logits (156 MB), 63.5 us or 2.4 TB/s (fp32: 79, 3.9), are bound
 // by instructions (15 on each element of 2 bytes by the counters: unpacking, maxima, exp2, compare), then by the last request's join.
 #include "gsk_dev.h"
@@ -29,6 +30,7 @@ constexpr uint32_t BS = 8192;      // tokens of a slice
 constexpr int BE = BS / BT;        // a thread's elements
 constexpr uint32_t BL = 1024;      // entries of the list
 constexpr uint32_t LISTS = 1024;   // a request's lists, at most
+constexpr float LOG2E = 0x1.715476p+0f, LOG2E_REST = 0x1.4ae0cp-26f;
 constexpr int AHEAD = 8;           // entries of its request's lists that a thread reads at once in the join
 
 struct ListSum {  // a workgroup's part of its row's sum
@@ -148,12 +150,14 @@ __global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts
       }
     }
     if (slice + 1 < end) load(slice + 1);
-    float most = -INFINITY;
+    float of8[BE / 8], most = -INFINITY;
 #pragma unroll
     for (int e = 0; e < BE; ++e) {
       v[e] = fmaxf(v[e], -INFINITY);  // (NaN counts as -inf)
-      most = fmaxf(most, v[e]);
+      of8[e / 8] = e % 8 ? fmaxf(of8[e / 8], v[e]) : v[e];
     }
+#pragma unroll
+    for (int e = 0; e < BE / 8; ++e) most = fmaxf(most, of8[e]);
     // each wave's bound, of the values' upper 16 bits; the slice's maximum
     const uint32_t kth = wave_kth_largest_u16(fkey(most) >> 16, (int)(n + 3) / 4) << 16, wave_most = wave_max_u32(fkey(most));
     __syncthreads();  // (the slice before is done with the list)
@@ -177,17 +181,28 @@ __global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts
     top = now;
     if (now_key <= KEY_NEGINF || now_key >= KEY_POSINF) continue;  // (nothing yet; or +inf: the row gives nothing)
     const float bound = bound_key > KEY_NEGINF ? fkey_inv(bound_key) : -FLT_MAX;
-    auto term = [&](float y) { return __builtin_amdgcn_exp2f((y - now) * 1.44269504f); };
-    float rest = 0;
+    auto term = [&](float y) {  // (log2 e as two numbers, so that a term's error has either sign)
+      const float d = y - now;
+      return __builtin_amdgcn_exp2f(__builtin_fmaf(d, LOG2E, d * LOG2E_REST));
+    };
 #pragma unroll
-    for (int e = 0; e < BE; ++e) {
-      rest += term(v[e]);
-      if (v[e] >= bound) {
-        const uint32_t k = atomicAdd(&sh.n, 1u);
-        if (k < BL) sh.list[k] = pack(fkey(v[e]), token(slice, e));
+    for (int g = 0; g < BE / 8; ++g) {
+      if (ballot64(of8[g] >= bound) == 0) continue;  // (after a row's first slice most have none)
+#pragma unroll
+      for (int e = 8 * g; e < 8 * g + 8; ++e) {
+        if (v[e] >= bound) {
+          const uint32_t k = atomicAdd(&sh.n, 1u);
+          if (k < BL) sh.list[k] = pack(fkey(v[e]), token(slice, e));
+        }
       }
     }
-    sum += (double)rest;
+    double odd = 0;  // (fp64 from the first term on: small ones next to a large one are not lost)
+#pragma unroll
+    for (int e = 0; e < BE; e += 2) {
+      sum += (double)term(v[e]);
+      odd += (double)term(v[e + 1]);
+    }
+    sum += odd;
     __syncthreads();
     uint32_t count = sh.n;
     if (count > BL) {

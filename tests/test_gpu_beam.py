@@ -124,3 +124,48 @@ def test_calls_share_a_stream(ge, gpu):
         _check(o, *cases[0])
         with torch.cuda.stream(stream):
             _check(ge.beam.select(*cases[1]), *cases[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("far", [16.875, 12.5, 9.0])
+@pytest.mark.parametrize("peaks,n", [(1, 1), (1, 4), (3, 1), (40, 2), (700, 64), (2000, 8)])
+def test_sums_of_peaked_rows(ge, gpu, dtype, far, peaks, n):
+    """A few tokens (or more than a list holds) at 0 and a hundred thousand others far below, all alike or spread out: a row's sum is
+    off by its far terms' own errors, never by what adding them to the large ones costs. Of each term below the listed ones, with t
+    its distance from the maximum: t's rounding and its product's with log2 e, 2^-24 |t| each, and exp2's, 2^-23; so 2^-24 (2 |t| + 4)
+    of it is allowed. Terms at the maximum itself are exact. Two beams whose sums differ by 2^-20.5 come in their order."""
+    v = 128256
+    g = torch.Generator(device=gpu).manual_seed(peaks)
+    x = torch.full((4, v), -far, device=gpu)
+    x[1] -= torch.rand(v, generator=g, device=gpu) * 4
+    x[3] = 50 - far
+    for i in range(4):
+        x[i, torch.randperm(v, generator=g, device=gpu)[:peaks]] = 50.0 if i == 3 else 0.0
+    x = x.to(dtype)
+    s = torch.tensor([[0.0, -0.25, -0.5, -0.75]], device=gpu)
+    for rows in ([0], [1], [2], [3], [0, 1, 2, 3]):
+        o = ge.beam.select(x[rows], s[:, :len(rows)].contiguous(), n)
+        xs = kr._np(x[rows])
+        t = xs.max(1, keepdims=True) - xs
+        w = np.exp(-t)
+        lse = xs.max(1) + np.log(w.sum(1))
+        near = [np.flatnonzero(z >= np.partition(z, -n)[-n]).tolist() for z in xs]
+        want = sorted((lse[b] - xs[b, i] + 0.25 * b, b, i) for b in range(len(rows)) for i in near[b])[:n]
+        tol = ((w * (2 * t + 4) * 2.0 ** -24 * (t > 0)).sum(1) / w.sum(1)).max()
+        got = o.scores.cpu().numpy()[0]
+        for k, (less, beam, token) in enumerate(want):
+            score = -less
+            assert abs(float(got[k]) - score) <= tol + abs(score) * 2.0 ** -24 + 1e-11, (rows, k, float(got[k]) - score, tol)
+            assert (int(o.tokens[0, k]), int(o.parents[0, k])) == (token, beam), (rows, k)
+
+
+def test_close_beams_in_order(ge, gpu):
+    """Beams whose rows have one peak, in the first slice or the last, and whose far tokens are a few more or fewer: their order is that
+    of their sums, whose differences (9e-8 and more) are above their errors (2^-24 * 38 of the far terms' 0.0059, 1.4e-8)."""
+    v = 128256
+    x = torch.full((4, v), -16.875, device=gpu)
+    for i, (cut, peak) in enumerate([(0, 5), (4, 124240), (2, 5), (6, 124240)]):
+        x[i, 100:100 + cut] = -float("inf")
+        x[i, peak] = 0
+    o = ge.beam.select(x, torch.zeros((1, 4), device=gpu), 4)
+    assert o.parents.tolist() == [[3, 1, 2, 0]] and o.tokens.tolist() == [[124240, 124240, 5, 5]]

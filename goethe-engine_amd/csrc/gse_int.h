@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>  // (host code says std::min and std::max: without std:: they are of ints there)
+
 #include "../../include/gse.h"
 
 namespace gse {

@@ -932,7 +932,7 @@ RowSlices slices_of(const RowsWs &w, int V, int *rows) {
     sub = (ns + cap - 1) / cap;
     ns = (V + RS * sub - 1) / (RS * sub);
   }
-  *rows = (int)min(min(cap / ns, (int64_t)w.rows), (int64_t)65535);
+  *rows = (int)std::min(std::min(cap / ns, (int64_t)w.rows), (int64_t)65535);
   return RowSlices{(int)ns, (int)sub};
 }
 

@@ -400,8 +400,8 @@ __global__ __launch_bounds__(BT, 4) void beam_kernel(gsk_beams a, uint32_t parts
 // CU 82).
 static uint32_t beam_parts(const gsk_beams &a, int cus) {
   const uint64_t slices = (a.vocab + BS - 1) / BS, rows = (uint64_t)a.requests * a.beams;
-  const uint64_t most = max((uint64_t)4 * cus / max(rows, (uint64_t)1), (uint64_t)1);
-  return (uint32_t)min(min(slices, most), (uint64_t)(LISTS / a.beams));
+  const uint64_t most = std::max((uint64_t)4 * cus / std::max(rows, (uint64_t)1), (uint64_t)1);
+  return (uint32_t)std::min(std::min(slices, most), (uint64_t)(LISTS / a.beams));
 }
 
 int64_t beam_work(const gsk_beams &a, int cus) {
@@ -411,10 +411,10 @@ int64_t beam_work(const gsk_beams &a, int cus) {
 hipError_t launch_beam(const gsk_beams &a, int cus, uint32_t *tick, uint32_t tickets, hipStream_t s) {
   const uint32_t parts = beam_parts(a, cus);
   // a launch takes a ticket per request, and 65535 rows at most
-  const uint32_t most = min(tickets, 65535u / a.beams);
+  const uint32_t most = std::min(tickets, 65535u / a.beams);
   auto go = [&](auto type, auto wide) {
     for (uint32_t r0 = 0; r0 < a.requests; r0 += most)
-      hipLaunchKernelGGL((beam_kernel<type(), wide()>), dim3(parts, min(most, a.requests - r0) * a.beams), dim3(BT), 0, s, a, parts,
+      hipLaunchKernelGGL((beam_kernel<type(), wide()>), dim3(parts, std::min(most, a.requests - r0) * a.beams), dim3(BT), 0, s, a, parts,
                          div_by(parts * a.n), tick, r0);
   };
   const uint64_t size = a.type == GSK_F32 ? 4 : 2;

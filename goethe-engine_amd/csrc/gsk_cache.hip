@@ -286,13 +286,13 @@ hipError_t launch_reorder(const gsk_reorder_beams &in, hipStream_t s) {
     const int64_t blocks = ((int64_t)in.max_pages * in.page + CT / MB - 1) / (CT / MB);
     for (uint32_t g0 = 0; g0 < in.groups; g0 += 65535) {
       gsk_reorder_beams a = in;
-      a.groups = min(in.groups - g0, 65535u);
+      a.groups = std::min(in.groups - g0, 65535u);
       a.table += (int64_t)g0 * in.beams * in.table_ld;
       a.seq_len += (int64_t)g0 * in.beams;
       a.parent += (int64_t)g0 * in.beams;
       if (a.first) a.first += g0;
-      const int64_t x = max(min((columns + EACH * CT - 1) / (EACH * CT), WGS / a.groups), (int64_t)1);
-      const int64_t y = min(min(blocks, (int64_t)65535), max((int64_t)1, WGS / (a.groups * x)));
+      const int64_t x = std::max(std::min((columns + EACH * CT - 1) / (EACH * CT), WGS / a.groups), (int64_t)1);
+      const int64_t y = std::min(std::min(blocks, (int64_t)65535), std::max((int64_t)1, WGS / (a.groups * x)));
       hipLaunchKernelGGL((reorder_kernel<V, MB>), dim3((uint32_t)x, (uint32_t)y, a.groups), dim3(CT), 0, s, a, div_by(vecs),
                          div_by(in.chunks));
     }

@@ -390,30 +390,30 @@ hipError_t launch_chains(const RowsWs &w, const gsp_chains &c, hipStream_t s) {
     a.tick = w.tick;
     const int64_t nv = (int64_t)c.vocab / VEC;
     const int64_t cap = (int64_t)w.rows * w.slices * 64;         // segment sums that the workspace holds
-    const int64_t rows = min((int64_t)c.requests, min((int64_t)w.ticks, (int64_t)65535));  // requests of a launch, at most
+    const int64_t rows = std::min((int64_t)c.requests, std::min((int64_t)w.ticks, (int64_t)65535));  // requests of a launch, at most
     // One resident round of workgroups over the launch, as long as a wave has a segment; the longest segments that leave every
     // wave one (the last workgroup reads their sums). Where a wave would have eight of the longest or more, four times as
     // many workgroups: rows with and without q even out (512 chains over 262144 bf16 tokens 84 -> 78 us; 64 over 128256 fp32
     // tokens, a segment or two a wave, are slower so: 15.3 -> 21).
-    auto segs = [&](int64_t S) { return max((int64_t)1, (nv + S * WAVE - 1) / (S * WAVE)); };
-    int64_t most = max((int64_t)1, min((int64_t)(w.round) / rows, (int64_t)WGS_MAX));
+    auto segs = [&](int64_t S) { return std::max((int64_t)1, (nv + S * WAVE - 1) / (S * WAVE)); };
+    int64_t most = std::max((int64_t)1, std::min((int64_t)(w.round) / rows, (int64_t)WGS_MAX));
     if (segs(8) >= 8 * CW * most) most *= 4;
     int S = 8;
     while (S > 1 && segs(S) < most * CW) S /= 2;
     while (S < 8 && segs(S) > cap) S *= 2;
     a.nseg = (int)segs(S);
-    const int64_t wgs = min(most, (a.nseg + CW - 1) / (int64_t)CW);
-    const int64_t per = min(rows, cap / a.nseg);
+    const int64_t wgs = std::min(most, (a.nseg + CW - 1) / (int64_t)CW);
+    const int64_t per = std::min(rows, cap / a.nseg);
     // Rows that together pass the last-level cache are read around it. Bytes of one row of p and q a request, us a call over
     // inputs in turn / the same input, cached and around: 134 MB (bf16 128 x 262144) 24.4 / 24.2 and 24.4 / 23.6; 233 MB (fp32
     // 192 x 151936) 41.2 / 31.1 and 37.7 / 35.3; 268 MB (bf16 256 x 262144) 44.7 / 37.0 and 40.5 / 37.5; 311 MB (fp32 256) 53.4 /
     // 44.3 and 48.6 / 46.6; 537 MB (bf16 512) 78.3 / 68.7 and 71.4 / 68.4. Smaller calls lose: 64 fp32 rows 15.0 -> 15.5. So do
     // fp64 rows: 525 MB (256 x 128256) 83.2 / 80.2 and 90.4 / 86.9.
     const bool past = (int64_t)c.requests * c.vocab * (PS + QS) >= (int64_t)256 << 20;
-    a.tstride = (int)min((int64_t)w.ticks / per, (int64_t)64);
+    a.tstride = (int)std::min((int64_t)w.ticks / per, (int64_t)64);
     for (int64_t r0 = 0; r0 < (int64_t)c.requests; r0 += per) {
       a.r0 = (int)r0;
-      const dim3 grid((uint32_t)wgs, (uint32_t)min(per, (int64_t)c.requests - r0));
+      const dim3 grid((uint32_t)wgs, (uint32_t)std::min(per, (int64_t)c.requests - r0));
       if (S == 1) hipLaunchKernelGGL((chain_kernel<P, Q, 1, false>), grid, dim3(CT), 0, s, a);
       else if (S == 2) hipLaunchKernelGGL((chain_kernel<P, Q, 2, false>), grid, dim3(CT), 0, s, a);
       else if (S == 4) hipLaunchKernelGGL((chain_kernel<P, Q, 4, false>), grid, dim3(CT), 0, s, a);

@@ -301,7 +301,7 @@ hipError_t launch_pages(const gsp_pages &p, const gsp_step &t, hipStream_t s) {
   auto go = [&](auto st) {
     constexpr int ST = decltype(st)::value;
     const int64_t tiles = ((int64_t)t.max_tokens + ST - 1) / ST;
-    const dim3 grid((uint32_t)max((int64_t)1, min(tiles, threads / ST)));
+    const dim3 grid((uint32_t)std::max((int64_t)1, std::min(tiles, threads / ST)));
     if (p.counters_out != p.counters) {
       hipLaunchKernelGGL((step_kernel<ST, true, true>), grid, dim3(ST), 0, s, p, t);
     } else {
@@ -320,10 +320,10 @@ hipError_t launch_path(const gsp_path &p, hipStream_t s) {
     using V = decltype(v);
     const uint32_t vecs = (uint32_t)(p.chunk_bytes / sizeof(V));
     const int64_t ids = (int64_t)p.caches * p.chunks * vecs;  // (at most 2^30)
-    const int64_t all = (ids + PT - 1) / PT, wgs = min(all, max((int64_t)1, PATH_WGS / p.requests));
+    const int64_t all = (ids + PT - 1) / PT, wgs = std::min(all, std::max((int64_t)1, PATH_WGS / p.requests));
     for (uint32_t r0 = 0; r0 < p.requests; r0 += 65535) {
       gsp_path a = p;
-      a.requests = min(p.requests - r0, 65535u);
+      a.requests = std::min(p.requests - r0, 65535u);
       a.anchor += r0;
       a.emit_len += r0;
       a.emit_nodes += r0 * p.emit_ld;

@@ -113,3 +113,24 @@ def test_attend_values_of_every_size(ge, gpu, cache):
             assert np.isfinite(want).all() and np.abs(want).max() > 0
             assert np.isfinite(got).all(), (rising, size)
             assert (np.abs(got - want) <= tol).all(), (rising, size, float((np.abs(got - want) / tol).max()))
+
+
+def test_attend_under_a_bound_far_above_its_rows(ge, gpu):
+    """A max_new of 2^24 over four new tokens of 256 query heads a head (2^32 rows at most, 2^31 with 128): the scratch memory is that of
+    any bound that fills the row tiles, and so are the results."""
+    lib, kv = ge._lib, ge.kv
+    rows = lib.handle(gpu.index, 1, 1).rows
+    size, at = (kv._CACHE.size, lib.K_BF16, 200, 16, 1, 64), (1024, 64, 64)
+    for heads in (128, 130, 200, 256):
+        wide, some = (kv._work_bytes(gpu.index, rows, size, at, (1, 4, heads, lib.K_BF16, m, 200)) for m in (1 << 24, 1000))
+        assert wide == some > 0
+    g = _gen(gpu, 34)
+    lengths, news = [3001], [4]
+    table, pages = _pages(g, lengths, 16)
+    keys, values, scales = _cache(g, BF, pages, 16, 1, 64, False)
+    for heads in (128, 200, 256):
+        q = _rand(g, 4, heads, 64).to(BF)
+        got, want, tol = _both(ge, q, keys, values, scales, table, lengths, news)
+        assert (np.abs(got - want) <= tol).all()
+        wide = ge.kv.attend(q, keys, values, table, lengths, begin=[0, 4], max_new=1 << 24)
+        assert (np.abs(kr._np(wide) - want) <= tol).all()

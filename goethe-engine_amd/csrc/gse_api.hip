@@ -764,7 +764,10 @@ int check_attention(gse_handle *h, const gsk_cache &c, const gsk_attention &a) {
   if (a.requests > (1u << 30) || a.tokens > (1u << 30) || a.max_new > (1u << 24))
     return fail(h, GSE_E_UNSUPPORTED, "%u requests, %u tokens, %u a request: at most 2^30, 2^30 and 2^24", a.requests, a.tokens,
                 a.max_new);
-  // blocks of 32 tokens are counted, for each tile of a request's rows
+  // rows are counted, and blocks of 32 tokens for each tile of a request's rows
+  if ((uint64_t)std::min(a.max_new, a.tokens) * (a.heads / c.heads) > UINT32_MAX - 48)
+    return fail(h, GSE_E_UNSUPPORTED, "%u new tokens a request of %u query heads a head: fewer new ones a call",
+                std::min(a.max_new, a.tokens), a.heads / c.heads);
   const uint64_t blocks = a.requests * (16 + (uint64_t)a.max_pages * c.page / 32), tiles = gse::attend_tiles(c, a);
   if (blocks > (uint64_t)UINT32_MAX)
     return fail(h, GSE_E_UNSUPPORTED, "%u requests of up to %llu tokens: at most 2^37 in all", a.requests,

@@ -260,7 +260,7 @@ def attend(q, keys, values, table, seq_len, begin=None, status=None, parents=Non
         raise ValueError(f"max_new {max_new} is not in [1, 2^24]")
     rows = min(max_new, n) * (hq // heads)
     tiles = -(-rows // (16 if rows <= 16 else 32 if rows <= 32 or dim > 128 else 48))
-    if r * (16 + width * page // 32) * max(tiles, 1) >= 1 << 32:
+    if rows >= (1 << 32) - 48 or r * (16 + width * page // 32) * max(tiles, 1) >= 1 << 32:
         raise ValueError(f"{r} requests of up to {min(max_new, n)} new tokens over up to {width * page}: fewer new ones a call")
     if parents is not None and (_count(parents) < n or max_new > _lib.MAX_TREE):
         raise ValueError(f"parents must have {n} entries, for trees of at most {_lib.MAX_TREE} new tokens")

@@ -179,7 +179,7 @@ GSE_API int gsk_read(gse_handle *h, const gsk_cache *cache, const gsk_read_rows 
 /* Attention of new tokens, in one launch. gsk_attention_work: the scratch bytes that it needs for these sizes on this device
  * (0: none; negative: an error); of the structs no pointer is read, and neither q's strides nor the scales'. Up to 2^37 tokens in all:
  * requests * (16 + max_pages * page / 32) < 2^32, and so much times the tiles of min(max_new, tokens) * heads / cache heads rows (of
- * 48; 32 where there are no more or dim > 128; 16): longer prompts go in parts. */
+ * 48; 32 where there are no more or dim > 128; 16), and fewer than 2^32 - 48 such rows a request: longer prompts go in parts. */
 GSE_API int64_t gsk_attention_work(gse_handle *h, const gsk_cache *cache, const gsk_attention *in);
 GSE_API int gsk_attend(gse_handle *h, const gsk_cache *cache, const gsk_attention *in);
 

@@ -134,3 +134,14 @@ def test_attend_under_a_bound_far_above_its_rows(ge, gpu):
         assert (np.abs(got - want) <= tol).all()
         wide = ge.kv.attend(q, keys, values, table, lengths, begin=[0, 4], max_new=1 << 24)
         assert (np.abs(kr._np(wide) - want) <= tol).all()
+
+
+def test_attention_work_counts_its_rows(ge, gpu):
+    """New tokens times a head's query heads past 2^32, over one page of one token: the library refuses them too."""
+    lib, kv = ge._lib, ge.kv
+    size, at = (kv._CACHE.size, lib.K_BF16, 1, 1, 1, 8), (8, 8, 8)
+    rows = lib.handle(gpu.index, 1, 1).rows
+    assert kv._work_bytes(gpu.index, rows, size, at, (1, 1 << 24, 255, lib.K_BF16, 1 << 24, 1)) > 0
+    for heads in (256, 300, 512):
+        with pytest.raises(RuntimeError, match="fewer new ones"):
+            kv._work_bytes(gpu.index, rows, size, at, (1, 1 << 24, heads, lib.K_BF16, 1 << 24, 1))

@@ -189,3 +189,11 @@ def test_packed_structs_are_the_headers(ge):
         assert [kinds[C.sizeof(t)][t] for _, t in cls._fields_] == list(flat)
         raw = cls.from_buffer_copy(packed.pack(*range(1, len(flat) + 1)))
         assert [getattr(raw, f) for f, _ in cls._fields_] == list(range(1, len(flat) + 1))
+
+
+def test_attend_refuses_more_rows_than_are_counted(ge):
+    """New tokens times a head's query heads past 2^32."""
+    k = torch.zeros((1, 1, 1, 8), dtype=BF)
+    ok = dict(q=torch.zeros((1, 1, 8), dtype=BF).expand(1 << 24, 255, 8), keys=k, values=k.clone(), begin=[0, 1], max_new=1 << 24, seq_len=[1],
+              table=torch.zeros((1, 1), dtype=torch.int32))
+    _refusals(ge.kv.attend, ok, [dict(q=torch.zeros((1, 1, 8), dtype=BF).expand(1 << 24, hq, 8)) for hq in (256, 300, 512)])

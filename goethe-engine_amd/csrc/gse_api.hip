@@ -757,6 +757,7 @@ int check_attention(gse_handle *h, const gsk_cache &c, const gsk_attention &a) {
   if (type_bytes(c.type) == 2 && c.type != a.type) return fail(h, GSE_E_ARG, "q of type %u over a cache of type %u", a.type, c.type);
   if (a.heads == 0 || a.heads % c.heads || a.heads > (1u << 16))
     return fail(h, GSE_E_ARG, "%u query heads over %u cache heads", a.heads, c.heads);
+  if (!(std::abs(a.scale) <= 0x1p127f)) return fail(h, GSE_E_ARG, "scale %g is not in [-2^127, 2^127]", a.scale);
   if (a.max_pages == 0) return fail(h, GSE_E_ARG, "max_pages must be > 0");
   if (a.max_new == 0 && a.tokens > 0) return fail(h, GSE_E_ARG, "max_new must be > 0");
   if ((uint64_t)a.max_pages * c.page > (uint64_t)INT32_MAX)

@@ -265,8 +265,8 @@ def attend(q, keys, values, table, seq_len, begin=None, status=None, parents=Non
     if parents is not None and (_count(parents) < n or max_new > _lib.MAX_TREE):
         raise ValueError(f"parents must have {n} entries, for trees of at most {_lib.MAX_TREE} new tokens")
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not abs(scale) <= 3.4e38:
-        raise ValueError(f"scale {scale}")
+    if not abs(scale) <= 2.0 ** 127:
+        raise ValueError(f"scale {scale} is not in [-2^127, 2^127]")
     if out is not None:
         if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be a contiguous tensor like q, at a multiple of 16 bytes")

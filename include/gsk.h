@@ -102,7 +102,7 @@ typedef struct gsk_attention {
   const int32_t *table;
   int64_t table_ld;
   uint32_t max_pages;       /* entries of a table row; max_pages * page < 2^31 */
-  float scale;              /* of the scores */
+  float scale;              /* of the scores; at most 2^127 in size */
   const int32_t *begin;     /* [requests + 1], or NULL: one new token a request, row r */
   const int32_t *seq_len;   /* [requests] */
   const uint32_t *status;   /* [requests] gsp_step's, or NULL: every request is served */

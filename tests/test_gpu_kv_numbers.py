@@ -145,3 +145,23 @@ def test_attention_work_counts_its_rows(ge, gpu):
     for heads in (256, 300, 512):
         with pytest.raises(RuntimeError, match="fewer new ones"):
             kv._work_bytes(gpu.index, rows, size, at, (1, 1 << 24, heads, lib.K_BF16, 1 << 24, 1))
+
+
+def test_attention_takes_scales_to_2_to_127(ge, gpu):
+    """Scores of a scale of 2^127 that are 0 are 0, and equal; the library refuses what is past it."""
+    g = _gen(gpu, 35)
+    table, pages = _pages(g, [40], 16)
+    keys, values, _ = _cache(g, BF, pages, 16, 1, 64, False)
+    q = torch.zeros((1, 2, 64), device=gpu).to(BF)
+    for scale in (2.0 ** 127, -(2.0 ** 127)):
+        got, want, tol = _both(ge, q, keys, values, None, table, [40], [1], scale=scale)
+        assert (np.abs(got - want) <= tol).all()
+    lib, kv = ge._lib, ge.kv
+    c = kv._CACHE.pack(kv._CACHE.size, lib.K_BF16, 1, 1, 1, 8, 0, 0, 8, 8, 8, *[0] * 5)
+    for scale, ok in ((2.0 ** 127, True), (3e38, False), (-3e38, False), (float("inf"), False), (float("nan"), False)):
+        a = kv._ATTEND.pack(kv._ATTEND.size, 1, 1, 1, lib.K_BF16, 1, *[0] * 6, 1, scale, *[0] * 7)
+        if ok:
+            assert lib.handle(gpu.index, 1, 1).call("gsk_attention_work", c, a) >= 0
+            continue
+        with pytest.raises(RuntimeError, match="scale"):
+            lib.handle(gpu.index, 1, 1).call("gsk_attention_work", c, a)

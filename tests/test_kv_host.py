@@ -197,3 +197,11 @@ def test_attend_refuses_more_rows_than_are_counted(ge):
     ok = dict(q=torch.zeros((1, 1, 8), dtype=BF).expand(1 << 24, 255, 8), keys=k, values=k.clone(), begin=[0, 1], max_new=1 << 24, seq_len=[1],
               table=torch.zeros((1, 1), dtype=torch.int32))
     _refusals(ge.kv.attend, ok, [dict(q=torch.zeros((1, 1, 8), dtype=BF).expand(1 << 24, hq, 8)) for hq in (256, 300, 512)])
+
+
+def test_attend_refuses_scales_past_2_to_127(ge):
+    """A scale times log2 e is to be finite in fp32."""
+    k, v = _caches()
+    ok = dict(q=torch.zeros(7, 6, 16, dtype=BF), keys=k, values=v, table=torch.zeros(2, 5, dtype=torch.int32), seq_len=[9, 9], begin=[0, 3, 7],
+              scale=2.0 ** 127)
+    _refusals(ge.kv.attend, ok, [dict(scale=s) for s in (3e38, -3e38, 2.0 ** 127 * 1.001, -1e300)])

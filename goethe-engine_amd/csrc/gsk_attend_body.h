@@ -17,11 +17,12 @@
 // instruction e of eight has element 8c + e as its row c. So nothing goes through LDS but the tokens' offsets (a lane finds one
 // token's, a block ahead) and 8-bit scales. 8-bit elements are exact in 16 bits; their scales multiply S and p in fp32.
 //
-// The weights p (up to 2^8: the maximum lags) go into the second product as two 16-bit numbers, so that results are off by little more than
-// their own rounding (with one, half a step of each weight, bfloat16's rms error was up to a seventh more). Over a 16-bit cache a weight is cut
-// off and its rest rounded, off by 2^-15 of it in bfloat16 and 2^-20 in float16: both above 0, so that an infinite value times them is the
-// same infinity. Over an 8-bit cache, whose values are finite or NaN, a weight is p times the token's scale, which may leave
-// float16's range: two bfloat16 numbers, rounded and the rest (2^-16), whatever q's type.
+// The weights p (up to 2^8: the maximum lags) go into the second product as two 16-bit numbers, so that results are off by little
+// more than their own rounding (with one, half a step of each weight, bfloat16's rms error was up to a seventh more). Over a 16-bit
+// cache a weight is cut off and its rest rounded, off by 2^-15 of it in bfloat16 and 2^-20 in float16: both above 0, so that an
+// infinite value times them is the same infinity (float16: at weights down to 2^-20 of the largest; below, it may become NaN). Over
+// an 8-bit cache, whose values are finite or NaN, a weight is p times the token's scale, which may leave float16's range: two
+// bfloat16 numbers, rounded and the rest (2^-16), whatever q's type.
 //
 // Bound: memory, by how the rows lie and by how evenly the workgroups of a CU get on. 128 requests of up to 16384 tokens of 8 heads of
 // 128 8-bit elements (2.79 GB, 2.83 read by the counters), 8 rows a head: 534 us, 5.2 TB/s; with the heads ahead of a page's tokens 481 us,

@@ -14,8 +14,9 @@
 // lists: log of each beam's sum, then the n best of all entries by the same two steps.
 //
 // Bound: 4 beams of 128256 fp32 logits, 14.4 us, are a chain: a slice's load, its maxima, bound, list and ranks (8 us), the ticket, the
-// join's reads, logs and ranks. 64 requests of 8 beams of 151936 bf16 logits (156 MB), 63.5 us or 2.4 TB/s (fp32: 79, 3.9), are bound
-// by instructions (15 on each element of 2 bytes by the counters: unpacking, maxima, exp2, compare), then by the last request's join.
+// join's reads, logs and ranks. 64 requests of 8 beams of 151936 bf16 logits (156 MB), 66 us or 2.4 TB/s, are bound by what waves wait
+// for, 54 % of their cycles by the counters (three barriers a slice, the list and its ranks; the last request's join), then by
+// instructions (17 on each element of 2 bytes: unpacking, maxima, exp2, its sum in fp64, compare).
 #include "gsk_dev.h"
 #include "gsk_int.h"
 

@@ -155,8 +155,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // other; then its threads walk the (cache, chunk, token, place) of the block: neighbouring tokens of a chunk lie together
 // where the heads come first.
 //
-// Bound: memory where there is enough to move (8 groups of 8 beams, 256 tokens in 48 caches of 400 bytes: 550 MB, 99 us, 5.6 TB/s);
-// else the launch, the table and the rows one after the other (4 beams, 16 tokens, 64 caches of 2 KB rows: 5.9 us).
+// Bound: memory where there is enough to move (8 groups of 8 beams, 256 tokens in 48 caches of 400 bytes: 550 MB, 121 to 125 us over two
+// or three sets of arrays in turn, 4.5 TB/s; 99 us where calls repeat on one set, part of which the last-level cache holds); else the
+// launch, the table and the rows one after the other (4 beams, 16 tokens, 64 caches of 2 KB rows: 6.5 us in turn, 6.0 on one set).
 struct ReorderShared {
   int64_t src[CT], dst[CT];
   uint32_t n[CT];
@@ -274,9 +275,9 @@ hipError_t launch_read(const gsk_cache &c, const gsk_read_rows &a, hipStream_t s
 }
 
 hipError_t launch_reorder(const gsk_reorder_beams &in, hipStream_t s) {
-  // Workgroups of a launch to aim for, a thread's vectors of a block of tokens (8 x 8 beams, 256 and 16 tokens: 98 and 8.9 us; with four
-  // vectors 107 and 13.2, with two 103 and 10.3; with 2048 workgroups 101 and 8.1, with 8192 95 and 9.9, and 4 beams of 16
-  // tokens 5.5, 5.8 and 7.2 with 2048, 4096 and 8192).
+  // Workgroups of a launch to aim for, a thread's vectors of a block of tokens (calls on one set of arrays; 8 x 8 beams, 256 and
+  // 16 tokens: 98 and 8.9 us; with four vectors 107 and 13.2, with two 103 and 10.3; with 2048 workgroups 101 and 8.1, with 8192
+  // 95 and 9.9, and 4 beams of 16 tokens 5.5, 5.8 and 7.2 with 2048, 4096 and 8192).
   constexpr int64_t WGS = 4096, EACH = 1;
   auto go = [&](auto v, auto mb) {
     using V = decltype(v);

@@ -86,8 +86,8 @@ typedef struct gsk_read_rows {
  * of those itself and the earlier ones; with parent: itself, parent[row], that one's parent and so on (entries that are no
  * earlier row of the request end the path). Query head h reads head h / (heads / cache heads). Where nothing is seen, or every
  * score is -inf, the result is 0, as it is for a request with status[r] != 0 or with numbers out of range; cached tokens
- * whose page is out of range are not seen. A NaN or an infinity reaches the rows that see its token, and no other. Rows from
- * begin[requests] on are left as they were. */
+ * whose page is out of range are not seen. A NaN or an infinity reaches the rows that see its token, whatever the token's weight (a
+ * value's may stay out where its score is -inf), and no other. Rows from begin[requests] on are left as they were. */
 typedef struct gsk_attention {
   uint32_t size;
   uint32_t requests;

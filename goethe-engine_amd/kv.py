@@ -310,7 +310,8 @@ def reorder(caches, table, seq_len, parents, first=None, heads_first=False):
     table and seq_len, and gets the tokens first[g] <= t < seq_len of beam parents[g, b] as they were before the call (first: 0;
     what comes before it, a prompt, is alike in a group's beams). caches: a paged.Caches, or one stacked tensor [n, pages, page,
     ...] (heads_first: [n, pages, heads, page, ...]), of any type. table int32 [groups * beams, pages] (PageTable.table), a page in
-    one row. At most 32 beams; a parent out of range leaves its beam as it is, and tokens past either beam's length stay."""
+    one row. At most 32 beams; a parent out of range leaves its beam as it is, a negative first its group, and tokens past either
+    beam's length stay."""
     stacked = not isinstance(caches, Caches)
     if not stacked:
         n, layout, dev = len(caches.tensors), caches.layout, caches.device

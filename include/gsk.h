@@ -140,8 +140,8 @@ typedef struct gsk_beams {
 
 /* The cached tokens first[g] <= t < seq_len of each beam's row replaced by those of the beam that it continues, for every beam
  * of a group at once (as they were before the call): beam b of group g is table row g * beams + b, its source parent[g * beams +
- * b] in 0 .. beams - 1 (another value: left as it is). A token past either beam's length stays. Caches, strides and chunks as in
- * gsp_path; pages belong to one row. */
+ * b] in 0 .. beams - 1 (another value: left as it is). A token past either beam's length stays, as does a group whose first is
+ * negative. Caches, strides and chunks as in gsp_path; pages belong to one row. */
 typedef struct gsk_reorder_beams {
   uint32_t size;
   uint32_t groups;

@@ -133,7 +133,7 @@ def test_sums_of_peaked_rows(ge, gpu, dtype, far, peaks, n):
     """A few tokens (or more than a list holds) at 0 and a hundred thousand others far below, all alike or spread out: a row's sum is
     off by its far terms' own errors, never by what adding them to the large ones costs. Of each term below the listed ones, with t
     its distance from the maximum: t's rounding and its product's with log2 e, 2^-24 |t| each, and exp2's, 2^-23; so 2^-24 (2 |t| + 4)
-    of it is allowed. Terms at the maximum itself are exact. Two beams whose sums differ by 2^-20.5 come in their order."""
+    of it is allowed. Terms at the maximum itself are exact."""
     v = 128256
     g = torch.Generator(device=gpu).manual_seed(peaks)
     x = torch.full((4, v), -far, device=gpu)
